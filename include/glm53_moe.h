@@ -621,6 +621,105 @@ int glm_mxfp4_is_tiled(int rows, int K);
 int glm_scalex_decode(void *stream, const uint8_t *staging, int64_t staging_bytes,
                       const int64_t *records, int n, int64_t *device_table);
 
+/* ------------------------------------------------------------ paged attention cache */
+
+/*
+ * The cache of a decoder layer's attention for a batch of requests.  The
+ * reference keeps one request's history in arrays that grow (DSACache,
+ * cache.py:53-103); here a pool of num_pages pages of page_size positions
+ * serves many requests, and a block table [request][max_blocks] names each
+ * request's pages in order.  A slot is page * page_size + offset.
+ * Cache tensors: keys [num_pages][kv_heads][page_size][key_dim], values
+ * [num_pages][kv_heads][page_size][value_dim]; GLM_FMT_BF16 (bf16), or
+ * GLM_FMT_MXFP8: E4M3FN codes u8 of the same shape and E8M0 scales u8 with
+ * the last axis / 32.  A latent cache has keys alone: the values are the first
+ * value_dim channels of the key rows.
+ */
+
+/* status bits of glm_cache_step: nothing is changed where one is set */
+#define GLM_CACHE_OUT_OF_PAGES 1    /* more pages needed than are free */
+#define GLM_CACHE_TABLE_FULL 2      /* a request would pass max_blocks * page_size */
+#define GLM_CACHE_TOO_MANY_TOKENS 4 /* more new tokens than max_tokens */
+#define GLM_CACHE_BAD_STATE 8       /* lens, blocks or num_free are none that a step leaves */
+
+/*
+ * One step of B requests: pages given back and taken, on the GPU.
+ * new_lens i32 [B]: n >= 0 appends n tokens to request b; -1 - n gives the
+ * request's pages back first and starts a new one of n tokens in its place
+ * (-1: the request is over).  A request keeps max(blocks, ceil(length /
+ * page_size)) pages: a caller may lower a length (rejected tokens) and append
+ * again.
+ * lens i32 [B]: tokens held before the step.  State, updated in place:
+ * blocks i32 [B] (pages held), tables i32 [B][max_blocks] (entries past
+ * blocks are not read; those of a request given back become -1), free_pages
+ * i32 [num_pages] (a stack: the first *num_free entries are free),
+ * num_free i32 [1].  Pages given back go on top in request order; new pages
+ * are taken from the top, requests in order.
+ * Written: kv_lens i32 [B], the lengths after the step (may be lens itself);
+ * cu_new i32 [B + 1], exclusive sums of the new tokens; for each of the
+ * max_tokens token rows slots i32 (where it goes in the cache, -1 past the
+ * last token) and positions i32 (in its request, 0 past the last); status i32
+ * [1], 0 or GLM_CACHE_* bits.  Where a bit is set, the state stays as it was,
+ * kv_lens = lens, cu_new = 0 and every slot is -1.
+ * Limits: B <= 4096; num_pages * page_size and max_blocks * page_size below
+ * 2^31.  Calls on one state must be ordered.
+ */
+int glm_cache_step(void *stream, const int32_t *new_lens, int B, int num_pages, int page_size,
+                   int max_blocks, int max_tokens, const int32_t *lens, int32_t *blocks,
+                   int32_t *tables, int32_t *free_pages, int32_t *num_free, int32_t *kv_lens,
+                   int32_t *cu_new, int32_t *slots, int32_t *positions, int32_t *status);
+
+/*
+ * Writes N tokens' rows into their slots: keys bf16, token t's kv_heads x
+ * key_dim elements at t * key_stride (elements), values likewise; value_dim 0
+ * (and NULL values and value_cache) for a latent cache.  bf16 caches take the
+ * rows as they are.  MXFP8: per 32 channels the smallest E8M0 exponent (from
+ * 2^-124 on) that keeps the largest finite magnitude within 448, codes rounded
+ * to nearest even; an infinity or a NaN is stored as NaN.
+ * A token whose slot is not in [0, num_pages * page_size) is skipped.  Slots
+ * named twice in one call hold pieces of either row.
+ * Limits: widths multiples of 8 (MXFP8: 32) up to 1024; strides multiples of
+ * 8; num_pages * page_size * kv_heads < 2^31.
+ */
+int glm_cache_write(void *stream, const uint16_t *keys, int64_t key_stride,
+                    const uint16_t *values, int64_t value_stride, const int32_t *slots, int N,
+                    int num_pages, int page_size, int kv_heads, int key_dim, int value_dim,
+                    int fmt, void *key_cache, uint8_t *key_scales, void *value_cache,
+                    uint8_t *value_scales);
+
+/*
+ * Workspace bytes of glm_paged_attention; 0 for sizes that it refuses.
+ */
+size_t glm_paged_attention_workspace_bytes(int B, int q_len, int heads, int kv_heads, int key_dim,
+                                           int value_dim, int page_size, int max_blocks);
+
+/*
+ * Attention of the newest q_len tokens of B requests over their cached
+ * history (one token of a decode step, a few of a verify step; the reference's
+ * dense-equivalent attention, dsa.py:41-56).  q bf16, token (b, t) at
+ * (b * q_len + t) * q_stride elements, heads x key_dim; query head h reads kv
+ * head h / (heads / kv_heads).  lens i32 [B]: positions in the cache, the new
+ * tokens' own among them (glm_cache_step's kv_lens; clamped to [0, max_blocks
+ * * page_size]).  Token t sees the positions j < lens[b] - (q_len - 1 - t):
+ *   s_j = scale q . k_j,  out[b][t][h] = sum_j softmax(s)_j v_j
+ * in f32, the probabilities rounded to bf16 for their product with the values
+ * (the denominator is their f32 sum); out bf16 [B * q_len][heads][value_dim].
+ * A row that sees no position gives zeros.  A position whose table entry is
+ * not in [0, num_pages) is not seen; cache rows past a request's length are
+ * never used, whatever they hold.
+ * value_cache NULL: a latent cache (value_dim <= key_dim).
+ * Limits: heads % kv_heads == 0, heads <= 1024, q_len <= 16, B <= 65535, widths
+ * multiples of 8 (MXFP8: 32) up to 1024, num_pages * page_size * kv_heads and
+ * max_blocks * page_size + 64 < 2^31.  The workspace needs no clearing; calls
+ * that may overlap need their own.
+ */
+int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_stride, int B, int q_len,
+                        int heads, int kv_heads, int key_dim, int value_dim,
+                        const void *key_cache, const uint8_t *key_scales, const void *value_cache,
+                        const uint8_t *value_scales, int fmt, int num_pages, int page_size,
+                        const int32_t *tables, const int32_t *lens, int max_blocks, float scale,
+                        void *workspace, size_t workspace_bytes, uint16_t *out);
+
 #ifdef __cplusplus
 }
 #endif

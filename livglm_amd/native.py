@@ -42,6 +42,11 @@ GLM_READ_DROP_CACHE = 1
 GLM_HC_BF16_STREAMS = 1
 GLM_NOALLOC_SCRATCH_BYTES = 64 << 20
 
+GLM_CACHE_OUT_OF_PAGES = 1
+GLM_CACHE_TABLE_FULL = 2
+GLM_CACHE_TOO_MANY_TOKENS = 4
+GLM_CACHE_BAD_STATE = 8
+
 ABI_VERSION = 2
 
 _p = ctypes.c_void_p
@@ -104,6 +109,12 @@ SIGNATURES = {
     "glm_mxfp4_tile": (_i, [_p, _p, _p, _i64, _i, _i]),
     "glm_mxfp4_is_tiled": (_i, [_i, _i]),
     "glm_scalex_decode": (_i, [_p, _p, _i64, _p, _i, _p]),
+    "glm_cache_step": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "glm_cache_write": (_i, [_p, _p, _i64, _p, _i64, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p,
+                             _p]),
+    "glm_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "glm_paged_attention": (_i, [_p, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i, _i, _i,
+                                 _p, _p, _i, _f, _p, _sz, _p]),
 }
 
 

@@ -1,0 +1,208 @@
+"""The paged attention cache on the host: the oracle against plain statements,
+and every refusal of the C ABI and of the Python entry points (nothing here
+reaches a GPU)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from livglm_amd import native
+from oracle import paged_oracle as P
+
+FAKE = ctypes.c_void_p(0x10000)  # never dereferenced: validation fails first
+ODD = ctypes.c_void_p(0x10004)
+
+
+# ---------------------------------------------------------------- the oracle
+
+def test_oracle_step_keeps_every_page_once():
+    rng = np.random.default_rng(5)
+    B, page, width, pool = 7, 4, 12, 60
+    lens, blocks = np.zeros(B, int), np.zeros(B, int)
+    tables, free, top = np.full((B, width), -1, np.int32), np.arange(pool)[::-1].astype(np.int32), pool
+    for _ in range(60):
+        new = rng.integers(-9, 9, B)
+        r = P.step(new, lens, blocks, tables, free, top, page, 80)
+        if r["status"]:
+            new = np.full(B, -1)  # all over
+            r = P.step(new, lens, blocks, tables, free, top, page, 80)
+        assert r["status"] == 0
+        lens, blocks, tables, free, top = (r[k] for k in ("kv_lens", "blocks", "tables", "free_pages", "num_free"))
+        held = [tables[b, j] for b in range(B) for j in range(blocks[b])]
+        assert sorted(held + list(free[:top])) == list(range(pool))
+        assert (blocks * page >= lens).all()
+        used = r["slots"][: r["cu_new"][-1]]
+        assert len(set(used)) == len(used) and (used >= 0).all()
+        assert (r["slots"][r["cu_new"][-1]:] == -1).all()
+
+
+def test_oracle_mx_rows_are_the_nearest_codes():
+    rng = np.random.default_rng(6)
+    x = (rng.standard_normal((9, 64)) * np.exp2(rng.integers(-140, 120, (9, 1)))).astype(np.float32)
+    x = P.bf16_bits_to_f32((x.view(np.uint32) >> 16).astype(np.uint16)).astype(np.float64)
+    x[0], x[1, 3], x[1, 40], x[2, :32] = 0, np.nan, -np.inf, 448.0
+    codes, scales = P.mx_rows(x)
+    assert (scales >= 3).all()
+    v = P.mx_values(codes, scales)
+    fine = np.isfinite(x)
+    assert np.isnan(v[~fine]).all()
+    step = np.maximum(np.exp2(scales.astype(float) - 127 - 9).repeat(32, -1), np.abs(x) / 8)
+    assert (np.abs(v - x)[fine] <= 0.5 * step[fine] * (1 + 1e-12)).all()
+    assert (scales[2, 0] - 127, codes[2, 0]) == (0, 0x7e)
+
+
+# ---------------------------------------------------------------- the C ABI's refusals
+
+def _step_args(**kw):
+    a = dict(stream=None, new=FAKE, B=2, num_pages=8, page=16, max_blocks=4, max_tokens=8, lens=FAKE, blocks=FAKE,
+             tables=FAKE, free=FAKE, num_free=FAKE, kv=FAKE, cu=FAKE, slots=FAKE, positions=FAKE, status=FAKE)
+    a.update(kw)
+    return list(a.values())
+
+
+def _write_args(**kw):
+    a = dict(stream=None, keys=FAKE, ks=256, values=FAKE, vs=256, slots=FAKE, N=2, num_pages=8, page=16, heads=2,
+             dk=128, dv=128, fmt=native.GLM_FMT_BF16, kc=FAKE, ksc=None, vc=FAKE, vsc=None)
+    a.update(kw)
+    return list(a.values())
+
+
+def _attend_args(**kw):
+    a = dict(stream=None, q=FAKE, qs=1024, B=2, q_len=1, heads=8, kv_heads=2, dk=128, dv=128, kc=FAKE, ksc=None,
+             vc=FAKE, vsc=None, fmt=native.GLM_FMT_BF16, num_pages=8, page=16, tables=FAKE, lens=FAKE, max_blocks=4,
+             scale=0.1, ws=FAKE, nbytes=1 << 30, out=FAKE)
+    a.update(kw)
+    return list(a.values())
+
+
+INVALID, SHAPE, WORKSPACE = (native.GLM_ERR_INVALID_ARGUMENT, native.GLM_ERR_UNSUPPORTED_SHAPE,
+                             native.GLM_ERR_WORKSPACE)
+
+
+@pytest.mark.parametrize("code, change", [
+    *[(INVALID, {k: None}) for k in ("new", "lens", "blocks", "tables", "free", "num_free", "kv", "cu", "slots",
+                                     "positions", "status")],
+    (INVALID, {"B": 0}), (INVALID, {"B": -1}), (SHAPE, {"B": 4097}), (INVALID, {"num_pages": 0}),
+    (INVALID, {"page": 0}), (INVALID, {"max_blocks": 0}), (INVALID, {"max_tokens": -1}),
+    (SHAPE, {"num_pages": 1 << 27}), (SHAPE, {"max_blocks": 1 << 27}),
+])
+def test_step_refusals(code, change):
+    assert native.load().glm_cache_step(*_step_args(**change)) == code
+    assert native.load().glm_last_error()
+
+
+@pytest.mark.parametrize("code, change", [
+    *[(INVALID, {k: None}) for k in ("keys", "slots", "kc", "values", "vc")],
+    (INVALID, {"fmt": native.GLM_FMT_MXFP4}), (INVALID, {"fmt": native.GLM_FMT_MXFP8}),
+    (INVALID, {"fmt": native.GLM_FMT_MXFP8, "ksc": FAKE}), (INVALID, {"N": -1}), (INVALID, {"page": 0}),
+    (SHAPE, {"dk": 100}), (SHAPE, {"dv": 4}), (SHAPE, {"dk": 2048, "ks": 4096}), (INVALID, {"ks": 255}),
+    (INVALID, {"ks": 260}), (INVALID, {"vs": 248}), (INVALID, {"keys": ODD}), (INVALID, {"vc": ODD}),
+    (SHAPE, {"dk": 40, "fmt": native.GLM_FMT_MXFP8, "ksc": FAKE, "vsc": FAKE}),
+    (SHAPE, {"num_pages": 1 << 27}),
+])
+def test_write_refusals(code, change):
+    assert native.load().glm_cache_write(*_write_args(**change)) == code
+    assert native.load().glm_last_error()
+
+
+@pytest.mark.parametrize("code, change", [
+    *[(INVALID, {k: None}) for k in ("q", "kc", "tables", "lens", "ws", "out")],
+    (INVALID, {"fmt": native.GLM_FMT_MXFP4}), (INVALID, {"fmt": native.GLM_FMT_MXFP8}),
+    (INVALID, {"fmt": native.GLM_FMT_MXFP8, "ksc": FAKE}), (INVALID, {"B": -1}), (INVALID, {"q_len": 0}),
+    (SHAPE, {"q_len": 17}), (SHAPE, {"heads": 7}), (SHAPE, {"heads": 2048, "qs": 1 << 18}), (SHAPE, {"B": 65536}),
+    (SHAPE, {"dk": 100}), (SHAPE, {"dv": 1032}), (SHAPE, {"vc": None, "dv": 136}), (INVALID, {"qs": 1016}),
+    (INVALID, {"qs": 1028}), (INVALID, {"scale": float("nan")}), (INVALID, {"scale": float("inf")}),
+    (INVALID, {"q": ODD}), (INVALID, {"out": ODD}), (INVALID, {"ws": ODD}), (WORKSPACE, {"nbytes": 16}),
+    (SHAPE, {"num_pages": 1 << 27}), (SHAPE, {"max_blocks": 1 << 27}), (INVALID, {"max_blocks": 0}),
+])
+def test_attend_refusals(code, change):
+    assert native.load().glm_paged_attention(*_attend_args(**change)) == code
+    assert native.load().glm_last_error()
+
+
+def test_attend_workspace():
+    size = native.load().glm_paged_attention_workspace_bytes
+    need = size(2, 1, 8, 2, 128, 128, 16, 4)
+    assert need > 0
+    assert native.load().glm_paged_attention(*_attend_args(nbytes=need - 1 - 256)) == WORKSPACE
+    assert size(2, 1, 7, 2, 128, 128, 16, 4) == 0 and size(-1, 1, 8, 2, 128, 128, 16, 4) == 0
+    # bounded by the work that the chip takes at once, not by the batch
+    assert size(4096, 1, 128, 8, 128, 128, 16, 8192) < 512 << 20
+
+
+def test_empty_batches_are_no_ops():
+    assert native.load().glm_cache_write(*_write_args(N=0)) == native.GLM_OK
+    assert native.load().glm_paged_attention(*_attend_args(B=0)) == native.GLM_OK
+
+
+# ---------------------------------------------------------------- the Python refusals
+
+def test_python_refuses_host_tensors():
+    from glm53flash import paged_cache as C
+    from glm53flash.contract import ContractError
+    i = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ContractError):
+        C.cache_step(i, i, i, i.view(1, 4), i, i[:1], page_size=4, max_tokens=4)
+    x, cache = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 8, 64, dtype=torch.bfloat16)
+    with pytest.raises(ContractError):
+        C.cache_write(x, x, i, cache, cache)
+    with pytest.raises(ContractError):
+        C.paged_attention(x, cache, cache, i.view(4, 1), i, scale=1.0)
+
+
+def test_python_objects():
+    from glm53flash import paged_cache as C
+    from glm53flash.contract import ContractError
+    from glm53flash.model_config import GLMTextConfig
+    table = C.PageTable(8, 16, 4, 6, device="cpu")
+    assert table.free_pages.tolist() == list(range(7, -1, -1)) and table.num_free.item() == 8
+    cfg = GLMTextConfig(kv_lora_rank=512, qk_rope_head_dim=64)
+    cache = C.PagedKVCache.from_config(cfg, table, quantization_mode="mxfp8")
+    assert cache.keys.shape == (8, 1, 16, 576) and cache.key_scales.shape == (8, 1, 16, 18)
+    assert cache.latent and cache.values is None and cache.value_dim == 512
+    cfg = GLMTextConfig(num_key_value_heads=2, qk_nope_head_dim=64, qk_rope_head_dim=64, v_head_dim=96)
+    cache = C.PagedKVCache.from_config(cfg, table)
+    assert cache.keys.shape == (8, 2, 16, 128) and cache.values.shape == (8, 2, 16, 96)
+    with pytest.raises(ContractError):
+        C.PagedKVCache.from_config(GLMTextConfig(), table)
+    with pytest.raises(ContractError):
+        C.PagedKVCache(table, 1, 64, 128, latent=True)
+    with pytest.raises(ContractError):
+        C.PagedKVCache(table, 1, 72, 72, quantization_mode="mxfp8")
+    with pytest.raises(ContractError):
+        C.PagedKVCache(table, 1, 64, 64, quantization_mode="int8")
+    with pytest.raises(ContractError):
+        C.PageTable(0, 16, 4, 6, device="cpu")
+
+
+def test_token_rows_strides():
+    from glm53flash.contract import ContractError
+    from glm53flash import paged_cache as C
+    qkv = torch.zeros(6, 10, 64, dtype=torch.bfloat16, device="meta")
+
+    class OnGpu:  # the check reads shapes and strides alone
+        def __init__(self, t):
+            self.shape, self.dtype, self.is_cuda, self.device = t.shape, t.dtype, True, "cuda"
+            self.stride = t.stride
+
+    def rows(t):
+        real, torch.Tensor_ = torch.Tensor, None
+        try:
+            C.torch = type("T", (), {"Tensor": (OnGpu, real), "bfloat16": torch.bfloat16})
+            return C._token_rows(OnGpu(t), "t")
+        finally:
+            C.torch = torch
+            del torch.Tensor_
+
+    assert rows(qkv[:, 2:6]) == 640
+    assert rows(qkv[:1, 2:6]) == 256
+    assert rows(qkv.view(3, 2, 10, 64)[:, :, :4]) == 640
+    assert rows(qkv.view(3, 2, 10, 64)[:, :1, :4]) == 1280
+    assert rows(qkv.view(3, 2, 10, 64)[:1, :, :4]) == 640
+    for bad in (qkv.transpose(1, 2), qkv[:, ::2], qkv.view(2, 3, 10, 64)[:, :2], qkv[0]):
+        with pytest.raises(ContractError):
+            rows(bad)
