@@ -27,6 +27,7 @@ struct AttnArgs {
   int2 *plan;        // [B] {splits, first partial}, for the join
   float *part, *ml;  // partial results [item][rows][dv], [item][rows][2]
   int B, q_len, heads, kv_heads, dk, dv, num_pages, page, max_blocks;
+  int page_shift;  // log2 of page, -1 where it is no power of two
   int rows;     // rows of an item: one kv head's row block
   int hblocks;  // kv_heads x row blocks
   int target, min_c;  // items wanted over all, fewest tiles of an item
@@ -195,6 +196,349 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// Grouped heads on the matrix cores.  A workgroup's item is 16 MT query rows
+// of one kv head (its group's heads, times the new tokens) over a range of
+// positions; its four waves take 32 positions in turn, each by itself, and
+// are joined in LDS at the item's end.  A wave forms
+//   S^T = K Q^T   (A: 16 positions x 32 channels straight from the cache,
+//                  B: the rows, in registers for good),
+//   O^T += V^T P^T (A: V^T by transposing LDS reads, B: P^T)
+// with v_mfma_f32_16x16x32_bf16.  S^T leaves lane (n, quad) with row n's
+// scores of positions 4 quad .. + 3 of two 16-position tiles: exactly the
+// eight k-slots of the B operand P^T, if V^T's slots are given the same
+// order, so the probabilities never leave their lane, and a row's maximum,
+// sum and rescaling are one lane column's own.  Only V goes through LDS (a
+// wave's own part: no barrier in the loop).  The next tile's keys are loaded
+// as soon as the products with this one's are formed, its values as soon as
+// these are in LDS, its page numbers a tile earlier.
+// Bound by the cache's bytes; a wave holds 32 positions of keys and values in
+// flight.
+// Masks: rows of a tile see the same positions but where it ends, so only
+// tiles with a position that some row does not see take the masked form.
+// ---------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+
+// One cache row's channels as lane (n, quad) holds them: pieces of 16 bytes,
+// 64 bytes of four quads in turn, and the scales of its pieces.
+template <int FMT, int D>
+struct CacheRow {
+  static constexpr int kPieces = FMT == GLM_FMT_BF16 ? D / 32 : D / 64;
+  glm_u32x4 v[kPieces];
+  uint32_t sc[FMT == GLM_FMT_BF16 ? 1 : (D + 127) / 128];
+
+  __device__ __forceinline__ void load(const void *cache, const uint8_t *scales, long long row,
+                                       int dim, int quad) {
+    const uint8_t *p = (const uint8_t *)cache + row * (FMT == GLM_FMT_BF16 ? 2 * dim : dim) + 16 * quad;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      v[i] = __builtin_nontemporal_load(reinterpret_cast<const glm_u32x4 *>(p + 64 * i));
+    if constexpr (FMT != GLM_FMT_BF16) {
+      const uint8_t *s = scales + row * (dim / 32);
+#pragma unroll
+      for (int i = 0; i < (D + 127) / 128; ++i) {  // (a row's scales need not be 4-byte aligned)
+        if (128 * (i + 1) <= D) {
+          __builtin_memcpy(&sc[i], s + 4 * i, 4);
+        } else {
+          uint16_t two;
+          __builtin_memcpy(&two, s + 4 * i, 2);
+          sc[i] = two;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) v[i] = glm_u32x4{0, 0, 0, 0};
+  }
+  // channels of MFMA step s: bf16 32 s + 8 quad .. + 7; MXFP8 64 (s / 2) + 16 quad + 8 (s % 2) .. + 7
+  __device__ __forceinline__ glm_bf16x8 step(int s, int quad) const {
+    if constexpr (FMT == GLM_FMT_BF16) {
+      return __builtin_bit_cast(glm_bf16x8, v[s]);
+    } else {
+      const int j = s / 2, h = s % 2;
+      const uint32_t byte = (sc[j / 2] >> (16 * (j % 2) + 8 * (quad >> 1))) & 0xffu;
+      return mxfp8_words_to_bf16x8(v[j][2 * h], v[j][2 * h + 1], e8m0_to_f32(byte));
+    }
+  }
+  static __device__ __forceinline__ int channel(int s, int quad) {
+    return FMT == GLM_FMT_BF16 ? 32 * s + 8 * quad : 64 * (s / 2) + 16 * quad + 8 * (s % 2);
+  }
+};
+
+__device__ __forceinline__ bf16x4 lds_read_tr(const uint16_t *p) {
+  typedef __attribute__((ext_vector_type(4))) short s16x4;
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  return __builtin_bit_cast(
+      bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(__attribute__((address_space(3))) void *)p));
+}
+
+__device__ __forceinline__ float max_over_quads(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, kWave));
+  return fmaxf(x, __shfl_xor(x, 32, kWave));
+}
+__device__ __forceinline__ float sum_over_quads(float x) {
+  x += __shfl_xor(x, 16, kWave);
+  return x + __shfl_xor(x, 32, kWave);
+}
+
+// Cache rows of the positions of two 16-position tiles, lane (n, .) position
+// p + 16 u + n; a position past `end` or on a page that is not one of the
+// cache's gets row 0 and a cleared bit.
+struct TileRows {
+  int row[2];
+  uint32_t seen;  // bit 16 u + n
+};
+__device__ __forceinline__ void page_of(const AttnArgs &a, int pos, int &block, int &off) {
+  if (a.page_shift >= 0) {
+    block = pos >> a.page_shift;
+    off = pos & (a.page - 1);
+  } else {
+    block = (uint32_t)pos / (uint32_t)a.page;
+    off = pos - block * a.page;
+  }
+}
+__device__ __forceinline__ TileRows tile_rows(const AttnArgs &a, const int32_t *table, int head, int p,
+                                              int end, int n) {
+  TileRows t;
+  uint32_t seen[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int pos = p + 16 * u + n;
+    int block, off;
+    page_of(a, min(pos, end - 1), block, off);
+    const int id = table[block];
+    const bool fine = (uint32_t)id < (uint32_t)a.num_pages;
+    t.row[u] = fine ? (id * a.kv_heads + head) * a.page + off : 0;
+    seen[u] = (uint32_t)__ballot(fine && pos < end) & 0xffffu;
+  }
+  t.seen = seen[0] | (seen[1] << 16);
+  return t;
+}
+
+template <int DK, int DV, int MT, int FMT, int OCC>
+__global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
+  constexpr int kStride = DV + 16;      // of a position's values in LDS, elements
+  constexpr int kAccStride = DV + 4;    // of a row's sums in LDS, floats
+  constexpr int kLds = 4 * (32 * kStride * 2 > 16 * kAccStride * 4 ? 32 * kStride * 2 : 16 * kAccStride * 4);
+  __shared__ __align__(16) uint8_t s_buf[kLds];
+  __shared__ float s_m[4][16 * MT], s_l[4][16 * MT];
+  AttnItem it;
+  if (!attn_item(a, blockIdx.x, it)) return;
+  attn_plan(a, it);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
+  const int R = attn_rows(a), group = a.heads / a.kv_heads, rb = a.hblocks / a.kv_heads;
+  const int head = it.hb / rb, r0 = (it.hb - head * rb) * 16 * MT;
+  const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
+  const void *vc = a.vc ? a.vc : a.kc;
+  const uint8_t *vs = a.vc ? a.vs : a.ks;
+  const int vdim = a.vc ? DV : DK;
+  typedef CacheRow<FMT, DK> KRow;
+  typedef CacheRow<FMT, DV> VRow;
+
+  glm_bf16x8 q[MT][DK / 32];
+  int tok[MT];  // this lane's rows' new token
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int r = min(r0 + 16 * m + n, R - 1);
+    tok[m] = r / group;
+    const uint16_t *p = a.q + ((long long)it.b * a.q_len + tok[m]) * a.q_stride +
+                        (head * group + r - tok[m] * group) * DK;
+#pragma unroll
+    for (int s = 0; s < DK / 32; ++s)
+      q[m][s] = *reinterpret_cast<const glm_bf16x8 *>(p + KRow::channel(s, quad));
+  }
+  glm_f32x4 acc[DV / 16][MT];
+  float top[MT], sum[MT];  // running maximum; this lane's part of the running sum
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    top[m] = -INFINITY;
+    sum[m] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DV / 16; ++d) acc[d][m] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  uint16_t *lv = reinterpret_cast<uint16_t *>(s_buf) + wave * 32 * kStride;
+  const uint16_t *lt = lv + (4 * quad + (n >> 2)) * kStride + 4 * (n & 3);  // transposing reads
+  const int end = min(it.t1 * kAttnTile, it.len);
+  const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
+
+  int p = it.t0 * kAttnTile + 32 * wave;
+  if (p < end) {
+    TileRows cur = tile_rows(a, table, head, p, end, n), nxt = cur;
+    KRow k[2];
+    VRow v[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) k[u].load(a.kc, a.ks, cur.row[u], DK, quad);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) v[u].load(vc, vs, cur.row[u], vdim, quad);
+    if (p + 128 < end) nxt = tile_rows(a, table, head, p + 128, end, n);
+    while (true) {
+      const bool more = p + 128 < end;
+      glm_f32x4 s[2][MT];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) s[u][m] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < DK / 32; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const glm_bf16x8 kf = k[u].step(i, quad);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            s[u][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[m][i], s[u][m], 0, 0, 0);
+        }
+      if (more) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) k[u].load(a.kc, a.ks, nxt.row[u], DK, quad);
+      }
+      const bool whole = cur.seen == 0xffffffffu && p + 32 <= all_see;  // (uniform)
+      glm_bf16x8 prob[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = s[i / 4][m][i % 4] * a.scale_log2;
+        if (!whole) {
+          const int below = all_see + tok[m];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = 16 * (i / 4) + 4 * quad + i % 4;
+            if (!((cur.seen >> at) & 1u) || p + at >= below) x[i] = -INFINITY;
+          }
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+        const float next = fmaxf(top[m], max_over_quads(mx));
+        const float from = next == -INFINITY ? 0.0f : next;
+        if (__any(next != top[m])) {
+          const float keep = __builtin_amdgcn_exp2f(top[m] - from);
+          sum[m] *= keep;
+#pragma unroll
+          for (int d = 0; d < DV / 16; ++d) acc[d][m] *= keep;
+        }
+        top[m] = next;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float e = __builtin_amdgcn_exp2f(x[i] - from);
+          sum[m] += e;
+          // bf16 for the matrix product: 2^-9 of each weight, as the output's own rounding
+          prob[m][i] = (__bf16)e;
+        }
+      }
+      if (whole) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < DV / 32; ++i)
+            *reinterpret_cast<glm_bf16x8 *>(lv + (16 * u + n) * kStride + VRow::channel(i, quad)) =
+                v[u].step(i, quad);
+        if (more) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) v[u].load(vc, vs, nxt.row[u], vdim, quad);
+        }
+#pragma unroll
+        for (int d = 0; d < DV / 16; ++d) {
+          const bf16x4 lo = lds_read_tr(lt + 16 * d), hi = lds_read_tr(lt + 16 * kStride + 16 * d);
+          const glm_bf16x8 vt = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            acc[d][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, prob[m], acc[d][m], 0, 0, 0);
+        }
+      } else {
+        // a value that a row does not see must not meet its zero weight (it may be an infinity or
+        // a NaN): one turn for each new token, with the values that it does not see as zeros, whose
+        // sums only that token's rows take
+        for (int t = p + 32 > all_see ? 0 : a.q_len - 1; t < a.q_len; ++t) {
+          const int below = all_see + t;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int at = 16 * u + n;
+            const bool fine = ((cur.seen >> at) & 1u) && p + at < below;
+#pragma unroll
+            for (int i = 0; i < DV / 32; ++i)
+              *reinterpret_cast<glm_u32x4 *>(lv + at * kStride + VRow::channel(i, quad)) =
+                  fine ? __builtin_bit_cast(glm_u32x4, v[u].step(i, quad)) : glm_u32x4{0, 0, 0, 0};
+          }
+          const bool every = p + 32 <= all_see;  // one turn for all rows
+#pragma unroll
+          for (int d = 0; d < DV / 16; ++d) {
+            const bf16x4 lo = lds_read_tr(lt + 16 * d), hi = lds_read_tr(lt + 16 * kStride + 16 * d);
+            const glm_bf16x8 vt = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              const glm_f32x4 with =
+                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, prob[m], acc[d][m], 0, 0, 0);
+              if (every || tok[m] == t) acc[d][m] = with;
+            }
+          }
+        }
+        if (more) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) v[u].load(vc, vs, nxt.row[u], vdim, quad);
+        }
+      }
+      if (!more) break;
+      p += 128;
+      cur = nxt;
+      if (p + 128 < end) nxt = tile_rows(a, table, head, p + 128, end, n);
+    }
+  }
+
+  // the four waves joined, row tile by row tile
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    sum[m] = sum_over_quads(sum[m]);
+    if (quad == 0) {
+      s_m[wave][16 * m + n] = top[m];
+      s_l[wave][16 * m + n] = sum[m];
+    }
+  }
+  __syncthreads();
+  float *la = reinterpret_cast<float *>(s_buf);
+  const long long part = attn_partial(a, it);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const float mt = fmaxf(fmaxf(s_m[0][16 * m + n], s_m[1][16 * m + n]),
+                           fmaxf(s_m[2][16 * m + n], s_m[3][16 * m + n]));
+    const float w = __builtin_amdgcn_exp2f(top[m] - (mt == -INFINITY ? 0.0f : mt));
+    if (m) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < DV / 16; ++d)
+      *reinterpret_cast<glm_f32x4 *>(la + (wave * 16 + n) * kAccStride + 16 * d + 4 * quad) =
+          acc[d][m] * w;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * DV / 4; i += 256) {
+      const int row = i / (DV / 4), ch = 4 * (i % (DV / 4)), r = r0 + 16 * m + row;
+      float mr = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int w4 = 0; w4 < 4; ++w4) mr = fmaxf(mr, s_m[w4][16 * m + row]);
+      const float from = mr == -INFINITY ? 0.0f : mr;
+      glm_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w4 = 0; w4 < 4; ++w4) {
+        l += s_l[w4][16 * m + row] * __builtin_amdgcn_exp2f(s_m[w4][16 * m + row] - from);
+        o += *reinterpret_cast<const glm_f32x4 *>(la + (w4 * 16 + row) * kAccStride + ch);
+      }
+      if (r >= R) continue;
+      if (it.splits == 1) {
+        const int t = r / group;
+        uint32_t b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = f32_to_bf16(l == 0.0f ? 0.0f : o[j] / l);
+        *reinterpret_cast<uint2 *>(
+            a.out + (((long long)it.b * a.q_len + t) * a.heads + head * group + r - t * group) * DV + ch) =
+            uint2{b[0] | (b[1] << 16), b[2] | (b[3] << 16)};
+      } else {
+        const long long at = part * a.rows + 16 * m + row;
+        *reinterpret_cast<glm_f32x4 *>(a.part + at * DV + ch) = o;
+        if (ch == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{mr, l};
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // The requests that were cut into several items: out = sum_i 2^(m_i - m) acc_i
 // / sum_i 2^(m_i - m) l_i over the items in order.  A thread has four channels
 // of a row.
@@ -236,13 +580,49 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 namespace {
 
+enum AttnForm { kAttnAny, kAttnGroup };
+
 struct AttnSizes {
+  AttnForm form;
   int rows, hblocks, target, min_c;
   long long grid, partials;  // workgroups; partial results
   size_t plan_bytes, part_bytes, ml_bytes;
 };
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// The widths that attn_group_kernel is built for.
+bool group_widths(int key_dim, int value_dim) {
+  return (key_dim == value_dim && (key_dim == 64 || key_dim == 128 || key_dim == 256)) ||
+         (key_dim == 192 && value_dim == 128);
+}
+
+template <int DK, int DV, int FMT>
+void launch_group(hipStream_t s, dim3 grid, const glm::AttnArgs &a) {
+  // two workgroups a CU where the registers allow it
+  if (a.rows == 16)
+    hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 1, FMT, (DV > 128 ? 1 : 2)>), grid, dim3(256), 0, s, a);
+  else if constexpr (DK <= 192) {
+    if (a.rows == 32)
+      hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 2, FMT, (DK > 128 ? 1 : 2)>), grid, dim3(256), 0, s, a);
+    else if constexpr (DK == 64)
+      hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 4, FMT, 1>), grid, dim3(256), 0, s, a);
+  }
+}
+
+template <int FMT>
+void launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnArgs &a) {
+  if (form == kAttnAny)
+    hipLaunchKernelGGL(glm::attn_any_kernel<FMT>, grid, dim3(256), 0, s, a);
+  else if (a.dk == 64)
+    launch_group<64, 64, FMT>(s, grid, a);
+  else if (a.dk == 128)
+    launch_group<128, 128, FMT>(s, grid, a);
+  else if (a.dk == 192)
+    launch_group<192, 128, FMT>(s, grid, a);
+  else
+    launch_group<256, 256, FMT>(s, grid, a);
+}
 
 // Sizes that follow from a call's shape; false for shapes that are refused.
 bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int value_dim, int page_size,
@@ -253,10 +633,20 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
   if (B > 65535 || q_len > 16 || heads > 1024 || (long long)max_blocks * page_size > INT_MAX - glm::kAttnTile)
     return false;
   const int R = q_len * (heads / kv_heads);
-  z.rows = 1;
-  z.hblocks = kv_heads * R;
-  z.target = 2048;
-  z.min_c = 4;
+  if (group_widths(key_dim, value_dim)) {
+    z.form = kAttnGroup;
+    const int most = key_dim == 64 ? 64 : key_dim <= 192 ? 32 : 16;  // rows that fit the registers
+    z.rows = R <= 16 || most == 16 ? 16 : R <= 32 || most == 32 ? 32 : 64;
+    z.hblocks = kv_heads * ((R + z.rows - 1) / z.rows);
+    z.target = 1024;
+    z.min_c = 2;
+  } else {
+    z.form = kAttnAny;
+    z.rows = 1;
+    z.hblocks = kv_heads * R;
+    z.target = 2048;
+    z.min_c = 4;
+  }
   const long long tiles = ((long long)max_blocks * page_size + glm::kAttnTile - 1) / glm::kAttnTile;
   if (tiles * B > INT_MAX / 2 || (long long)B * z.hblocks > INT_MAX / 2) return false;
   const long long splits = (tiles + z.min_c - 1) / z.min_c;
@@ -350,6 +740,7 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
   a.num_pages = num_pages;
   a.page = page_size;
   a.max_blocks = max_blocks;
+  a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   a.rows = z.rows;
   a.hblocks = z.hblocks;
   a.target = z.target;
@@ -358,10 +749,10 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)z.grid);
   if (mx)
-    hipLaunchKernelGGL(glm::attn_any_kernel<GLM_FMT_MXFP8>, grid, dim3(256), 0, s, a);
+    launch_attention<GLM_FMT_MXFP8>(s, grid, z.form, a);
   else
-    hipLaunchKernelGGL(glm::attn_any_kernel<GLM_FMT_BF16>, grid, dim3(256), 0, s, a);
-  GLM_LAUNCH_CHECK("attn_any_kernel");
+    launch_attention<GLM_FMT_BF16>(s, grid, z.form, a);
+  GLM_LAUNCH_CHECK("paged_attention");
   if (z.partials > 0) {
     const long long quads = (long long)q_len * heads * value_dim / 4;
     hipLaunchKernelGGL(glm::attn_join_kernel, dim3((unsigned)((quads + 255) / 256), B), dim3(256), 0,
