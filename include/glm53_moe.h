@@ -688,10 +688,12 @@ int glm_cache_write(void *stream, const uint16_t *keys, int64_t key_stride,
                     uint8_t *value_scales);
 
 /*
- * Workspace bytes of glm_paged_attention; 0 for sizes that it refuses.
+ * Workspace bytes of glm_paged_attention (latent: value_cache is NULL); 0 for
+ * sizes that it refuses.
  */
 size_t glm_paged_attention_workspace_bytes(int B, int q_len, int heads, int kv_heads, int key_dim,
-                                           int value_dim, int page_size, int max_blocks);
+                                           int value_dim, int latent, int page_size,
+                                           int max_blocks);
 
 /*
  * Attention of the newest q_len tokens of B requests over their cached

@@ -58,8 +58,14 @@ __device__ __forceinline__ bool attn_item(const AttnArgs &a, int block, AttnItem
   for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, kWave);
   const int c =
       max(a.min_c, (int)(((long long)total * a.hblocks + a.target - 1) / a.target));
-  const int s = block / a.hblocks;
+  int s = block / a.hblocks;
   it.hb = block - s * a.hblocks;
+  if (a.hblocks > a.kv_heads) {
+    // a head's row blocks read the same positions: consecutive workgroups go to the eight XCDs in
+    // turn, so the row blocks of eight items are dealt out eight apart and share an XCD's cache
+    s = block / (8 * a.hblocks) * 8 + block % 8;
+    it.hb = block / 8 % a.hblocks;
+  }
   int upto_s = 0, upto_p = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
     const int b = b0 + lane;
@@ -539,6 +545,249 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// The latent cache on the matrix cores: values are the first DV channels of
+// the key rows, so a tile is read once and serves both products, and many
+// heads share one row, so a workgroup takes 64 query rows, 16 a wave, and its
+// waves share each tile of 32 positions through LDS (two tiles in turn; a
+// barrier a tile).  The products, and the probabilities that stay in their
+// lane, are those of attn_group_kernel; the sums of 16 rows x 512 channels
+// take 128 registers, the rows 72, so two workgroups fit a CU and one's loads
+// and barriers hide behind the other's products.
+// LDS holds a tile as blocks of 1 KB, 8 positions x 64 channels, the 16-byte
+// piece c of position t at 128 t + 16 (c ^ t): a wave's load of one block
+// reads eight whole 128-byte lines, and neither the products' reads (16
+// positions x 4 pieces) nor the transposing ones (8 positions x 2 pieces a
+// half wave) meet on a bank.  bf16 goes there directly, by the swizzled
+// source address; MXFP8 through registers, a tile ahead, converted on its way
+// (exact).
+// Bound by the cache's bytes up to some 64 rows and by LDS reads beyond: a
+// tile's 68 KB for 16 rows feed 68 MFMAs.
+// ---------------------------------------------------------------------------
+template <int DK, int DV, int FMT>
+__global__ __launch_bounds__(256, 2) void attn_latent_kernel(AttnArgs a) {
+  constexpr int kG = DK / 64;               // blocks of eight positions
+  constexpr int kTile = 4 * kG * 1024;      // bytes of 32 positions
+  constexpr bool kMx = FMT != GLM_FMT_BF16;
+  constexpr int kRaw = (DK / 16 + 7) / 8;   // MXFP8: pieces of a thread's eighth of a row
+  __shared__ __align__(16) uint8_t s_kv[2][kTile];
+  AttnItem it;
+  if (!attn_item(a, blockIdx.x, it)) return;
+  attn_plan(a, it);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
+  const int R = attn_rows(a), group = a.heads / a.kv_heads, rb = a.hblocks / a.kv_heads;
+  const int head = it.hb / rb, r0 = (it.hb - head * rb) * 64 + 16 * wave;
+  const bool active = r0 < R;  // (uniform in a wave)
+  const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
+  const int end = min(it.t1 * kAttnTile, it.len);
+  const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
+
+  const int r = min(r0 + n, R - 1), tok = r / group;
+  glm_bf16x8 q[DK / 32];
+  {
+    const uint16_t *p = a.q + ((long long)it.b * a.q_len + tok) * a.q_stride +
+                        (head * group + r - tok * group) * DK + 8 * quad;
+#pragma unroll
+    for (int s = 0; s < DK / 32; ++s) q[s] = *reinterpret_cast<const glm_bf16x8 *>(p + 32 * s);
+  }
+  glm_f32x4 acc[DV / 16];
+#pragma unroll
+  for (int d = 0; d < DV / 16; ++d) acc[d] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, sum = 0.0f;
+
+  // this thread's share of a tile: an eighth of position `mine`
+  const int tl = lane >> 3, pc = lane & 7, mine = 8 * wave + tl;
+  // the products' reads: position n, piece 4 (s % 2) + quad of 64 channels s / 2; even s, odd s + 64 ^
+  const int kread = (n >> 3) * kG * 1024 + (n & 7) * 128 + ((quad ^ (n & 7)) << 4);
+  // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
+  const int vt = 4 * quad + (n >> 2);
+  const int vread = (vt >> 3) * kG * 1024 + (vt & 7) * 128 + ((((n & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (n & 1);
+
+  struct Rows {
+    int row;        // of this thread's position
+    uint32_t seen;  // of the tile's 32
+  };
+  const auto rows_at = [&](int p) {
+    const int pos = p + (lane & 31);
+    int block, off;
+    page_of(a, min(pos, end - 1), block, off);
+    const int id = table[block];
+    const bool fine = (uint32_t)id < (uint32_t)a.num_pages;
+    const int row = fine ? (id * a.kv_heads + head) * a.page + off : 0;
+    return Rows{__shfl(row, mine, kWave), (uint32_t)__ballot(fine && pos < end)};
+  };
+  glm_u32x4 raw[kRaw];
+  uint32_t rsc[kRaw];
+  const auto fetch = [&](const Rows &at, int buf) {  // bf16: into LDS; MXFP8: into registers
+    if constexpr (!kMx) {
+      const uint8_t *src = (const uint8_t *)a.kc + (long long)at.row * (2 * DK) + ((pc ^ tl) << 4);
+#pragma unroll
+      for (int i = 0; i < kG; ++i)
+        __builtin_amdgcn_global_load_lds(
+            (__attribute__((address_space(1))) void *)(src + 128 * i),
+            (__attribute__((address_space(3))) void *)(s_kv[buf] + (wave * kG + i) * 1024), 16, 0, 0);
+    } else {
+      const uint8_t *src = (const uint8_t *)a.kc + (long long)at.row * DK;
+      const uint8_t *sc = a.ks + (long long)at.row * (DK / 32);
+#pragma unroll
+      for (int i = 0; i < kRaw; ++i) {
+        const int c = min(8 * i + pc, DK / 16 - 1);
+        raw[i] = __builtin_nontemporal_load(reinterpret_cast<const glm_u32x4 *>(src + 16 * c));
+        rsc[i] = sc[c >> 1];
+      }
+    }
+  };
+  const auto store = [&](int buf) {  // MXFP8: the registers' tile as bf16
+    if constexpr (kMx) {
+#pragma unroll
+      for (int i = 0; i < kRaw; ++i) {
+        const int c = 8 * i + pc;
+        if (c < DK / 16) {
+          const float sc = e8m0_to_f32(rsc[i]);
+          uint8_t *dst = s_kv[buf] + (wave * kG + (c >> 2)) * 1024 + tl * 128;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<glm_bf16x8 *>(dst + (((2 * (c & 3) + h) ^ tl) << 4)) =
+                mxfp8_words_to_bf16x8(raw[i][2 * h], raw[i][2 * h + 1], sc);
+        }
+      }
+    }
+  };
+
+  int p = it.t0 * kAttnTile;
+  if (p < end) {
+    Rows cur = rows_at(p), nxt = cur, far = cur;
+    fetch(cur, 0);
+    if (p + 32 < end) nxt = rows_at(p + 32);
+    if constexpr (kMx) {
+      store(0);
+      if (p + 32 < end) {
+        fetch(nxt, 0);
+        if (p + 64 < end) far = rows_at(p + 64);
+      }
+    }
+    __syncthreads();
+    for (int buf = 0;; buf ^= 1) {
+      const bool more = p + 32 < end;
+      if (more) {
+        if constexpr (kMx) {
+          store(buf ^ 1);
+          if (p + 64 < end) fetch(far, 0);
+        } else {
+          fetch(nxt, buf ^ 1);
+          if (p + 64 < end) far = rows_at(p + 64);
+        }
+      }
+      const uint8_t *kv = s_kv[buf];
+      const bool whole = cur.seen == 0xffffffffu && p + 32 <= all_see;  // (uniform)
+      glm_bf16x8 prob = {};
+      if (active) {
+        glm_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int i = 0; i < DK / 32; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const glm_bf16x8 kf = *reinterpret_cast<const glm_bf16x8 *>(
+                kv + ((kread ^ (64 * (i & 1))) + (2 * u * kG + (i >> 1)) * 1024));
+            s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[i], s[u], 0, 0, 0);
+          }
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4] * a.scale_log2;
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = 16 * (i / 4) + 4 * quad + i % 4;
+            if (!((cur.seen >> at) & 1u) || p + at >= all_see + tok) x[i] = -INFINITY;
+          }
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+        const float next = fmaxf(top, max_over_quads(mx));
+        const float from = next == -INFINITY ? 0.0f : next;
+        if (__any(next != top)) {
+          const float keep = __builtin_amdgcn_exp2f(top - from);
+          sum *= keep;
+#pragma unroll
+          for (int d = 0; d < DV / 16; ++d) acc[d] *= keep;
+        }
+        top = next;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float e = __builtin_amdgcn_exp2f(x[i] - from);
+          sum += e;
+          prob[i] = (__bf16)e;  // (see attn_group_kernel)
+        }
+      }
+      const auto values = [&](int d) {
+        const uint16_t *at = reinterpret_cast<const uint16_t *>(
+            kv + ((vread ^ (32 * (d & 3))) + (d >> 2) * 1024));
+        const bf16x4 lo = lds_read_tr(at), hi = lds_read_tr(at + 2 * kG * 512);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      if (whole) {
+        if (active) {
+#pragma unroll
+          for (int d = 0; d < DV / 16; ++d)
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values(d), prob, acc[d], 0, 0, 0);
+        }
+      } else {
+        // as in attn_group_kernel, a turn for each token from the last on, with ever more of the
+        // tile's rows set to zero; the scores are done with them
+        const bool every = p + 32 <= all_see;
+        for (int t = a.q_len - 1; t >= (every ? a.q_len - 1 : 0); --t) {
+          __syncthreads();
+          if (!((cur.seen >> mine) & 1u) || p + mine >= all_see + t) {
+#pragma unroll
+            for (int i = 0; i < kG; ++i)
+              *reinterpret_cast<glm_u32x4 *>(s_kv[buf] + (wave * kG + i) * 1024 + 16 * lane) =
+                  glm_u32x4{0, 0, 0, 0};
+          }
+          __syncthreads();
+          if (active) {
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) {
+              const glm_f32x4 with =
+                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(values(d), prob, acc[d], 0, 0, 0);
+              if (every || tok == t) acc[d] = with;
+            }
+          }
+        }
+      }
+      if (!more) break;
+      __syncthreads();
+      p += 32;
+      cur = nxt;
+      nxt = far;
+      if constexpr (kMx) {
+        if (p + 64 < end) far = rows_at(p + 64);
+      }
+    }
+  }
+
+  sum = sum_over_quads(sum);
+  if (!active || r0 + n >= R) return;
+  if (it.splits == 1) {
+    uint16_t *out = a.out + (((long long)it.b * a.q_len + tok) * a.heads + head * group + r - tok * group) * DV +
+                    4 * quad;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < DV / 16; ++d) {
+      uint32_t b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = f32_to_bf16(acc[d][j] * inv);
+      *reinterpret_cast<uint2 *>(out + 16 * d) = uint2{b[0] | (b[1] << 16), b[2] | (b[3] << 16)};
+    }
+  } else {
+    const long long at = attn_partial(a, it) * a.rows + 16 * wave + n;
+#pragma unroll
+    for (int d = 0; d < DV / 16; ++d)
+      *reinterpret_cast<glm_f32x4 *>(a.part + at * DV + 16 * d + 4 * quad) = acc[d];
+    if (quad == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{top, sum};
+  }
+}
+
+// ---------------------------------------------------------------------------
 // The requests that were cut into several items: out = sum_i 2^(m_i - m) acc_i
 // / sum_i 2^(m_i - m) l_i over the items in order.  A thread has four channels
 // of a row.
@@ -580,7 +829,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 
 namespace {
 
-enum AttnForm { kAttnAny, kAttnGroup };
+enum AttnForm { kAttnAny, kAttnGroup, kAttnLatent };
 
 struct AttnSizes {
   AttnForm form;
@@ -614,6 +863,8 @@ template <int FMT>
 void launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnArgs &a) {
   if (form == kAttnAny)
     hipLaunchKernelGGL(glm::attn_any_kernel<FMT>, grid, dim3(256), 0, s, a);
+  else if (form == kAttnLatent)
+    hipLaunchKernelGGL((glm::attn_latent_kernel<576, 512, FMT>), grid, dim3(256), 0, s, a);
   else if (a.dk == 64)
     launch_group<64, 64, FMT>(s, grid, a);
   else if (a.dk == 128)
@@ -625,15 +876,21 @@ void launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnAr
 }
 
 // Sizes that follow from a call's shape; false for shapes that are refused.
-bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int value_dim, int page_size,
-                int max_blocks, AttnSizes &z) {
+bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int value_dim, bool latent,
+                int page_size, int max_blocks, AttnSizes &z) {
   if (B < 0 || q_len < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || key_dim < 1 ||
       value_dim < 1 || page_size < 1 || max_blocks < 1)
     return false;
   if (B > 65535 || q_len > 16 || heads > 1024 || (long long)max_blocks * page_size > INT_MAX - glm::kAttnTile)
     return false;
   const int R = q_len * (heads / kv_heads);
-  if (group_widths(key_dim, value_dim)) {
+  if (latent && key_dim == 576 && value_dim == 512) {
+    z.form = kAttnLatent;
+    z.rows = 64;
+    z.hblocks = kv_heads * ((R + 63) / 64);
+    z.target = 512;
+    z.min_c = 2;
+  } else if (group_widths(key_dim, value_dim)) {
     z.form = kAttnGroup;
     const int most = key_dim == 64 ? 64 : key_dim <= 192 ? 32 : 16;  // rows that fit the registers
     z.rows = R <= 16 || most == 16 ? 16 : R <= 32 || most == 32 ? 32 : 64;
@@ -652,6 +909,7 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
   const long long splits = (tiles + z.min_c - 1) / z.min_c;
   z.grid = z.hblocks * B * splits;
   if (z.grid > z.target + (long long)z.hblocks * B) z.grid = z.target + (long long)z.hblocks * B;
+  if (z.hblocks > kv_heads) z.grid = (z.grid + 8 * z.hblocks - 1) / (8 * z.hblocks) * (8 * z.hblocks);
   // a request of nt > c tiles has at most 2 nt / c items, so at most 2 target / hblocks over all
   long long p = B * splits;
   if (p > 2LL * z.target / z.hblocks) p = 2LL * z.target / z.hblocks;
@@ -666,10 +924,11 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
 }  // namespace
 
 extern "C" size_t glm_paged_attention_workspace_bytes(int B, int q_len, int heads, int kv_heads,
-                                                      int key_dim, int value_dim, int page_size,
-                                                      int max_blocks) {
+                                                      int key_dim, int value_dim, int latent,
+                                                      int page_size, int max_blocks) {
   AttnSizes z;
-  if (!attn_sizes(B, q_len, heads, kv_heads, key_dim, value_dim, page_size, max_blocks, z)) return 0;
+  if (!attn_sizes(B, q_len, heads, kv_heads, key_dim, value_dim, latent != 0, page_size, max_blocks, z))
+    return 0;
   return z.plan_bytes + z.part_bytes + z.ml_bytes + 256;
 }
 
@@ -704,7 +963,7 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
               "paged_attention: %d pages of %d x %d rows pass 32 bits", num_pages, kv_heads,
               page_size);
   AttnSizes z;
-  GLM_REQUIRE(attn_sizes(B, q_len, heads, kv_heads, key_dim, value_dim, page_size, max_blocks, z),
+  GLM_REQUIRE(attn_sizes(B, q_len, heads, kv_heads, key_dim, value_dim, shared, page_size, max_blocks, z),
               GLM_ERR_UNSUPPORTED_SHAPE,
               "paged_attention: batch %d, %d tokens, %d heads or %d blocks of %d are too many", B,
               q_len, heads, max_blocks, page_size);

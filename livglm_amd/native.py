@@ -112,7 +112,7 @@ SIGNATURES = {
     "glm_cache_step": (_i, [_p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
     "glm_cache_write": (_i, [_p, _p, _i64, _p, _i64, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p,
                              _p]),
-    "glm_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "glm_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "glm_paged_attention": (_i, [_p, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i, _i, _i,
                                  _p, _p, _i, _f, _p, _sz, _p]),
 }

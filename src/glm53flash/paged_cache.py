@@ -184,9 +184,9 @@ def cache_write(keys: torch.Tensor, values: torch.Tensor | None, slots: torch.Te
 
 @lru_cache(maxsize=256)  # a function of the sizes alone
 def _attention_workspace(B: int, q_len: int, heads: int, kv_heads: int, key_dim: int,
-                         value_dim: int, page: int, max_blocks: int) -> int:
+                         value_dim: int, latent: int, page: int, max_blocks: int) -> int:
     return int(N.native.load().glm_paged_attention_workspace_bytes(
-        B, q_len, heads, kv_heads, key_dim, value_dim, page, max_blocks))
+        B, q_len, heads, kv_heads, key_dim, value_dim, latent, page, max_blocks))
 
 
 def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
@@ -235,7 +235,8 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
     if B == 0 or q_len == 0:
         return out
     max_blocks = tables.shape[1]
-    need = _attention_workspace(B, q_len, heads, kv_heads, key_dim, value_dim, page, max_blocks)
+    need = _attention_workspace(B, q_len, heads, kv_heads, key_dim, value_dim,
+                                int(value_cache is None), page, max_blocks)
     ws = torch.empty(need, dtype=_U8, device=dev)
     _call(dev, "glm_paged_attention", N.stream_of(query), query.data_ptr(), q_stride, B, q_len, heads,
            kv_heads, key_dim, value_dim, key_cache.data_ptr(), N.ptr(key_scales),

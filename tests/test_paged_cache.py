@@ -126,12 +126,13 @@ def test_attend_refusals(code, change):
 
 def test_attend_workspace():
     size = native.load().glm_paged_attention_workspace_bytes
-    need = size(2, 1, 8, 2, 128, 128, 16, 4)
+    need = size(2, 1, 8, 2, 128, 128, 0, 16, 4)
     assert need > 0
     assert native.load().glm_paged_attention(*_attend_args(nbytes=need - 1 - 256)) == WORKSPACE
-    assert size(2, 1, 7, 2, 128, 128, 16, 4) == 0 and size(-1, 1, 8, 2, 128, 128, 16, 4) == 0
+    assert size(2, 1, 7, 2, 128, 128, 0, 16, 4) == 0 and size(-1, 1, 8, 2, 128, 128, 0, 16, 4) == 0
     # bounded by the work that the chip takes at once, not by the batch
-    assert size(4096, 1, 128, 8, 128, 128, 16, 8192) < 512 << 20
+    assert 0 < size(4096, 1, 128, 8, 128, 128, 0, 16, 8192) < 512 << 20
+    assert 0 < size(4096, 2, 128, 1, 576, 512, 1, 64, 2048) < 512 << 20
 
 
 def test_empty_batches_are_no_ops():
