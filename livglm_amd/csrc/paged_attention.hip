@@ -2,19 +2,25 @@
 //
 // Row (b, t, h) sees the positions j < len_b - (q_len - 1 - t) of request b:
 //   s_j = scale q . k_j,  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  m = max_j s_j.
-// The cache is read once, so the positions are cut into items that fill the
-// chip whatever the lengths are: every workgroup reads the lengths and cuts
-// them alike (attn_item), keeps a running maximum and sum over its item's
-// positions, and a request cut into several items is joined by a second
-// launch (attn_join_kernel) from their partial results (m, l, acc).
+// The cache is read once, and the chip is filled whatever the lengths are: the
+// tiles of all requests and kv heads, one after the other, are cut into as
+// many equal parts as workgroups fit the chip (AttnWalk: every wave finds its
+// part from the lengths), and a workgroup walks through its part, request by
+// request, keeping a running maximum and sum.  What a cut leaves of a request
+// on either side goes to the workspace as (m, l, acc), and a second launch
+// (attn_join_kernel) joins it.
 #include <climits>
 #include <cmath>
 
 #include "glm_common.h"
+#include "lds_stage.h"
 
 namespace glm {
 
-constexpr int kAttnTile = 64;  // positions; items are whole tiles
+constexpr int kAttnTile = 64;  // positions; parts are cut between tiles
+// What a request costs a workgroup beside its tiles (its rows, the first loads' latency, the
+// result), in tiles.
+constexpr int kAttnOver = 1;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct AttnArgs {
@@ -24,13 +30,13 @@ struct AttnArgs {
   const uint8_t *ks, *vs;
   const int32_t *tables, *lens;
   uint16_t *out;
-  int2 *plan;        // [B] {splits, first partial}, for the join
-  float *part, *ml;  // partial results [item][rows][dv], [item][rows][2]
+  int2 *plan;        // [B] {units before the request, units of a part}, for the join
+  float *part, *ml;  // partial results [2 part + end][row block][rows][dv], [..][2]
   int B, q_len, heads, kv_heads, dk, dv, num_pages, page, max_blocks;
-  int page_shift;  // log2 of page, -1 where it is no power of two
-  int rows;     // rows of an item: one kv head's row block
-  int hblocks;  // kv_heads x row blocks
-  int target, min_c;  // items wanted over all, fewest tiles of an item
+  uint32_t page_magic;   // floor(2^32 / page), at most 2^32 - 1
+  uint32_t cache_bytes;  // of kc where they fit 32 bits
+  int rows, rblocks;    // query rows a workgroup takes, blocks of them in a kv head
+  int parts, min_part;  // most parts, fewest units of a part
   float scale_log2;
 };
 
@@ -41,71 +47,99 @@ __device__ __forceinline__ int attn_len(const AttnArgs &a, int b) {
   return max(0, min(a.lens[b], a.max_blocks * a.page));
 }
 
+// Tiles [t0, t1) of one request, kv head and row block.
 struct AttnItem {
-  int b, hb, len, t0, t1;      // request, head block, its length, tile range
-  int splits, split, partial;  // of the request; this item's, and the request's first partial
+  int b, head, rb, len, t0, t1;
+  bool whole;     // all of the request's
+  int partial;    // else where its partial result goes
 };
 
-// This workgroup's item: c tiles of one request and head block, c the least
-// that gives at most `target` items beyond one a request.  Every wave finds it
-// by itself from the lengths (no barrier, no plan from the host).  False for a
-// workgroup past the last item.
-__device__ __forceinline__ bool attn_item(const AttnArgs &a, int block, AttnItem &it) {
-  const int lane = threadIdx.x & 63;
-  int total = 0;
-  for (int b = lane; b < a.B; b += kWave) total += (attn_len(a, b) + kAttnTile - 1) / kAttnTile;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, kWave);
-  const int c =
-      max(a.min_c, (int)(((long long)total * a.hblocks + a.target - 1) / a.target));
-  int s = block / a.hblocks;
-  it.hb = block - s * a.hblocks;
-  if (a.hblocks > a.kv_heads) {
-    // a head's row blocks read the same positions: consecutive workgroups go to the eight XCDs in
-    // turn, so the row blocks of eight items are dealt out eight apart and share an XCD's cache
-    s = block / (8 * a.hblocks) * 8 + block % 8;
-    it.hb = block / 8 % a.hblocks;
-  }
-  int upto_s = 0, upto_p = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kWave) {
-    const int b = b0 + lane;
-    const int len = b < a.B ? attn_len(a, b) : 0;
-    const int nt = (len + kAttnTile - 1) / kAttnTile;
-    const int mine = b < a.B ? max(1, (nt + c - 1) / c) : 0;
-    int sum_s = mine, sum_p = mine > 1 ? mine : 0;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const int vs = __shfl_up(sum_s, off, kWave), vp = __shfl_up(sum_p, off, kWave);
-      if (lane >= off) {
-        sum_s += vs;
-        sum_p += vp;
-      }
-    }
-    const int first = upto_s + sum_s - mine;
-    const unsigned long long hit = __ballot(s >= first && s < first + mine);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      it.b = b0 + l;
-      it.len = __builtin_amdgcn_readlane(len, l);
-      it.splits = __builtin_amdgcn_readlane(mine, l);
-      it.split = s - __builtin_amdgcn_readlane(first, l);
-      it.partial = upto_p + __builtin_amdgcn_readlane(sum_p, l) - (it.splits > 1 ? it.splits : 0);
-      it.t0 = it.split * c;
-      it.t1 = min((it.len + kAttnTile - 1) / kAttnTile, it.t0 + c);
-      return true;
-    }
-    upto_s += __builtin_amdgcn_readlane(sum_s, kWave - 1);
-    upto_p += __builtin_amdgcn_readlane(sum_p, kWave - 1);
-  }
-  return false;
-}
+// A workgroup's part of the work.  Requests in order, kv heads in order, a
+// pair of them takes kAttnOver units and one for each of its tiles; part i has
+// the units [i u, (i + 1) u), u the least that makes do with `parts` parts.
+// At most one pair began before the part and one ends after it: partial
+// results 2 i and 2 i + 1.
+struct AttnWalk {
+  int x, x1, u, part, rb;  // units left [x, x1)
+  int b, head, before, len, w;  // the pair: the request's units before it (of one kv head), its units
 
-__device__ __forceinline__ void attn_plan(const AttnArgs &a, const AttnItem &it) {
-  if (it.split == 0 && it.hb == 0 && threadIdx.x == 0) a.plan[it.b] = int2{it.splits, it.partial};
-}
-__device__ __forceinline__ long long attn_partial(const AttnArgs &a, const AttnItem &it) {
-  return (long long)(it.partial + it.split) * a.hblocks + it.hb;
-}
+  __device__ __forceinline__ int units(int len_b) const {
+    return kAttnOver + (len_b + kAttnTile - 1) / kAttnTile;
+  }
+
+  // False where the part is empty.  Every wave does this by itself, without a barrier.
+  __device__ __forceinline__ bool start(const AttnArgs &a, int block) {
+    const int lane = threadIdx.x & 63;
+    part = block;
+    rb = 0;
+    if (a.rblocks > 1) {
+      // a head's row blocks read the same positions: consecutive workgroups go to the eight XCDs
+      // in turn, so the row blocks of a part are dealt out eight apart and share an XCD's cache
+      part = block / (8 * a.rblocks) * 8 + block % 8;
+      rb = block / 8 % a.rblocks;
+    }
+    int total = 0;
+    for (int i = lane; i < a.B; i += kWave) total += units(attn_len(a, i));
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, kWave);
+    total = __builtin_amdgcn_readfirstlane(total) * a.kv_heads;
+    u = max(a.min_part, (total + a.parts - 1) / a.parts);
+    if (part > (total - 1) / u) return false;
+    x = part * u;
+    x1 = min(total, x + u);
+    before = 0;
+    for (int b0 = 0;; b0 += kWave) {
+      const int i = b0 + lane;
+      const int len_i = i < a.B ? attn_len(a, i) : 0, w_i = i < a.B ? units(len_i) : 0;
+      int upto = w_i;
+#pragma unroll
+      for (int off = 1; off < kWave; off <<= 1) {
+        const int v = __shfl_up(upto, off, kWave);
+        if (lane >= off) upto += v;
+      }
+      const int first = before + upto - w_i;
+      const unsigned long long hit = __ballot(x >= first * a.kv_heads && x < (first + w_i) * a.kv_heads);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        b = b0 + l;
+        len = __builtin_amdgcn_readlane(len_i, l);
+        before = __builtin_amdgcn_readlane(first, l);
+        w = __builtin_amdgcn_readlane(w_i, l);
+        head = (x - before * a.kv_heads) / w;
+        return true;
+      }
+      before += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+  }
+
+  // The part's next item; also leaves the request's place for the join.
+  __device__ __forceinline__ bool next(const AttnArgs &a, AttnItem &it) {
+    while (x < x1) {
+      const int first = before * a.kv_heads + head * w, from = x - first, to = min(x1 - first, w);
+      it.b = b;
+      it.head = head;
+      it.rb = rb;
+      it.len = len;
+      it.t0 = max(0, from - kAttnOver);
+      it.t1 = to - kAttnOver;
+      it.whole = it.t0 == 0 && it.t1 == w - kAttnOver;
+      it.partial = (2 * part + (it.t0 == 0)) * a.rblocks + rb;
+      if (from == 0 && head == 0 && rb == 0 && threadIdx.x == 0) a.plan[b] = int2{before, u};
+      const bool some = it.t1 > it.t0 || (w == kAttnOver && from == 0);
+      x = first + w;
+      if (++head == a.kv_heads) {
+        head = 0;
+        before += w;
+        if (++b < a.B) {
+          len = attn_len(a, b);
+          w = units(len);
+        }
+      }
+      if (some) return true;
+    }
+    return false;
+  }
+};
 
 // The cache row (of dk or dv elements) of a request's position, -1 where its
 // page is not one of the cache's.
@@ -134,78 +168,80 @@ template <int FMT>
 __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
   __shared__ float s_q[kAnyDim], s_p[256], s_red[4];
   __shared__ long long s_row[256];
-  AttnItem it;
-  if (!attn_item(a, blockIdx.x, it)) return;
-  attn_plan(a, it);
-  const int tid = threadIdx.x, R = attn_rows(a), group = a.heads / a.kv_heads;
-  const int head = it.hb / R, r = it.hb - head * R, t = r / group;
-  const uint16_t *q = a.q + ((long long)it.b * a.q_len + t) * a.q_stride +
-                      (head * group + r % group) * a.dk;
-  for (int ch = tid; ch < a.dk; ch += 256) s_q[ch] = bf16_to_f32(q[ch]);
-  const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
-  const int end = min(it.t1 * kAttnTile, it.len - (a.q_len - 1 - t));
-  const void *vc = a.vc ? a.vc : a.kc;
-  const uint8_t *vs = a.vc ? a.vs : a.ks;
-  const int vdim = a.vc ? a.dv : a.dk;
-  float m = -INFINITY, l = 0.0f, acc[kAnyDim / 256] = {};
-  __syncthreads();
-  for (int p0 = it.t0 * kAttnTile; p0 < end; p0 += 256) {
-    const int pos = p0 + tid;
-    const long long row = pos < end ? cache_row(a, table, head, pos) : -1;
-    float s = -INFINITY;
-    if (row >= 0) {
-      s = 0.0f;
-      for (int ch = 0; ch < a.dk; ++ch)
-        s += s_q[ch] * cache_value(a.kc, a.ks, FMT, row, a.dk, ch);
-      s *= a.scale_log2;
+  AttnWalk walk;
+  if (!walk.start(a, blockIdx.x)) return;
+  const int tid = threadIdx.x, group = a.heads / a.kv_heads;
+  for (AttnItem it; walk.next(a, it);) {
+    const int head = it.head, r = it.rb, t = r / group;
+    const uint16_t *q = a.q + ((long long)it.b * a.q_len + t) * a.q_stride +
+                        (head * group + r % group) * a.dk;
+    for (int ch = tid; ch < a.dk; ch += 256) s_q[ch] = bf16_to_f32(q[ch]);
+    const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
+    const int end = min(it.t1 * kAttnTile, it.len - (a.q_len - 1 - t));
+    const void *vc = a.vc ? a.vc : a.kc;
+    const uint8_t *vs = a.vc ? a.vs : a.ks;
+    const int vdim = a.vc ? a.dv : a.dk;
+    float m = -INFINITY, l = 0.0f, acc[kAnyDim / 256] = {};
+    __syncthreads();
+    for (int p0 = it.t0 * kAttnTile; p0 < end; p0 += 256) {
+      const int pos = p0 + tid;
+      const long long row = pos < end ? cache_row(a, table, head, pos) : -1;
+      float s = -INFINITY;
+      if (row >= 0) {
+        s = 0.0f;
+        for (int ch = 0; ch < a.dk; ++ch)
+          s += s_q[ch] * cache_value(a.kc, a.ks, FMT, row, a.dk, ch);
+        s *= a.scale_log2;
+      }
+      float top = s;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+      if ((tid & 63) == 0) s_red[tid >> 6] = top;
+      __syncthreads();
+      const float next = fmaxf(m, fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])));
+      const float from = next == -INFINITY ? 0.0f : next;
+      const float keep = exp2f(m - from);
+      m = next;
+      const float p = row >= 0 ? exp2f(s - from) : 0.0f;
+      s_p[tid] = p;
+      s_row[tid] = row;
+      __syncthreads();
+      l *= keep;
+#pragma unroll
+      for (int i = 0; i < kAnyDim / 256; ++i) acc[i] *= keep;
+      const int n = min(256, end - p0);
+      for (int j = 0; j < n; ++j) {
+        const float pj = s_p[j];
+        l += pj;
+        const long long rj = s_row[j];
+        if (rj < 0) continue;
+#pragma unroll
+        for (int i = 0; i < kAnyDim / 256; ++i)
+          if (tid + 256 * i < a.dv) acc[i] += pj * cache_value(vc, vs, FMT, rj, vdim, tid + 256 * i);
+      }
+      __syncthreads();
     }
-    float top = s;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-    if ((tid & 63) == 0) s_red[tid >> 6] = top;
-    __syncthreads();
-    const float next = fmaxf(m, fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3])));
-    const float from = next == -INFINITY ? 0.0f : next;
-    const float keep = exp2f(m - from);
-    m = next;
-    const float p = row >= 0 ? exp2f(s - from) : 0.0f;
-    s_p[tid] = p;
-    s_row[tid] = row;
-    __syncthreads();
-    l *= keep;
-#pragma unroll
-    for (int i = 0; i < kAnyDim / 256; ++i) acc[i] *= keep;
-    const int n = min(256, end - p0);
-    for (int j = 0; j < n; ++j) {
-      const float pj = s_p[j];
-      l += pj;
-      const long long rj = s_row[j];
-      if (rj < 0) continue;
+    if (it.whole) {
+      uint16_t *out = a.out + (((long long)it.b * a.q_len + t) * a.heads + head * group + r % group) * a.dv;
 #pragma unroll
       for (int i = 0; i < kAnyDim / 256; ++i)
-        if (tid + 256 * i < a.dv) acc[i] += pj * cache_value(vc, vs, FMT, rj, vdim, tid + 256 * i);
+        if (tid + 256 * i < a.dv) out[tid + 256 * i] = (uint16_t)f32_to_bf16(l == 0.0f ? 0.0f : acc[i] / l);
+    } else {
+      const long long at = it.partial;
+#pragma unroll
+      for (int i = 0; i < kAnyDim / 256; ++i)
+        if (tid + 256 * i < a.dv) a.part[at * a.dv + tid + 256 * i] = acc[i];
+      if (tid == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{m, l};
     }
     __syncthreads();
-  }
-  if (it.splits == 1) {
-    uint16_t *out = a.out + (((long long)it.b * a.q_len + t) * a.heads + head * group + r % group) * a.dv;
-#pragma unroll
-    for (int i = 0; i < kAnyDim / 256; ++i)
-      if (tid + 256 * i < a.dv) out[tid + 256 * i] = (uint16_t)f32_to_bf16(l == 0.0f ? 0.0f : acc[i] / l);
-  } else {
-    const long long at = attn_partial(a, it);
-#pragma unroll
-    for (int i = 0; i < kAnyDim / 256; ++i)
-      if (tid + 256 * i < a.dv) a.part[at * a.dv + tid + 256 * i] = acc[i];
-    if (tid == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{m, l};
   }
 }
 
 // ---------------------------------------------------------------------------
-// Grouped heads on the matrix cores.  A workgroup's item is 16 MT query rows
+// Grouped heads on the matrix cores.  A workgroup takes 16 MT query rows
 // of one kv head (its group's heads, times the new tokens) over a range of
 // positions; its four waves take 32 positions in turn, each by itself, and
-// are joined in LDS at the item's end.  A wave forms
+// are joined in LDS at the range's end.  A wave forms
 //   S^T = K Q^T   (A: 16 positions x 32 channels straight from the cache,
 //                  B: the rows, in registers for good),
 //   O^T += V^T P^T (A: V^T by transposing LDS reads, B: P^T)
@@ -294,13 +330,13 @@ struct TileRows {
   int row[2];
   uint32_t seen;  // bit 16 u + n
 };
+// pos / page and the rest, by a product: the quotient is one short at most.
 __device__ __forceinline__ void page_of(const AttnArgs &a, int pos, int &block, int &off) {
-  if (a.page_shift >= 0) {
-    block = pos >> a.page_shift;
-    off = pos & (a.page - 1);
-  } else {
-    block = (uint32_t)pos / (uint32_t)a.page;
-    off = pos - block * a.page;
+  block = (int)__umulhi((uint32_t)pos, a.page_magic);
+  off = pos - block * a.page;
+  if (off >= a.page) {
+    ++block;
+    off -= a.page;
   }
 }
 __device__ __forceinline__ TileRows tile_rows(const AttnArgs &a, const int32_t *table, int head, int p,
@@ -328,376 +364,420 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
   constexpr int kLds = 4 * (32 * kStride * 2 > 16 * kAccStride * 4 ? 32 * kStride * 2 : 16 * kAccStride * 4);
   __shared__ __align__(16) uint8_t s_buf[kLds];
   __shared__ float s_m[4][16 * MT], s_l[4][16 * MT];
-  AttnItem it;
-  if (!attn_item(a, blockIdx.x, it)) return;
-  attn_plan(a, it);
+  AttnWalk walk;
+  if (!walk.start(a, blockIdx.x)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
-  const int R = attn_rows(a), group = a.heads / a.kv_heads, rb = a.hblocks / a.kv_heads;
-  const int head = it.hb / rb, r0 = (it.hb - head * rb) * 16 * MT;
-  const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
+  const int R = attn_rows(a), group = a.heads / a.kv_heads;
   const void *vc = a.vc ? a.vc : a.kc;
   const uint8_t *vs = a.vc ? a.vs : a.ks;
   const int vdim = a.vc ? DV : DK;
   typedef CacheRow<FMT, DK> KRow;
   typedef CacheRow<FMT, DV> VRow;
 
-  glm_bf16x8 q[MT][DK / 32];
-  int tok[MT];  // this lane's rows' new token
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int r = min(r0 + 16 * m + n, R - 1);
-    tok[m] = r / group;
-    const uint16_t *p = a.q + ((long long)it.b * a.q_len + tok[m]) * a.q_stride +
-                        (head * group + r - tok[m] * group) * DK;
-#pragma unroll
-    for (int s = 0; s < DK / 32; ++s)
-      q[m][s] = *reinterpret_cast<const glm_bf16x8 *>(p + KRow::channel(s, quad));
-  }
-  glm_f32x4 acc[DV / 16][MT];
-  float top[MT], sum[MT];  // running maximum; this lane's part of the running sum
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    top[m] = -INFINITY;
-    sum[m] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DV / 16; ++d) acc[d][m] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
-  }
   uint16_t *lv = reinterpret_cast<uint16_t *>(s_buf) + wave * 32 * kStride;
   const uint16_t *lt = lv + (4 * quad + (n >> 2)) * kStride + 4 * (n & 3);  // transposing reads
-  const int end = min(it.t1 * kAttnTile, it.len);
-  const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
+  for (AttnItem it; walk.next(a, it);) {
+    const int head = it.head, r0 = it.rb * 16 * MT;
+    const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
+    glm_bf16x8 q[MT][DK / 32];
+    int tok[MT];  // this lane's rows' new token
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r = min(r0 + 16 * m + n, R - 1);
+      tok[m] = r / group;
+      const uint16_t *p = a.q + ((long long)it.b * a.q_len + tok[m]) * a.q_stride +
+                          (head * group + r - tok[m] * group) * DK;
+#pragma unroll
+      for (int s = 0; s < DK / 32; ++s)
+        q[m][s] = *reinterpret_cast<const glm_bf16x8 *>(p + KRow::channel(s, quad));
+    }
+    glm_f32x4 acc[DV / 16][MT];
+    float top[MT], sum[MT];  // running maximum; this lane's part of the running sum
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      top[m] = -INFINITY;
+      sum[m] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DV / 16; ++d) acc[d][m] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int end = min(it.t1 * kAttnTile, it.len);
+    const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
 
-  int p = it.t0 * kAttnTile + 32 * wave;
-  if (p < end) {
-    TileRows cur = tile_rows(a, table, head, p, end, n), nxt = cur;
-    KRow k[2];
-    VRow v[2];
+    int p = it.t0 * kAttnTile + 32 * wave;
+    if (p < end) {
+      TileRows cur = tile_rows(a, table, head, p, end, n), nxt = cur;
+      KRow k[2];
+      VRow v[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) k[u].load(a.kc, a.ks, cur.row[u], DK, quad);
+      for (int u = 0; u < 2; ++u) k[u].load(a.kc, a.ks, cur.row[u], DK, quad);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) v[u].load(vc, vs, cur.row[u], vdim, quad);
-    if (p + 128 < end) nxt = tile_rows(a, table, head, p + 128, end, n);
-    while (true) {
-      const bool more = p + 128 < end;
-      glm_f32x4 s[2][MT];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) s[u][m] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < DK / 32; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const glm_bf16x8 kf = k[u].step(i, quad);
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-            s[u][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[m][i], s[u][m], 0, 0, 0);
-        }
-      if (more) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) k[u].load(a.kc, a.ks, nxt.row[u], DK, quad);
-      }
-      const bool whole = cur.seen == 0xffffffffu && p + 32 <= all_see;  // (uniform)
-      glm_bf16x8 prob[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[i / 4][m][i % 4] * a.scale_log2;
-        if (!whole) {
-          const int below = all_see + tok[m];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = 16 * (i / 4) + 4 * quad + i % 4;
-            if (!((cur.seen >> at) & 1u) || p + at >= below) x[i] = -INFINITY;
-          }
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-        const float next = fmaxf(top[m], max_over_quads(mx));
-        const float from = next == -INFINITY ? 0.0f : next;
-        if (__any(next != top[m])) {
-          const float keep = __builtin_amdgcn_exp2f(top[m] - from);
-          sum[m] *= keep;
-#pragma unroll
-          for (int d = 0; d < DV / 16; ++d) acc[d][m] *= keep;
-        }
-        top[m] = next;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float e = __builtin_amdgcn_exp2f(x[i] - from);
-          sum[m] += e;
-          // bf16 for the matrix product: 2^-9 of each weight, as the output's own rounding
-          prob[m][i] = (__bf16)e;
-        }
-      }
-      if (whole) {
+      for (int u = 0; u < 2; ++u) v[u].load(vc, vs, cur.row[u], vdim, quad);
+      if (p + 128 < end) nxt = tile_rows(a, table, head, p + 128, end, n);
+      while (true) {
+        const bool more = p + 128 < end;
+        glm_f32x4 s[2][MT];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < DV / 32; ++i)
-            *reinterpret_cast<glm_bf16x8 *>(lv + (16 * u + n) * kStride + VRow::channel(i, quad)) =
-                v[u].step(i, quad);
-        if (more) {
+          for (int m = 0; m < MT; ++m) s[u][m] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int u = 0; u < 2; ++u) v[u].load(vc, vs, nxt.row[u], vdim, quad);
-        }
-#pragma unroll
-        for (int d = 0; d < DV / 16; ++d) {
-          const bf16x4 lo = lds_read_tr(lt + 16 * d), hi = lds_read_tr(lt + 16 * kStride + 16 * d);
-          const glm_bf16x8 vt = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-            acc[d][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, prob[m], acc[d][m], 0, 0, 0);
-        }
-      } else {
-        // a value that a row does not see must not meet its zero weight (it may be an infinity or
-        // a NaN): one turn for each new token, with the values that it does not see as zeros, whose
-        // sums only that token's rows take
-        for (int t = p + 32 > all_see ? 0 : a.q_len - 1; t < a.q_len; ++t) {
-          const int below = all_see + t;
+        for (int i = 0; i < DK / 32; ++i)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int at = 16 * u + n;
-            const bool fine = ((cur.seen >> at) & 1u) && p + at < below;
+            const glm_bf16x8 kf = k[u].step(i, quad);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+              s[u][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[m][i], s[u][m], 0, 0, 0);
+          }
+        if (more) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) k[u].load(a.kc, a.ks, nxt.row[u], DK, quad);
+        }
+        const bool whole = cur.seen == 0xffffffffu && p + 32 <= all_see;  // (uniform)
+        glm_bf16x8 prob[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = s[i / 4][m][i % 4] * a.scale_log2;
+          if (!whole) {
+            const uint32_t bits = cur.seen >> (4 * quad);
+            const int left = all_see + tok[m] - p - 4 * quad;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int at = 16 * (i / 4) + i % 4;
+              if (!((bits >> at) & 1u) || at >= left) x[i] = -INFINITY;
+            }
+          }
+          float mx = x[0];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+          const float next = fmaxf(top[m], max_over_quads(mx));
+          const float from = next == -INFINITY ? 0.0f : next;
+          if (__any(next != top[m])) {
+            const float keep = __builtin_amdgcn_exp2f(top[m] - from);
+            sum[m] *= keep;
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) acc[d][m] *= keep;
+          }
+          top[m] = next;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float e = __builtin_amdgcn_exp2f(x[i] - from);
+            sum[m] += e;
+            // bf16 for the matrix product: 2^-9 of each weight, as the output's own rounding
+            prob[m][i] = (__bf16)e;
+          }
+        }
+        if (whole) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < DV / 32; ++i)
-              *reinterpret_cast<glm_u32x4 *>(lv + at * kStride + VRow::channel(i, quad)) =
-                  fine ? __builtin_bit_cast(glm_u32x4, v[u].step(i, quad)) : glm_u32x4{0, 0, 0, 0};
+              *reinterpret_cast<glm_bf16x8 *>(lv + (16 * u + n) * kStride + VRow::channel(i, quad)) =
+                  v[u].step(i, quad);
+          if (more) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) v[u].load(vc, vs, nxt.row[u], vdim, quad);
           }
-          const bool every = p + 32 <= all_see;  // one turn for all rows
 #pragma unroll
           for (int d = 0; d < DV / 16; ++d) {
             const bf16x4 lo = lds_read_tr(lt + 16 * d), hi = lds_read_tr(lt + 16 * kStride + 16 * d);
             const glm_bf16x8 vt = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const glm_f32x4 with =
-                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, prob[m], acc[d][m], 0, 0, 0);
-              if (every || tok[m] == t) acc[d][m] = with;
+            for (int m = 0; m < MT; ++m)
+              acc[d][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, prob[m], acc[d][m], 0, 0, 0);
+          }
+        } else {
+          // a value that a row does not see must not meet its zero weight (it may be an infinity or
+          // a NaN): one turn for each new token, with the values that it does not see as zeros, whose
+          // sums only that token's rows take
+          for (int t = p + 32 > all_see ? 0 : a.q_len - 1; t < a.q_len; ++t) {
+            const int below = all_see + t;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int at = 16 * u + n;
+              const bool fine = ((cur.seen >> at) & 1u) && p + at < below;
+#pragma unroll
+              for (int i = 0; i < DV / 32; ++i)
+                *reinterpret_cast<glm_u32x4 *>(lv + at * kStride + VRow::channel(i, quad)) =
+                    fine ? __builtin_bit_cast(glm_u32x4, v[u].step(i, quad)) : glm_u32x4{0, 0, 0, 0};
+            }
+            const bool every = p + 32 <= all_see;  // one turn for all rows
+#pragma unroll
+            for (int d = 0; d < DV / 16; ++d) {
+              const bf16x4 lo = lds_read_tr(lt + 16 * d), hi = lds_read_tr(lt + 16 * kStride + 16 * d);
+              const glm_bf16x8 vt = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const glm_f32x4 with =
+                    __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, prob[m], acc[d][m], 0, 0, 0);
+                if (every || tok[m] == t) acc[d][m] = with;
+              }
             }
           }
-        }
-        if (more) {
+          if (more) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) v[u].load(vc, vs, nxt.row[u], vdim, quad);
+            for (int u = 0; u < 2; ++u) v[u].load(vc, vs, nxt.row[u], vdim, quad);
+          }
         }
+        if (!more) break;
+        p += 128;
+        cur = nxt;
+        if (p + 128 < end) nxt = tile_rows(a, table, head, p + 128, end, n);
       }
-      if (!more) break;
-      p += 128;
-      cur = nxt;
-      if (p + 128 < end) nxt = tile_rows(a, table, head, p + 128, end, n);
     }
-  }
 
-  // the four waves joined, row tile by row tile
+    // the four waves joined, row tile by row tile
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    sum[m] = sum_over_quads(sum[m]);
-    if (quad == 0) {
-      s_m[wave][16 * m + n] = top[m];
-      s_l[wave][16 * m + n] = sum[m];
+    for (int m = 0; m < MT; ++m) {
+      sum[m] = sum_over_quads(sum[m]);
+      if (quad == 0) {
+        s_m[wave][16 * m + n] = top[m];
+        s_l[wave][16 * m + n] = sum[m];
+      }
     }
-  }
-  __syncthreads();
-  float *la = reinterpret_cast<float *>(s_buf);
-  const long long part = attn_partial(a, it);
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const float mt = fmaxf(fmaxf(s_m[0][16 * m + n], s_m[1][16 * m + n]),
-                           fmaxf(s_m[2][16 * m + n], s_m[3][16 * m + n]));
-    const float w = __builtin_amdgcn_exp2f(top[m] - (mt == -INFINITY ? 0.0f : mt));
-    if (m) __syncthreads();
-#pragma unroll
-    for (int d = 0; d < DV / 16; ++d)
-      *reinterpret_cast<glm_f32x4 *>(la + (wave * 16 + n) * kAccStride + 16 * d + 4 * quad) =
-          acc[d][m] * w;
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * DV / 4; i += 256) {
-      const int row = i / (DV / 4), ch = 4 * (i % (DV / 4)), r = r0 + 16 * m + row;
-      float mr = -INFINITY, l = 0.0f;
+    float *la = reinterpret_cast<float *>(s_buf);
 #pragma unroll
-      for (int w4 = 0; w4 < 4; ++w4) mr = fmaxf(mr, s_m[w4][16 * m + row]);
-      const float from = mr == -INFINITY ? 0.0f : mr;
-      glm_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int m = 0; m < MT; ++m) {
+      const float mt = fmaxf(fmaxf(s_m[0][16 * m + n], s_m[1][16 * m + n]),
+                             fmaxf(s_m[2][16 * m + n], s_m[3][16 * m + n]));
+      const float w = __builtin_amdgcn_exp2f(top[m] - (mt == -INFINITY ? 0.0f : mt));
+      if (m) __syncthreads();
 #pragma unroll
-      for (int w4 = 0; w4 < 4; ++w4) {
-        l += s_l[w4][16 * m + row] * __builtin_amdgcn_exp2f(s_m[w4][16 * m + row] - from);
-        o += *reinterpret_cast<const glm_f32x4 *>(la + (w4 * 16 + row) * kAccStride + ch);
-      }
-      if (r >= R) continue;
-      if (it.splits == 1) {
-        const int t = r / group;
-        uint32_t b[4];
+      for (int d = 0; d < DV / 16; ++d)
+        *reinterpret_cast<glm_f32x4 *>(la + (wave * 16 + n) * kAccStride + 16 * d + 4 * quad) =
+            acc[d][m] * w;
+      __syncthreads();
+      for (int i = threadIdx.x; i < 16 * DV / 4; i += 256) {
+        const int row = i / (DV / 4), ch = 4 * (i % (DV / 4)), r = r0 + 16 * m + row;
+        float mr = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) b[j] = f32_to_bf16(l == 0.0f ? 0.0f : o[j] / l);
-        *reinterpret_cast<uint2 *>(
-            a.out + (((long long)it.b * a.q_len + t) * a.heads + head * group + r - t * group) * DV + ch) =
-            uint2{b[0] | (b[1] << 16), b[2] | (b[3] << 16)};
-      } else {
-        const long long at = part * a.rows + 16 * m + row;
-        *reinterpret_cast<glm_f32x4 *>(a.part + at * DV + ch) = o;
-        if (ch == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{mr, l};
+        for (int w4 = 0; w4 < 4; ++w4) mr = fmaxf(mr, s_m[w4][16 * m + row]);
+        const float from = mr == -INFINITY ? 0.0f : mr;
+        glm_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w4 = 0; w4 < 4; ++w4) {
+          l += s_l[w4][16 * m + row] * __builtin_amdgcn_exp2f(s_m[w4][16 * m + row] - from);
+          o += *reinterpret_cast<const glm_f32x4 *>(la + (w4 * 16 + row) * kAccStride + ch);
+        }
+        if (r >= R) continue;
+        if (it.whole) {
+          const int t = r / group;
+          uint32_t b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = f32_to_bf16(l == 0.0f ? 0.0f : o[j] / l);
+          *reinterpret_cast<uint2 *>(
+              a.out + (((long long)it.b * a.q_len + t) * a.heads + head * group + r - t * group) * DV + ch) =
+              uint2{b[0] | (b[1] << 16), b[2] | (b[3] << 16)};
+        } else {
+          const long long at = (long long)it.partial * a.rows + 16 * m + row;
+          *reinterpret_cast<glm_f32x4 *>(a.part + at * DV + ch) = o;
+          if (ch == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{mr, l};
+        }
       }
     }
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------
 // The latent cache on the matrix cores: values are the first DV channels of
 // the key rows, so a tile is read once and serves both products, and many
-// heads share one row, so a workgroup takes 64 query rows, 16 a wave, and its
-// waves share each tile of 32 positions through LDS (two tiles in turn; a
-// barrier a tile).  The products, and the probabilities that stay in their
-// lane, are those of attn_group_kernel; the sums of 16 rows x 512 channels
-// take 128 registers, the rows 72, so two workgroups fit a CU and one's loads
-// and barriers hide behind the other's products.
+// heads share one row, so a workgroup takes 64 query rows and its eight waves
+// share each tile of 32 positions through LDS.  Two waves have 16 rows: each
+// forms the scores of 16 of the positions, they exchange them through LDS
+// (lane for lane, so both know all 32 and hold the same maximum, sum and
+// probabilities), and each adds half of the channels to the sums.  A wave
+// alone with its rows would need 128 registers for the sums beside 72 for the
+// rows, which left none to read ahead with; a pair's 64 do.  Products and
+// operand layouts are those of attn_group_kernel.
 // LDS holds a tile as blocks of 1 KB, 8 positions x 64 channels, the 16-byte
 // piece c of position t at 128 t + 16 (c ^ t): a wave's load of one block
 // reads eight whole 128-byte lines, and neither the products' reads (16
 // positions x 4 pieces) nor the transposing ones (8 positions x 2 pieces a
-// half wave) meet on a bank.  bf16 goes there directly, by the swizzled
-// source address; MXFP8 through registers, a tile ahead, converted on its way
-// (exact).
-// Bound by the cache's bytes up to some 64 rows and by LDS reads beyond: a
-// tile's 68 KB for 16 rows feed 68 MFMAs.
+// half wave) meet on a bank.  DIRECT: bf16 goes there by buffer loads with
+// swizzled source addresses, into a ring of four tiles, three of them in
+// flight; rows that are not seen are asked for past the buffer's end and come
+// as zeros.  Else (MXFP8, converted on its way, exact; bf16 caches past a
+// buffer's 4 GB) through registers, two tiles ahead.
+// Bound by the cache's bytes for some 64 rows and by LDS reads beyond: 34 KB
+// for each wave's 34 MFMAs.
 // ---------------------------------------------------------------------------
-template <int DK, int DV, int FMT>
-__global__ __launch_bounds__(256, 2) void attn_latent_kernel(AttnArgs a) {
-  constexpr int kG = DK / 64;               // blocks of eight positions
-  constexpr int kTile = 4 * kG * 1024;      // bytes of 32 positions
+template <int DK, int DV, int FMT, bool DIRECT>
+__global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
+  static_assert(!DIRECT || FMT == GLM_FMT_BF16, "MXFP8 is converted in registers");
+  constexpr int kG = DK / 64;              // blocks of eight positions
+  constexpr int kTile = 4 * kG * 1024;     // bytes of 32 positions
   constexpr bool kMx = FMT != GLM_FMT_BF16;
-  constexpr int kRaw = (DK / 16 + 7) / 8;   // MXFP8: pieces of a thread's eighth of a row
-  __shared__ __align__(16) uint8_t s_kv[2][kTile];
-  AttnItem it;
-  if (!attn_item(a, blockIdx.x, it)) return;
-  attn_plan(a, it);
+  constexpr int kLoads = (kG + 1) / 2;     // blocks of a wave (a pair's middle one is both's)
+  constexpr int kPieces = DK / (kMx ? 16 : 8);   // 16-byte pieces of a row
+  constexpr int kRaw = (kPieces + 15) / 16;      // through registers: a thread's
+  constexpr int kD = DV / 32;              // 16-channel tiles of a wave's half
+  constexpr int kAhead = DIRECT ? 8 : 4;   // operands read ahead of the products
+  // (one dynamic array: for reads of a static one the compiler waits for every load on its way to it)
+  extern __shared__ __align__(16) uint8_t smem[];
+  const auto s_kv = [&](int buf) { return smem + buf * kTile; };
+  glm_f32x4(*s_x)[2][64] = reinterpret_cast<glm_f32x4(*)[2][64]>(smem + (DIRECT ? 4 : 2) * kTile);
+  int(*s_id)[64] = reinterpret_cast<int(*)[64]>(s_x + 4);  // DIRECT: page numbers of the tiles ahead
+  AttnWalk walk;
+  if (!walk.start(a, blockIdx.x)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
-  const int R = attn_rows(a), group = a.heads / a.kv_heads, rb = a.hblocks / a.kv_heads;
-  const int head = it.hb / rb, r0 = (it.hb - head * rb) * 64 + 16 * wave;
-  const bool active = r0 < R;  // (uniform in a wave)
-  const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
-  const int end = min(it.t1 * kAttnTile, it.len);
-  const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
-
-  const int r = min(r0 + n, R - 1), tok = r / group;
-  glm_bf16x8 q[DK / 32];
-  {
-    const uint16_t *p = a.q + ((long long)it.b * a.q_len + tok) * a.q_stride +
-                        (head * group + r - tok * group) * DK + 8 * quad;
-#pragma unroll
-    for (int s = 0; s < DK / 32; ++s) q[s] = *reinterpret_cast<const glm_bf16x8 *>(p + 32 * s);
-  }
-  glm_f32x4 acc[DV / 16];
-#pragma unroll
-  for (int d = 0; d < DV / 16; ++d) acc[d] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
-  float top = -INFINITY, sum = 0.0f;
-
-  // this thread's share of a tile: an eighth of position `mine`
-  const int tl = lane >> 3, pc = lane & 7, mine = 8 * wave + tl;
-  // the products' reads: position n, piece 4 (s % 2) + quad of 64 channels s / 2; even s, odd s + 64 ^
-  const int kread = (n >> 3) * kG * 1024 + (n & 7) * 128 + ((quad ^ (n & 7)) << 4);
+  const int rg = wave >> 1, half = wave & 1;
+  const int R = attn_rows(a), group = a.heads / a.kv_heads;
+  // this lane's piece of the wave's blocks: piece pc ^ tl of position `mine`
+  const int tl = lane >> 3, pc = lane & 7, mine = 8 * rg + tl;
+  const int g0 = half ? kG - kLoads : 0;  // the wave's blocks
+  // the products' reads: position 16 half + n, piece 4 (s % 2) + quad of 64 channels s / 2
+  const int kread = (2 * half + (n >> 3)) * kG * 1024 + (n & 7) * 128 + ((quad ^ (n & 7)) << 4);
   // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
   const int vt = 4 * quad + (n >> 2);
-  const int vread = (vt >> 3) * kG * 1024 + (vt & 7) * 128 + ((((n & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (n & 1);
+  const int vread = ((vt >> 3) * kG + half * kD / 4) * 1024 + (vt & 7) * 128 +
+                    ((((n & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (n & 1);
 
-  struct Rows {
-    int row;        // of this thread's position
-    uint32_t seen;  // of the tile's 32
-  };
-  const auto rows_at = [&](int p) {
-    const int pos = p + (lane & 31);
-    int block, off;
-    page_of(a, min(pos, end - 1), block, off);
-    const int id = table[block];
-    const bool fine = (uint32_t)id < (uint32_t)a.num_pages;
-    const int row = fine ? (id * a.kv_heads + head) * a.page + off : 0;
-    return Rows{__shfl(row, mine, kWave), (uint32_t)__ballot(fine && pos < end)};
-  };
-  glm_u32x4 raw[kRaw];
-  uint32_t rsc[kRaw];
-  const auto fetch = [&](const Rows &at, int buf) {  // bf16: into LDS; MXFP8: into registers
-    if constexpr (!kMx) {
-      const uint8_t *src = (const uint8_t *)a.kc + (long long)at.row * (2 * DK) + ((pc ^ tl) << 4);
+  // through registers: sixteen threads a position
+  const int xt = 4 * wave + (lane >> 4), xc = lane & 15;
+  const __amdgpu_buffer_rsrc_t kvrs = make_rsrc(a.kc, a.cache_bytes);
+  for (AttnItem it; walk.next(a, it);) {
+    const int head = it.head, r0 = it.rb * 64 + 16 * rg;
+    const bool active = r0 < R;  // (uniform in a wave)
+    const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
+    const int end = min(it.t1 * kAttnTile, it.len);
+    const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
+
+    const int r = min(r0 + n, R - 1), tok = r / group;
+    glm_bf16x8 q[DK / 32];
+    {
+      const uint16_t *p = a.q + ((long long)it.b * a.q_len + tok) * a.q_stride +
+                          (head * group + r - tok * group) * DK + 8 * quad;
 #pragma unroll
-      for (int i = 0; i < kG; ++i)
-        __builtin_amdgcn_global_load_lds(
-            (__attribute__((address_space(1))) void *)(src + 128 * i),
-            (__attribute__((address_space(3))) void *)(s_kv[buf] + (wave * kG + i) * 1024), 16, 0, 0);
-    } else {
-      const uint8_t *src = (const uint8_t *)a.kc + (long long)at.row * DK;
-      const uint8_t *sc = a.ks + (long long)at.row * (DK / 32);
+      for (int s = 0; s < DK / 32; ++s) q[s] = *reinterpret_cast<const glm_bf16x8 *>(p + 32 * s);
+    }
+    glm_f32x4 acc[kD];
+#pragma unroll
+    for (int d = 0; d < kD; ++d) acc[d] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, sum = 0.0f;
+
+    // Page numbers are asked for two tiles before the rows, so that waiting for them waits for no
+    // row that is still wanted in flight.  Past the end: the last position's, not seen.
+    struct Rows {
+      int row;        // lane l: of position l % 32, -1 where it is not seen
+      uint32_t seen;  // of the tile's 32
+    };
+    const auto rows_of = [&](int id, int p) {
+      int block, off;
+      page_of(a, p + (lane & 31), block, off);
+      const bool fine = (uint32_t)id < (uint32_t)a.num_pages && p + (lane & 31) < end;
+      return Rows{fine ? (id * a.kv_heads + head) * a.page + off : -1, (uint32_t)__ballot(fine)};
+    };
+    const auto block_of = [&](int p) {
+      int block, off;
+      page_of(a, min(p + (lane & 31), end - 1), block, off);
+      return block;
+    };
+    const __amdgpu_buffer_rsrc_t idrs = make_rsrc(table, (uint32_t)a.max_blocks * 4u);
+    const auto load_ids = [&](int p, int slot) {  // DIRECT: straight into LDS, every wave the same
+      buf4_to_lds(idrs, s_id[slot], 4u * block_of(p), 0);
+    };
+    const auto load_lds = [&](int rows, int buf) {  // DIRECT
+      const int row = __shfl(rows, mine, kWave);
+      const uint32_t at = row < 0 ? 0xfffff000u : (uint32_t)row * (2 * DK) + ((pc ^ tl) << 4) + 128 * g0;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        buf16_to_lds(kvrs, s_kv(buf) + (rg * kG + g0 + i) * 1024, at, 128 * i);
+    };
+    // a tile on its way to LDS through registers, sixteen threads a position
+    struct Raw {
+      glm_u32x4 v[kRaw];
+      uint32_t sc[kMx ? kRaw : 1];
+      bool fine;
+    };
+    const auto load_raw = [&](Raw &x, int rows) {
+      const int row = __shfl(rows, xt, kWave);
+      x.fine = row >= 0;
+      const long long at = max(row, 0);
+      const uint8_t *src = (const uint8_t *)a.kc + at * (16 * kPieces), *sc = a.ks + at * (DK / 32);
 #pragma unroll
       for (int i = 0; i < kRaw; ++i) {
-        const int c = min(8 * i + pc, DK / 16 - 1);
-        raw[i] = __builtin_nontemporal_load(reinterpret_cast<const glm_u32x4 *>(src + 16 * c));
-        rsc[i] = sc[c >> 1];
+        const int c = min(16 * i + xc, kPieces - 1);
+        x.v[i] = __builtin_nontemporal_load(reinterpret_cast<const glm_u32x4 *>(src + 16 * c));
+        if constexpr (kMx) x.sc[i] = sc[c >> 1];
       }
-    }
-  };
-  const auto store = [&](int buf) {  // MXFP8: the registers' tile as bf16
-    if constexpr (kMx) {
+    };
+    const auto store_raw = [&](const Raw &x, int buf) {
+      uint8_t *row = s_kv(buf) + (xt >> 3) * kG * 1024 + (xt & 7) * 128;
 #pragma unroll
       for (int i = 0; i < kRaw; ++i) {
-        const int c = 8 * i + pc;
-        if (c < DK / 16) {
-          const float sc = e8m0_to_f32(rsc[i]);
-          uint8_t *dst = s_kv[buf] + (wave * kG + (c >> 2)) * 1024 + tl * 128;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<glm_bf16x8 *>(dst + (((2 * (c & 3) + h) ^ tl) << 4)) =
-                mxfp8_words_to_bf16x8(raw[i][2 * h], raw[i][2 * h + 1], sc);
-        }
-      }
-    }
-  };
-
-  int p = it.t0 * kAttnTile;
-  if (p < end) {
-    Rows cur = rows_at(p), nxt = cur, far = cur;
-    fetch(cur, 0);
-    if (p + 32 < end) nxt = rows_at(p + 32);
-    if constexpr (kMx) {
-      store(0);
-      if (p + 32 < end) {
-        fetch(nxt, 0);
-        if (p + 64 < end) far = rows_at(p + 64);
-      }
-    }
-    __syncthreads();
-    for (int buf = 0;; buf ^= 1) {
-      const bool more = p + 32 < end;
-      if (more) {
+        const int c = 16 * i + xc;
+        if (c >= kPieces) continue;
         if constexpr (kMx) {
-          store(buf ^ 1);
-          if (p + 64 < end) fetch(far, 0);
+          const float sc = e8m0_to_f32(x.sc[i]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const glm_u32x4 o = __builtin_bit_cast(
+                glm_u32x4, mxfp8_words_to_bf16x8(x.v[i][2 * h], x.v[i][2 * h + 1], sc));
+            *reinterpret_cast<glm_u32x4 *>(row + (c >> 2) * 1024 + (((2 * (c & 3) + h) ^ (xt & 7)) << 4)) =
+                x.fine ? o : glm_u32x4{0, 0, 0, 0};
+          }
         } else {
-          fetch(nxt, buf ^ 1);
-          if (p + 64 < end) far = rows_at(p + 64);
+          *reinterpret_cast<glm_u32x4 *>(row + (c >> 3) * 1024 + (((c & 7) ^ (xt & 7)) << 4)) =
+              x.fine ? x.v[i] : glm_u32x4{0, 0, 0, 0};
         }
       }
-      const uint8_t *kv = s_kv[buf];
-      const bool whole = cur.seen == 0xffffffffu && p + 32 <= all_see;  // (uniform)
+    };
+    // this wave's LDS writes are done, and every wave has come here
+    const auto meet = [&]() {
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(63) & ~(15 << 8));
+      ring_barrier();
+    };
+
+    // one tile's products, from LDS; every wave comes here with the same tile
+    const auto tile = [&](int p, uint32_t seen, int buf) {
+      const uint8_t *kv = s_kv(buf);
+      const bool every = p + 32 <= all_see || a.q_len == 1;  // (uniform) all rows see the same
+      const bool whole = seen == 0xffffffffu && p + 32 <= all_see;
+      glm_f32x4 own = {0.f, 0.f, 0.f, 0.f};
+      if (active) {
+        glm_f32x4 odd = {0.f, 0.f, 0.f, 0.f};
+        // a ring of operands: one pair is read when the pair kAhead before it has been multiplied
+        glm_bf16x8 k[kAhead];
+        const auto key = [&](int i) {
+          return *reinterpret_cast<const glm_bf16x8 *>(kv + (kread ^ (64 * (i & 1))) + (i >> 1) * 1024);
+        };
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) k[i] = key(i);
+#pragma unroll
+        for (int i = 0; i < DK / 32; i += 2) {
+          __builtin_amdgcn_sched_barrier(0);
+          own = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i % kAhead], q[i], own, 0, 0, 0);
+          odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[(i + 1) % kAhead], q[i + 1], odd, 0, 0, 0);
+          if (i + kAhead < DK / 32) {
+            k[i % kAhead] = key(i + kAhead);
+            k[(i + 1) % kAhead] = key(i + 1 + kAhead);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        own += odd;
+        s_x[rg][half][lane] = own;
+      }
+      meet();
       glm_bf16x8 prob = {};
       if (active) {
-        glm_f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-        for (int i = 0; i < DK / 32; ++i)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const glm_bf16x8 kf = *reinterpret_cast<const glm_bf16x8 *>(
-                kv + ((kread ^ (64 * (i & 1))) + (2 * u * kG + (i >> 1)) * 1024));
-            s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[i], s[u], 0, 0, 0);
-          }
+        const glm_f32x4 other = s_x[rg][half ^ 1][lane];
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4] * a.scale_log2;
+        for (int i = 0; i < 4; ++i) {
+          x[i] = (half ? other[i] : own[i]) * a.scale_log2;
+          x[4 + i] = (half ? own[i] : other[i]) * a.scale_log2;
+        }
         if (!whole) {
+          const uint32_t bits = seen >> (4 * quad);
+          const int left = all_see + tok - p - 4 * quad;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int at = 16 * (i / 4) + 4 * quad + i % 4;
-            if (!((cur.seen >> at) & 1u) || p + at >= all_see + tok) x[i] = -INFINITY;
+            const int at = 16 * (i / 4) + i % 4;
+            if (!((bits >> at) & 1u) || at >= left) x[i] = -INFINITY;
           }
         }
         float mx = x[0];
@@ -709,7 +789,7 @@ __global__ __launch_bounds__(256, 2) void attn_latent_kernel(AttnArgs a) {
           const float keep = __builtin_amdgcn_exp2f(top - from);
           sum *= keep;
 #pragma unroll
-          for (int d = 0; d < DV / 16; ++d) acc[d] *= keep;
+          for (int d = 0; d < kD; ++d) acc[d] *= keep;
         }
         top = next;
 #pragma unroll
@@ -725,97 +805,163 @@ __global__ __launch_bounds__(256, 2) void attn_latent_kernel(AttnArgs a) {
         const bf16x4 lo = lds_read_tr(at), hi = lds_read_tr(at + 2 * kG * 512);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       };
-      if (whole) {
+      if (every) {
         if (active) {
+          glm_bf16x8 v[kAhead];
 #pragma unroll
-          for (int d = 0; d < DV / 16; ++d)
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values(d), prob, acc[d], 0, 0, 0);
+          for (int d = 0; d < kAhead; ++d) v[d] = values(d);
+#pragma unroll
+          for (int d = 0; d < kD; ++d) {
+            __builtin_amdgcn_sched_barrier(0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[d % kAhead], prob, acc[d], 0, 0, 0);
+            if (d + kAhead < kD) v[d % kAhead] = values(d + kAhead);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       } else {
         // as in attn_group_kernel, a turn for each token from the last on, with ever more of the
         // tile's rows set to zero; the scores are done with them
-        const bool every = p + 32 <= all_see;
-        for (int t = a.q_len - 1; t >= (every ? a.q_len - 1 : 0); --t) {
-          __syncthreads();
-          if (!((cur.seen >> mine) & 1u) || p + mine >= all_see + t) {
+        for (int t = a.q_len - 1; t >= 0; --t) {
+          meet();
+          if (p + mine >= all_see + t) {
 #pragma unroll
-            for (int i = 0; i < kG; ++i)
-              *reinterpret_cast<glm_u32x4 *>(s_kv[buf] + (wave * kG + i) * 1024 + 16 * lane) =
+            for (int i = 0; i < kLoads; ++i)
+              *reinterpret_cast<glm_u32x4 *>(s_kv(buf) + (rg * kG + g0 + i) * 1024 + 16 * lane) =
                   glm_u32x4{0, 0, 0, 0};
           }
-          __syncthreads();
+          meet();
           if (active) {
 #pragma unroll
-            for (int d = 0; d < DV / 16; ++d) {
+            for (int d = 0; d < kD; ++d) {
               const glm_f32x4 with =
                   __builtin_amdgcn_mfma_f32_16x16x32_bf16(values(d), prob, acc[d], 0, 0, 0);
-              if (every || tok == t) acc[d] = with;
+              if (tok == t) acc[d] = with;
+              __builtin_amdgcn_sched_barrier(0);
             }
           }
         }
       }
-      if (!more) break;
-      __syncthreads();
-      p += 32;
-      cur = nxt;
-      nxt = far;
-      if constexpr (kMx) {
-        if (p + 64 < end) far = rows_at(p + 64);
+    };
+
+    const int p0 = it.t0 * kAttnTile, tiles = end > p0 ? (end - p0 + 31) / 32 : 0;
+    if (tiles > 0) {
+      uint32_t seen0, seen1, seen2;
+      const auto id_at = [&](int p) { return table[block_of(p)]; };
+      const int i0 = id_at(p0), i1 = id_at(p0 + 32), i2 = id_at(p0 + 64);
+      const Rows r0_ = rows_of(i0, p0), r1_ = rows_of(i1, p0 + 32), r2_ = rows_of(i2, p0 + 64);
+      seen0 = r0_.seen;
+      seen1 = r1_.seen;
+      seen2 = r2_.seen;
+      if constexpr (DIRECT) {
+        // tile i's rows are loaded three tiles ahead, its page numbers five; past the last tile the
+        // rows are none (zeros, no traffic), so that every turn issues the same count
+        load_lds(r0_.row, 0);
+        load_ids(p0 + 96, 3);
+        load_lds(r1_.row, 1);
+        load_ids(p0 + 128, 4);
+        load_lds(r2_.row, 2);
+        for (int i = 0; i < tiles; ++i) {
+          // tile i and the page numbers of tile i + 3 have landed; buffer i + 3 is free
+          __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads + 1) & ~(15 << 8));
+          ring_barrier();
+          __builtin_amdgcn_sched_barrier(0);
+          const int p = p0 + 32 * i;
+          const Rows next = rows_of(s_id[(i + 3) & 7][lane & 31], p + 96);
+          load_ids(p + 160, (i + 5) & 7);
+          load_lds(next.row, (i + 3) & 3);
+          __builtin_amdgcn_sched_barrier(0);
+          tile(p, seen0, i & 3);
+          seen0 = seen1;
+          seen1 = seen2;
+          seen2 = next.seen;
+        }
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // nothing may land in LDS that is left
+      } else {
+        // tile i + 1 goes from registers to LDS and tile i + 3 is loaded while tile i is worked on
+        Raw x0, x1;
+        int near = id_at(p0 + 96);
+        load_raw(x0, r0_.row);
+        load_raw(x1, r1_.row);
+        store_raw(x0, 0);
+        load_raw(x0, r2_.row);
+        const auto turn = [&](int i, Raw &here) {  // (tile i + 1 is in `here`)
+          meet();
+          const int p = p0 + 32 * i;
+          store_raw(here, (i + 1) & 1);
+          const Rows next = rows_of(near, p + 96);
+          near = id_at(p + 128);
+          load_raw(here, next.row);
+          tile(p, seen0, i & 1);
+          seen0 = seen1;
+          seen1 = seen2;
+          seen2 = next.seen;
+        };
+        for (int i = 0; i < tiles; i += 2) {
+          turn(i, x1);
+          if (i + 1 < tiles) turn(i + 1, x0);
+        }
       }
     }
-  }
 
-  sum = sum_over_quads(sum);
-  if (!active || r0 + n >= R) return;
-  if (it.splits == 1) {
-    uint16_t *out = a.out + (((long long)it.b * a.q_len + tok) * a.heads + head * group + r - tok * group) * DV +
-                    4 * quad;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    sum = sum_over_quads(sum);
+    if (!active || r0 + n >= R) {
+      // (a row past the last, or a wave of them)
+    } else if (it.whole) {
+      uint16_t *out = a.out + (((long long)it.b * a.q_len + tok) * a.heads + head * group + r - tok * group) * DV +
+                      half * (DV / 2) + 4 * quad;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-    for (int d = 0; d < DV / 16; ++d) {
-      uint32_t b[4];
+      for (int d = 0; d < kD; ++d) {
+        uint32_t b[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = f32_to_bf16(acc[d][j] * inv);
-      *reinterpret_cast<uint2 *>(out + 16 * d) = uint2{b[0] | (b[1] << 16), b[2] | (b[3] << 16)};
+        for (int j = 0; j < 4; ++j) b[j] = f32_to_bf16(acc[d][j] * inv);
+        *reinterpret_cast<uint2 *>(out + 16 * d) = uint2{b[0] | (b[1] << 16), b[2] | (b[3] << 16)};
+      }
+    } else {
+      const long long at = (long long)it.partial * a.rows + 16 * rg + n;
+#pragma unroll
+      for (int d = 0; d < kD; ++d)
+        *reinterpret_cast<glm_f32x4 *>(a.part + at * DV + half * (DV / 2) + 16 * d + 4 * quad) = acc[d];
+      if (half == 0 && quad == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{top, sum};
     }
-  } else {
-    const long long at = attn_partial(a, it) * a.rows + 16 * wave + n;
-#pragma unroll
-    for (int d = 0; d < DV / 16; ++d)
-      *reinterpret_cast<glm_f32x4 *>(a.part + at * DV + 16 * d + 4 * quad) = acc[d];
-    if (quad == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{top, sum};
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------
-// The requests that were cut into several items: out = sum_i 2^(m_i - m) acc_i
-// / sum_i 2^(m_i - m) l_i over the items in order.  A thread has four channels
-// of a row.
+// The pairs of request and kv head that were cut: out = sum_i 2^(m_i - m) acc_i
+// / sum_i 2^(m_i - m) l_i over their pieces in order.  A thread has four
+// channels of a row.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int b = blockIdx.y;
   const int2 plan = a.plan[b];
-  if (plan.x <= 1) return;
-  const int R = attn_rows(a), group = a.heads / a.kv_heads, rb = a.hblocks / a.kv_heads;
+  const int tiles = (attn_len(a, b) + kAttnTile - 1) / kAttnTile, w = kAttnOver + tiles;
+  const int R = attn_rows(a), group = a.heads / a.kv_heads;
   const int i = blockIdx.x * 256 + threadIdx.x, quads = a.dv / 4;
   const int row = i / quads, ch = 4 * (i - row * quads);
-  if (row >= a.kv_heads * R) return;
+  if (row >= a.kv_heads * R || tiles == 0) return;
   const int head = row / R, r = row - head * R;
-  const int hb = head * rb + r / a.rows;
-  const long long first = (long long)plan.y * a.hblocks + hb;
+  // the parts that the pair's tiles lie in; the first holds its beginning
+  const int first = plan.x * a.kv_heads + head * w;
+  const int g0 = (first + kAttnOver) / plan.y, g1 = (first + w - 1) / plan.y;
+  if (g0 == g1) return;
+  const auto at = [&](int g) {
+    return ((long long)(2 * g + (g == g0)) * a.rblocks + r / a.rows) * a.rows + r % a.rows;
+  };
   float m = -INFINITY;
-  for (int s = 0; s < plan.x; ++s)
-    m = fmaxf(m, a.ml[2 * ((first + (long long)s * a.hblocks) * a.rows + r % a.rows)]);
+#pragma unroll 4
+  for (int g = g0; g <= g1; ++g) m = fmaxf(m, a.ml[2 * at(g)]);
   const float from = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
   glm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < plan.x; ++s) {
-    const long long at = (first + (long long)s * a.hblocks) * a.rows + r % a.rows;
-    const float2 ml = *reinterpret_cast<const float2 *>(a.ml + 2 * at);
-    const float w = exp2f(ml.x - from);
-    l += w * ml.y;
-    acc += w * *reinterpret_cast<const glm_f32x4 *>(a.part + at * a.dv + ch);
+  for (int g = g0; g <= g1; ++g) {
+    const float2 ml = *reinterpret_cast<const float2 *>(a.ml + 2 * at(g));
+    const float scale = exp2f(ml.x - from);
+    l += scale * ml.y;
+    acc += scale * *reinterpret_cast<const glm_f32x4 *>(a.part + at(g) * a.dv + ch);
   }
   uint32_t o[4];
 #pragma unroll
@@ -833,8 +979,8 @@ enum AttnForm { kAttnAny, kAttnGroup, kAttnLatent };
 
 struct AttnSizes {
   AttnForm form;
-  int rows, hblocks, target, min_c;
-  long long grid, partials;  // workgroups; partial results
+  int rows, rblocks, parts, min_part;
+  unsigned grid;
   size_t plan_bytes, part_bytes, ml_bytes;
 };
 
@@ -859,12 +1005,24 @@ void launch_group(hipStream_t s, dim3 grid, const glm::AttnArgs &a) {
   }
 }
 
+template <int DK, int DV, int FMT, bool DIRECT>
+int launch_latent(hipStream_t s, dim3 grid, const glm::AttnArgs &a) {
+  // tiles of 32 positions, the scores' exchange, page numbers
+  constexpr int kLds = (DIRECT ? 4 : 2) * 32 * DK * 2 + 4 * 2 * 64 * 16 + (DIRECT ? 8 * 64 * 4 : 0);
+  hipLaunchKernelGGL((glm::attn_latent_kernel<DK, DV, FMT, DIRECT>), grid, dim3(512), kLds, s, a);
+  return GLM_OK;
+}
+
 template <int FMT>
-void launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnArgs &a) {
+int launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnArgs &a) {
   if (form == kAttnAny)
     hipLaunchKernelGGL(glm::attn_any_kernel<FMT>, grid, dim3(256), 0, s, a);
-  else if (form == kAttnLatent)
-    hipLaunchKernelGGL((glm::attn_latent_kernel<576, 512, FMT>), grid, dim3(256), 0, s, a);
+  else if (form == kAttnLatent) {
+    // direct loads where 32-bit offsets (and those past the end, from 2^32 - 4096 on) reach
+    if constexpr (FMT == GLM_FMT_BF16)
+      if (a.cache_bytes) return launch_latent<576, 512, FMT, true>(s, grid, a);
+    return launch_latent<576, 512, FMT, false>(s, grid, a);
+  }
   else if (a.dk == 64)
     launch_group<64, 64, FMT>(s, grid, a);
   else if (a.dk == 128)
@@ -873,6 +1031,7 @@ void launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnAr
     launch_group<192, 128, FMT>(s, grid, a);
   else
     launch_group<256, 256, FMT>(s, grid, a);
+  return GLM_OK;
 }
 
 // Sizes that follow from a call's shape; false for shapes that are refused.
@@ -884,40 +1043,36 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
   if (B > 65535 || q_len > 16 || heads > 1024 || (long long)max_blocks * page_size > INT_MAX - glm::kAttnTile)
     return false;
   const int R = q_len * (heads / kv_heads);
+  int slots;  // workgroups that the chip holds at once
   if (latent && key_dim == 576 && value_dim == 512) {
     z.form = kAttnLatent;
     z.rows = 64;
-    z.hblocks = kv_heads * ((R + 63) / 64);
-    z.target = 512;
-    z.min_c = 2;
+    slots = 256;
+    z.min_part = glm::kAttnOver + 1;
   } else if (group_widths(key_dim, value_dim)) {
     z.form = kAttnGroup;
     const int most = key_dim == 64 ? 64 : key_dim <= 192 ? 32 : 16;  // rows that fit the registers
     z.rows = R <= 16 || most == 16 ? 16 : R <= 32 || most == 32 ? 32 : 64;
-    z.hblocks = kv_heads * ((R + z.rows - 1) / z.rows);
-    z.target = 1024;
-    z.min_c = 2;
+    slots = 512;
+    z.min_part = glm::kAttnOver + 2;
   } else {
     z.form = kAttnAny;
     z.rows = 1;
-    z.hblocks = kv_heads * R;
-    z.target = 2048;
-    z.min_c = 4;
+    slots = 2048;
+    z.min_part = glm::kAttnOver + 4;
   }
+  z.rblocks = (R + z.rows - 1) / z.rows;
+  z.parts = slots / z.rblocks > 1 ? slots / z.rblocks : 1;
   const long long tiles = ((long long)max_blocks * page_size + glm::kAttnTile - 1) / glm::kAttnTile;
-  if (tiles * B > INT_MAX / 2 || (long long)B * z.hblocks > INT_MAX / 2) return false;
-  const long long splits = (tiles + z.min_c - 1) / z.min_c;
-  z.grid = z.hblocks * B * splits;
-  if (z.grid > z.target + (long long)z.hblocks * B) z.grid = z.target + (long long)z.hblocks * B;
-  if (z.hblocks > kv_heads) z.grid = (z.grid + 8 * z.hblocks - 1) / (8 * z.hblocks) * (8 * z.hblocks);
-  // a request of nt > c tiles has at most 2 nt / c items, so at most 2 target / hblocks over all
-  long long p = B * splits;
-  if (p > 2LL * z.target / z.hblocks) p = 2LL * z.target / z.hblocks;
-  if (splits == 1) p = 0;
-  z.partials = p * z.hblocks;
+  const long long units = (tiles + glm::kAttnOver) * B * kv_heads;
+  if (units > INT_MAX / 2) return false;
+  const long long most_parts = (units + z.min_part - 1) / z.min_part;
+  if (z.parts > most_parts) z.parts = most_parts > 1 ? (int)most_parts : 1;
+  z.grid = z.rblocks > 1 ? (unsigned)((z.parts + 7) / 8 * 8 * z.rblocks) : (unsigned)z.parts;
+  const size_t results = (size_t)2 * z.parts * z.rblocks * z.rows;
   z.plan_bytes = up256((size_t)B * sizeof(int2));
-  z.part_bytes = up256((size_t)z.partials * z.rows * value_dim * sizeof(float));
-  z.ml_bytes = up256((size_t)z.partials * z.rows * 2 * sizeof(float));
+  z.part_bytes = up256(results * value_dim * sizeof(float));
+  z.ml_bytes = up256(results * 2 * sizeof(float));
   return true;
 }
 
@@ -999,20 +1154,21 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
   a.num_pages = num_pages;
   a.page = page_size;
   a.max_blocks = max_blocks;
-  a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
+  const unsigned long long bytes = (unsigned long long)num_pages * page_size * kv_heads * key_dim * 2;
+  a.cache_bytes = bytes <= 0xffff0000ull && max_blocks <= 1 << 29 ? (uint32_t)bytes : 0;
+  a.page_magic = page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / page_size);
   a.rows = z.rows;
-  a.hblocks = z.hblocks;
-  a.target = z.target;
-  a.min_c = z.min_c;
+  a.rblocks = z.rblocks;
+  a.parts = z.parts;
+  a.min_part = z.min_part;
   a.scale_log2 = scale * glm::kLog2e;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)z.grid);
-  if (mx)
-    launch_attention<GLM_FMT_MXFP8>(s, grid, z.form, a);
-  else
-    launch_attention<GLM_FMT_BF16>(s, grid, z.form, a);
+  const int rc = mx ? launch_attention<GLM_FMT_MXFP8>(s, grid, z.form, a)
+                    : launch_attention<GLM_FMT_BF16>(s, grid, z.form, a);
+  if (rc != GLM_OK) return rc;
   GLM_LAUNCH_CHECK("paged_attention");
-  if (z.partials > 0) {
+  if (z.parts > 1) {
     const long long quads = (long long)q_len * heads * value_dim / 4;
     hipLaunchKernelGGL(glm::attn_join_kernel, dim3((unsigned)((quads + 255) / 256), B), dim3(256), 0,
                        s, a);
