@@ -18,9 +18,6 @@
 namespace glm {
 
 constexpr int kAttnTile = 64;  // positions; parts are cut between tiles
-// What a request costs a workgroup beside its tiles (its rows, the first loads' latency, the
-// result), in tiles.
-constexpr int kAttnOver = 1;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct AttnArgs {
@@ -34,9 +31,9 @@ struct AttnArgs {
   float *part, *ml;  // partial results [2 part + end][row block][rows][dv], [..][2]
   int B, q_len, heads, kv_heads, dk, dv, num_pages, page, max_blocks;
   uint32_t page_magic;   // floor(2^32 / page), at most 2^32 - 1
-  uint32_t cache_bytes;  // of kc where they fit 32 bits
   int rows, rblocks;    // query rows a workgroup takes, blocks of them in a kv head
   int parts, min_part;  // most parts, fewest units of a part
+  int over;  // what a request costs a workgroup beside its tiles (its rows, the first loads' latency, the result), in tiles
   float scale_log2;
 };
 
@@ -55,16 +52,16 @@ struct AttnItem {
 };
 
 // A workgroup's part of the work.  Requests in order, kv heads in order, a
-// pair of them takes kAttnOver units and one for each of its tiles; part i has
+// pair of them takes a.over units and one for each of its tiles; part i has
 // the units [i u, (i + 1) u), u the least that makes do with `parts` parts.
 // At most one pair began before the part and one ends after it: partial
 // results 2 i and 2 i + 1.
 struct AttnWalk {
-  int x, x1, u, part, rb;  // units left [x, x1)
+  int x, x1, u, part, rb, over;  // units left [x, x1)
   int b, head, before, len, w;  // the pair: the request's units before it (of one kv head), its units
 
   __device__ __forceinline__ int units(int len_b) const {
-    return kAttnOver + (len_b + kAttnTile - 1) / kAttnTile;
+    return over + (len_b + kAttnTile - 1) / kAttnTile;
   }
 
   // False where the part is empty.  Every wave does this by itself, without a barrier.
@@ -72,6 +69,7 @@ struct AttnWalk {
     const int lane = threadIdx.x & 63;
     part = block;
     rb = 0;
+    over = a.over;
     if (a.rblocks > 1) {
       // a head's row blocks read the same positions: consecutive workgroups go to the eight XCDs
       // in turn, so the row blocks of a part are dealt out eight apart and share an XCD's cache
@@ -113,6 +111,7 @@ struct AttnWalk {
   }
 
   // The part's next item; also leaves the request's place for the join.
+  template <bool PLAN = true>
   __device__ __forceinline__ bool next(const AttnArgs &a, AttnItem &it) {
     while (x < x1) {
       const int first = before * a.kv_heads + head * w, from = x - first, to = min(x1 - first, w);
@@ -120,18 +119,20 @@ struct AttnWalk {
       it.head = head;
       it.rb = rb;
       it.len = len;
-      it.t0 = max(0, from - kAttnOver);
-      it.t1 = to - kAttnOver;
-      it.whole = it.t0 == 0 && it.t1 == w - kAttnOver;
+      it.t0 = max(0, from - over);
+      it.t1 = to - over;
+      it.whole = w == over || (it.t0 == 0 && it.t1 == w - over);  // (an empty request: wherever it begins)
       it.partial = (2 * part + (it.t0 == 0)) * a.rblocks + rb;
-      if (from == 0 && head == 0 && rb == 0 && threadIdx.x == 0) a.plan[b] = int2{before, u};
-      const bool some = it.t1 > it.t0 || (w == kAttnOver && from == 0);
+      if (PLAN && from == 0 && head == 0 && rb == 0 && threadIdx.x == 0) a.plan[b] = int2{before, u};
+      const bool some = it.t1 > it.t0 || (w == over && from == 0);
       x = first + w;
       if (++head == a.kv_heads) {
         head = 0;
         before += w;
         if (++b < a.B) {
-          len = attn_len(a, b);
+          // (a scalar load: a vector one would wait for the rows in flight)
+          const auto lens = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)a.lens;
+          len = max(0, min(lens[b], a.max_blocks * a.page));
           w = units(len);
         }
       }
@@ -597,38 +598,66 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
 // piece c of position t at 128 t + 16 (c ^ t): a wave's load of one block
 // reads eight whole 128-byte lines, and neither the products' reads (16
 // positions x 4 pieces) nor the transposing ones (8 positions x 2 pieces a
-// half wave) meet on a bank.  DIRECT: bf16 goes there by buffer loads with
-// swizzled source addresses, into a ring of four tiles, three of them in
-// flight; rows that are not seen are asked for past the buffer's end and come
-// as zeros.  Else (MXFP8, converted on its way, exact; bf16 caches past a
-// buffer's 4 GB) through registers, two tiles ahead.
+// half wave) meet on a bank.  Rows go from the cache to LDS directly: bf16
+// into a ring of four such tiles, by swizzled source addresses; MXFP8 codes
+// and scales into a ring of three, from where the wave that loaded them
+// converts them (exact) into one of two tiles.  Three tiles (two) are in
+// flight, across the requests of a workgroup's part too; positions that are
+// not seen read a row of zeros.
 // Bound by the cache's bytes for some 64 rows and by LDS reads beyond: 34 KB
 // for each wave's 34 MFMAs.
 // ---------------------------------------------------------------------------
-template <int DK, int DV, int FMT, bool DIRECT>
+__device__ uint8_t attn_zero_row[2048];
+
+// N bytes a lane (2, 4 or 16) from global memory to LDS: lane l's to lds + l * max(N, 4).
+template <int N>
+__device__ __forceinline__ void load_to_lds(const void *src, void *lds) {
+  const auto from = (__attribute__((address_space(1))) void *)(const_cast<void *>(src));
+  const auto to = (__attribute__((address_space(3))) void *)lds;
+  static_assert(N == 2 || N == 4 || N == 16, "sizes used here");
+  if constexpr (N == 2)
+    __builtin_amdgcn_global_load_lds(from, to, 2, 0, 0);
+  else if constexpr (N == 4)
+    __builtin_amdgcn_global_load_lds(from, to, 4, 0, 0);
+  else
+    __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
+}
+
+template <int DK, int DV, int FMT>
+struct LatentLds {
+  static constexpr bool kMx = FMT != GLM_FMT_BF16;
+  static constexpr int kG = DK / 64;           // blocks of eight positions
+  static constexpr int kTile = 4 * kG * 1024;  // bytes of 32 positions
+  static constexpr int kTiles = kMx ? 2 : 4;
+  static constexpr int kRaw = kMx ? 4 * DK + 256 : 0;  // MXFP8: a wave's four rows and their scales
+  static constexpr int kX = kTiles * kTile;            // the exchanged scores
+  static constexpr int kId = kX + 4 * 2 * 64 * 16;     // page numbers of the tiles ahead
+  static constexpr int kRawAt = kId + 8 * 64 * 4;
+  static constexpr int kBytes = kRawAt + 3 * 8 * kRaw;
+  static_assert(kBytes <= 160 * 1024, "one workgroup a CU");
+};
+
+template <int DK, int DV, int FMT>
 __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
-  static_assert(!DIRECT || FMT == GLM_FMT_BF16, "MXFP8 is converted in registers");
-  constexpr int kG = DK / 64;              // blocks of eight positions
-  constexpr int kTile = 4 * kG * 1024;     // bytes of 32 positions
-  constexpr bool kMx = FMT != GLM_FMT_BF16;
-  constexpr int kLoads = (kG + 1) / 2;     // blocks of a wave (a pair's middle one is both's)
-  constexpr int kPieces = DK / (kMx ? 16 : 8);   // 16-byte pieces of a row
-  constexpr int kRaw = (kPieces + 15) / 16;      // through registers: a thread's
-  constexpr int kD = DV / 32;              // 16-channel tiles of a wave's half
-  constexpr int kAhead = DIRECT ? 8 : 4;   // operands read ahead of the products
+  typedef LatentLds<DK, DV, FMT> L;
+  constexpr bool kMx = L::kMx;
+  constexpr int kG = L::kG, kTile = L::kTile;
+  constexpr int kD = DV / 32;   // 16-channel tiles of a wave's half
+  constexpr int kAhead = kMx ? 6 : 8;  // operands read ahead of the products
+  constexpr int kLoads = kMx ? 4 : (kG + 1) / 2;  // of a wave and tile (bf16: a pair's middle block is both's)
+  static_assert(!kMx || DK == 576, "36 pieces of 16 codes, 18 scales a row");
   // (one dynamic array: for reads of a static one the compiler waits for every load on its way to it)
   extern __shared__ __align__(16) uint8_t smem[];
-  const auto s_kv = [&](int buf) { return smem + buf * kTile; };
-  glm_f32x4(*s_x)[2][64] = reinterpret_cast<glm_f32x4(*)[2][64]>(smem + (DIRECT ? 4 : 2) * kTile);
-  int(*s_id)[64] = reinterpret_cast<int(*)[64]>(s_x + 4);  // DIRECT: page numbers of the tiles ahead
+  uint8_t *const s_kv = smem;
+  glm_f32x4(*const s_x)[2][64] = reinterpret_cast<glm_f32x4(*)[2][64]>(smem + L::kX);
+  int(*const s_id)[64] = reinterpret_cast<int(*)[64]>(smem + L::kId);
   AttnWalk walk;
   if (!walk.start(a, blockIdx.x)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
   const int rg = wave >> 1, half = wave & 1;
   const int R = attn_rows(a), group = a.heads / a.kv_heads;
-  // this lane's piece of the wave's blocks: piece pc ^ tl of position `mine`
-  const int tl = lane >> 3, pc = lane & 7, mine = 8 * rg + tl;
-  const int g0 = half ? kG - kLoads : 0;  // the wave's blocks
+  constexpr int kHalf = (kG + 1) / 2;
+  const int g0 = half ? kG - kHalf : 0;  // the wave's blocks
   // the products' reads: position 16 half + n, piece 4 (s % 2) + quad of 64 channels s / 2
   const int kread = (2 * half + (n >> 3)) * kG * 1024 + (n & 7) * 128 + ((quad ^ (n & 7)) << 4);
   // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
@@ -636,16 +665,160 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   const int vread = ((vt >> 3) * kG + half * kD / 4) * 1024 + (vt & 7) * 128 +
                     ((((n & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (n & 1);
 
-  // through registers: sixteen threads a position
-  const int xt = 4 * wave + (lane >> 4), xc = lane & 15;
-  const __amdgpu_buffer_rsrc_t kvrs = make_rsrc(a.kc, a.cache_bytes);
+  // ---- the tiles of the part, one after the other: their page numbers are asked for five tiles
+  // ahead and their rows three, so that waiting for page numbers waits for no row that is still
+  // wanted in flight; past the last tile for nothing (zeros), so that every turn issues the same
+  struct Place {
+    int b, head, p, end;  // a tile's request, kv head, first position, end of the item
+  };
+  AttnWalk ahead = walk;
+  AttnItem next_it;
+  Place place = {0, 0, 0, 0};
+  const auto next_place = [&]() {
+    while (place.p >= place.end) {
+      if (!ahead.template next<false>(a, next_it)) return Place{0, 0, 0, 0};
+      place = {next_it.b, next_it.head, next_it.t0 * kAttnTile, min(next_it.t1 * kAttnTile, next_it.len)};
+    }
+    const Place now = place;
+    place.p += 32;
+    return now;
+  };
+  const auto id_of = [&](const Place &t) {
+    int block, off;
+    page_of(a, max(0, min(t.p + (lane & 31), t.end - 1)), block, off);
+    return a.tables + (long long)t.b * a.max_blocks + block;
+  };
+  struct Rows {
+    int row;        // lane l: of position l % 32, -1 where it is not seen
+    uint32_t seen;  // of the tile's 32
+  };
+  const auto rows_of = [&](int id, const Place &t) {
+    int block, off;
+    page_of(a, t.p + (lane & 31), block, off);
+    const bool fine = (uint32_t)id < (uint32_t)a.num_pages && t.p + (lane & 31) < t.end;
+    return Rows{fine ? (id * a.kv_heads + t.head) * a.page + off : -1, (uint32_t)__ballot(fine)};
+  };
+  // (what follows from the lane alone is formed anew in every turn: held over the loop, it would not
+  // leave the products their registers)
+  const auto this_lane = [&]() {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  const auto load_rows = [&](int rows, int slot) {
+    const int l = this_lane();
+    if constexpr (!kMx) {
+      const int row = __shfl(rows, 8 * rg + (l >> 3), kWave);
+      const uint8_t *src = (row < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)row * (2 * DK)) +
+                           (((l & 7) ^ (l >> 3)) << 4) + 128 * g0;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        load_to_lds<16>(src + 128 * i, s_kv + slot * kTile + (rg * kG + g0 + i) * 1024);
+    } else {
+      // four rows of 36 pieces: 16 lanes a row twice, then four lanes a row; 9 lanes a row for the scales
+      uint8_t *raw = smem + L::kRawAt + (slot * 8 + wave) * L::kRaw;
+      const auto code = [&](int t, int c) {
+        const int row = __shfl(rows, 4 * wave + t, kWave);
+        return (row < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)row * DK) + 16 * c;
+      };
+      const uint8_t *src = code(l >> 4, l & 15);
+      load_to_lds<16>(src, raw);
+      load_to_lds<16>(src + 256, raw + 1024);
+      const uint8_t *rest = code((l & 15) >> 2, 32 + (l & 3));
+      const int st = min(l / 9, 3), row = __shfl(rows, 4 * wave + st, kWave);
+      const uint8_t *sc = (row < 0 ? attn_zero_row : a.ks + (long long)row * (DK / 32)) + 2 * (l - 9 * st);
+      if (l < 16) load_to_lds<16>(rest, raw + 2048);
+      if (l < 36) load_to_lds<2>(sc, raw + 4 * DK);
+    }
+  };
+  // MXFP8: this wave's rows of a tile, from codes to bf16: piece c of row t to the tile's pieces 2 c,
+  // 2 c + 1 (the swizzle keeps them neighbours)
+  const auto convert = [&](int slot, int buf) {
+    const int l = this_lane(), t = l >> 4, c = l & 15;
+    const uint8_t *raw = smem + L::kRawAt + (slot * 8 + wave) * L::kRaw;
+    const auto place = [&](int t, int c) {
+      const int pos = 4 * wave + t;
+      return buf * kTile + ((pos >> 3) * kG + (c >> 2)) * 1024 + (pos & 7) * 128 +
+             (((2 * (c & 3)) ^ (pos & 7)) << 4);
+    };
+    const auto put = [&](int at0, int at1, const glm_u32x4 &v, uint32_t two) {
+      const float sc = e8m0_to_f32((two >> (8 * ((l >> 1) & 1))) & 0xffu);
+      *reinterpret_cast<glm_bf16x8 *>(s_kv + at0) = mxfp8_words_to_bf16x8(v[0], v[1], sc);
+      *reinterpret_cast<glm_bf16x8 *>(s_kv + at1) = mxfp8_words_to_bf16x8(v[2], v[3], sc);
+    };
+    const uint8_t *sc = raw + 4 * DK + 36 * t + 4 * (c >> 2);
+    const int at = place(t, c);
+    const glm_u32x4 v0 = *reinterpret_cast<const glm_u32x4 *>(raw + 16 * l);
+    const glm_u32x4 v1 = *reinterpret_cast<const glm_u32x4 *>(raw + 1024 + 16 * l);
+    const uint32_t s0 = *reinterpret_cast<const uint32_t *>(sc);
+    const uint32_t s1 = *reinterpret_cast<const uint32_t *>(sc + 16);
+    put(at, at ^ 16, v0, s0);
+    put(at + 4096, (at ^ 16) + 4096, v1, s1);
+    if (l < 16) {
+      const int rest = place(c >> 2, 32 + (c & 3));
+      put(rest, rest ^ 16, *reinterpret_cast<const glm_u32x4 *>(raw + 2048 + 16 * l),
+          *reinterpret_cast<const uint32_t *>(raw + 4 * DK + 36 * (c >> 2) + 32));
+    }
+  };
+  // this wave's LDS writes are done, and every wave has come here
+  const auto meet = [&]() {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(63) & ~(15 << 8));
+    ring_barrier();
+  };
+
+  int k = 0, slot = 0;  // the tile's number in the part; MXFP8: its place in the ring of codes
+  uint32_t seen0, seen1, seen2;
+  Place near, far;
+  {
+    const Place t0 = next_place(), t1 = next_place(), t2 = next_place();
+    near = next_place();
+    far = next_place();
+    const int i0 = *id_of(t0), i1 = *id_of(t1), i2 = *id_of(t2);
+    const Rows r0 = rows_of(i0, t0), r1 = rows_of(i1, t1), r2 = rows_of(i2, t2);
+    seen0 = r0.seen;
+    seen1 = r1.seen;
+    seen2 = r2.seen;
+    load_rows(r0.row, 0);
+    load_to_lds<4>(id_of(near), s_id[3]);
+    load_rows(r1.row, 1);
+    load_to_lds<4>(id_of(far), s_id[4]);
+    load_rows(r2.row, 2);
+    if constexpr (kMx) {
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * (kLoads + 1)));
+      __builtin_amdgcn_sched_barrier(0);
+      convert(0, 0);
+    }
+  }
+  // tile k is in LDS for every wave; what comes after it is on its way
+  const auto turn = [&]() {
+    // bf16: tile k has landed, and the page numbers of tile k + 3; buffer k + 3 is free
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads + 1) & ~(15 << 8));
+    ring_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    const Rows rows = rows_of(s_id[(k + 3) & 7][lane & 31], near);
+    near = far;
+    far = next_place();
+    load_to_lds<4>(id_of(far), s_id[(k + 5) & 7]);
+    load_rows(rows.row, kMx ? slot : (k + 3) & 3);
+    if constexpr (kMx) {
+      // this wave's codes of tile k + 1 have landed
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * (kLoads + 1)));
+      __builtin_amdgcn_sched_barrier(0);
+      slot = slot == 2 ? 0 : slot + 1;
+      convert(slot, (k + 1) & 1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    return rows.seen;
+  };
+
   for (AttnItem it; walk.next(a, it);) {
     const int head = it.head, r0 = it.rb * 64 + 16 * rg;
     const bool active = r0 < R;  // (uniform in a wave)
-    const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
     const int end = min(it.t1 * kAttnTile, it.len);
     const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
-
     const int r = min(r0 + n, R - 1), tok = r / group;
     glm_bf16x8 q[DK / 32];
     {
@@ -653,88 +826,17 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
                           (head * group + r - tok * group) * DK + 8 * quad;
 #pragma unroll
       for (int s = 0; s < DK / 32; ++s) q[s] = *reinterpret_cast<const glm_bf16x8 *>(p + 32 * s);
+      // (here once, or the compiler waits for them, and with them for all rows in flight, in every turn)
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     }
     glm_f32x4 acc[kD];
 #pragma unroll
     for (int d = 0; d < kD; ++d) acc[d] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, sum = 0.0f;
 
-    // Page numbers are asked for two tiles before the rows, so that waiting for them waits for no
-    // row that is still wanted in flight.  Past the end: the last position's, not seen.
-    struct Rows {
-      int row;        // lane l: of position l % 32, -1 where it is not seen
-      uint32_t seen;  // of the tile's 32
-    };
-    const auto rows_of = [&](int id, int p) {
-      int block, off;
-      page_of(a, p + (lane & 31), block, off);
-      const bool fine = (uint32_t)id < (uint32_t)a.num_pages && p + (lane & 31) < end;
-      return Rows{fine ? (id * a.kv_heads + head) * a.page + off : -1, (uint32_t)__ballot(fine)};
-    };
-    const auto block_of = [&](int p) {
-      int block, off;
-      page_of(a, min(p + (lane & 31), end - 1), block, off);
-      return block;
-    };
-    const __amdgpu_buffer_rsrc_t idrs = make_rsrc(table, (uint32_t)a.max_blocks * 4u);
-    const auto load_ids = [&](int p, int slot) {  // DIRECT: straight into LDS, every wave the same
-      buf4_to_lds(idrs, s_id[slot], 4u * block_of(p), 0);
-    };
-    const auto load_lds = [&](int rows, int buf) {  // DIRECT
-      const int row = __shfl(rows, mine, kWave);
-      const uint32_t at = row < 0 ? 0xfffff000u : (uint32_t)row * (2 * DK) + ((pc ^ tl) << 4) + 128 * g0;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        buf16_to_lds(kvrs, s_kv(buf) + (rg * kG + g0 + i) * 1024, at, 128 * i);
-    };
-    // a tile on its way to LDS through registers, sixteen threads a position
-    struct Raw {
-      glm_u32x4 v[kRaw];
-      uint32_t sc[kMx ? kRaw : 1];
-      bool fine;
-    };
-    const auto load_raw = [&](Raw &x, int rows) {
-      const int row = __shfl(rows, xt, kWave);
-      x.fine = row >= 0;
-      const long long at = max(row, 0);
-      const uint8_t *src = (const uint8_t *)a.kc + at * (16 * kPieces), *sc = a.ks + at * (DK / 32);
-#pragma unroll
-      for (int i = 0; i < kRaw; ++i) {
-        const int c = min(16 * i + xc, kPieces - 1);
-        x.v[i] = __builtin_nontemporal_load(reinterpret_cast<const glm_u32x4 *>(src + 16 * c));
-        if constexpr (kMx) x.sc[i] = sc[c >> 1];
-      }
-    };
-    const auto store_raw = [&](const Raw &x, int buf) {
-      uint8_t *row = s_kv(buf) + (xt >> 3) * kG * 1024 + (xt & 7) * 128;
-#pragma unroll
-      for (int i = 0; i < kRaw; ++i) {
-        const int c = 16 * i + xc;
-        if (c >= kPieces) continue;
-        if constexpr (kMx) {
-          const float sc = e8m0_to_f32(x.sc[i]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const glm_u32x4 o = __builtin_bit_cast(
-                glm_u32x4, mxfp8_words_to_bf16x8(x.v[i][2 * h], x.v[i][2 * h + 1], sc));
-            *reinterpret_cast<glm_u32x4 *>(row + (c >> 2) * 1024 + (((2 * (c & 3) + h) ^ (xt & 7)) << 4)) =
-                x.fine ? o : glm_u32x4{0, 0, 0, 0};
-          }
-        } else {
-          *reinterpret_cast<glm_u32x4 *>(row + (c >> 3) * 1024 + (((c & 7) ^ (xt & 7)) << 4)) =
-              x.fine ? x.v[i] : glm_u32x4{0, 0, 0, 0};
-        }
-      }
-    };
-    // this wave's LDS writes are done, and every wave has come here
-    const auto meet = [&]() {
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(63) & ~(15 << 8));
-      ring_barrier();
-    };
-
     // one tile's products, from LDS; every wave comes here with the same tile
     const auto tile = [&](int p, uint32_t seen, int buf) {
-      const uint8_t *kv = s_kv(buf);
+      const uint8_t *kv = s_kv + buf * kTile;
       const bool every = p + 32 <= all_see || a.q_len == 1;  // (uniform) all rows see the same
       const bool whole = seen == 0xffffffffu && p + 32 <= all_see;
       glm_f32x4 own = {0.f, 0.f, 0.f, 0.f};
@@ -823,10 +925,11 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         // tile's rows set to zero; the scores are done with them
         for (int t = a.q_len - 1; t >= 0; --t) {
           meet();
+          const int mine = 8 * rg + (this_lane() >> 3);  // the position of this lane's pieces in the wave's blocks
           if (p + mine >= all_see + t) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-              *reinterpret_cast<glm_u32x4 *>(s_kv(buf) + (rg * kG + g0 + i) * 1024 + 16 * lane) =
+            for (int i = 0; i < kHalf; ++i)
+              *reinterpret_cast<glm_u32x4 *>(s_kv + buf * kTile + (rg * kG + g0 + i) * 1024 + 16 * lane) =
                   glm_u32x4{0, 0, 0, 0};
           }
           meet();
@@ -843,65 +946,13 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       }
     };
 
-    const int p0 = it.t0 * kAttnTile, tiles = end > p0 ? (end - p0 + 31) / 32 : 0;
-    if (tiles > 0) {
-      uint32_t seen0, seen1, seen2;
-      const auto id_at = [&](int p) { return table[block_of(p)]; };
-      const int i0 = id_at(p0), i1 = id_at(p0 + 32), i2 = id_at(p0 + 64);
-      const Rows r0_ = rows_of(i0, p0), r1_ = rows_of(i1, p0 + 32), r2_ = rows_of(i2, p0 + 64);
-      seen0 = r0_.seen;
-      seen1 = r1_.seen;
-      seen2 = r2_.seen;
-      if constexpr (DIRECT) {
-        // tile i's rows are loaded three tiles ahead, its page numbers five; past the last tile the
-        // rows are none (zeros, no traffic), so that every turn issues the same count
-        load_lds(r0_.row, 0);
-        load_ids(p0 + 96, 3);
-        load_lds(r1_.row, 1);
-        load_ids(p0 + 128, 4);
-        load_lds(r2_.row, 2);
-        for (int i = 0; i < tiles; ++i) {
-          // tile i and the page numbers of tile i + 3 have landed; buffer i + 3 is free
-          __builtin_amdgcn_sched_barrier(0);
-          __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads + 1) & ~(15 << 8));
-          ring_barrier();
-          __builtin_amdgcn_sched_barrier(0);
-          const int p = p0 + 32 * i;
-          const Rows next = rows_of(s_id[(i + 3) & 7][lane & 31], p + 96);
-          load_ids(p + 160, (i + 5) & 7);
-          load_lds(next.row, (i + 3) & 3);
-          __builtin_amdgcn_sched_barrier(0);
-          tile(p, seen0, i & 3);
-          seen0 = seen1;
-          seen1 = seen2;
-          seen2 = next.seen;
-        }
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // nothing may land in LDS that is left
-      } else {
-        // tile i + 1 goes from registers to LDS and tile i + 3 is loaded while tile i is worked on
-        Raw x0, x1;
-        int near = id_at(p0 + 96);
-        load_raw(x0, r0_.row);
-        load_raw(x1, r1_.row);
-        store_raw(x0, 0);
-        load_raw(x0, r2_.row);
-        const auto turn = [&](int i, Raw &here) {  // (tile i + 1 is in `here`)
-          meet();
-          const int p = p0 + 32 * i;
-          store_raw(here, (i + 1) & 1);
-          const Rows next = rows_of(near, p + 96);
-          near = id_at(p + 128);
-          load_raw(here, next.row);
-          tile(p, seen0, i & 1);
-          seen0 = seen1;
-          seen1 = seen2;
-          seen2 = next.seen;
-        };
-        for (int i = 0; i < tiles; i += 2) {
-          turn(i, x1);
-          if (i + 1 < tiles) turn(i + 1, x0);
-        }
-      }
+    for (int p = it.t0 * kAttnTile; p < end; p += 32) {
+      const uint32_t seen3 = turn();
+      tile(p, seen0, k & (L::kTiles - 1));
+      seen0 = seen1;
+      seen1 = seen2;
+      seen2 = seen3;
+      ++k;
     }
 
     sum = sum_over_quads(sum);
@@ -925,8 +976,8 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         *reinterpret_cast<glm_f32x4 *>(a.part + at * DV + half * (DV / 2) + 16 * d + 4 * quad) = acc[d];
       if (half == 0 && quad == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{top, sum};
     }
-    __syncthreads();
   }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // nothing may land in LDS that is left
 }
 
 // ---------------------------------------------------------------------------
@@ -937,7 +988,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int b = blockIdx.y;
   const int2 plan = a.plan[b];
-  const int tiles = (attn_len(a, b) + kAttnTile - 1) / kAttnTile, w = kAttnOver + tiles;
+  const int tiles = (attn_len(a, b) + kAttnTile - 1) / kAttnTile, w = a.over + tiles;
   const int R = attn_rows(a), group = a.heads / a.kv_heads;
   const int i = blockIdx.x * 256 + threadIdx.x, quads = a.dv / 4;
   const int row = i / quads, ch = 4 * (i - row * quads);
@@ -945,7 +996,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int head = row / R, r = row - head * R;
   // the parts that the pair's tiles lie in; the first holds its beginning
   const int first = plan.x * a.kv_heads + head * w;
-  const int g0 = (first + kAttnOver) / plan.y, g1 = (first + w - 1) / plan.y;
+  const int g0 = (first + a.over) / plan.y, g1 = (first + w - 1) / plan.y;
   if (g0 == g1) return;
   const auto at = [&](int g) {
     return ((long long)(2 * g + (g == g0)) * a.rblocks + r / a.rows) * a.rows + r % a.rows;
@@ -979,7 +1030,7 @@ enum AttnForm { kAttnAny, kAttnGroup, kAttnLatent };
 
 struct AttnSizes {
   AttnForm form;
-  int rows, rblocks, parts, min_part;
+  int rows, rblocks, parts, min_part, over;
   unsigned grid;
   size_t plan_bytes, part_bytes, ml_bytes;
 };
@@ -1005,24 +1056,13 @@ void launch_group(hipStream_t s, dim3 grid, const glm::AttnArgs &a) {
   }
 }
 
-template <int DK, int DV, int FMT, bool DIRECT>
-int launch_latent(hipStream_t s, dim3 grid, const glm::AttnArgs &a) {
-  // tiles of 32 positions, the scores' exchange, page numbers
-  constexpr int kLds = (DIRECT ? 4 : 2) * 32 * DK * 2 + 4 * 2 * 64 * 16 + (DIRECT ? 8 * 64 * 4 : 0);
-  hipLaunchKernelGGL((glm::attn_latent_kernel<DK, DV, FMT, DIRECT>), grid, dim3(512), kLds, s, a);
-  return GLM_OK;
-}
-
 template <int FMT>
-int launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnArgs &a) {
+void launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnArgs &a) {
   if (form == kAttnAny)
     hipLaunchKernelGGL(glm::attn_any_kernel<FMT>, grid, dim3(256), 0, s, a);
-  else if (form == kAttnLatent) {
-    // direct loads where 32-bit offsets (and those past the end, from 2^32 - 4096 on) reach
-    if constexpr (FMT == GLM_FMT_BF16)
-      if (a.cache_bytes) return launch_latent<576, 512, FMT, true>(s, grid, a);
-    return launch_latent<576, 512, FMT, false>(s, grid, a);
-  }
+  else if (form == kAttnLatent)
+    hipLaunchKernelGGL((glm::attn_latent_kernel<576, 512, FMT>), grid, dim3(512),
+                       (glm::LatentLds<576, 512, FMT>::kBytes), s, a);
   else if (a.dk == 64)
     launch_group<64, 64, FMT>(s, grid, a);
   else if (a.dk == 128)
@@ -1031,7 +1071,6 @@ int launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnArg
     launch_group<192, 128, FMT>(s, grid, a);
   else
     launch_group<256, 256, FMT>(s, grid, a);
-  return GLM_OK;
 }
 
 // Sizes that follow from a call's shape; false for shapes that are refused.
@@ -1048,23 +1087,26 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
     z.form = kAttnLatent;
     z.rows = 64;
     slots = 256;
-    z.min_part = glm::kAttnOver + 1;
+    z.over = 2;
+    z.min_part = z.over + 1;
   } else if (group_widths(key_dim, value_dim)) {
     z.form = kAttnGroup;
     const int most = key_dim == 64 ? 64 : key_dim <= 192 ? 32 : 16;  // rows that fit the registers
     z.rows = R <= 16 || most == 16 ? 16 : R <= 32 || most == 32 ? 32 : 64;
     slots = 512;
-    z.min_part = glm::kAttnOver + 2;
+    z.over = 1;
+    z.min_part = z.over + 2;
   } else {
     z.form = kAttnAny;
     z.rows = 1;
     slots = 2048;
-    z.min_part = glm::kAttnOver + 4;
+    z.over = 1;
+    z.min_part = z.over + 4;
   }
   z.rblocks = (R + z.rows - 1) / z.rows;
   z.parts = slots / z.rblocks > 1 ? slots / z.rblocks : 1;
   const long long tiles = ((long long)max_blocks * page_size + glm::kAttnTile - 1) / glm::kAttnTile;
-  const long long units = (tiles + glm::kAttnOver) * B * kv_heads;
+  const long long units = (tiles + z.over) * B * kv_heads;
   if (units > INT_MAX / 2) return false;
   const long long most_parts = (units + z.min_part - 1) / z.min_part;
   if (z.parts > most_parts) z.parts = most_parts > 1 ? (int)most_parts : 1;
@@ -1154,19 +1196,19 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
   a.num_pages = num_pages;
   a.page = page_size;
   a.max_blocks = max_blocks;
-  const unsigned long long bytes = (unsigned long long)num_pages * page_size * kv_heads * key_dim * 2;
-  a.cache_bytes = bytes <= 0xffff0000ull && max_blocks <= 1 << 29 ? (uint32_t)bytes : 0;
   a.page_magic = page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / page_size);
   a.rows = z.rows;
   a.rblocks = z.rblocks;
   a.parts = z.parts;
   a.min_part = z.min_part;
+  a.over = z.over;
   a.scale_log2 = scale * glm::kLog2e;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)z.grid);
-  const int rc = mx ? launch_attention<GLM_FMT_MXFP8>(s, grid, z.form, a)
-                    : launch_attention<GLM_FMT_BF16>(s, grid, z.form, a);
-  if (rc != GLM_OK) return rc;
+  if (mx)
+    launch_attention<GLM_FMT_MXFP8>(s, grid, z.form, a);
+  else
+    launch_attention<GLM_FMT_BF16>(s, grid, z.form, a);
   GLM_LAUNCH_CHECK("paged_attention");
   if (z.parts > 1) {
     const long long quads = (long long)q_len * heads * value_dim / 4;
