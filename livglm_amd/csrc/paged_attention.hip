@@ -623,6 +623,39 @@ __device__ __forceinline__ void load_to_lds(const void *src, void *lds) {
     __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
 }
 
+// V^T operands of eight 16-channel tiles from LDS at at[i % 4] + 1024 (i / 4): the transposing reads
+// of positions 0 .. 15 and, HI bytes on, 16 .. 31, and the wait for them in one statement.  (Of the
+// builtin's reads the compiler does not know the place, and waits for every load on its way to LDS.)
+template <int HI>
+__device__ __forceinline__ void lds_read_tr8(glm_bf16x8 (&v)[8], const uint32_t (&at)[4]) {
+  bf16x4 lo[8], hi[8];
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %16\n\t"
+      "ds_read_b64_tr_b16 %8, %16 offset:%20\n\t"
+      "ds_read_b64_tr_b16 %1, %17\n\t"
+      "ds_read_b64_tr_b16 %9, %17 offset:%20\n\t"
+      "ds_read_b64_tr_b16 %2, %18\n\t"
+      "ds_read_b64_tr_b16 %10, %18 offset:%20\n\t"
+      "ds_read_b64_tr_b16 %3, %19\n\t"
+      "ds_read_b64_tr_b16 %11, %19 offset:%20\n\t"
+      "ds_read_b64_tr_b16 %4, %16 offset:1024\n\t"
+      "ds_read_b64_tr_b16 %12, %16 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %5, %17 offset:1024\n\t"
+      "ds_read_b64_tr_b16 %13, %17 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %6, %18 offset:1024\n\t"
+      "ds_read_b64_tr_b16 %14, %18 offset:%21\n\t"
+      "ds_read_b64_tr_b16 %7, %19 offset:1024\n\t"
+      "ds_read_b64_tr_b16 %15, %19 offset:%21\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(lo[4]), "=&v"(lo[5]),
+        "=&v"(lo[6]), "=&v"(lo[7]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3]),
+        "=&v"(hi[4]), "=&v"(hi[5]), "=&v"(hi[6]), "=&v"(hi[7])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "i"(HI), "i"(HI + 1024)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 template <int DK, int DV, int FMT>
 struct LatentLds {
   static constexpr bool kMx = FMT != GLM_FMT_BF16;
@@ -643,7 +676,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   constexpr bool kMx = L::kMx;
   constexpr int kG = L::kG, kTile = L::kTile;
   constexpr int kD = DV / 32;   // 16-channel tiles of a wave's half
-  constexpr int kAhead = kMx ? 6 : 8;  // operands read ahead of the products
+  constexpr int kAhead = 6;     // operands read ahead of the products
   constexpr int kLoads = kMx ? 4 : (kG + 1) / 2;  // of a wave and tile (bf16: a pair's middle block is both's)
   static_assert(!kMx || DK == 576, "36 pieces of 16 codes, 18 scales a row");
   // (one dynamic array: for reads of a static one the compiler waits for every load on its way to it)
@@ -653,17 +686,18 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   int(*const s_id)[64] = reinterpret_cast<int(*)[64]>(smem + L::kId);
   AttnWalk walk;
   if (!walk.start(a, blockIdx.x)) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
-  const int rg = wave >> 1, half = wave & 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, quad = lane >> 4, rg = wave >> 1, half = wave & 1;
   const int R = attn_rows(a), group = a.heads / a.kv_heads;
   constexpr int kHalf = (kG + 1) / 2;
   const int g0 = half ? kG - kHalf : 0;  // the wave's blocks
-  // the products' reads: position 16 half + n, piece 4 (s % 2) + quad of 64 channels s / 2
-  const int kread = (2 * half + (n >> 3)) * kG * 1024 + (n & 7) * 128 + ((quad ^ (n & 7)) << 4);
-  // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
-  const int vt = 4 * quad + (n >> 2);
-  const int vread = ((vt >> 3) * kG + half * kD / 4) * 1024 + (vt & 7) * 128 +
-                    ((((n & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (n & 1);
+  // (what follows from the lane alone is formed anew for every tile: held over the loop, it would not
+  // leave the products their registers)
+  const auto this_lane = [&]() {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    return l;
+  };
 
   // ---- the tiles of the part, one after the other: their page numbers are asked for five tiles
   // ahead and their rows three, so that waiting for page numbers waits for no row that is still
@@ -697,13 +731,6 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     page_of(a, t.p + (lane & 31), block, off);
     const bool fine = (uint32_t)id < (uint32_t)a.num_pages && t.p + (lane & 31) < t.end;
     return Rows{fine ? (id * a.kv_heads + t.head) * a.page + off : -1, (uint32_t)__ballot(fine)};
-  };
-  // (what follows from the lane alone is formed anew in every turn: held over the loop, it would not
-  // leave the products their registers)
-  const auto this_lane = [&]() {
-    int l = lane;
-    asm volatile("" : "+v"(l));
-    return l;
   };
   const auto load_rows = [&](int rows, int slot) {
     const int l = this_lane();
@@ -783,36 +810,39 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     load_rows(r1.row, 1);
     load_to_lds<4>(id_of(far), s_id[4]);
     load_rows(r2.row, 2);
-    if constexpr (kMx) {
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * (kLoads + 1)));
-      __builtin_amdgcn_sched_barrier(0);
-      convert(0, 0);
-    }
   }
-  // tile k is in LDS for every wave; what comes after it is on its way
-  const auto turn = [&]() {
-    // bf16: tile k has landed, and the page numbers of tile k + 3; buffer k + 3 is free
+  // The loads of tile k + 3, into the place of tile k - 1, and the page numbers of tile k + 5.
+  const auto issue = [&]() {
     __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads + 1) & ~(15 << 8));
-    ring_barrier();
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads + 1));  // the page numbers of tile k + 3
     __builtin_amdgcn_sched_barrier(0);
-    const Rows rows = rows_of(s_id[(k + 3) & 7][lane & 31], near);
+    const Rows rows = rows_of(s_id[(k + 3) & 7][this_lane() & 31], near);
     near = far;
     far = next_place();
     load_to_lds<4>(id_of(far), s_id[(k + 5) & 7]);
     load_rows(rows.row, kMx ? slot : (k + 3) & 3);
-    if constexpr (kMx) {
-      // this wave's codes of tile k + 1 have landed
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * (kLoads + 1)));
-      __builtin_amdgcn_sched_barrier(0);
-      slot = slot == 2 ? 0 : slot + 1;
-      convert(slot, (k + 1) & 1);
-    }
     __builtin_amdgcn_sched_barrier(0);
+    slot = slot == 2 ? 0 : slot + 1;
     return rows.seen;
   };
+  // This wave's part of tile k + 1 is in LDS: what is newer are the loads of two tiles.
+  const auto land = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * (kLoads + 1)));
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kMx) convert(slot, (k + 1) & 1);
+  };
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * (kLoads + 1)));
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (kMx) convert(0, 0);
+  meet();
+  // The four waves of rows 32 .. 63 are half a tile behind the others, so that each SIMD has a wave
+  // at the scores and one at the sums, and one's latencies hide behind the other's products.  Tile
+  // k is read in three spans between barriers, 2 k to 2 k + 2; its place is filled from span 2 k + 3
+  // on: in odd spans, by the early waves beside their sums, by the late ones beside their scores.
+  const bool late = wave >= 4;
+  if (late) meet();
 
   for (AttnItem it; walk.next(a, it);) {
     const int head = it.head, r0 = it.rb * 64 + 16 * rg;
@@ -833,126 +863,148 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < kD; ++d) acc[d] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, sum = 0.0f;
+    constexpr glm_f32x4 odd_zero = {0.f, 0.f, 0.f, 0.f};
+    glm_f32x4 own = odd_zero;
 
-    // one tile's products, from LDS; every wave comes here with the same tile
-    const auto tile = [&](int p, uint32_t seen, int buf) {
+    // one tile's scores of this wave's 16 positions, to LDS
+    const auto scores = [&](int buf) {
+      if (!active) return;
       const uint8_t *kv = s_kv + buf * kTile;
-      const bool every = p + 32 <= all_see || a.q_len == 1;  // (uniform) all rows see the same
-      const bool whole = seen == 0xffffffffu && p + 32 <= all_see;
-      glm_f32x4 own = {0.f, 0.f, 0.f, 0.f};
-      if (active) {
-        glm_f32x4 odd = {0.f, 0.f, 0.f, 0.f};
-        // a ring of operands: one pair is read when the pair kAhead before it has been multiplied
-        glm_bf16x8 k[kAhead];
-        const auto key = [&](int i) {
-          return *reinterpret_cast<const glm_bf16x8 *>(kv + (kread ^ (64 * (i & 1))) + (i >> 1) * 1024);
-        };
+      own = odd_zero;
+      glm_f32x4 odd = odd_zero;
+      // position 16 half + n, piece 4 (i % 2) + quad of 64 channels i / 2
+      const int l = this_lane();
+      const int kread = (2 * half + ((l >> 3) & 1)) * kG * 1024 + (l & 7) * 128 + (((l >> 4) ^ (l & 7)) << 4);
+      // a ring of operands: one pair is read when the pair kAhead before it has been multiplied
+      glm_bf16x8 k[kAhead];
+      const auto key = [&](int i) {
+        return *reinterpret_cast<const glm_bf16x8 *>(kv + (kread ^ (64 * (i & 1))) + (i >> 1) * 1024);
+      };
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) k[i] = key(i);
+      for (int i = 0; i < kAhead; ++i) k[i] = key(i);
 #pragma unroll
-        for (int i = 0; i < DK / 32; i += 2) {
-          __builtin_amdgcn_sched_barrier(0);
-          own = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i % kAhead], q[i], own, 0, 0, 0);
-          odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[(i + 1) % kAhead], q[i + 1], odd, 0, 0, 0);
-          if (i + kAhead < DK / 32) {
-            k[i % kAhead] = key(i + kAhead);
-            k[(i + 1) % kAhead] = key(i + 1 + kAhead);
-          }
-        }
+      for (int i = 0; i < DK / 32; i += 2) {
         __builtin_amdgcn_sched_barrier(0);
-        own += odd;
-        s_x[rg][half][lane] = own;
+        own = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i % kAhead], q[i], own, 0, 0, 0);
+        odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[(i + 1) % kAhead], q[i + 1], odd, 0, 0, 0);
+        if (i + kAhead < DK / 32) {
+          k[i % kAhead] = key(i + kAhead);
+          k[(i + 1) % kAhead] = key(i + 1 + kAhead);
+        }
       }
-      meet();
-      glm_bf16x8 prob = {};
-      if (active) {
-        const glm_f32x4 other = s_x[rg][half ^ 1][lane];
-        float x[8];
+      __builtin_amdgcn_sched_barrier(0);
+      own += odd;
+      s_x[rg][half][l] = own;
+    };
+    // with the pair's other 16: the probabilities, and this wave's half of the channels
+    const auto sums = [&](int p, uint32_t seen, int buf) {
+      if (!active) return;
+      const uint8_t *kv = s_kv + buf * kTile;
+      const glm_f32x4 other = s_x[rg][half ^ 1][this_lane()];
+      float x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = (half ? other[i] : own[i]) * a.scale_log2;
-          x[4 + i] = (half ? own[i] : other[i]) * a.scale_log2;
-        }
-        if (!whole) {
-          const uint32_t bits = seen >> (4 * quad);
-          const int left = all_see + tok - p - 4 * quad;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = 16 * (i / 4) + i % 4;
-            if (!((bits >> at) & 1u) || at >= left) x[i] = -INFINITY;
-          }
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-        const float next = fmaxf(top, max_over_quads(mx));
-        const float from = next == -INFINITY ? 0.0f : next;
-        if (__any(next != top)) {
-          const float keep = __builtin_amdgcn_exp2f(top - from);
-          sum *= keep;
-#pragma unroll
-          for (int d = 0; d < kD; ++d) acc[d] *= keep;
-        }
-        top = next;
+      for (int i = 0; i < 4; ++i) {
+        x[i] = (half ? other[i] : own[i]) * a.scale_log2;
+        x[4 + i] = (half ? own[i] : other[i]) * a.scale_log2;
+      }
+      if (seen != 0xffffffffu || p + 32 > all_see) {  // (uniform)
+        const uint32_t bits = seen >> (4 * quad);
+        const int left = all_see + tok - p - 4 * quad;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float e = __builtin_amdgcn_exp2f(x[i] - from);
-          sum += e;
-          prob[i] = (__bf16)e;  // (see attn_group_kernel)
+          const int at = 16 * (i / 4) + i % 4;
+          if (!((bits >> at) & 1u) || at >= left) x[i] = -INFINITY;
         }
       }
-      const auto values = [&](int d) {
-        const uint16_t *at = reinterpret_cast<const uint16_t *>(
-            kv + ((vread ^ (32 * (d & 3))) + (d >> 2) * 1024));
-        const bf16x4 lo = lds_read_tr(at), hi = lds_read_tr(at + 2 * kG * 512);
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      };
-      if (every) {
-        if (active) {
-          glm_bf16x8 v[kAhead];
+      float mx = x[0];
 #pragma unroll
-          for (int d = 0; d < kAhead; ++d) v[d] = values(d);
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+      const float next = fmaxf(top, max_over_quads(mx));
+      const float from = next == -INFINITY ? 0.0f : next;
+      if (__any(next != top)) {
+        const float keep = __builtin_amdgcn_exp2f(top - from);
+        sum *= keep;
+#pragma unroll
+        for (int d = 0; d < kD; ++d) acc[d] *= keep;
+      }
+      top = next;
+      // positions that only later tokens see: a value there must not meet an earlier token's zero
+      // weight (it may be an infinity or a NaN), so they stay out of the matrix product
+      const bool fringe = p + 32 > all_see && a.q_len > 1;  // (uniform)
+      const int l = this_lane(), common = fringe ? all_see - p - 4 * (l >> 4) : 32;
+      glm_bf16x8 prob;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __builtin_amdgcn_exp2f(x[i] - from);
+        sum += x[i];
+        prob[i] = 16 * (i / 4) + i % 4 < common ? (__bf16)x[i] : (__bf16)0.0f;  // (see attn_group_kernel)
+      }
+      // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
+      const int vt = 4 * (l >> 4) + ((l >> 2) & 3);
+      const int vread = ((vt >> 3) * kG + half * kD / 4) * 1024 + (vt & 7) * 128 +
+                        ((((l & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (l & 1);
+      const uint32_t kv0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)kv;
+#pragma unroll
+      for (int d = 0; d < kD; d += 8) {
+        const uint32_t from = kv0 + (d >> 2) * 1024;
+        const uint32_t at[4] = {from + vread, from + (vread ^ 32), from + (vread ^ 64), from + (vread ^ 96)};
+        glm_bf16x8 v[8];
+        lds_read_tr8<2 * kG * 1024>(v, at);
+        if (fringe) {
+          glm_u32x4 mask;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = 16 * (j / 2) + 2 * (j % 2);
+            mask[j] = (c < common ? 0xffffu : 0u) | (c + 1 < common ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            v[i] = __builtin_bit_cast(glm_bf16x8, __builtin_bit_cast(glm_u32x4, v[i]) & mask);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], prob, acc[d + i], 0, 0, 0);
+      }
+      if (fringe) {
+        // one position after the other: the rows of the tokens that see it add its weight's share
+        for (int j = max(0, all_see - p); j < min(32, it.len - p); ++j) {
+          float w = 0.0f;  // of this lane's row: quad j / 4 % 4 has it
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w = 16 * (i / 4) + i % 4 == (j & 19) ? x[i] : w;
+          w = __shfl(w, n + 16 * ((j >> 2) & 3), kWave);
+          const bool sees = p + j < all_see + tok && ((seen >> j) & 1u);
 #pragma unroll
           for (int d = 0; d < kD; ++d) {
-            __builtin_amdgcn_sched_barrier(0);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[d % kAhead], prob, acc[d], 0, 0, 0);
-            if (d + kAhead < kD) v[d % kAhead] = values(d + kAhead);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
-        // as in attn_group_kernel, a turn for each token from the last on, with ever more of the
-        // tile's rows set to zero; the scores are done with them
-        for (int t = a.q_len - 1; t >= 0; --t) {
-          meet();
-          const int mine = 8 * rg + (this_lane() >> 3);  // the position of this lane's pieces in the wave's blocks
-          if (p + mine >= all_see + t) {
-#pragma unroll
-            for (int i = 0; i < kHalf; ++i)
-              *reinterpret_cast<glm_u32x4 *>(s_kv + buf * kTile + (rg * kG + g0 + i) * 1024 + 16 * lane) =
-                  glm_u32x4{0, 0, 0, 0};
-          }
-          meet();
-          if (active) {
-#pragma unroll
-            for (int d = 0; d < kD; ++d) {
-              const glm_f32x4 with =
-                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(values(d), prob, acc[d], 0, 0, 0);
-              if (tok == t) acc[d] = with;
-              __builtin_amdgcn_sched_barrier(0);
+            // channels 16 d + 4 quad .. + 3 of the wave's half: half of a piece
+            const int c = half * kD + d, piece = 2 * c + (quad >> 1);
+            const uint2 v = *reinterpret_cast<const uint2 *>(
+                kv + ((j >> 3) * kG + (piece >> 3)) * 1024 + (j & 7) * 128 +
+                (((piece & 7) ^ (j & 7)) << 4) + 8 * (quad & 1));
+            if (sees) {
+              acc[d][0] += w * bf16_to_f32(v.x & 0xffffu);
+              acc[d][1] += w * __uint_as_float(v.x & 0xffff0000u);
+              acc[d][2] += w * bf16_to_f32(v.y & 0xffffu);
+              acc[d][3] += w * __uint_as_float(v.y & 0xffff0000u);
             }
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
     };
 
-    for (int p = it.t0 * kAttnTile; p < end; p += 32) {
-      const uint32_t seen3 = turn();
-      tile(p, seen0, k & (L::kTiles - 1));
+    for (int p = it.t0 * kAttnTile; p < end; p += 32, ++k) {
+      uint32_t seen3 = 0;
+      if (late) seen3 = issue();
+      scores(k & (L::kTiles - 1));
+      if (late) land();
+      meet();
+      if (!late) seen3 = issue();
+      sums(p, seen0, k & (L::kTiles - 1));
+      if (!late) land();
+      meet();
       seen0 = seen1;
       seen1 = seen2;
       seen2 = seen3;
-      ++k;
     }
 
     sum = sum_over_quads(sum);
@@ -977,6 +1029,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       if (half == 0 && quad == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{top, sum};
     }
   }
+  if (!late) meet();
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // nothing may land in LDS that is left
 }
 
