@@ -315,13 +315,18 @@ __device__ __forceinline__ bf16x4 lds_read_tr(const uint16_t *p) {
       bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(__attribute__((address_space(3))) void *)p));
 }
 
+// Over the four lanes n, n + 16, n + 32, n + 48, for all of them.
 __device__ __forceinline__ float max_over_quads(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16, kWave));
-  return fmaxf(x, __shfl_xor(x, 32, kWave));
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float sum_over_quads(float x) {
-  x += __shfl_xor(x, 16, kWave);
-  return x + __shfl_xor(x, 32, kWave);
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // Cache rows of the positions of two 16-position tiles, lane (n, .) position
@@ -656,17 +661,26 @@ __device__ __forceinline__ void lds_read_tr8(glm_bf16x8 (&v)[8], const uint32_t 
   for (int i = 0; i < 8; ++i) v[i] = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// At most LEFT of the wave's loads are outstanding, and nothing is moved across.
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(LEFT));
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 template <int DK, int DV, int FMT>
 struct LatentLds {
   static constexpr bool kMx = FMT != GLM_FMT_BF16;
-  static constexpr int kG = DK / 64;           // blocks of eight positions
-  static constexpr int kTile = 4 * kG * 1024;  // bytes of 32 positions
-  static constexpr int kTiles = kMx ? 2 : 4;
-  static constexpr int kRaw = kMx ? 4 * DK + 256 : 0;  // MXFP8: a wave's four rows and their scales
-  static constexpr int kX = kTiles * kTile;            // the exchanged scores
-  static constexpr int kId = kX + 4 * 2 * 64 * 16;     // page numbers of the tiles ahead
-  static constexpr int kRawAt = kId + 8 * 64 * 4;
-  static constexpr int kBytes = kRawAt + 3 * 8 * kRaw;
+  static constexpr int kG = DV / 64, kGR = (DK - DV) / 64;  // 64-channel blocks: values and keys, keys alone
+  static constexpr int kMain = 4 * kG * 1024, kRest = 4 * kGR * 1024;  // bytes of 32 positions
+  static constexpr int kMains = kMx ? 3 : 4, kRests = kMx ? 2 : 3;     // tiles
+  static constexpr int kRaw = kMx ? 4 * DK + 144 : 0;  // MXFP8: a wave's four rows and their scales
+  static constexpr int kRestAt = kMains * kMain;
+  static constexpr int kX = kRestAt + kRests * kRest;  // the exchanged scores of two tiles
+  static constexpr int kId = kX + 2 * 4 * 2 * 64 * 16;  // page numbers of the tiles ahead
+  static constexpr int kRawAt = kId + 4 * 64 * 4;
+  static constexpr int kBytes = kRawAt + 2 * 8 * kRaw;
   static_assert(kBytes <= 160 * 1024, "one workgroup a CU");
 };
 
@@ -674,23 +688,20 @@ template <int DK, int DV, int FMT>
 __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   typedef LatentLds<DK, DV, FMT> L;
   constexpr bool kMx = L::kMx;
-  constexpr int kG = L::kG, kTile = L::kTile;
-  constexpr int kD = DV / 32;   // 16-channel tiles of a wave's half
-  constexpr int kAhead = 6;     // operands read ahead of the products
-  constexpr int kLoads = kMx ? 4 : (kG + 1) / 2;  // of a wave and tile (bf16: a pair's middle block is both's)
-  static_assert(!kMx || DK == 576, "36 pieces of 16 codes, 18 scales a row");
+  constexpr int kG = L::kG;
+  constexpr int kD = DV / 32;  // 16-channel tiles of a wave's half
+  constexpr int kKeys = 6;     // operands of the scores read ahead
+  constexpr int kLoads = kMx ? 4 : 5;  // of a wave and tile (bf16: a pair's middle block is both's)
+  static_assert(DK == 576 && DV == 512, "nine blocks of 64 channels; MXFP8: 36 pieces of 16 codes, 18 scales a row");
   // (one dynamic array: for reads of a static one the compiler waits for every load on its way to it)
   extern __shared__ __align__(16) uint8_t smem[];
-  uint8_t *const s_kv = smem;
-  glm_f32x4(*const s_x)[2][64] = reinterpret_cast<glm_f32x4(*)[2][64]>(smem + L::kX);
+  glm_f32x4(*const s_x)[4][2][64] = reinterpret_cast<glm_f32x4(*)[4][2][64]>(smem + L::kX);
   int(*const s_id)[64] = reinterpret_cast<int(*)[64]>(smem + L::kId);
   AttnWalk walk;
   if (!walk.start(a, blockIdx.x)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4, rg = wave >> 1, half = wave & 1;
   const int R = attn_rows(a), group = a.heads / a.kv_heads;
-  constexpr int kHalf = (kG + 1) / 2;
-  const int g0 = half ? kG - kHalf : 0;  // the wave's blocks
   // (what follows from the lane alone is formed anew for every tile: held over the loop, it would not
   // leave the products their registers)
   const auto this_lane = [&]() {
@@ -699,9 +710,8 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     return l;
   };
 
-  // ---- the tiles of the part, one after the other: their page numbers are asked for five tiles
-  // ahead and their rows three, so that waiting for page numbers waits for no row that is still
-  // wanted in flight; past the last tile for nothing (zeros), so that every turn issues the same
+  // ---- the tiles of the part, one after the other; past the last one zeros, so that every tile's
+  // turn issues the same
   struct Place {
     int b, head, p, end;  // a tile's request, kv head, first position, end of the item
   };
@@ -732,18 +742,20 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     const bool fine = (uint32_t)id < (uint32_t)a.num_pages && t.p + (lane & 31) < t.end;
     return Rows{fine ? (id * a.kv_heads + t.head) * a.page + off : -1, (uint32_t)__ballot(fine)};
   };
-  const auto load_rows = [&](int rows, int slot) {
+  // bf16: into the tile's places `main` and `rest`; MXFP8: into the place `main` of codes
+  const auto load_rows = [&](int rows, int main, int rest) {
     const int l = this_lane();
     if constexpr (!kMx) {
-      const int row = __shfl(rows, 8 * rg + (l >> 3), kWave);
+      const int row = __shfl(rows, 8 * rg + (l >> 3), kWave), g0 = 4 * half;
       const uint8_t *src = (row < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)row * (2 * DK)) +
                            (((l & 7) ^ (l >> 3)) << 4) + 128 * g0;
+      uint8_t *to = smem + main * L::kMain + (rg * kG + g0) * 1024;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        load_to_lds<16>(src + 128 * i, s_kv + slot * kTile + (rg * kG + g0 + i) * 1024);
+      for (int i = 0; i < 4; ++i) load_to_lds<16>(src + 128 * i, to + 1024 * i);
+      load_to_lds<16>(src + 512, half ? smem + L::kRestAt + rest * L::kRest + rg * 1024 : to + 4096);
     } else {
       // four rows of 36 pieces: 16 lanes a row twice, then four lanes a row; 9 lanes a row for the scales
-      uint8_t *raw = smem + L::kRawAt + (slot * 8 + wave) * L::kRaw;
+      uint8_t *raw = smem + L::kRawAt + (main * 8 + wave) * L::kRaw;
       const auto code = [&](int t, int c) {
         const int row = __shfl(rows, 4 * wave + t, kWave);
         return (row < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)row * DK) + 16 * c;
@@ -751,103 +763,112 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       const uint8_t *src = code(l >> 4, l & 15);
       load_to_lds<16>(src, raw);
       load_to_lds<16>(src + 256, raw + 1024);
-      const uint8_t *rest = code((l & 15) >> 2, 32 + (l & 3));
+      const uint8_t *last = code((l & 15) >> 2, 32 + (l & 3));
       const int st = min(l / 9, 3), row = __shfl(rows, 4 * wave + st, kWave);
       const uint8_t *sc = (row < 0 ? attn_zero_row : a.ks + (long long)row * (DK / 32)) + 2 * (l - 9 * st);
-      if (l < 16) load_to_lds<16>(rest, raw + 2048);
+      if (l < 16) load_to_lds<16>(last, raw + 2048);
       if (l < 36) load_to_lds<2>(sc, raw + 4 * DK);
     }
   };
   // MXFP8: this wave's rows of a tile, from codes to bf16: piece c of row t to the tile's pieces 2 c,
   // 2 c + 1 (the swizzle keeps them neighbours)
-  const auto convert = [&](int slot, int buf) {
+  const auto convert = [&](int from, int main, int rest) {
     const int l = this_lane(), t = l >> 4, c = l & 15;
-    const uint8_t *raw = smem + L::kRawAt + (slot * 8 + wave) * L::kRaw;
-    const auto place = [&](int t, int c) {
-      const int pos = 4 * wave + t;
-      return buf * kTile + ((pos >> 3) * kG + (c >> 2)) * 1024 + (pos & 7) * 128 +
-             (((2 * (c & 3)) ^ (pos & 7)) << 4);
+    const uint8_t *raw = smem + L::kRawAt + (from * 8 + wave) * L::kRaw;
+    const auto swizzled = [&](int pos, int c) {
+      return (pos & 7) * 128 + (((2 * (c & 3)) ^ (pos & 7)) << 4);
     };
-    const auto put = [&](int at0, int at1, const glm_u32x4 &v, uint32_t two) {
+    const auto put = [&](uint8_t *tile, int at, const glm_u32x4 &v, uint32_t two) {
       const float sc = e8m0_to_f32((two >> (8 * ((l >> 1) & 1))) & 0xffu);
-      *reinterpret_cast<glm_bf16x8 *>(s_kv + at0) = mxfp8_words_to_bf16x8(v[0], v[1], sc);
-      *reinterpret_cast<glm_bf16x8 *>(s_kv + at1) = mxfp8_words_to_bf16x8(v[2], v[3], sc);
+      *reinterpret_cast<glm_bf16x8 *>(tile + at) = mxfp8_words_to_bf16x8(v[0], v[1], sc);
+      *reinterpret_cast<glm_bf16x8 *>(tile + (at ^ 16)) = mxfp8_words_to_bf16x8(v[2], v[3], sc);
     };
     const uint8_t *sc = raw + 4 * DK + 36 * t + 4 * (c >> 2);
-    const int at = place(t, c);
     const glm_u32x4 v0 = *reinterpret_cast<const glm_u32x4 *>(raw + 16 * l);
     const glm_u32x4 v1 = *reinterpret_cast<const glm_u32x4 *>(raw + 1024 + 16 * l);
     const uint32_t s0 = *reinterpret_cast<const uint32_t *>(sc);
     const uint32_t s1 = *reinterpret_cast<const uint32_t *>(sc + 16);
-    put(at, at ^ 16, v0, s0);
-    put(at + 4096, (at ^ 16) + 4096, v1, s1);
-    if (l < 16) {
-      const int rest = place(c >> 2, 32 + (c & 3));
-      put(rest, rest ^ 16, *reinterpret_cast<const glm_u32x4 *>(raw + 2048 + 16 * l),
+    // (a wave's four positions lie in one block of eight)
+    uint8_t *tile = smem + main * L::kMain + ((wave >> 1) * kG + (c >> 2)) * 1024;
+    put(tile, swizzled(4 * wave + t, c), v0, s0);
+    put(tile + 4096, swizzled(4 * wave + t, c), v1, s1);
+    if (l < 16)
+      put(smem + L::kRestAt + rest * L::kRest + (wave >> 1) * 1024, swizzled(4 * wave + (c >> 2), c & 3),
+          *reinterpret_cast<const glm_u32x4 *>(raw + 2048 + 16 * l),
           *reinterpret_cast<const uint32_t *>(raw + 4 * DK + 36 * (c >> 2) + 32));
-    }
   };
   // this wave's LDS writes are done, and every wave has come here
   const auto meet = [&]() {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(63) & ~(15 << 8));
     ring_barrier();
   };
+  constexpr int kTwoTiles = 2 * kLoads + 1, kOneTile = kLoads + 1;  // loads, with the page numbers between
 
-  int k = 0, slot = 0;  // the tile's number in the part; MXFP8: its place in the ring of codes
-  uint32_t seen0, seen1, seen2;
+  // Tile k's turn multiplies its values, and tile k + 1's keys for the next.  Page numbers are asked for
+  // two turns before the rows that they name, so that waiting for them waits for no row that is still
+  // wanted in flight.
+  //   bf16   turn k loads tile k + 3, into the place of tile k - 1, and ends when tile k + 2 has landed
+  //   MXFP8  turn k converts tile k + 2, loads the codes of tile k + 4 into its place
+  constexpr int kAhead = kMx ? 4 : 3;
+  int k = 0;
+  int main_k = 0, rest_k = 1 % L::kRests;  // tile k's place among the mains, tile k + 1's among the rests
+  const auto plus = [](int at, int by, int ring) { return at + by >= ring ? at + by - ring : at + by; };
+  uint32_t seen[kAhead];  // of tiles k, k + 1, ..
   Place near, far;
   {
-    const Place t0 = next_place(), t1 = next_place(), t2 = next_place();
+    Place t[kAhead];
+    int id[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) t[i] = next_place();
     near = next_place();
     far = next_place();
-    const int i0 = *id_of(t0), i1 = *id_of(t1), i2 = *id_of(t2);
-    const Rows r0 = rows_of(i0, t0), r1 = rows_of(i1, t1), r2 = rows_of(i2, t2);
-    seen0 = r0.seen;
-    seen1 = r1.seen;
-    seen2 = r2.seen;
-    load_rows(r0.row, 0);
-    load_to_lds<4>(id_of(near), s_id[3]);
-    load_rows(r1.row, 1);
-    load_to_lds<4>(id_of(far), s_id[4]);
-    load_rows(r2.row, 2);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) id[i] = *id_of(t[i]);
+    int row[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const Rows r = rows_of(id[i], t[i]);
+      row[i] = r.row;
+      seen[i] = r.seen;
+    }
+    load_rows(row[0], 0, 0);
+    if constexpr (kMx) {
+      load_rows(row[1], 1, 0);
+      wait_loads<kLoads>();
+      convert(0, 0, 0);
+      load_to_lds<4>(id_of(near), s_id[0]);
+      load_rows(row[2], 0, 0);
+      wait_loads<kOneTile>();
+      convert(1, 1, 1);
+      load_to_lds<4>(id_of(far), s_id[1]);
+      load_rows(row[kAhead - 1], 1, 0);
+    } else {
+      load_to_lds<4>(id_of(near), s_id[3]);
+      load_rows(row[1], 1, 1);
+      load_to_lds<4>(id_of(far), s_id[0]);
+      load_rows(row[2], 2, 2);
+      wait_loads<kOneTile>();
+    }
   }
-  // The loads of tile k + 3, into the place of tile k - 1, and the page numbers of tile k + 5.
+  meet();
+  // the loads of tile k + kAhead, and the page numbers of tile k + kAhead + 2
   const auto issue = [&]() {
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads + 1));  // the page numbers of tile k + 3
-    __builtin_amdgcn_sched_barrier(0);
-    const Rows rows = rows_of(s_id[(k + 3) & 7][this_lane() & 31], near);
+    const Rows rows = rows_of(s_id[(k + kAhead) & 3][this_lane() & 31], near);
     near = far;
     far = next_place();
-    load_to_lds<4>(id_of(far), s_id[(k + 5) & 7]);
-    load_rows(rows.row, kMx ? slot : (k + 3) & 3);
+    load_to_lds<4>(id_of(far), s_id[(k + kAhead + 2) & 3]);
+    if constexpr (kMx)
+      load_rows(rows.row, k & 1, 0);
+    else
+      load_rows(rows.row, plus(main_k, 3, 4), plus(rest_k, 2, 3));
     __builtin_amdgcn_sched_barrier(0);
-    slot = slot == 2 ? 0 : slot + 1;
     return rows.seen;
   };
-  // This wave's part of tile k + 1 is in LDS: what is newer are the loads of two tiles.
-  const auto land = [&]() {
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * (kLoads + 1)));
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (kMx) convert(slot, (k + 1) & 1);
-  };
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * (kLoads + 1)));
-  __builtin_amdgcn_sched_barrier(0);
-  if constexpr (kMx) convert(0, 0);
-  meet();
-  // The four waves of rows 32 .. 63 are half a tile behind the others, so that each SIMD has a wave
-  // at the scores and one at the sums, and one's latencies hide behind the other's products.  Tile
-  // k is read in three spans between barriers, 2 k to 2 k + 2; its place is filled from span 2 k + 3
-  // on: in odd spans, by the early waves beside their sums, by the late ones beside their scores.
-  const bool late = wave >= 4;
-  if (late) meet();
 
   for (AttnItem it; walk.next(a, it);) {
     const int head = it.head, r0 = it.rb * 64 + 16 * rg;
     const bool active = r0 < R;  // (uniform in a wave)
-    const int end = min(it.t1 * kAttnTile, it.len);
+    const int begin = it.t0 * kAttnTile, end = min(it.t1 * kAttnTile, it.len);
     const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
     const int r = min(r0 + n, R - 1), tok = r / group;
     glm_bf16x8 q[DK / 32];
@@ -859,152 +880,167 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       // (here once, or the compiler waits for them, and with them for all rows in flight, in every turn)
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     }
-    glm_f32x4 acc[kD];
+    constexpr glm_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    glm_f32x4 acc[kD], own = zero;  // own: this wave's scores, of 16 positions of the tile to come
 #pragma unroll
-    for (int d = 0; d < kD; ++d) acc[d] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < kD; ++d) acc[d] = zero;
     float top = -INFINITY, sum = 0.0f;
-    constexpr glm_f32x4 odd_zero = {0.f, 0.f, 0.f, 0.f};
-    glm_f32x4 own = odd_zero;
 
-    // one tile's scores of this wave's 16 positions, to LDS
-    const auto scores = [&](int buf) {
-      if (!active) return;
-      const uint8_t *kv = s_kv + buf * kTile;
-      own = odd_zero;
-      glm_f32x4 odd = odd_zero;
+    // this wave's scores of tile k + 1 (its places: main, rest)
+    const auto scores = [&](int main, int rest) {
       // position 16 half + n, piece 4 (i % 2) + quad of 64 channels i / 2
-      const int l = this_lane();
-      const int kread = (2 * half + ((l >> 3) & 1)) * kG * 1024 + (l & 7) * 128 + (((l >> 4) ^ (l & 7)) << 4);
-      // a ring of operands: one pair is read when the pair kAhead before it has been multiplied
-      glm_bf16x8 k[kAhead];
+      const int l = this_lane(), pos = 2 * half + ((l >> 3) & 1);
+      const int at = (l & 7) * 128 + (((l >> 4) ^ (l & 7)) << 4);
+      const uint8_t *km = smem + main * L::kMain + pos * kG * 1024 + at;
+      const uint8_t *km1 = smem + main * L::kMain + pos * kG * 1024 + (at ^ 64);
+      const uint8_t *kr = smem + L::kRestAt + rest * L::kRest + pos * 1024;
       const auto key = [&](int i) {
-        return *reinterpret_cast<const glm_bf16x8 *>(kv + (kread ^ (64 * (i & 1))) + (i >> 1) * 1024);
+        const uint8_t *from = i < DV / 32 ? (i & 1 ? km1 : km) + (i >> 1) * 1024 : kr + (at ^ (64 * (i & 1)));
+        return *reinterpret_cast<const glm_bf16x8 *>(from);
       };
+      glm_f32x4 even = zero, odd = zero;
+      // a ring of operands: one pair is read when the pair kKeys before it has been multiplied
+      glm_bf16x8 kf[kKeys];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) k[i] = key(i);
+      for (int i = 0; i < kKeys; ++i) kf[i] = key(i);
 #pragma unroll
       for (int i = 0; i < DK / 32; i += 2) {
-        __builtin_amdgcn_sched_barrier(0);
-        own = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i % kAhead], q[i], own, 0, 0, 0);
-        odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[(i + 1) % kAhead], q[i + 1], odd, 0, 0, 0);
-        if (i + kAhead < DK / 32) {
-          k[i % kAhead] = key(i + kAhead);
-          k[(i + 1) % kAhead] = key(i + 1 + kAhead);
+        even = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i % kKeys], q[i], even, 0, 0, 0);
+        odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[(i + 1) % kKeys], q[i + 1], odd, 0, 0, 0);
+        if (i + kKeys < DK / 32) {
+          kf[i % kKeys] = key(i + kKeys);
+          kf[(i + 1) % kKeys] = key(i + 1 + kKeys);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
-      own += odd;
-      s_x[rg][half][l] = own;
+      return even + odd;
     };
-    // with the pair's other 16: the probabilities, and this wave's half of the channels
-    const auto sums = [&](int p, uint32_t seen, int buf) {
-      if (!active) return;
-      const uint8_t *kv = s_kv + buf * kTile;
-      const glm_f32x4 other = s_x[rg][half ^ 1][this_lane()];
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = (half ? other[i] : own[i]) * a.scale_log2;
-        x[4 + i] = (half ? own[i] : other[i]) * a.scale_log2;
+
+    if (begin < end) {  // the first tile's scores
+      if (active) {
+        own = scores(main_k, plus(rest_k, L::kRests - 1, L::kRests));
+        s_x[k & 1][rg][half][lane] = own;
       }
-      if (seen != 0xffffffffu || p + 32 > all_see) {  // (uniform)
-        const uint32_t bits = seen >> (4 * quad);
-        const int left = all_see + tok - p - 4 * quad;
+      meet();
+    }
+    for (int p = begin; p < end; p += 32, ++k) {
+      uint32_t last_seen = 0;
+      if constexpr (!kMx) {
+        wait_loads<kTwoTiles>();  // the page numbers of tile k + 3
+        last_seen = issue();
+      }
+      if (active) {
+        const int l0 = this_lane();
+        const glm_f32x4 other = s_x[k & 1][rg][half ^ 1][l0];
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int at = 16 * (i / 4) + i % 4;
-          if (!((bits >> at) & 1u) || at >= left) x[i] = -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+          x[i] = (half ? other[i] : own[i]) * a.scale_log2;
+          x[4 + i] = (half ? own[i] : other[i]) * a.scale_log2;
         }
-      }
-      float mx = x[0];
+        if (seen[0] != 0xffffffffu || p + 32 > all_see) {  // (uniform)
+          const uint32_t bits = seen[0] >> (4 * quad);
+          const int left = all_see + tok - p - 4 * quad;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-      const float next = fmaxf(top, max_over_quads(mx));
-      const float from = next == -INFINITY ? 0.0f : next;
-      if (__any(next != top)) {
+          for (int i = 0; i < 8; ++i) {
+            const int at = 16 * (i / 4) + i % 4;
+            if (!((bits >> at) & 1u) || at >= left) x[i] = -INFINITY;
+          }
+        }
+        // positions that only later tokens see: a value there must not meet an earlier token's zero
+        // weight (it may be an infinity or a NaN), so they stay out of the matrix product
+        const bool fringe = p + 32 > all_see && a.q_len > 1;  // (uniform)
+        // the next tile's scores beside this one's probabilities (past the item's end: of whatever
+        // tile follows, and not used)
+        const glm_f32x4 next_own = scores(plus(main_k, 1, L::kMains), rest_k);
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+        const float next = fmaxf(top, max_over_quads(mx));
+        const float from = next == -INFINITY ? 0.0f : next;
         const float keep = __builtin_amdgcn_exp2f(top - from);
+        const int l = this_lane(), common = fringe ? all_see - p - 4 * (l >> 4) : 32;
+        glm_bf16x8 prob;
         sum *= keep;
 #pragma unroll
-        for (int d = 0; d < kD; ++d) acc[d] *= keep;
-      }
-      top = next;
-      // positions that only later tokens see: a value there must not meet an earlier token's zero
-      // weight (it may be an infinity or a NaN), so they stay out of the matrix product
-      const bool fringe = p + 32 > all_see && a.q_len > 1;  // (uniform)
-      const int l = this_lane(), common = fringe ? all_see - p - 4 * (l >> 4) : 32;
-      glm_bf16x8 prob;
+        for (int i = 0; i < 8; ++i) {
+          x[i] = __builtin_amdgcn_exp2f(x[i] - from);
+          sum += x[i];
+          prob[i] = 16 * (i / 4) + i % 4 < common ? (__bf16)x[i] : (__bf16)0.0f;  // (see attn_group_kernel)
+        }
+        own = next_own;
+        s_x[(k + 1) & 1][rg][half][l] = own;
+        if (__any(next != top)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - from);
-        sum += x[i];
-        prob[i] = 16 * (i / 4) + i % 4 < common ? (__bf16)x[i] : (__bf16)0.0f;  // (see attn_group_kernel)
-      }
-      // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
-      const int vt = 4 * (l >> 4) + ((l >> 2) & 3);
-      const int vread = ((vt >> 3) * kG + half * kD / 4) * 1024 + (vt & 7) * 128 +
-                        ((((l & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (l & 1);
-      const uint32_t kv0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)kv;
+          for (int d = 0; d < kD; ++d) acc[d] *= keep;
+        }
+        top = next;
+        // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
+        const uint8_t *kv = smem + main_k * L::kMain;
+        const int vt = 4 * (l >> 4) + ((l >> 2) & 3);
+        const int vread = ((vt >> 3) * kG + half * kD / 4) * 1024 + (vt & 7) * 128 +
+                          ((((l & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (l & 1);
+        const uint32_t kv0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)kv;
 #pragma unroll
-      for (int d = 0; d < kD; d += 8) {
-        const uint32_t from = kv0 + (d >> 2) * 1024;
-        const uint32_t at[4] = {from + vread, from + (vread ^ 32), from + (vread ^ 64), from + (vread ^ 96)};
-        glm_bf16x8 v[8];
-        lds_read_tr8<2 * kG * 1024>(v, at);
-        if (fringe) {
-          glm_u32x4 mask;
+        for (int d = 0; d < kD; d += 8) {
+          const uint32_t from = kv0 + (d >> 2) * 1024;
+          const uint32_t at[4] = {from + vread, from + (vread ^ 32), from + (vread ^ 64), from + (vread ^ 96)};
+          glm_bf16x8 v[8];
+          lds_read_tr8<2 * kG * 1024>(v, at);
+          if (fringe) {
+            glm_u32x4 mask;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int c = 16 * (j / 2) + 2 * (j % 2);
-            mask[j] = (c < common ? 0xffffu : 0u) | (c + 1 < common ? 0xffff0000u : 0u);
+            for (int j = 0; j < 4; ++j) {
+              const int c = 16 * (j / 2) + 2 * (j % 2);
+              mask[j] = (c < common ? 0xffffu : 0u) | (c + 1 < common ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              v[i] = __builtin_bit_cast(glm_bf16x8, __builtin_bit_cast(glm_u32x4, v[i]) & mask);
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            v[i] = __builtin_bit_cast(glm_bf16x8, __builtin_bit_cast(glm_u32x4, v[i]) & mask);
+            acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], prob, acc[d + i], 0, 0, 0);
         }
+        if (fringe) {
+          // one position after the other: the rows of the tokens that see it add its weight's share
+          for (int j = max(0, all_see - p); j < min(32, it.len - p); ++j) {
+            float w = 0.0f;  // of this lane's row: quad j / 4 % 4 has it
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], prob, acc[d + i], 0, 0, 0);
-      }
-      if (fringe) {
-        // one position after the other: the rows of the tokens that see it add its weight's share
-        for (int j = max(0, all_see - p); j < min(32, it.len - p); ++j) {
-          float w = 0.0f;  // of this lane's row: quad j / 4 % 4 has it
+            for (int i = 0; i < 8; ++i) w = 16 * (i / 4) + i % 4 == (j & 19) ? x[i] : w;
+            w = __shfl(w, n + 16 * ((j >> 2) & 3), kWave);
+            const bool sees = p + j < all_see + tok && ((seen[0] >> j) & 1u);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w = 16 * (i / 4) + i % 4 == (j & 19) ? x[i] : w;
-          w = __shfl(w, n + 16 * ((j >> 2) & 3), kWave);
-          const bool sees = p + j < all_see + tok && ((seen >> j) & 1u);
-#pragma unroll
-          for (int d = 0; d < kD; ++d) {
-            // channels 16 d + 4 quad .. + 3 of the wave's half: half of a piece
-            const int c = half * kD + d, piece = 2 * c + (quad >> 1);
-            const uint2 v = *reinterpret_cast<const uint2 *>(
-                kv + ((j >> 3) * kG + (piece >> 3)) * 1024 + (j & 7) * 128 +
-                (((piece & 7) ^ (j & 7)) << 4) + 8 * (quad & 1));
-            if (sees) {
-              acc[d][0] += w * bf16_to_f32(v.x & 0xffffu);
-              acc[d][1] += w * __uint_as_float(v.x & 0xffff0000u);
-              acc[d][2] += w * bf16_to_f32(v.y & 0xffffu);
-              acc[d][3] += w * __uint_as_float(v.y & 0xffff0000u);
+            for (int d = 0; d < kD; ++d) {
+              // channels 16 d + 4 quad .. + 3 of the wave's half: half of a piece
+              const int c = half * kD + d, piece = 2 * c + (quad >> 1);
+              const uint2 v = *reinterpret_cast<const uint2 *>(
+                  kv + ((j >> 3) * kG + (piece >> 3)) * 1024 + (j & 7) * 128 +
+                  (((piece & 7) ^ (j & 7)) << 4) + 8 * (quad & 1));
+              if (sees) {
+                acc[d][0] += w * bf16_to_f32(v.x & 0xffffu);
+                acc[d][1] += w * __uint_as_float(v.x & 0xffff0000u);
+                acc[d][2] += w * bf16_to_f32(v.y & 0xffffu);
+                acc[d][3] += w * __uint_as_float(v.y & 0xffff0000u);
+              }
+              __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
-    };
-
-    for (int p = it.t0 * kAttnTile; p < end; p += 32, ++k) {
-      uint32_t seen3 = 0;
-      if (late) seen3 = issue();
-      scores(k & (L::kTiles - 1));
-      if (late) land();
+      if constexpr (kMx) {
+        wait_loads<kOneTile>();  // the codes of tile k + 2, the page numbers of tile k + 4
+        convert(k & 1, plus(main_k, 2, 3), rest_k ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+        last_seen = issue();
+      } else {
+        wait_loads<kOneTile>();  // tile k + 2
+      }
       meet();
-      if (!late) seen3 = issue();
-      sums(p, seen0, k & (L::kTiles - 1));
-      if (!late) land();
-      meet();
-      seen0 = seen1;
-      seen1 = seen2;
-      seen2 = seen3;
+      main_k = plus(main_k, 1, L::kMains);
+      rest_k = plus(rest_k, 1, L::kRests);
+#pragma unroll
+      for (int i = 0; i + 1 < kAhead; ++i) seen[i] = seen[i + 1];
+      seen[kAhead - 1] = last_seen;
     }
 
     sum = sum_over_quads(sum);
@@ -1029,7 +1065,6 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       if (half == 0 && quad == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{top, sum};
     }
   }
-  if (!late) meet();
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // nothing may land in LDS that is left
 }
 
