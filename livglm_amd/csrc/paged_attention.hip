@@ -678,8 +678,10 @@ struct LatentLds {
   static constexpr int kRaw = kMx ? 4 * DK + 144 : 0;  // MXFP8: a wave's four rows and their scales
   static constexpr int kRestAt = kMains * kMain;
   static constexpr int kX = kRestAt + kRests * kRest;  // the exchanged scores of two tiles
-  static constexpr int kId = kX + 2 * 4 * 2 * 64 * 16;  // page numbers of the tiles ahead
-  static constexpr int kRawAt = kId + 4 * 64 * 4;
+  static constexpr int kId = kX + 2 * 4 * 2 * 64 * 16;  // page numbers of four tiles
+  static constexpr int kRow = kId + 4 * 32 * 4;         // cache rows of two times four tiles
+  static constexpr int kSeen = kRow + 2 * 4 * 32 * 4;   // which of them are seen
+  static constexpr int kRawAt = kSeen + 2 * 4 * 4;
   static constexpr int kBytes = kRawAt + 2 * 8 * kRaw;
   static_assert(kBytes <= 160 * 1024, "one workgroup a CU");
 };
@@ -696,7 +698,9 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   // (one dynamic array: for reads of a static one the compiler waits for every load on its way to it)
   extern __shared__ __align__(16) uint8_t smem[];
   glm_f32x4(*const s_x)[4][2][64] = reinterpret_cast<glm_f32x4(*)[4][2][64]>(smem + L::kX);
-  int(*const s_id)[64] = reinterpret_cast<int(*)[64]>(smem + L::kId);
+  int *const s_id = reinterpret_cast<int *>(smem + L::kId);
+  int(*const s_row)[4][32] = reinterpret_cast<int(*)[4][32]>(smem + L::kRow);
+  uint32_t(*const s_seen)[4] = reinterpret_cast<uint32_t(*)[4]>(smem + L::kSeen);
   AttnWalk walk;
   if (!walk.start(a, blockIdx.x)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -710,8 +714,8 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     return l;
   };
 
-  // ---- the tiles of the part, one after the other; past the last one zeros, so that every tile's
-  // turn issues the same
+  // ---- the tiles of the part, one after the other, and past the last one zeros, so that every tile's
+  // turn issues the same.  Four tiles' cache rows are found at once, by two waves.
   struct Place {
     int b, head, p, end;  // a tile's request, kv head, first position, end of the item
   };
@@ -727,26 +731,33 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     place.p += 32;
     return now;
   };
-  const auto id_of = [&](const Place &t) {
+  // wave w < 2, lane l: position l % 32 of tile 2 w + l / 32 of the next four: its entry of the block
+  // table, and its row within the page (-1: not seen)
+  int within = -1;
+  const auto entry = [&]() {
+    Place t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = next_place();
+    const Place t0 = wave & 1 ? t[2] : t[0], t1 = wave & 1 ? t[3] : t[1];
+    const bool up = lane >= 32;
+    const int pos = (up ? t1.p : t0.p) + (lane & 31), end = up ? t1.end : t0.end;
     int block, off;
-    page_of(a, max(0, min(t.p + (lane & 31), t.end - 1)), block, off);
-    return a.tables + (long long)t.b * a.max_blocks + block;
+    page_of(a, max(0, min(pos, end - 1)), block, off);
+    within = pos < end ? (up ? t1.head : t0.head) * a.page + off : -1;
+    return a.tables + (long long)(up ? t1.b : t0.b) * a.max_blocks + block;
   };
-  struct Rows {
-    int row;        // lane l: of position l % 32, -1 where it is not seen
-    uint32_t seen;  // of the tile's 32
-  };
-  const auto rows_of = [&](int id, const Place &t) {
-    int block, off;
-    page_of(a, t.p + (lane & 31), block, off);
-    const bool fine = (uint32_t)id < (uint32_t)a.num_pages && t.p + (lane & 31) < t.end;
-    return Rows{fine ? (id * a.kv_heads + t.head) * a.page + off : -1, (uint32_t)__ballot(fine)};
+  const auto put_rows = [&](int id, int slot) {
+    const bool fine = (uint32_t)id < (uint32_t)a.num_pages && within >= 0;
+    (&s_row[slot][0][0])[64 * (wave & 1) + lane] = fine ? id * a.kv_heads * a.page + within : -1;
+    const unsigned long long seen = __ballot(fine);
+    if ((lane & 31) == 0) s_seen[slot][2 * (wave & 1) + (lane >> 5)] = (uint32_t)(seen >> (lane & 32));
   };
   // bf16: into the tile's places `main` and `rest`; MXFP8: into the place `main` of codes
-  const auto load_rows = [&](int rows, int main, int rest) {
+  const auto load_rows = [&](int tile, int main, int rest) {
     const int l = this_lane();
+    const int *rows = s_row[(tile >> 2) & 1][tile & 3];
     if constexpr (!kMx) {
-      const int row = __shfl(rows, 8 * rg + (l >> 3), kWave), g0 = 4 * half;
+      const int row = rows[8 * rg + (l >> 3)], g0 = 4 * half;
       const uint8_t *src = (row < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)row * (2 * DK)) +
                            (((l & 7) ^ (l >> 3)) << 4) + 128 * g0;
       uint8_t *to = smem + main * L::kMain + (rg * kG + g0) * 1024;
@@ -757,14 +768,14 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       // four rows of 36 pieces: 16 lanes a row twice, then four lanes a row; 9 lanes a row for the scales
       uint8_t *raw = smem + L::kRawAt + (main * 8 + wave) * L::kRaw;
       const auto code = [&](int t, int c) {
-        const int row = __shfl(rows, 4 * wave + t, kWave);
+        const int row = rows[4 * wave + t];
         return (row < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)row * DK) + 16 * c;
       };
       const uint8_t *src = code(l >> 4, l & 15);
       load_to_lds<16>(src, raw);
       load_to_lds<16>(src + 256, raw + 1024);
       const uint8_t *last = code((l & 15) >> 2, 32 + (l & 3));
-      const int st = min(l / 9, 3), row = __shfl(rows, 4 * wave + st, kWave);
+      const int st = min(l / 9, 3), row = rows[4 * wave + st];
       const uint8_t *sc = (row < 0 ? attn_zero_row : a.ks + (long long)row * (DK / 32)) + 2 * (l - 9 * st);
       if (l < 16) load_to_lds<16>(last, raw + 2048);
       if (l < 36) load_to_lds<2>(sc, raw + 4 * DK);
@@ -802,67 +813,43 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(63) & ~(15 << 8));
     ring_barrier();
   };
-  constexpr int kTwoTiles = 2 * kLoads + 1, kOneTile = kLoads + 1;  // loads, with the page numbers between
-
-  // Tile k's turn multiplies its values, and tile k + 1's keys for the next.  Page numbers are asked for
-  // two turns before the rows that they name, so that waiting for them waits for no row that is still
-  // wanted in flight.
+  // Tile k's turn multiplies its values, and tile k + 1's keys for the next.
   //   bf16   turn k loads tile k + 3, into the place of tile k - 1, and ends when tile k + 2 has landed
-  //   MXFP8  turn k converts tile k + 2, loads the codes of tile k + 4 into its place
+  //   MXFP8  turn k converts tile k + 2 and loads the codes of tile k + 4 into its place
+  // Turn 4 c asks for the page numbers of tiles 4 c + 8 .. + 11, turn 4 c + 3 finds their rows.
   constexpr int kAhead = kMx ? 4 : 3;
   int k = 0;
   int main_k = 0, rest_k = 1 % L::kRests;  // tile k's place among the mains, tile k + 1's among the rests
   const auto plus = [](int at, int by, int ring) { return at + by >= ring ? at + by - ring : at + by; };
   uint32_t seen[kAhead];  // of tiles k, k + 1, ..
-  Place near, far;
-  {
-    Place t[kAhead];
-    int id[kAhead];
+  const auto seen_of = [&](int tile) {
+    return (uint32_t)__builtin_amdgcn_readfirstlane(s_seen[(tile >> 2) & 1][tile & 3]);
+  };
+  if (wave < 2) {
+    const int32_t *first = entry();
+    put_rows(*first, 0);
+    const int32_t *second = entry();
+    put_rows(*second, 1);
+  }
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) t[i] = next_place();
-    near = next_place();
-    far = next_place();
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) id[i] = *id_of(t[i]);
-    int row[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const Rows r = rows_of(id[i], t[i]);
-      row[i] = r.row;
-      seen[i] = r.seen;
-    }
-    load_rows(row[0], 0, 0);
-    if constexpr (kMx) {
-      load_rows(row[1], 1, 0);
-      wait_loads<kLoads>();
-      convert(0, 0, 0);
-      load_to_lds<4>(id_of(near), s_id[0]);
-      load_rows(row[2], 0, 0);
-      wait_loads<kOneTile>();
-      convert(1, 1, 1);
-      load_to_lds<4>(id_of(far), s_id[1]);
-      load_rows(row[kAhead - 1], 1, 0);
-    } else {
-      load_to_lds<4>(id_of(near), s_id[3]);
-      load_rows(row[1], 1, 1);
-      load_to_lds<4>(id_of(far), s_id[0]);
-      load_rows(row[2], 2, 2);
-      wait_loads<kOneTile>();
-    }
+  for (int i = 0; i < kAhead; ++i) seen[i] = seen_of(i);
+  load_rows(0, 0, 0);
+  load_rows(1, 1, 1);
+  if constexpr (kMx) {
+    wait_loads<kLoads>();
+    convert(0, 0, 0);
+    load_rows(2, 0, 0);
+    wait_loads<kLoads>();
+    convert(1, 1, 1);
+    load_rows(3, 1, 0);
+  } else {
+    load_rows(2, 2, 2);
+    wait_loads<kLoads>();
   }
   meet();
-  // the loads of tile k + kAhead, and the page numbers of tile k + kAhead + 2
-  const auto issue = [&]() {
-    const Rows rows = rows_of(s_id[(k + kAhead) & 3][this_lane() & 31], near);
-    near = far;
-    far = next_place();
-    load_to_lds<4>(id_of(far), s_id[(k + kAhead + 2) & 3]);
-    if constexpr (kMx)
-      load_rows(rows.row, k & 1, 0);
-    else
-      load_rows(rows.row, plus(main_k, 3, 4), plus(rest_k, 2, 3));
-    __builtin_amdgcn_sched_barrier(0);
-    return rows.seen;
+  const auto load_ids = [&]() {
+    if ((k & 3) == 0 && wave < 2) load_to_lds<4>(entry(), s_id + 64 * wave);
   };
 
   for (AttnItem it; walk.next(a, it);) {
@@ -923,11 +910,12 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       meet();
     }
     for (int p = begin; p < end; p += 32, ++k) {
-      uint32_t last_seen = 0;
+      const uint32_t last_seen = seen_of(k + kAhead);
       if constexpr (!kMx) {
-        wait_loads<kTwoTiles>();  // the page numbers of tile k + 3
-        last_seen = issue();
+        load_rows(k + 3, plus(main_k, 3, 4), plus(rest_k, 2, 3));
+        __builtin_amdgcn_sched_barrier(0);
       }
+      if ((k & 3) == 3 && wave < 2) put_rows(s_id[64 * wave + this_lane()], ((k >> 2) + 2) & 1);
       if (active) {
         const int l0 = this_lane();
         const glm_f32x4 other = s_x[k & 1][rg][half ^ 1][l0];
@@ -958,14 +946,19 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         const float next = fmaxf(top, max_over_quads(mx));
         const float from = next == -INFINITY ? 0.0f : next;
         const float keep = __builtin_amdgcn_exp2f(top - from);
-        const int l = this_lane(), common = fringe ? all_see - p - 4 * (l >> 4) : 32;
+        const int l = this_lane(), common = all_see - p - 4 * (l >> 4);
         glm_bf16x8 prob;
         sum *= keep;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[i] = __builtin_amdgcn_exp2f(x[i] - from);
           sum += x[i];
-          prob[i] = 16 * (i / 4) + i % 4 < common ? (__bf16)x[i] : (__bf16)0.0f;  // (see attn_group_kernel)
+          prob[i] = (__bf16)x[i];  // (see attn_group_kernel)
+        }
+        if (fringe) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (16 * (i / 4) + i % 4 >= common) prob[i] = (__bf16)0.0f;
         }
         own = next_own;
         s_x[(k + 1) & 1][rg][half][l] = own;
@@ -1027,13 +1020,14 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
           }
         }
       }
+      wait_loads<kLoads>();  // bf16: tile k + 2; MXFP8: the codes of tile k + 2
       if constexpr (kMx) {
-        wait_loads<kOneTile>();  // the codes of tile k + 2, the page numbers of tile k + 4
         convert(k & 1, plus(main_k, 2, 3), rest_k ^ 1);
         __builtin_amdgcn_sched_barrier(0);
-        last_seen = issue();
+        load_ids();
+        load_rows(k + 4, k & 1, 0);
       } else {
-        wait_loads<kOneTile>();  // tile k + 2
+        load_ids();
       }
       meet();
       main_k = plus(main_k, 1, L::kMains);
