@@ -692,7 +692,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   constexpr bool kMx = L::kMx;
   constexpr int kG = L::kG;
   constexpr int kD = DV / 32;  // 16-channel tiles of a wave's half
-  constexpr int kKeys = 6;     // operands of the scores read ahead
+  constexpr int kKeys = 8;     // operands of the scores read ahead
   constexpr int kLoads = kMx ? 4 : 5;  // of a wave and tile (bf16: a pair's middle block is both's)
   static_assert(DK == 576 && DV == 512, "nine blocks of 64 channels; MXFP8: 36 pieces of 16 codes, 18 scales a row");
   // (one dynamic array: for reads of a static one the compiler waits for every load on its way to it)
@@ -720,7 +720,8 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     int b, head, p, end;  // a tile's request, kv head, first position, end of the item
   };
   AttnWalk ahead = walk;
-  AttnItem next_it;
+  AttnItem it, next_it;
+  bool more = walk.next(a, it);
   Place place = {0, 0, 0, 0};
   const auto next_place = [&]() {
     while (place.p >= place.end) {
@@ -825,11 +826,30 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   const auto seen_of = [&](int tile) {
     return (uint32_t)__builtin_amdgcn_readfirstlane(s_seen[(tile >> 2) & 1][tile & 3]);
   };
+  // the query rows of an item, in registers for its tiles
+  glm_bf16x8 q[DK / 32];
+  const auto load_q = [&]() {
+    const int r = min(it.rb * 64 + 16 * rg + n, R - 1), tok = r / group;
+    const uint16_t *p = a.q + ((long long)it.b * a.q_len + tok) * a.q_stride +
+                        (it.head * group + r - tok * group) * DK + 8 * quad;
+#pragma unroll
+    for (int s = 0; s < DK / 32; ++s) q[s] = *reinterpret_cast<const glm_bf16x8 *>(p + 32 * s);
+  };
+  int id0 = -1, id1 = -1, within0 = -1;
   if (wave < 2) {
-    const int32_t *first = entry();
-    put_rows(*first, 0);
-    const int32_t *second = entry();
-    put_rows(*second, 1);
+    id0 = *entry();
+    within0 = within;
+    id1 = *entry();
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  if (more) load_q();  // (behind the page numbers: loads return in order)
+  __builtin_amdgcn_sched_barrier(0);
+  if (wave < 2) {
+    const int within1 = within;
+    within = within0;
+    put_rows(id0, 0);
+    within = within1;
+    put_rows(id1, 1);
   }
   __syncthreads();
 #pragma unroll
@@ -852,21 +872,15 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     if ((k & 3) == 0 && wave < 2) load_to_lds<4>(entry(), s_id + 64 * wave);
   };
 
-  for (AttnItem it; walk.next(a, it);) {
+  while (more) {
     const int head = it.head, r0 = it.rb * 64 + 16 * rg;
     const bool active = r0 < R;  // (uniform in a wave)
     const int begin = it.t0 * kAttnTile, end = min(it.t1 * kAttnTile, it.len);
     const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
     const int r = min(r0 + n, R - 1), tok = r / group;
-    glm_bf16x8 q[DK / 32];
-    {
-      const uint16_t *p = a.q + ((long long)it.b * a.q_len + tok) * a.q_stride +
-                          (head * group + r - tok * group) * DK + 8 * quad;
-#pragma unroll
-      for (int s = 0; s < DK / 32; ++s) q[s] = *reinterpret_cast<const glm_bf16x8 *>(p + 32 * s);
-      // (here once, or the compiler waits for them, and with them for all rows in flight, in every turn)
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-    }
+    // (the rows' loads are waited for here once, or the compiler waits for them, and with them for all
+    // rows in flight, in every turn)
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     constexpr glm_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     glm_f32x4 acc[kD], own = zero;  // own: this wave's scores, of 16 positions of the tile to come
 #pragma unroll
@@ -892,6 +906,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       for (int i = 0; i < kKeys; ++i) kf[i] = key(i);
 #pragma unroll
       for (int i = 0; i < DK / 32; i += 2) {
+        __builtin_amdgcn_sched_barrier(0);  // (else each read is waited for by itself)
         even = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i % kKeys], q[i], even, 0, 0, 0);
         odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[(i + 1) % kKeys], q[i + 1], odd, 0, 0, 0);
         if (i + kKeys < DK / 32) {
@@ -899,6 +914,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
           kf[(i + 1) % kKeys] = key(i + 1 + kKeys);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
       return even + odd;
     };
 
@@ -1037,11 +1053,15 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       seen[kAhead - 1] = last_seen;
     }
 
+    const AttnItem done = it;
+    more = walk.next(a, it);
+    if (more) load_q();  // the next item's, while this one's results are written
+    __builtin_amdgcn_sched_barrier(0);
     sum = sum_over_quads(sum);
     if (!active || r0 + n >= R) {
       // (a row past the last, or a wave of them)
-    } else if (it.whole) {
-      uint16_t *out = a.out + (((long long)it.b * a.q_len + tok) * a.heads + head * group + r - tok * group) * DV +
+    } else if (done.whole) {
+      uint16_t *out = a.out + (((long long)done.b * a.q_len + tok) * a.heads + head * group + r - tok * group) * DV +
                       half * (DV / 2) + 4 * quad;
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -1052,7 +1072,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         *reinterpret_cast<uint2 *>(out + 16 * d) = uint2{b[0] | (b[1] << 16), b[2] | (b[3] << 16)};
       }
     } else {
-      const long long at = (long long)it.partial * a.rows + 16 * rg + n;
+      const long long at = (long long)done.partial * a.rows + 16 * rg + n;
 #pragma unroll
       for (int d = 0; d < kD; ++d)
         *reinterpret_cast<glm_f32x4 *>(a.part + at * DV + half * (DV / 2) + 16 * d + 4 * quad) = acc[d];
@@ -1064,10 +1084,12 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
 
 // ---------------------------------------------------------------------------
 // The pairs of request and kv head that were cut: out = sum_i 2^(m_i - m) acc_i
-// / sum_i 2^(m_i - m) l_i over their pieces in order.  A thread has four
-// channels of a row.
+// / sum_i 2^(m_i - m) l_i over their pieces in order, with a running maximum,
+// so that a piece's weight and sums are asked for together.  A thread has four
+// channels of a row and eight pieces in flight.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  constexpr int kFlight = 8;
   const int b = blockIdx.y;
   const int2 plan = a.plan[b];
   const int tiles = (attn_len(a, b) + kAttnTile - 1) / kAttnTile, w = a.over + tiles;
@@ -1080,21 +1102,32 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int first = plan.x * a.kv_heads + head * w;
   const int g0 = (first + a.over) / plan.y, g1 = (first + w - 1) / plan.y;
   if (g0 == g1) return;
-  const auto at = [&](int g) {
-    return ((long long)(2 * g + (g == g0)) * a.rblocks + r / a.rows) * a.rows + r % a.rows;
-  };
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int g = g0; g <= g1; ++g) m = fmaxf(m, a.ml[2 * at(g)]);
-  const float from = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
+  float m = -INFINITY, l = 0.0f;
   glm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int g = g0; g <= g1; ++g) {
-    const float2 ml = *reinterpret_cast<const float2 *>(a.ml + 2 * at(g));
-    const float scale = exp2f(ml.x - from);
-    l += scale * ml.y;
-    acc += scale * *reinterpret_cast<const glm_f32x4 *>(a.part + at(g) * a.dv + ch);
+  for (int g = g0; g <= g1; g += kFlight) {
+    float2 ml[kFlight];
+    glm_f32x4 part[kFlight];
+    float next = m;
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) {
+      const int from = min(g + j, g1);
+      const long long at =
+          ((long long)(2 * from + (from == g0)) * a.rblocks + r / a.rows) * a.rows + r % a.rows;
+      ml[j] = *reinterpret_cast<const float2 *>(a.ml + 2 * at);
+      part[j] = *reinterpret_cast<const glm_f32x4 *>(a.part + at * a.dv + ch);
+      next = fmaxf(next, ml[j].x);
+    }
+    const float from = next == -INFINITY ? 0.0f : next, keep = exp2f(m - from);
+    m = next;
+    l *= keep;
+    acc *= keep;
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) {
+      if (g + j > g1) break;
+      const float scale = exp2f(ml[j].x - from);
+      l += scale * ml[j].y;
+      acc += scale * part[j];
+    }
   }
   uint32_t o[4];
 #pragma unroll
