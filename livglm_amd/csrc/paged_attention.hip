@@ -20,6 +20,17 @@ namespace glm {
 constexpr int kAttnTile = 64;  // positions; parts are cut between tiles
 constexpr float kLog2e = 1.44269504088896341f;
 
+// Sums over the wave by DPP: row_shr 1, 2, 4, 8, then a row's last lane to the next rows.
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 struct AttnArgs {
   const uint16_t *q;
   long long q_stride;  // elements from token to token
@@ -27,7 +38,7 @@ struct AttnArgs {
   const uint8_t *ks, *vs;
   const int32_t *tables, *lens;
   uint16_t *out;
-  int2 *plan;        // [B] {units before the request, units of a part}, for the join
+  int4 *plan;        // [parts] the pair that ends in a part and was cut: {b, head, its first part, 0}, b -1 for none
   float *part, *ml;  // partial results [2 part + end][row block][rows][dv], [..][2]
   int B, q_len, heads, kv_heads, dk, dv, num_pages, page, max_blocks;
   uint32_t page_magic;   // floor(2^32 / page), at most 2^32 - 1
@@ -76,25 +87,35 @@ struct AttnWalk {
       part = block / (8 * a.rblocks) * 8 + block % 8;
       rb = block / 8 % a.rblocks;
     }
-    int total = 0;
-    for (int i = lane; i < a.B; i += kWave) total += units(attn_len(a, i));
+    // the first 256 requests' lengths stay in registers
+    constexpr int kHold = 4;
+    int held[kHold], total = 0;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, kWave);
-    total = __builtin_amdgcn_readfirstlane(total) * a.kv_heads;
+    for (int j = 0; j < kHold; ++j) {
+      const int i = lane + kWave * j;
+      held[j] = i < a.B ? attn_len(a, i) : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) total += held[j] >= 0 ? units(held[j]) : 0;
+    for (int i = lane + kWave * kHold; i < a.B; i += kWave) total += units(attn_len(a, i));
+    total = __builtin_amdgcn_readlane(wave_scan(total), kWave - 1) * a.kv_heads;
     u = max(a.min_part, (total + a.parts - 1) / a.parts);
-    if (part > (total - 1) / u) return false;
+    const bool writes = rb == 0 && threadIdx.x == 0 && part < a.parts;
+    if (part > (total - 1) / u) {
+      if (writes) a.plan[part] = int4{-1, 0, 0, 0};
+      return false;
+    }
     x = part * u;
     x1 = min(total, x + u);
     before = 0;
     for (int b0 = 0;; b0 += kWave) {
       const int i = b0 + lane;
-      const int len_i = i < a.B ? attn_len(a, i) : 0, w_i = i < a.B ? units(len_i) : 0;
-      int upto = w_i;
+      int len_i = -1;
 #pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) {
-        const int v = __shfl_up(upto, off, kWave);
-        if (lane >= off) upto += v;
-      }
+      for (int j = 0; j < kHold; ++j) len_i = b0 == kWave * j ? held[j] : len_i;
+      if (b0 >= kWave * kHold) len_i = i < a.B ? attn_len(a, i) : -1;
+      const int w_i = len_i >= 0 ? units(len_i) : 0;
+      const int upto = wave_scan(w_i);
       const int first = before + upto - w_i;
       const unsigned long long hit = __ballot(x >= first * a.kv_heads && x < (first + w_i) * a.kv_heads);
       if (hit) {
@@ -104,14 +125,18 @@ struct AttnWalk {
         before = __builtin_amdgcn_readlane(first, l);
         w = __builtin_amdgcn_readlane(w_i, l);
         head = (x - before * a.kv_heads) / w;
+        // for the join: a pair that has tiles before the part and ends in it
+        const int begin = before * a.kv_heads + head * w;
+        if (writes)
+          a.plan[part] = x - begin > over && begin + w <= x1 ? int4{b, head, (begin + over) / u, 0}
+                                                             : int4{-1, 0, 0, 0};
         return true;
       }
       before += __builtin_amdgcn_readlane(upto, kWave - 1);
     }
   }
 
-  // The part's next item; also leaves the request's place for the join.
-  template <bool PLAN = true>
+  // The part's next item.
   __device__ __forceinline__ bool next(const AttnArgs &a, AttnItem &it) {
     while (x < x1) {
       const int first = before * a.kv_heads + head * w, from = x - first, to = min(x1 - first, w);
@@ -123,7 +148,6 @@ struct AttnWalk {
       it.t1 = to - over;
       it.whole = w == over || (it.t0 == 0 && it.t1 == w - over);  // (an empty request: wherever it begins)
       it.partial = (2 * part + (it.t0 == 0)) * a.rblocks + rb;
-      if (PLAN && from == 0 && head == 0 && rb == 0 && threadIdx.x == 0) a.plan[b] = int2{before, u};
       const bool some = it.t1 > it.t0 || (w == over && from == 0);
       x = first + w;
       if (++head == a.kv_heads) {
@@ -725,7 +749,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   Place place = {0, 0, 0, 0};
   const auto next_place = [&]() {
     while (place.p >= place.end) {
-      if (!ahead.template next<false>(a, next_it)) return Place{0, 0, 0, 0};
+      if (!ahead.next(a, next_it)) return Place{0, 0, 0, 0};
       place = {next_it.b, next_it.head, next_it.t0 * kAttnTile, min(next_it.t1 * kAttnTile, next_it.len)};
     }
     const Place now = place;
@@ -1085,56 +1109,52 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------
 // The pairs of request and kv head that were cut: out = sum_i 2^(m_i - m) acc_i
 // / sum_i 2^(m_i - m) l_i over their pieces in order, with a running maximum,
-// so that a piece's weight and sums are asked for together.  A thread has four
-// channels of a row and eight pieces in flight.
+// so that a piece's weight and sums are asked for together.  A part has the
+// end of at most one of them, so the launch goes by parts and not by requests.
+// A thread has four channels of a row and eight pieces in flight.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int kFlight = 8;
-  const int b = blockIdx.y;
-  const int2 plan = a.plan[b];
-  const int tiles = (attn_len(a, b) + kAttnTile - 1) / kAttnTile, w = a.over + tiles;
-  const int R = attn_rows(a), group = a.heads / a.kv_heads;
-  const int i = blockIdx.x * 256 + threadIdx.x, quads = a.dv / 4;
-  const int row = i / quads, ch = 4 * (i - row * quads);
-  if (row >= a.kv_heads * R || tiles == 0) return;
-  const int head = row / R, r = row - head * R;
-  // the parts that the pair's tiles lie in; the first holds its beginning
-  const int first = plan.x * a.kv_heads + head * w;
-  const int g0 = (first + a.over) / plan.y, g1 = (first + w - 1) / plan.y;
-  if (g0 == g1) return;
-  float m = -INFINITY, l = 0.0f;
-  glm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int g = g0; g <= g1; g += kFlight) {
-    float2 ml[kFlight];
-    glm_f32x4 part[kFlight];
-    float next = m;
+  const int4 pair = a.plan[blockIdx.y];
+  if (pair.x < 0) return;
+  const int b = pair.x, head = pair.y, g0 = pair.z, g1 = blockIdx.y;  // (g0: the pair's beginning)
+  const int R = attn_rows(a), group = a.heads / a.kv_heads, quads = a.dv / 4;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < R * quads; i += gridDim.x * 256) {
+    const int r = i / quads, ch = 4 * (i - r * quads);
+    float m = -INFINITY, l = 0.0f;
+    glm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int g = g0; g <= g1; g += kFlight) {
+      float2 ml[kFlight];
+      glm_f32x4 part[kFlight];
+      float next = m;
 #pragma unroll
-    for (int j = 0; j < kFlight; ++j) {
-      const int from = min(g + j, g1);
-      const long long at =
-          ((long long)(2 * from + (from == g0)) * a.rblocks + r / a.rows) * a.rows + r % a.rows;
-      ml[j] = *reinterpret_cast<const float2 *>(a.ml + 2 * at);
-      part[j] = *reinterpret_cast<const glm_f32x4 *>(a.part + at * a.dv + ch);
-      next = fmaxf(next, ml[j].x);
-    }
-    const float from = next == -INFINITY ? 0.0f : next, keep = exp2f(m - from);
-    m = next;
-    l *= keep;
-    acc *= keep;
+      for (int j = 0; j < kFlight; ++j) {
+        const int from = min(g + j, g1);
+        const long long at =
+            ((long long)(2 * from + (from == g0)) * a.rblocks + r / a.rows) * a.rows + r % a.rows;
+        ml[j] = *reinterpret_cast<const float2 *>(a.ml + 2 * at);
+        part[j] = *reinterpret_cast<const glm_f32x4 *>(a.part + at * a.dv + ch);
+        next = fmaxf(next, ml[j].x);
+      }
+      const float from = next == -INFINITY ? 0.0f : next, keep = exp2f(m - from);
+      m = next;
+      l *= keep;
+      acc *= keep;
 #pragma unroll
-    for (int j = 0; j < kFlight; ++j) {
-      if (g + j > g1) break;
-      const float scale = exp2f(ml[j].x - from);
-      l += scale * ml[j].y;
-      acc += scale * part[j];
+      for (int j = 0; j < kFlight; ++j) {
+        if (g + j > g1) break;
+        const float scale = exp2f(ml[j].x - from);
+        l += scale * ml[j].y;
+        acc += scale * part[j];
+      }
     }
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = f32_to_bf16(l == 0.0f ? 0.0f : acc[j] / l);
+    const int t = r / group;
+    uint16_t *out = a.out + (((long long)b * a.q_len + t) * a.heads + head * group + r % group) * a.dv + ch;
+    *reinterpret_cast<uint2 *>(out) = uint2{o[0] | (o[1] << 16), o[2] | (o[3] << 16)};
   }
-  uint32_t o[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) o[j] = f32_to_bf16(l == 0.0f ? 0.0f : acc[j] / l);
-  const int t = r / group;
-  uint16_t *out = a.out + (((long long)b * a.q_len + t) * a.heads + head * group + r % group) * a.dv + ch;
-  *reinterpret_cast<uint2 *>(out) = uint2{o[0] | (o[1] << 16), o[2] | (o[3] << 16)};
 }
 
 }  // namespace glm
@@ -1227,7 +1247,7 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
   if (z.parts > most_parts) z.parts = most_parts > 1 ? (int)most_parts : 1;
   z.grid = z.rblocks > 1 ? (unsigned)((z.parts + 7) / 8 * 8 * z.rblocks) : (unsigned)z.parts;
   const size_t results = (size_t)2 * z.parts * z.rblocks * z.rows;
-  z.plan_bytes = up256((size_t)B * sizeof(int2));
+  z.plan_bytes = up256((size_t)z.parts * sizeof(int4));
   z.part_bytes = up256(results * value_dim * sizeof(float));
   z.ml_bytes = up256(results * 2 * sizeof(float));
   return true;
@@ -1299,7 +1319,7 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
   a.tables = tables;
   a.lens = lens;
   a.out = out;
-  a.plan = (int2 *)ws;
+  a.plan = (int4 *)ws;
   a.part = (float *)(ws + z.plan_bytes);
   a.ml = (float *)(ws + z.plan_bytes + z.part_bytes);
   a.B = B;
@@ -1326,9 +1346,12 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
     launch_attention<GLM_FMT_BF16>(s, grid, z.form, a);
   GLM_LAUNCH_CHECK("paged_attention");
   if (z.parts > 1) {
-    const long long quads = (long long)q_len * heads * value_dim / 4;
-    hipLaunchKernelGGL(glm::attn_join_kernel, dim3((unsigned)((quads + 255) / 256), B), dim3(256), 0,
-                       s, a);
+    // as many workgroups as have work for few cut pairs, and no more than fill the chip for many
+    const int quads = q_len * (heads / kv_heads) * value_dim / 4;
+    const int pairs = z.parts < (long long)B * kv_heads ? z.parts : B * kv_heads;
+    int ways = (quads + 255) / 256;
+    if (ways > 4096 / pairs) ways = 4096 / pairs > 1 ? 4096 / pairs : 1;
+    hipLaunchKernelGGL(glm::attn_join_kernel, dim3(ways, z.parts), dim3(256), 0, s, a);
     GLM_LAUNCH_CHECK("attn_join_kernel");
   }
   return GLM_OK;
