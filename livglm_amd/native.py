@@ -138,6 +138,8 @@ def library_path() -> str:
 def load(path: str | None = None):
     """Load (once) and return the ctypes library with typed signatures."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

@@ -53,10 +53,22 @@ def call(name: str, *args) -> None:
     try:
         native.call(name, *args)
     except native.NativeError as err:
-        if err.code in (native.GLM_ERR_INVALID_ARGUMENT, native.GLM_ERR_UNSUPPORTED_SHAPE,
-                        native.GLM_ERR_WORKSPACE):
-            raise ContractError(str(err)) from err
-        raise
+        _refused(err)
+
+
+def check(name: str, code: int) -> None:
+    """The same mapping for an entry point that was called directly."""
+    try:
+        native.check(name, code)
+    except native.NativeError as err:
+        _refused(err)
+
+
+def _refused(err: native.NativeError) -> None:
+    if err.code in (native.GLM_ERR_INVALID_ARGUMENT, native.GLM_ERR_UNSUPPORTED_SHAPE,
+                    native.GLM_ERR_WORKSPACE):
+        raise ContractError(str(err)) from err
+    raise err
 
 
 @lru_cache(maxsize=256)  # a function of the sizes alone

@@ -38,11 +38,19 @@ BAD_STATE = N.native.GLM_CACHE_BAD_STATE
 _BF16, _U8, _I32 = torch.bfloat16, torch.uint8, torch.int32
 
 
-def _check(t: torch.Tensor, name: str, dtype: torch.dtype, device) -> None:
+# The calls here are a few microseconds of GPU work each, so what the host does
+# before them counts: devices are compared as numbers, and the library's
+# functions are called without a wrapper in between.
+_getDevice = torch._C._cuda_getDevice
+_getStream = torch._C._cuda_getCurrentRawStream
+_empty = torch.empty
+
+
+def _check(t: torch.Tensor, name: str, dtype: torch.dtype, device: int) -> None:
     """A contiguous tensor of the call's device and the dtype it has to have."""
-    if t is None or t.dtype is not dtype or t.device != device or not t.is_contiguous():
+    if t is None or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
         N.require_device(t, name, (dtype,))
-        raise ContractError(f"{name} is on {t.device}, the call's tensors on {device}")
+        raise ContractError(f"{name} is on {t.device}, the call's tensors on device {device}")
 
 
 def _token_rows(t: torch.Tensor, name: str) -> int:
@@ -54,39 +62,46 @@ def _token_rows(t: torch.Tensor, name: str) -> int:
         raise ContractError(f"{name} must live on the GPU (got {t.device})")
     if t.dtype is not _BF16:
         raise ContractError(f"{name} has dtype {t.dtype}, expected {_BF16}")
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
     if len(shape) not in (3, 4):
         raise ContractError(f"{name} must be [tokens, heads, dim] rows, got {tuple(shape)}")
+    row = shape[-1] * shape[-2]
+    if t.is_contiguous():
+        return row
+    stride = t.stride()
     if stride[-1] != 1 and shape[-1] != 1 or stride[-2] != shape[-1] and shape[-2] != 1:
         raise ContractError(f"{name}: a token's heads must lie together, strides {stride}")
     if len(shape) == 4 and stride[0] != shape[1] * stride[1] and shape[0] != 1 and shape[1] != 1:
         raise ContractError(f"{name}: the tokens must lie at one stride, strides {stride}")
-    if shape[0] > 1:  # (the stride of an axis of one says nothing)
-        return stride[1] if len(shape) == 4 and shape[1] > 1 else stride[0]
-    return stride[1] if len(shape) == 4 and shape[1] > 1 else shape[-1] * shape[-2]
+    if len(shape) == 4 and shape[1] > 1:  # (the stride of an axis of one says nothing)
+        return stride[1]
+    return stride[0] if shape[0] > 1 else row
 
 
-def _call(device, name: str, *args) -> None:
-    """The native call with the tensors' device current, as a launch needs it."""
-    if device.index == torch.cuda.current_device():
-        N.call(name, *args)
+def _run(device: int, name: str, function, *args) -> None:
+    """A native call on the current stream of the tensors' device, which is the
+    current one meanwhile, as a launch needs it."""
+    if device == _getDevice():
+        code = function(_getStream(device), *args)
     else:
         with torch.cuda.device(device):
-            N.call(name, *args)
+            code = function(_getStream(device), *args)
+    if code:
+        N.check(name, code)
 
 
-def _cache_format(cache: torch.Tensor, scales: torch.Tensor | None, name: str, device) -> int:
-    if cache.ndim != 4:
-        raise ContractError(f"{name} must be [pages, kv_heads, page_size, dim], got "
-                            f"{tuple(cache.shape)}")
+def _cache_format(cache: torch.Tensor, scales: torch.Tensor | None, name: str, device: int) -> int:
     if scales is None:
         _check(cache, name, _BF16, device)
+        if cache.dim() != 4:
+            raise ContractError(f"{name} must be [pages, kv_heads, page_size, dim], got "
+                                f"{tuple(cache.shape)}")
         return N.FMT_BF16
     _check(cache, name, _U8, device)
     _check(scales, f"{name} scales", _U8, device)
-    if cache.shape[3] % 32 or scales.shape != (*cache.shape[:3], cache.shape[3] // 32):
-        raise ContractError(f"{name} scales {tuple(scales.shape)} do not fit codes "
-                            f"{tuple(cache.shape)}")
+    shape = cache.shape
+    if len(shape) != 4 or shape[3] % 32 or scales.shape != (*shape[:3], shape[3] // 32):
+        raise ContractError(f"{name} scales {tuple(scales.shape)} do not fit codes {tuple(shape)}")
     return N.FMT_MXFP8
 
 
@@ -114,12 +129,13 @@ def cache_step(new_lens: torch.Tensor, lens: torch.Tensor, blocks: torch.Tensor,
     place.  ``kv_lens`` (allocated when not given; may be ``lens``) receives the
     lengths after the step.  Slots and positions have ``max_tokens`` rows.
     """
-    dev = new_lens.device
-    if not new_lens.is_cuda:
-        N.require_device(new_lens, "new_lens")
-    for t, name in ((new_lens, "new_lens"), (lens, "lens"), (blocks, "blocks"),
-                    (tables, "tables"), (free_pages, "free_pages"), (num_free, "num_free")):
-        _check(t, name, _I32, dev)
+    N.require_device(new_lens, "new_lens", (_I32,))
+    dev = new_lens.get_device()
+    _check(lens, "lens", _I32, dev)
+    _check(blocks, "blocks", _I32, dev)
+    _check(tables, "tables", _I32, dev)
+    _check(free_pages, "free_pages", _I32, dev)
+    _check(num_free, "num_free", _I32, dev)
     B = new_lens.numel()
     if tables.ndim != 2 or tables.shape[0] < B or lens.numel() < B or blocks.numel() < B:
         raise ContractError(f"cache_step: {B} requests, tables {tuple(tables.shape)}, "
@@ -133,15 +149,17 @@ def cache_step(new_lens: torch.Tensor, lens: torch.Tensor, blocks: torch.Tensor,
         if kv_lens.numel() < B:
             raise ContractError(f"cache_step: kv_lens for {kv_lens.numel()} of {B} requests")
     # one allocation: cu_new | status | slots | positions | kv_lens
-    buf = torch.empty(2 * B + 2 + 2 * max_tokens, dtype=_I32, device=dev)
-    cu, status, slots, positions, after = buf.split((B + 1, 1, max_tokens, max_tokens, B))
+    buf = _empty(2 * B + 2 + 2 * max_tokens, dtype=_I32, device=new_lens.device)
+    cu, status, slots, positions, after = buf.split_with_sizes(
+        (B + 1, 1, max_tokens, max_tokens, B))
     if kv_lens is None:
         kv_lens = after
     base = buf.data_ptr()
-    _call(dev, "glm_cache_step", N.stream_of(new_lens), new_lens.data_ptr(), B, free_pages.numel(),
-           page_size, tables.shape[1], max_tokens, lens.data_ptr(), blocks.data_ptr(),
-           tables.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(), kv_lens.data_ptr(),
-           base, base + 4 * (B + 2), base + 4 * (B + 2 + max_tokens), base + 4 * (B + 1))
+    _run(dev, "glm_cache_step", N.native.load().glm_cache_step, new_lens.data_ptr(), B,
+         free_pages.numel(), page_size, tables.shape[1], max_tokens, lens.data_ptr(),
+         blocks.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
+         kv_lens.data_ptr(), base, base + 4 * (B + 2), base + 4 * (B + 2 + max_tokens),
+         base + 4 * (B + 1))
     return CacheStep(kv_lens, cu, slots, positions, status)
 
 
@@ -155,7 +173,7 @@ def cache_write(keys: torch.Tensor, values: torch.Tensor | None, slots: torch.Te
     ``values`` and ``value_cache`` are None for a latent cache.  With scales the
     caches are MXFP8."""
     key_stride = _token_rows(keys, "keys")
-    dev = keys.device
+    dev = keys.get_device()
     fmt = _cache_format(key_cache, key_scales, "key_cache", dev)
     _check(slots, "slots", _I32, dev)
     pages, heads, page, key_dim = key_cache.shape
@@ -172,14 +190,14 @@ def cache_write(keys: torch.Tensor, values: torch.Tensor | None, slots: torch.Te
             raise ContractError("key_cache and value_cache must share one format")
         value_dim = value_cache.shape[3]
         if value_cache.shape[:3] != key_cache.shape[:3] or \
-                values.shape != (n, heads, value_dim) or values.device != dev:
+                values.shape != (n, heads, value_dim) or values.get_device() != dev:
             raise ContractError(f"values {tuple(values.shape)} and value_cache "
                                 f"{tuple(value_cache.shape)} do not fit the keys")
     if n == 0:
         return
-    _call(dev, "glm_cache_write", N.stream_of(keys), keys.data_ptr(), key_stride, N.ptr(values),
-           value_stride, slots.data_ptr(), n, pages, page, heads, key_dim, value_dim, fmt,
-           key_cache.data_ptr(), N.ptr(key_scales), N.ptr(value_cache), N.ptr(value_scales))
+    _run(dev, "glm_cache_write", N.native.load().glm_cache_write, keys.data_ptr(), key_stride,
+         N.ptr(values), value_stride, slots.data_ptr(), n, pages, page, heads, key_dim, value_dim,
+         fmt, key_cache.data_ptr(), N.ptr(key_scales), N.ptr(value_cache), N.ptr(value_scales))
 
 
 @lru_cache(maxsize=256)  # a function of the sizes alone
@@ -204,7 +222,7 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
     key rows.  Returns bf16 of the query's shape with ``value_dim`` channels; a
     row that sees nothing gives zeros."""
     q_stride = _token_rows(query, "query")
-    dev = query.device
+    dev = query.get_device()
     shape = query.shape
     B, heads = shape[0], shape[-2]
     q_len = shape[1] if len(shape) == 4 else 1
@@ -227,7 +245,7 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
     elif value_dim is None or value_scales is not None:
         raise ContractError("a latent cache needs value_dim and has no value scales")
     if out is None:
-        out = torch.empty((*shape[:-1], value_dim), dtype=_BF16, device=dev)
+        out = _empty((*shape[:-1], value_dim), dtype=_BF16, device=query.device)
     else:
         _check(out, "out", _BF16, dev)
         if out.shape != (*shape[:-1], value_dim):
@@ -237,11 +255,12 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
     max_blocks = tables.shape[1]
     need = _attention_workspace(B, q_len, heads, kv_heads, key_dim, value_dim,
                                 int(value_cache is None), page, max_blocks)
-    ws = torch.empty(need, dtype=_U8, device=dev)
-    _call(dev, "glm_paged_attention", N.stream_of(query), query.data_ptr(), q_stride, B, q_len, heads,
-           kv_heads, key_dim, value_dim, key_cache.data_ptr(), N.ptr(key_scales),
-           N.ptr(value_cache), N.ptr(value_scales), fmt, pages, page, tables.data_ptr(),
-           lens.data_ptr(), max_blocks, scale, ws.data_ptr(), need, out.data_ptr())
+    ws = _empty(need, dtype=_U8, device=query.device)
+    _run(dev, "glm_paged_attention", N.native.load().glm_paged_attention, query.data_ptr(),
+         q_stride, B, q_len, heads, kv_heads, key_dim, value_dim, key_cache.data_ptr(),
+         N.ptr(key_scales), N.ptr(value_cache), N.ptr(value_scales), fmt, pages, page,
+         tables.data_ptr(), lens.data_ptr(), max_blocks, scale, ws.data_ptr(), need,
+         out.data_ptr())
     return out
 
 

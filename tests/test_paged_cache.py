@@ -188,7 +188,7 @@ def test_token_rows_strides():
     class OnGpu:  # the check reads shapes and strides alone
         def __init__(self, t):
             self.shape, self.dtype, self.is_cuda, self.device = t.shape, t.dtype, True, "cuda"
-            self.stride = t.stride
+            self.stride, self.is_contiguous = t.stride, t.is_contiguous
 
     def rows(t):
         real, torch.Tensor_ = torch.Tensor, None
