@@ -678,8 +678,8 @@ int glm_cache_step(void *stream, const int32_t *new_lens, int B, int num_pages, 
  * to nearest even; an infinity or a NaN is stored as NaN.
  * A token whose slot is not in [0, num_pages * page_size) is skipped.  Slots
  * named twice in one call hold pieces of either row.
- * Limits: widths multiples of 8 (MXFP8: 32) up to 1024; strides multiples of
- * 8; num_pages * page_size * kv_heads < 2^31.
+ * Limits: N <= 2^30, kv_heads <= 65536, widths multiples of 8 (MXFP8: 32) up to
+ * 1024, strides multiples of 8, num_pages * page_size * kv_heads < 2^31.
  */
 int glm_cache_write(void *stream, const uint16_t *keys, int64_t key_stride,
                     const uint16_t *values, int64_t value_stride, const int32_t *slots, int N,

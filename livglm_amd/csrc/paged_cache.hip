@@ -193,10 +193,11 @@ __global__ __launch_bounds__(256) void cache_slots_kernel(
 // ---------------------------------------------------------------------------
 // New rows into their slots.  Cache layout [page][kv head][page size][dim]:
 // a head's rows of one page lie together, so the attention streams them.
-// A thread moves eight channels (16 bytes of bf16); consecutive threads take
-// consecutive channels of a token's keys, then of its values.  bf16 rows are
-// copied; MXFP8 groups of 32 channels lie in four lanes, which find the
-// group's largest magnitude by DPP and its exponent
+// A thread moves eight channels (16 bytes of bf16) of every so many tokens:
+// what follows from the channel is formed once, and four tokens are in flight.
+// Consecutive threads take consecutive channels of a token's keys, then of its
+// values.  bf16 rows are copied; MXFP8 groups of 32 channels lie in four lanes,
+// which find the group's largest magnitude by DPP and its exponent
 //   e = the smallest >= -124 with amax <= 448 2^e
 // from the bf16 bits alone (448 = 1.75 2^8), so no code saturates -- the
 // rounding rules of glm_mx_quantize may cut a group's largest element by up
@@ -212,53 +213,75 @@ struct CacheWrite {
   int dim[2];
   const int32_t *slots;
   int N, heads, page, num_slots;
+  uint32_t page_magic;  // floor(2^32 / page), at most 2^32 - 1
 };
+
+// Eight bf16 channels as MXFP8, four lanes a group.
+__device__ __forceinline__ uint2 mxfp8_codes(const glm_u32x4 &x, uint32_t &scale) {
+  float f[8];
+  int m = 0;  // largest finite magnitude's bf16 bits
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t bits = j % 2 ? x[j / 2] >> 16 : x[j / 2] & 0xffffu;
+    const int mag = bits & 0x7fffu;
+    m = mag < 0x7f80 ? max(m, mag) : m;
+    f[j] = mag < 0x7f80 ? __uint_as_float(bits << 16) : __uint_as_float(0x7fc00000u);
+  }
+  m = max(m, __builtin_amdgcn_mov_dpp(m, 0xB1, 0xf, 0xf, true));
+  m = max(m, __builtin_amdgcn_mov_dpp(m, 0x4E, 0xf, 0xf, true));
+  const int e = max((m >> 7) - 127 - 8 + ((m & 0x7f) > 0x60 ? 1 : 0), -124);
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e, exact
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] *= inv;  // exact, within 448
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  uint32_t code[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    s16x2 o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, f[4 * j], f[4 * j + 1], 1.0f, false);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, f[4 * j + 2], f[4 * j + 3], 1.0f, true);
+    code[j] = __builtin_bit_cast(uint32_t, o);
+  }
+  scale = (uint32_t)(e + 127);
+  return uint2{code[0], code[1]};
+}
 
 template <int FMT>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheWrite a) {
+  constexpr int kFlight = 4;
   const int keys = a.heads * a.dim[0] / 8, pieces = keys + a.heads * a.dim[1] / 8;
-  const long long all = (long long)a.N * pieces;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < all;
-       i += (long long)gridDim.x * blockDim.x) {  // (MXFP8: whole lane quads leave together)
-    const int token = (int)(i / pieces);
-    int c = (int)(i - (long long)token * pieces);
-    const int slot = a.slots[token];
-    if ((uint32_t)slot >= (uint32_t)a.num_slots) continue;
-    const int v = c >= keys;
-    c -= v ? keys : 0;
+  const int tokens = pieces < 256 ? 256 / pieces : 1;  // of a workgroup at once
+  const int tl = pieces < 256 ? threadIdx.x / pieces : 0;
+  const int step = gridDim.x * tokens;
+  for (int c0 = pieces < 256 ? threadIdx.x - tl * pieces : threadIdx.x; c0 < pieces && tl < tokens; c0 += 256) {
+    const int v = c0 >= keys, c = c0 - (v ? keys : 0);
     const int dim = a.dim[v], head = c / (dim / 8), ch = 8 * (c - head * (dim / 8));
-    const glm_u32x4 x = *reinterpret_cast<const glm_u32x4 *>(a.rows[v] + token * a.stride[v] + 8 * c);
-    const long long row =
-        ((long long)(slot / a.page) * a.heads + head) * a.page + slot % a.page;
-    if constexpr (FMT == GLM_FMT_BF16) {
-      *reinterpret_cast<glm_u32x4 *>((uint16_t *)a.cache[v] + row * dim + ch) = x;
-    } else {
-      float f[8];
-      int m = 0;  // largest finite magnitude's bf16 bits
+    const uint16_t *rows = a.rows[v] + 8 * c;
+    for (int t0 = blockIdx.x * tokens + tl; t0 < a.N; t0 += kFlight * step) {
+      int slot[kFlight];
+      glm_u32x4 x[kFlight];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t bits = j % 2 ? x[j / 2] >> 16 : x[j / 2] & 0xffffu;
-        const int mag = bits & 0x7fffu;
-        m = mag < 0x7f80 ? max(m, mag) : m;
-        f[j] = mag < 0x7f80 ? __uint_as_float(bits << 16) : __uint_as_float(0x7fc00000u);
+      for (int j = 0; j < kFlight; ++j) {
+        const int token = t0 + j * step;
+        slot[j] = token < a.N ? a.slots[token] : -1;
+        x[j] = *reinterpret_cast<const glm_u32x4 *>(rows + (long long)min(token, a.N - 1) * a.stride[v]);
       }
-      m = max(m, __builtin_amdgcn_mov_dpp(m, 0xB1, 0xf, 0xf, true));
-      m = max(m, __builtin_amdgcn_mov_dpp(m, 0x4E, 0xf, 0xf, true));
-      int e = (m >> 7) - 127 - 8 + ((m & 0x7f) > 0x60 ? 1 : 0);
-      e = max(e, -124);
-      const float inv = __uint_as_float((uint32_t)(127 - e) << 23);  // 2^-e, exact
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= inv;  // exact, within 448
-      typedef short s16x2 __attribute__((ext_vector_type(2)));
-      uint32_t code[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        s16x2 o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, f[4 * j], f[4 * j + 1], 1.0f, false);
-        o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, f[4 * j + 2], f[4 * j + 3], 1.0f, true);
-        code[j] = __builtin_bit_cast(uint32_t, o);
+      for (int j = 0; j < kFlight; ++j) {
+        if ((uint32_t)slot[j] >= (uint32_t)a.num_slots) continue;  // (a token's lanes leave together)
+        int page = (int)__umulhi((uint32_t)slot[j], a.page_magic), off = slot[j] - page * a.page;
+        if (off >= a.page) {  // the quotient is one short at most
+          ++page;
+          off -= a.page;
+        }
+        const long long row = ((long long)page * a.heads + head) * a.page + off;
+        if constexpr (FMT == GLM_FMT_BF16) {
+          *reinterpret_cast<glm_u32x4 *>((uint16_t *)a.cache[v] + row * dim + ch) = x[j];
+        } else {
+          uint32_t scale;
+          *reinterpret_cast<uint2 *>((uint8_t *)a.cache[v] + row * dim + ch) = mxfp8_codes(x[j], scale);
+          if ((c & 3) == 0) a.scales[v][row * (dim / 32) + ch / 32] = (uint8_t)scale;
+        }
       }
-      *reinterpret_cast<uint2 *>((uint8_t *)a.cache[v] + row * dim + ch) = uint2{code[0], code[1]};
-      if ((threadIdx.x & 3) == 0) a.scales[v][row * (dim / 32) + ch / 32] = (uint8_t)(e + 127);
     }
   }
 }
@@ -318,6 +341,7 @@ extern "C" int glm_cache_write(void *stream, const uint16_t *keys, int64_t key_s
               GLM_ERR_UNSUPPORTED_SHAPE,
               "cache_write: widths %d and %d must be multiples of %d up to 1024", key_dim,
               value_dim, unit);
+  GLM_REQUIRE(N <= 1 << 30, GLM_ERR_UNSUPPORTED_SHAPE, "cache_write: %d tokens, at most 2^30", N);
   GLM_REQUIRE((long long)num_pages * page_size * kv_heads <= INT_MAX && kv_heads <= 65536,
               GLM_ERR_UNSUPPORTED_SHAPE, "cache_write: %d pages of %d x %d rows pass 32 bits",
               num_pages, kv_heads, page_size);
@@ -332,9 +356,12 @@ extern "C" int glm_cache_write(void *stream, const uint16_t *keys, int64_t key_s
   if (N == 0) return GLM_OK;
   glm::CacheWrite a{{keys, values}, {key_stride, value_stride}, {key_cache, value_cache},
                     {key_scales, value_scales}, {key_dim, value_dim}, slots, N, kv_heads,
-                    page_size, num_pages * page_size};
-  const long long blocks = ((long long)N * kv_heads * (key_dim + value_dim) / 8 + 255) / 256;
-  const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536));
+                    page_size, num_pages * page_size,
+                    page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / page_size)};
+  // as many workgroups as the chip holds: a thread's channels serve all its tokens
+  const int pieces = kv_heads * (key_dim + value_dim) / 8, tokens = pieces < 256 ? 256 / pieces : 1;
+  const int blocks = (N - 1) / tokens + 1;
+  const dim3 grid(blocks < 2048 ? blocks : 2048);
   if (mx)
     hipLaunchKernelGGL(glm::cache_write_kernel<GLM_FMT_MXFP8>, grid, dim3(256), 0,
                        (hipStream_t)stream, a);

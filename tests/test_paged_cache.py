@@ -101,6 +101,7 @@ def test_step_refusals(code, change):
     (INVALID, {"fmt": native.GLM_FMT_MXFP8, "ksc": FAKE}), (INVALID, {"N": -1}), (INVALID, {"page": 0}),
     (SHAPE, {"dk": 100}), (SHAPE, {"dv": 4}), (SHAPE, {"dk": 2048, "ks": 4096}), (INVALID, {"ks": 255}),
     (INVALID, {"ks": 260}), (INVALID, {"vs": 248}), (INVALID, {"keys": ODD}), (INVALID, {"vc": ODD}),
+    (SHAPE, {"N": (1 << 30) + 1}), (SHAPE, {"heads": 65537, "ks": 1 << 24, "vs": 1 << 24}),
     (SHAPE, {"dk": 40, "fmt": native.GLM_FMT_MXFP8, "ksc": FAKE, "vsc": FAKE}),
     (SHAPE, {"num_pages": 1 << 27}),
 ])
