@@ -369,22 +369,31 @@ __device__ __forceinline__ void page_of(const AttnArgs &a, int pos, int &block, 
     off -= a.page;
   }
 }
-__device__ __forceinline__ TileRows tile_rows(const AttnArgs &a, const int32_t *table, int head, int p,
-                                              int end, int n) {
-  TileRows t;
+struct TileIds {
+  int id[2], off[2];
+};
+__device__ __forceinline__ TileIds tile_ids(const AttnArgs &a, const int32_t *table, int p, int end, int n) {
+  TileIds t;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    int block;
+    page_of(a, min(p + 16 * u + n, end - 1), block, t.off[u]);
+    t.id[u] = table[block];
+  }
+  return t;
+}
+__device__ __forceinline__ TileRows tile_rows(const AttnArgs &a, const TileIds &t, int head, int p, int end,
+                                              int n) {
+  TileRows r;
   uint32_t seen[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int pos = p + 16 * u + n;
-    int block, off;
-    page_of(a, min(pos, end - 1), block, off);
-    const int id = table[block];
-    const bool fine = (uint32_t)id < (uint32_t)a.num_pages;
-    t.row[u] = fine ? (id * a.kv_heads + head) * a.page + off : 0;
-    seen[u] = (uint32_t)__ballot(fine && pos < end) & 0xffffu;
+    const bool fine = (uint32_t)t.id[u] < (uint32_t)a.num_pages;
+    r.row[u] = fine ? (t.id[u] * a.kv_heads + head) * a.page + t.off[u] : 0;
+    seen[u] = (uint32_t)__ballot(fine && p + 16 * u + n < end) & 0xffffu;
   }
-  t.seen = seen[0] | (seen[1] << 16);
-  return t;
+  r.seen = seen[0] | (seen[1] << 16);
+  return r;
 }
 
 template <int DK, int DV, int MT, int FMT, int OCC>
@@ -409,6 +418,11 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
   for (AttnItem it; walk.next(a, it);) {
     const int head = it.head, r0 = it.rb * 16 * MT;
     const int32_t *table = a.tables + (long long)it.b * a.max_blocks;
+    const int end = min(it.t1 * kAttnTile, it.len);
+    const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
+    int p = it.t0 * kAttnTile + 32 * wave;
+    // (ahead of the query rows: loads return in order, and the first keys wait for these)
+    const TileIds ids = tile_ids(a, table, max(0, min(p, end - 1)), max(1, end), n);
     glm_bf16x8 q[MT][DK / 32];
     int tok[MT];  // this lane's rows' new token
 #pragma unroll
@@ -430,19 +444,15 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
 #pragma unroll
       for (int d = 0; d < DV / 16; ++d) acc[d][m] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const int end = min(it.t1 * kAttnTile, it.len);
-    const int all_see = it.len - (a.q_len - 1);  // positions below it are seen by every token
-
-    int p = it.t0 * kAttnTile + 32 * wave;
     if (p < end) {
-      TileRows cur = tile_rows(a, table, head, p, end, n), nxt = cur;
+      TileRows cur = tile_rows(a, ids, head, p, end, n), nxt = cur;
       KRow k[2];
       VRow v[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) k[u].load(a.kc, a.ks, cur.row[u], DK, quad);
 #pragma unroll
       for (int u = 0; u < 2; ++u) v[u].load(vc, vs, cur.row[u], vdim, quad);
-      if (p + 128 < end) nxt = tile_rows(a, table, head, p + 128, end, n);
+      if (p + 128 < end) nxt = tile_rows(a, tile_ids(a, table, p + 128, end, n), head, p + 128, end, n);
       while (true) {
         const bool more = p + 128 < end;
         glm_f32x4 s[2][MT];
@@ -554,7 +564,7 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
         if (!more) break;
         p += 128;
         cur = nxt;
-        if (p + 128 < end) nxt = tile_rows(a, table, head, p + 128, end, n);
+        if (p + 128 < end) nxt = tile_rows(a, tile_ids(a, table, p + 128, end, n), head, p + 128, end, n);
       }
     }
 
@@ -1180,9 +1190,10 @@ bool group_widths(int key_dim, int value_dim) {
 
 template <int DK, int DV, int FMT>
 void launch_group(hipStream_t s, dim3 grid, const glm::AttnArgs &a) {
-  // two workgroups a CU where the registers allow it
+  // workgroups a CU: what the registers allow (and attn_sizes counts on)
   if (a.rows == 16)
-    hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 1, FMT, (DV > 128 ? 1 : 2)>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 1, FMT, (DV > 128 ? 1 : DK == 64 ? 3 : 2)>), grid,
+                       dim3(256), 0, s, a);
   else if constexpr (DK <= 192) {
     if (a.rows == 32)
       hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 2, FMT, (DK > 128 ? 1 : 2)>), grid, dim3(256), 0, s, a);
@@ -1228,9 +1239,9 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
     z.form = kAttnGroup;
     const int most = key_dim == 64 ? 64 : key_dim <= 192 ? 32 : 16;  // rows that fit the registers
     z.rows = R <= 16 || most == 16 ? 16 : R <= 32 || most == 32 ? 32 : 64;
-    slots = 512;
-    z.over = 1;
-    z.min_part = z.over + 2;
+    slots = 256 * (value_dim > 128 ? 1 : key_dim == 64 && z.rows == 16 ? 3 : 2);
+    z.over = 2;
+    z.min_part = 3;
   } else {
     z.form = kAttnAny;
     z.rows = 1;
