@@ -1118,52 +1118,83 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
 
 // ---------------------------------------------------------------------------
 // The pairs of request and kv head that were cut: out = sum_i 2^(m_i - m) acc_i
-// / sum_i 2^(m_i - m) l_i over their pieces in order, with a running maximum,
-// so that a piece's weight and sums are asked for together.  A part has the
-// end of at most one of them, so the launch goes by parts and not by requests.
-// A thread has four channels of a row and eight pieces in flight.
+// / sum_i 2^(m_i - m) l_i over their pieces, with a running maximum, so that a
+// piece's weight and sums are asked for together.  A part has the end of at
+// most one of them, so the launch goes by parts and not by requests.  A thread
+// has four channels of a row; a workgroup's four waves take every fourth piece
+// of the same 64 such quads, two in flight each, and are joined in LDS in
+// their order.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-  constexpr int kFlight = 8;
+  constexpr int kFlight = 2, kWaves = 4;
+  __shared__ glm_f32x4 s_acc[kWaves][kWave];
+  __shared__ float2 s_ml[kWaves][kWave];
   const int4 pair = a.plan[blockIdx.y];
   if (pair.x < 0) return;
   const int b = pair.x, head = pair.y, g0 = pair.z, g1 = blockIdx.y;  // (g0: the pair's beginning)
   const int R = attn_rows(a), group = a.heads / a.kv_heads, quads = a.dv / 4;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < R * quads; i += gridDim.x * 256) {
-    const int r = i / quads, ch = 4 * (i - r * quads);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int i0 = blockIdx.x * kWave; i0 < R * quads; i0 += gridDim.x * kWave) {
+    const int i = min(i0 + lane, R * quads - 1), r = i / quads, ch = 4 * (i - r * quads);
+    const int block = r / a.rows, row = r - block * a.rows;
     float m = -INFINITY, l = 0.0f;
     glm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int g = g0; g <= g1; g += kFlight) {
+    for (int g = g0 + wave; g <= g1; g += kWaves * kFlight) {
       float2 ml[kFlight];
       glm_f32x4 part[kFlight];
-      float next = m;
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        const int from = min(g + j, g1);
-        const long long at =
-            ((long long)(2 * from + (from == g0)) * a.rblocks + r / a.rows) * a.rows + r % a.rows;
+        const int from = g + kWaves * j;
+        ml[j] = float2{-INFINITY, 0.0f};
+        part[j] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+        if (from > g1) continue;  // (uniform)
+        const long long at = ((long long)(2 * from + (from == g0)) * a.rblocks + block) * a.rows + row;
         ml[j] = *reinterpret_cast<const float2 *>(a.ml + 2 * at);
         part[j] = *reinterpret_cast<const glm_f32x4 *>(a.part + at * a.dv + ch);
-        next = fmaxf(next, ml[j].x);
       }
+      float next = m;
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) next = fmaxf(next, ml[j].x);
       const float from = next == -INFINITY ? 0.0f : next, keep = exp2f(m - from);
       m = next;
       l *= keep;
       acc *= keep;
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        if (g + j > g1) break;
         const float scale = exp2f(ml[j].x - from);
         l += scale * ml[j].y;
         acc += scale * part[j];
       }
     }
-    uint32_t o[4];
+    s_ml[wave][lane] = float2{m, l};
+    s_acc[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && i0 + lane < R * quads) {
+      float2 ml[kWaves];
+      float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = f32_to_bf16(l == 0.0f ? 0.0f : acc[j] / l);
-    const int t = r / group;
-    uint16_t *out = a.out + (((long long)b * a.q_len + t) * a.heads + head * group + r % group) * a.dv + ch;
-    *reinterpret_cast<uint2 *>(out) = uint2{o[0] | (o[1] << 16), o[2] | (o[3] << 16)};
+      for (int w = 0; w < kWaves; ++w) {
+        ml[w] = s_ml[w][lane];
+        top = fmaxf(top, ml[w].x);
+      }
+      const float from = top == -INFINITY ? 0.0f : top;
+      l = 0.0f;
+      acc = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float scale = exp2f(ml[w].x - from);
+        l += scale * ml[w].y;
+        acc += scale * s_acc[w][lane];
+      }
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = f32_to_bf16(l == 0.0f ? 0.0f : acc[j] / l);
+      const int t = r / group;
+      uint16_t *out =
+          a.out + (((long long)b * a.q_len + t) * a.heads + head * group + r - t * group) * a.dv + ch;
+      *reinterpret_cast<uint2 *>(out) = uint2{o[0] | (o[1] << 16), o[2] | (o[3] << 16)};
+    }
+    __syncthreads();
   }
 }
 
@@ -1194,12 +1225,8 @@ void launch_group(hipStream_t s, dim3 grid, const glm::AttnArgs &a) {
   if (a.rows == 16)
     hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 1, FMT, (DV > 128 ? 1 : DK == 64 ? 3 : 2)>), grid,
                        dim3(256), 0, s, a);
-  else if constexpr (DK <= 192) {
-    if (a.rows == 32)
-      hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 2, FMT, (DK > 128 ? 1 : 2)>), grid, dim3(256), 0, s, a);
-    else if constexpr (DK == 64)
-      hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 4, FMT, 1>), grid, dim3(256), 0, s, a);
-  }
+  else if constexpr (DK <= 192)
+    hipLaunchKernelGGL((glm::attn_group_kernel<DK, DV, 2, FMT, (DK > 128 ? 1 : 2)>), grid, dim3(256), 0, s, a);
 }
 
 template <int FMT>
@@ -1237,9 +1264,8 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
     z.min_part = z.over + 1;
   } else if (group_widths(key_dim, value_dim)) {
     z.form = kAttnGroup;
-    const int most = key_dim == 64 ? 64 : key_dim <= 192 ? 32 : 16;  // rows that fit the registers
-    z.rows = R <= 16 || most == 16 ? 16 : R <= 32 || most == 32 ? 32 : 64;
-    slots = 256 * (value_dim > 128 ? 1 : key_dim == 64 && z.rows == 16 ? 3 : 2);
+    z.rows = R <= 16 || key_dim > 192 ? 16 : 32;
+    slots = 256 * (key_dim > 192 || (key_dim > 128 && z.rows == 32) ? 1 : key_dim == 64 && z.rows == 16 ? 3 : 2);
     z.over = 2;
     z.min_part = 3;
   } else {
@@ -1247,7 +1273,7 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
     z.rows = 1;
     slots = 2048;
     z.over = 1;
-    z.min_part = z.over + 4;
+    z.min_part = 2;
   }
   z.rblocks = (R + z.rows - 1) / z.rows;
   z.parts = slots / z.rblocks > 1 ? slots / z.rblocks : 1;
@@ -1360,7 +1386,7 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
     // as many workgroups as have work for few cut pairs, and no more than fill the chip for many
     const int quads = q_len * (heads / kv_heads) * value_dim / 4;
     const int pairs = z.parts < (long long)B * kv_heads ? z.parts : B * kv_heads;
-    int ways = (quads + 255) / 256;
+    int ways = (quads + 63) / 64;
     if (ways > 4096 / pairs) ways = 4096 / pairs > 1 ? 4096 / pairs : 1;
     hipLaunchKernelGGL(glm::attn_join_kernel, dim3(ways, z.parts), dim3(256), 0, s, a);
     GLM_LAUNCH_CHECK("attn_join_kernel");

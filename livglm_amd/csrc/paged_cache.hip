@@ -23,7 +23,7 @@ namespace glm {
 // ---------------------------------------------------------------------------
 constexpr int kStepThreads = 1024;
 constexpr int kStepRequests = 4096;  // three sums per request in LDS
-constexpr int kStepTokens = 4096;
+constexpr int kStepTokens = 8192;
 
 struct StepSums {
   long long given, need, tokens;
