@@ -662,37 +662,155 @@ __device__ __forceinline__ void load_to_lds(const void *src, void *lds) {
     __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
 }
 
-// V^T operands of eight 16-channel tiles from LDS at at[i % 4] + 1024 (i / 4): the transposing reads
-// of positions 0 .. 15 and, HI bytes on, 16 .. 31, and the wait for them in one statement.  (Of the
-// builtin's reads the compiler does not know the place, and waits for every load on its way to LDS.)
-template <int HI>
-__device__ __forceinline__ void lds_read_tr8(glm_bf16x8 (&v)[8], const uint32_t (&at)[4]) {
-  bf16x4 lo[8], hi[8];
+// A wave's scores of 16 positions: 18 steps of 32 channels, even ones from `km` and odd ones from `km1` (1 KB
+// on every second step), the last two from `kr` and `kr1`; eight operands are on their way ahead of the
+// products.  One statement, since the compiler waits for all reads wherever it needs the first of eight, and
+// for what it holds in flight there is no place in it that could be overwritten.  (v208 .. v239 hold the
+// operands; the no-ops are what a vector instruction has to stay behind a product's last.)
+__device__ __forceinline__ glm_f32x4 latent_scores(const glm_bf16x8 (&q)[18], uint32_t km, uint32_t km1,
+                                                   uint32_t kr, uint32_t kr1) {
+  glm_f32x4 even, odd;
   asm volatile(
-      "ds_read_b64_tr_b16 %0, %16\n\t"
-      "ds_read_b64_tr_b16 %8, %16 offset:%20\n\t"
-      "ds_read_b64_tr_b16 %1, %17\n\t"
-      "ds_read_b64_tr_b16 %9, %17 offset:%20\n\t"
-      "ds_read_b64_tr_b16 %2, %18\n\t"
-      "ds_read_b64_tr_b16 %10, %18 offset:%20\n\t"
-      "ds_read_b64_tr_b16 %3, %19\n\t"
-      "ds_read_b64_tr_b16 %11, %19 offset:%20\n\t"
-      "ds_read_b64_tr_b16 %4, %16 offset:1024\n\t"
-      "ds_read_b64_tr_b16 %12, %16 offset:%21\n\t"
-      "ds_read_b64_tr_b16 %5, %17 offset:1024\n\t"
-      "ds_read_b64_tr_b16 %13, %17 offset:%21\n\t"
-      "ds_read_b64_tr_b16 %6, %18 offset:1024\n\t"
-      "ds_read_b64_tr_b16 %14, %18 offset:%21\n\t"
-      "ds_read_b64_tr_b16 %7, %19 offset:1024\n\t"
-      "ds_read_b64_tr_b16 %15, %19 offset:%21\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(lo[4]), "=&v"(lo[5]),
-        "=&v"(lo[6]), "=&v"(lo[7]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3]),
-        "=&v"(hi[4]), "=&v"(hi[5]), "=&v"(hi[6]), "=&v"(hi[7])
-      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "i"(HI), "i"(HI + 1024)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7);
+      "ds_read_b128 v[224:227], %2 offset:0\n\t"
+      "ds_read_b128 v[228:231], %3 offset:0\n\t"
+      "ds_read_b128 v[232:235], %2 offset:1024\n\t"
+      "ds_read_b128 v[236:239], %3 offset:1024\n\t"
+      "ds_read_b128 v[240:243], %2 offset:2048\n\t"
+      "ds_read_b128 v[244:247], %3 offset:2048\n\t"
+      "ds_read_b128 v[248:251], %2 offset:3072\n\t"
+      "ds_read_b128 v[252:255], %3 offset:3072\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[224:227], %6, 0\n\t"
+      "ds_read_b128 v[224:227], %2 offset:4096\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[228:231], %7, 0\n\t"
+      "ds_read_b128 v[228:231], %3 offset:4096\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[232:235], %8, %0\n\t"
+      "ds_read_b128 v[232:235], %2 offset:5120\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[236:239], %9, %1\n\t"
+      "ds_read_b128 v[236:239], %3 offset:5120\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[240:243], %10, %0\n\t"
+      "ds_read_b128 v[240:243], %2 offset:6144\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[244:247], %11, %1\n\t"
+      "ds_read_b128 v[244:247], %3 offset:6144\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[248:251], %12, %0\n\t"
+      "ds_read_b128 v[248:251], %2 offset:7168\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[252:255], %13, %1\n\t"
+      "ds_read_b128 v[252:255], %3 offset:7168\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[224:227], %14, %0\n\t"
+      "ds_read_b128 v[224:227], %4\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[228:231], %15, %1\n\t"
+      "ds_read_b128 v[228:231], %5\n\t"
+      "s_waitcnt lgkmcnt(7)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[232:235], %16, %0\n\t"
+      "s_waitcnt lgkmcnt(6)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[236:239], %17, %1\n\t"
+      "s_waitcnt lgkmcnt(5)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[240:243], %18, %0\n\t"
+      "s_waitcnt lgkmcnt(4)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[244:247], %19, %1\n\t"
+      "s_waitcnt lgkmcnt(3)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[248:251], %20, %0\n\t"
+      "s_waitcnt lgkmcnt(2)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[252:255], %21, %1\n\t"
+      "s_waitcnt lgkmcnt(1)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[224:227], %22, %0\n\t"
+      "s_waitcnt lgkmcnt(0)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[228:231], %23, %1\n\t"
+      "s_nop 7\n\t"
+      "s_nop 7\n\t"
+      : "=&v"(even), "=&v"(odd)
+      : "v"(km), "v"(km1), "v"(kr), "v"(kr1), "v"(q[0]), "v"(q[1]), "v"(q[2]), "v"(q[3]), "v"(q[4]), "v"(q[5]), "v"(q[6]), "v"(q[7]), "v"(q[8]), "v"(q[9]), "v"(q[10]), "v"(q[11]), "v"(q[12]), "v"(q[13]), "v"(q[14]), "v"(q[15]), "v"(q[16]), "v"(q[17])
+      : "memory", "v224", "v225", "v226", "v227", "v228", "v229", "v230", "v231", "v232", "v233",
+        "v234", "v235", "v236", "v237", "v238", "v239", "v240", "v241", "v242", "v243", "v244",
+        "v245", "v246", "v247", "v248", "v249", "v250", "v251", "v252", "v253", "v254", "v255");
+  return even + odd;
+}
+
+// The products with a wave's 16 channel tiles of the values: tile d's transposed operand comes from at[d % 4]
+// + 1024 (d / 4), positions 16 .. 31 from 16 KB on, six tiles ahead of the products.  One statement, as above.
+__device__ __forceinline__ void latent_values(glm_f32x4 (&acc)[16], const glm_bf16x8 &prob,
+                                              const uint32_t (&at)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 v[224:225], %17 offset:0\n\t"
+      "ds_read_b64_tr_b16 v[226:227], %17 offset:16384\n\t"
+      "ds_read_b64_tr_b16 v[228:229], %18 offset:0\n\t"
+      "ds_read_b64_tr_b16 v[230:231], %18 offset:16384\n\t"
+      "ds_read_b64_tr_b16 v[232:233], %19 offset:0\n\t"
+      "ds_read_b64_tr_b16 v[234:235], %19 offset:16384\n\t"
+      "ds_read_b64_tr_b16 v[236:237], %20 offset:0\n\t"
+      "ds_read_b64_tr_b16 v[238:239], %20 offset:16384\n\t"
+      "ds_read_b64_tr_b16 v[240:241], %17 offset:1024\n\t"
+      "ds_read_b64_tr_b16 v[242:243], %17 offset:17408\n\t"
+      "ds_read_b64_tr_b16 v[244:245], %18 offset:1024\n\t"
+      "ds_read_b64_tr_b16 v[246:247], %18 offset:17408\n\t"
+      "ds_read_b64_tr_b16 v[248:249], %19 offset:1024\n\t"
+      "ds_read_b64_tr_b16 v[250:251], %19 offset:17408\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %0, v[224:227], %16, %0\n\t"
+      "ds_read_b64_tr_b16 v[224:225], %20 offset:1024\n\t"
+      "ds_read_b64_tr_b16 v[226:227], %20 offset:17408\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %1, v[228:231], %16, %1\n\t"
+      "ds_read_b64_tr_b16 v[228:229], %17 offset:2048\n\t"
+      "ds_read_b64_tr_b16 v[230:231], %17 offset:18432\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %2, v[232:235], %16, %2\n\t"
+      "ds_read_b64_tr_b16 v[232:233], %18 offset:2048\n\t"
+      "ds_read_b64_tr_b16 v[234:235], %18 offset:18432\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %3, v[236:239], %16, %3\n\t"
+      "ds_read_b64_tr_b16 v[236:237], %19 offset:2048\n\t"
+      "ds_read_b64_tr_b16 v[238:239], %19 offset:18432\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %4, v[240:243], %16, %4\n\t"
+      "ds_read_b64_tr_b16 v[240:241], %20 offset:2048\n\t"
+      "ds_read_b64_tr_b16 v[242:243], %20 offset:18432\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %5, v[244:247], %16, %5\n\t"
+      "ds_read_b64_tr_b16 v[244:245], %17 offset:3072\n\t"
+      "ds_read_b64_tr_b16 v[246:247], %17 offset:19456\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %6, v[248:251], %16, %6\n\t"
+      "ds_read_b64_tr_b16 v[248:249], %18 offset:3072\n\t"
+      "ds_read_b64_tr_b16 v[250:251], %18 offset:19456\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %7, v[224:227], %16, %7\n\t"
+      "ds_read_b64_tr_b16 v[224:225], %19 offset:3072\n\t"
+      "ds_read_b64_tr_b16 v[226:227], %19 offset:19456\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %8, v[228:231], %16, %8\n\t"
+      "ds_read_b64_tr_b16 v[228:229], %20 offset:3072\n\t"
+      "ds_read_b64_tr_b16 v[230:231], %20 offset:19456\n\t"
+      "s_waitcnt lgkmcnt(12)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %9, v[232:235], %16, %9\n\t"
+      "s_waitcnt lgkmcnt(10)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %10, v[236:239], %16, %10\n\t"
+      "s_waitcnt lgkmcnt(8)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %11, v[240:243], %16, %11\n\t"
+      "s_waitcnt lgkmcnt(6)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %12, v[244:247], %16, %12\n\t"
+      "s_waitcnt lgkmcnt(4)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %13, v[248:251], %16, %13\n\t"
+      "s_waitcnt lgkmcnt(2)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %14, v[224:227], %16, %14\n\t"
+      "s_waitcnt lgkmcnt(0)\n\t"
+      "v_mfma_f32_16x16x32_bf16 %15, v[228:231], %16, %15\n\t"
+      "s_nop 7\n\t"
+      "s_nop 7\n\t"
+      : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]), "+v"(acc[4]), "+v"(acc[5]), "+v"(acc[6]), "+v"(acc[7]), "+v"(acc[8]), "+v"(acc[9]), "+v"(acc[10]), "+v"(acc[11]), "+v"(acc[12]), "+v"(acc[13]), "+v"(acc[14]), "+v"(acc[15])
+      : "v"(prob), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+      : "memory", "v224", "v225", "v226", "v227", "v228", "v229", "v230", "v231", "v232", "v233",
+        "v234", "v235", "v236", "v237", "v238", "v239", "v240", "v241", "v242", "v243", "v244",
+        "v245", "v246", "v247", "v248", "v249", "v250", "v251");
 }
 
 // At most LEFT of the wave's loads are outstanding, and nothing is moved across.
@@ -726,7 +844,6 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   constexpr bool kMx = L::kMx;
   constexpr int kG = L::kG;
   constexpr int kD = DV / 32;  // 16-channel tiles of a wave's half
-  constexpr int kKeys = 8;     // operands of the scores read ahead
   constexpr int kLoads = kMx ? 4 : 5;  // of a wave and tile (bf16: a pair's middle block is both's)
   static_assert(DK == 576 && DV == 512, "nine blocks of 64 channels; MXFP8: 36 pieces of 16 codes, 18 scales a row");
   // (one dynamic array: for reads of a static one the compiler waits for every load on its way to it)
@@ -929,27 +1046,10 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
       const uint8_t *km = smem + main * L::kMain + pos * kG * 1024 + at;
       const uint8_t *km1 = smem + main * L::kMain + pos * kG * 1024 + (at ^ 64);
       const uint8_t *kr = smem + L::kRestAt + rest * L::kRest + pos * 1024;
-      const auto key = [&](int i) {
-        const uint8_t *from = i < DV / 32 ? (i & 1 ? km1 : km) + (i >> 1) * 1024 : kr + (at ^ (64 * (i & 1)));
-        return *reinterpret_cast<const glm_bf16x8 *>(from);
+      const auto lds = [](const uint8_t *p) {
+        return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
       };
-      glm_f32x4 even = zero, odd = zero;
-      // a ring of operands: one pair is read when the pair kKeys before it has been multiplied
-      glm_bf16x8 kf[kKeys];
-#pragma unroll
-      for (int i = 0; i < kKeys; ++i) kf[i] = key(i);
-#pragma unroll
-      for (int i = 0; i < DK / 32; i += 2) {
-        __builtin_amdgcn_sched_barrier(0);  // (else each read is waited for by itself)
-        even = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i % kKeys], q[i], even, 0, 0, 0);
-        odd = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[(i + 1) % kKeys], q[i + 1], odd, 0, 0, 0);
-        if (i + kKeys < DK / 32) {
-          kf[i % kKeys] = key(i + kKeys);
-          kf[(i + 1) % kKeys] = key(i + 1 + kKeys);
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      return even + odd;
+      return latent_scores(q, lds(km), lds(km1), lds(kr + at), lds(kr + (at ^ 64)));
     };
 
     if (begin < end) {  // the first tile's scores
@@ -966,6 +1066,11 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         __builtin_amdgcn_sched_barrier(0);
       }
       if ((k & 3) == 3 && wave < 2) put_rows(s_id[64 * wave + this_lane()], ((k >> 2) + 2) & 1);
+      // positions that only later tokens see: a value there must not meet an earlier token's zero weight (it
+      // may be an infinity or a NaN), so they stay out of the matrix product
+      const bool fringe = p + 32 > all_see && a.q_len > 1;  // (uniform)
+      uint8_t *kv = smem + main_k * L::kMain;
+      glm_bf16x8 prob;
       if (active) {
         const int l0 = this_lane();
         const glm_f32x4 other = s_x[k & 1][rg][half ^ 1][l0];
@@ -984,9 +1089,6 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
             if (!((bits >> at) & 1u) || at >= left) x[i] = -INFINITY;
           }
         }
-        // positions that only later tokens see: a value there must not meet an earlier token's zero
-        // weight (it may be an infinity or a NaN), so they stay out of the matrix product
-        const bool fringe = p + 32 > all_see && a.q_len > 1;  // (uniform)
         // the next tile's scores beside this one's probabilities (past the item's end: of whatever
         // tile follows, and not used)
         const glm_f32x4 next_own = scores(plus(main_k, 1, L::kMains), rest_k);
@@ -997,7 +1099,6 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         const float from = next == -INFINITY ? 0.0f : next;
         const float keep = __builtin_amdgcn_exp2f(top - from);
         const int l = this_lane(), common = all_see - p - 4 * (l >> 4);
-        glm_bf16x8 prob;
         sum *= keep;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -1017,33 +1118,6 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
           for (int d = 0; d < kD; ++d) acc[d] *= keep;
         }
         top = next;
-        // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
-        const uint8_t *kv = smem + main_k * L::kMain;
-        const int vt = 4 * (l >> 4) + ((l >> 2) & 3);
-        const int vread = ((vt >> 3) * kG + half * kD / 4) * 1024 + (vt & 7) * 128 +
-                          ((((l & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (l & 1);
-        const uint32_t kv0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)kv;
-#pragma unroll
-        for (int d = 0; d < kD; d += 8) {
-          const uint32_t from = kv0 + (d >> 2) * 1024;
-          const uint32_t at[4] = {from + vread, from + (vread ^ 32), from + (vread ^ 64), from + (vread ^ 96)};
-          glm_bf16x8 v[8];
-          lds_read_tr8<2 * kG * 1024>(v, at);
-          if (fringe) {
-            glm_u32x4 mask;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int c = 16 * (j / 2) + 2 * (j % 2);
-              mask[j] = (c < common ? 0xffffu : 0u) | (c + 1 < common ? 0xffff0000u : 0u);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              v[i] = __builtin_bit_cast(glm_bf16x8, __builtin_bit_cast(glm_u32x4, v[i]) & mask);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            acc[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i], prob, acc[d + i], 0, 0, 0);
-        }
         if (fringe) {
           // one position after the other: the rows of the tokens that see it add its weight's share
           for (int j = max(0, all_see - p); j < min(32, it.len - p); ++j) {
@@ -1069,6 +1143,23 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
             }
           }
         }
+      }
+      if (fringe) {  // zeros in their place, once every wave has added them
+        meet();
+        const int l = this_lane();
+        for (int j = max(0, all_see - p) + wave; j < 32; j += 8)
+          *reinterpret_cast<glm_u32x4 *>(kv + ((j >> 3) * kG + (l >> 3)) * 1024 + (j & 7) * 128 + 16 * (l & 7)) =
+              glm_u32x4{0, 0, 0, 0};
+        meet();
+      }
+      if (active) {
+        // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
+        const int l = this_lane(), vt = 4 * (l >> 4) + ((l >> 2) & 3);
+        const int vread = ((vt >> 3) * kG + half * kD / 4) * 1024 + (vt & 7) * 128 +
+                          ((((l & 3) >> 1) ^ (vt & 7)) << 4) + 8 * (l & 1);
+        const uint32_t kv0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)kv;
+        const uint32_t at[4] = {kv0 + vread, kv0 + (vread ^ 32), kv0 + (vread ^ 64), kv0 + (vread ^ 96)};
+        latent_values(acc, prob, at);
       }
       wait_loads<kLoads>();  // bf16: tile k + 2; MXFP8: the codes of tile k + 2
       if constexpr (kMx) {
