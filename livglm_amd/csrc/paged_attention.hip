@@ -904,61 +904,81 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     const unsigned long long seen = __ballot(fine);
     if ((lane & 31) == 0) s_seen[slot][2 * (wave & 1) + (lane >> 5)] = (uint32_t)(seen >> (lane & 32));
   };
-  // bf16: into the tile's places `main` and `rest`; MXFP8: into the place `main` of codes
-  const auto load_rows = [&](int tile, int main, int rest) {
+  // The cache rows that this lane loads a part of.  bf16: eight rows a wave, eight lanes a row; MXFP8: four
+  // rows of 36 pieces of 16 codes: 16 lanes a row twice, then four lanes a row, and 9 a row for the scales.
+  struct Rows {
+    int a, b, c;
+  };
+  const auto rows_of = [&](int tile) {
     const int l = this_lane();
     const int *rows = s_row[(tile >> 2) & 1][tile & 3];
+    if constexpr (!kMx)
+      return Rows{rows[8 * rg + (l >> 3)], 0, 0};
+    else
+      return Rows{rows[4 * wave + (l >> 4)], rows[4 * wave + ((l & 15) >> 2)], rows[4 * wave + min(l / 9, 3)]};
+  };
+  // bf16: into the tile's places `main` and `rest`; MXFP8: into the place `main` of codes
+  const auto load_rows = [&](const Rows &rows, int main, int rest) {
+    const int l = this_lane();
     if constexpr (!kMx) {
-      const int row = rows[8 * rg + (l >> 3)], g0 = 4 * half;
-      const uint8_t *src = (row < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)row * (2 * DK)) +
+      const int g0 = 4 * half;
+      const uint8_t *src = (rows.a < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)rows.a * (2 * DK)) +
                            (((l & 7) ^ (l >> 3)) << 4) + 128 * g0;
       uint8_t *to = smem + main * L::kMain + (rg * kG + g0) * 1024;
 #pragma unroll
       for (int i = 0; i < 4; ++i) load_to_lds<16>(src + 128 * i, to + 1024 * i);
       load_to_lds<16>(src + 512, half ? smem + L::kRestAt + rest * L::kRest + rg * 1024 : to + 4096);
     } else {
-      // four rows of 36 pieces: 16 lanes a row twice, then four lanes a row; 9 lanes a row for the scales
       uint8_t *raw = smem + L::kRawAt + (main * 8 + wave) * L::kRaw;
-      const auto code = [&](int t, int c) {
-        const int row = rows[4 * wave + t];
+      const auto code = [&](int row, int c) {
         return (row < 0 ? attn_zero_row : (const uint8_t *)a.kc + (long long)row * DK) + 16 * c;
       };
-      const uint8_t *src = code(l >> 4, l & 15);
+      const uint8_t *src = code(rows.a, l & 15);
       load_to_lds<16>(src, raw);
       load_to_lds<16>(src + 256, raw + 1024);
-      const uint8_t *last = code((l & 15) >> 2, 32 + (l & 3));
-      const int st = min(l / 9, 3), row = rows[4 * wave + st];
-      const uint8_t *sc = (row < 0 ? attn_zero_row : a.ks + (long long)row * (DK / 32)) + 2 * (l - 9 * st);
+      const uint8_t *last = code(rows.b, 32 + (l & 3));
+      const uint8_t *sc = (rows.c < 0 ? attn_zero_row : a.ks + (long long)rows.c * (DK / 32)) +
+                          2 * (l - 9 * min(l / 9, 3));
       if (l < 16) load_to_lds<16>(last, raw + 2048);
       if (l < 36) load_to_lds<2>(sc, raw + 4 * DK);
     }
   };
-  // MXFP8: this wave's rows of a tile, from codes to bf16: piece c of row t to the tile's pieces 2 c,
-  // 2 c + 1 (the swizzle keeps them neighbours)
-  const auto convert = [&](int from, int main, int rest) {
-    const int l = this_lane(), t = l >> 4, c = l & 15;
+  // MXFP8: this wave's rows of a tile: lane (t, c) = (l / 16, l % 16) has pieces c and 16 + c of row t, and
+  // four codes of its last 64
+  struct Codes {
+    glm_u32x4 v0, v1;
+    uint32_t last, s0, s1, s2;
+  };
+  const auto codes_of = [&](int from) {
+    const int l = this_lane();
     const uint8_t *raw = smem + L::kRawAt + (from * 8 + wave) * L::kRaw;
-    const auto swizzled = [&](int pos, int c) {
-      return (pos & 7) * 128 + (((2 * (c & 3)) ^ (pos & 7)) << 4);
+    const uint8_t *sc = raw + 4 * DK + 36 * (l >> 4);
+    const int at = 4 * ((l >> 2) & 3);
+    return Codes{*reinterpret_cast<const glm_u32x4 *>(raw + 16 * l),
+                 *reinterpret_cast<const glm_u32x4 *>(raw + 1024 + 16 * l),
+                 *reinterpret_cast<const uint32_t *>(raw + 2048 + 4 * l),
+                 *reinterpret_cast<const uint32_t *>(sc + at), *reinterpret_cast<const uint32_t *>(sc + at + 16),
+                 *reinterpret_cast<const uint32_t *>(sc + 32)};
+  };
+  // .. to bf16 (exact): piece c to the tile's pieces 2 c, 2 c + 1 (the swizzle keeps them neighbours)
+  const auto convert = [&](const Codes &codes, int main, int rest) {
+    const int l = this_lane(), c = l & 15, pos = (4 * wave + (l >> 4)) & 7;
+    const auto scale = [](uint32_t two, int second) { return e8m0_to_f32((two >> (8 * (second & 1))) & 0xffu); };
+    const auto put = [&](uint8_t *to, const glm_u32x4 &v, float sc) {
+      const int at = pos * 128 + (((2 * (c & 3)) ^ pos) << 4);
+      *reinterpret_cast<glm_bf16x8 *>(to + at) = mxfp8_words_to_bf16x8(v[0], v[1], sc);
+      *reinterpret_cast<glm_bf16x8 *>(to + (at ^ 16)) = mxfp8_words_to_bf16x8(v[2], v[3], sc);
     };
-    const auto put = [&](uint8_t *tile, int at, const glm_u32x4 &v, uint32_t two) {
-      const float sc = e8m0_to_f32((two >> (8 * ((l >> 1) & 1))) & 0xffu);
-      *reinterpret_cast<glm_bf16x8 *>(tile + at) = mxfp8_words_to_bf16x8(v[0], v[1], sc);
-      *reinterpret_cast<glm_bf16x8 *>(tile + (at ^ 16)) = mxfp8_words_to_bf16x8(v[2], v[3], sc);
-    };
-    const uint8_t *sc = raw + 4 * DK + 36 * t + 4 * (c >> 2);
-    const glm_u32x4 v0 = *reinterpret_cast<const glm_u32x4 *>(raw + 16 * l);
-    const glm_u32x4 v1 = *reinterpret_cast<const glm_u32x4 *>(raw + 1024 + 16 * l);
-    const uint32_t s0 = *reinterpret_cast<const uint32_t *>(sc);
-    const uint32_t s1 = *reinterpret_cast<const uint32_t *>(sc + 16);
     // (a wave's four positions lie in one block of eight)
     uint8_t *tile = smem + main * L::kMain + ((wave >> 1) * kG + (c >> 2)) * 1024;
-    put(tile, swizzled(4 * wave + t, c), v0, s0);
-    put(tile + 4096, swizzled(4 * wave + t, c), v1, s1);
-    if (l < 16)
-      put(smem + L::kRestAt + rest * L::kRest + (wave >> 1) * 1024, swizzled(4 * wave + (c >> 2), c & 3),
-          *reinterpret_cast<const glm_u32x4 *>(raw + 2048 + 16 * l),
-          *reinterpret_cast<const uint32_t *>(raw + 4 * DK + 36 * (c >> 2) + 32));
+    put(tile, codes.v0, scale(codes.s0, l >> 1));
+    put(tile + 4096, codes.v1, scale(codes.s1, l >> 1));
+    const float sc = scale(codes.s2, c >> 3);
+    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes.last, sc, false);
+    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes.last, sc, true);
+    *reinterpret_cast<uint2 *>(smem + L::kRestAt + rest * L::kRest + (wave >> 1) * 1024 + pos * 128 +
+                               (((c >> 1) ^ pos) << 4) + 8 * (c & 1)) =
+        uint2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
   };
   // this wave's LDS writes are done, and every wave has come here
   const auto meet = [&]() {
@@ -1005,17 +1025,19 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) seen[i] = seen_of(i);
-  load_rows(0, 0, 0);
-  load_rows(1, 1, 1);
+  load_rows(rows_of(0), 0, 0);
+  load_rows(rows_of(1), 1, 1);
+  Rows rows{};  // bf16: of tile k + 3
   if constexpr (kMx) {
     wait_loads<kLoads>();
-    convert(0, 0, 0);
-    load_rows(2, 0, 0);
+    convert(codes_of(0), 0, 0);
+    load_rows(rows_of(2), 0, 0);
     wait_loads<kLoads>();
-    convert(1, 1, 1);
-    load_rows(3, 1, 0);
+    convert(codes_of(1), 1, 1);
+    load_rows(rows_of(3), 1, 0);
   } else {
-    load_rows(2, 2, 2);
+    load_rows(rows_of(2), 2, 2);
+    rows = rows_of(3);
     wait_loads<kLoads>();
   }
   meet();
@@ -1062,7 +1084,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     for (int p = begin; p < end; p += 32, ++k) {
       const uint32_t last_seen = seen_of(k + kAhead);
       if constexpr (!kMx) {
-        load_rows(k + 3, plus(main_k, 3, 4), plus(rest_k, 2, 3));
+        load_rows(rows, plus(main_k, 3, 4), plus(rest_k, 2, 3));
         __builtin_amdgcn_sched_barrier(0);
       }
       if ((k & 3) == 3 && wave < 2) put_rows(s_id[64 * wave + this_lane()], ((k >> 2) + 2) & 1);
@@ -1152,6 +1174,13 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
               glm_u32x4{0, 0, 0, 0};
         meet();
       }
+      // MXFP8: tile k + 2's codes and tile k + 4's rows, asked for before the products with the values
+      Codes codes;
+      if constexpr (kMx) {
+        wait_loads<kLoads>();
+        codes = codes_of(k & 1);
+      }
+      rows = rows_of(k + 4);
       if (active) {
         // transposing reads: position 4 quad + n / 4, channels 4 (n % 4) of 16 d
         const int l = this_lane(), vt = 4 * (l >> 4) + ((l >> 2) & 3);
@@ -1161,13 +1190,13 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         const uint32_t at[4] = {kv0 + vread, kv0 + (vread ^ 32), kv0 + (vread ^ 64), kv0 + (vread ^ 96)};
         latent_values(acc, prob, at);
       }
-      wait_loads<kLoads>();  // bf16: tile k + 2; MXFP8: the codes of tile k + 2
       if constexpr (kMx) {
-        convert(k & 1, plus(main_k, 2, 3), rest_k ^ 1);
+        convert(codes, plus(main_k, 2, 3), rest_k ^ 1);
         __builtin_amdgcn_sched_barrier(0);
         load_ids();
-        load_rows(k + 4, k & 1, 0);
+        load_rows(rows, k & 1, 0);
       } else {
+        wait_loads<kLoads>();  // tile k + 2
         load_ids();
       }
       meet();
