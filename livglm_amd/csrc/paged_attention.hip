@@ -19,6 +19,9 @@ namespace glm {
 
 constexpr int kAttnTile = 64;  // positions; parts are cut between tiles
 constexpr float kLog2e = 1.44269504088896341f;
+// A running maximum is raised where a score passes it by more than this (in powers of two), so that the sums
+// are seldom rescaled: weights then lie up to 2^8, which costs neither bf16 nor the sums in 32 bits any digit.
+constexpr float kAttnSlack = 8.0f;
 
 // Sums over the wave by DPP: row_shr 1, 2, 4, 8, then a row's last lane to the next rows.
 __device__ __forceinline__ int wave_scan(int v) {  // inclusive
@@ -492,15 +495,16 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
           float mx = x[0];
 #pragma unroll
           for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-          const float next = fmaxf(top[m], max_over_quads(mx));
-          const float from = next == -INFINITY ? 0.0f : next;
-          if (__any(next != top[m])) {
-            const float keep = __builtin_amdgcn_exp2f(top[m] - from);
+          mx = max_over_quads(mx);
+          if (__any(mx > top[m] + kAttnSlack)) {
+            const float next = fmaxf(top[m], mx);
+            const float keep = __builtin_amdgcn_exp2f(top[m] - (next == -INFINITY ? 0.0f : next));
+            top[m] = next;
             sum[m] *= keep;
 #pragma unroll
             for (int d = 0; d < DV / 16; ++d) acc[d][m] *= keep;
           }
-          top[m] = next;
+          const float from = top[m] == -INFINITY ? 0.0f : top[m];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float e = __builtin_amdgcn_exp2f(x[i] - from);
@@ -976,9 +980,9 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
     const float sc = scale(codes.s2, c >> 3);
     const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes.last, sc, false);
     const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes.last, sc, true);
-    *reinterpret_cast<uint2 *>(smem + L::kRestAt + rest * L::kRest + (wave >> 1) * 1024 + pos * 128 +
-                               (((c >> 1) ^ pos) << 4) + 8 * (c & 1)) =
-        uint2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    // (a vector of bf16: for a uint2 the compiler waits for every load on its way to LDS)
+    *reinterpret_cast<bf16x4 *>(smem + L::kRestAt + rest * L::kRest + (wave >> 1) * 1024 + pos * 128 +
+                                (((c >> 1) ^ pos) << 4) + 8 * (c & 1)) = bf16x4{lo[0], lo[1], hi[0], hi[1]};
   };
   // this wave's LDS writes are done, and every wave has come here
   const auto meet = [&]() {
@@ -1117,11 +1121,17 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         float mx = x[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-        const float next = fmaxf(top, max_over_quads(mx));
-        const float from = next == -INFINITY ? 0.0f : next;
-        const float keep = __builtin_amdgcn_exp2f(top - from);
+        mx = max_over_quads(mx);
+        if (__any(mx > top + kAttnSlack)) {
+          const float next = fmaxf(top, mx);
+          const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.0f : next));
+          top = next;
+          sum *= keep;
+#pragma unroll
+          for (int d = 0; d < kD; ++d) acc[d] *= keep;
+        }
+        const float from = top == -INFINITY ? 0.0f : top;
         const int l = this_lane(), common = all_see - p - 4 * (l >> 4);
-        sum *= keep;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[i] = __builtin_amdgcn_exp2f(x[i] - from);
@@ -1135,11 +1145,6 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         }
         own = next_own;
         s_x[(k + 1) & 1][rg][half][l] = own;
-        if (__any(next != top)) {
-#pragma unroll
-          for (int d = 0; d < kD; ++d) acc[d] *= keep;
-        }
-        top = next;
         if (fringe) {
           // one position after the other: the rows of the tokens that see it add its weight's share
           for (int j = max(0, all_see - p); j < min(32, it.len - p); ++j) {
