@@ -9,6 +9,13 @@
 // request, keeping a running maximum and sum.  What a cut leaves of a request
 // on either side goes to the workspace as (m, l, acc), and a second launch
 // (attn_join_kernel) joins it.
+//
+// Three forms, by the widths alone: the grouped one for heads of 64, 128, 256
+// or 192 / 128 channels, the latent one for rows of 576 channels whose first
+// 512 are the values, and one for all other widths.  The last form on the
+// others' cases: 3554 us for 93 (32 ragged requests, 32 heads over 8 of 128),
+// 328 for 31 (45 requests, 16 heads of 64), 93 for 13 (one request of 517),
+// 15.9 ms for 58 us (64 latent requests).
 #include <climits>
 #include <cmath>
 
@@ -47,7 +54,7 @@ struct AttnArgs {
   uint32_t page_magic;   // floor(2^32 / page), at most 2^32 - 1
   int rows, rblocks;    // query rows a workgroup takes, blocks of them in a kv head
   int parts, min_part;  // most parts, fewest units of a part
-  int over;  // what a request costs a workgroup beside its tiles (its rows, the first loads' latency, the result), in tiles
+  int over;  // what a request costs beside its tiles (rows, the first loads' latency, the result), in tiles
   float scale_log2;
 };
 
@@ -189,6 +196,8 @@ __device__ __forceinline__ float cache_value(const void *cache, const uint8_t *s
 // ---------------------------------------------------------------------------
 // Any widths: one row a workgroup, 256 positions at a time.  A thread forms
 // one position's score, then the threads share the channels of the values.
+// Bound by latency and by the scalar products (no matrix instructions): 250 us
+// for 32 requests of 100 .. 4000 positions, 8 heads over 2 of 96 channels.
 // ---------------------------------------------------------------------------
 constexpr int kAnyDim = 1024;
 
@@ -282,7 +291,11 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // as soon as the products with this one's are formed, its values as soon as
 // these are in LDS, its page numbers a tile earlier.
 // Bound by the cache's bytes; a wave holds 32 positions of keys and values in
-// flight.
+// flight.  Measured, 128 channels in bf16: 91 us for 461 MB of 32 ragged
+// requests (5.1 TB/s), 197 us for 1.07 GB of two requests of 131000 positions
+// (5.4 TB/s; a large copy moves 4.9 TB/s, counting both ways).  96 requests of
+// two tokens on an MXFP8 cache, 164 MB: 46 us, where conversion and rescaling
+// show; 45 requests of 16 heads of 64 channels, 102 MB: 30 us.
 // Masks: rows of a tile see the same positions but where it ends, so only
 // tiles with a position that some row does not see take the masked form.
 // ---------------------------------------------------------------------------
@@ -636,19 +649,24 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
 // probabilities), and each adds half of the channels to the sums.  A wave
 // alone with its rows would need 128 registers for the sums beside 72 for the
 // rows, which left none to read ahead with; a pair's 64 do.  Products and
-// operand layouts are those of attn_group_kernel.
+// operand layouts are those of attn_group_kernel, but a value that only later
+// tokens see is added by itself and cleared in LDS before the matrix product.
 // LDS holds a tile as blocks of 1 KB, 8 positions x 64 channels, the 16-byte
 // piece c of position t at 128 t + 16 (c ^ t): a wave's load of one block
 // reads eight whole 128-byte lines, and neither the products' reads (16
 // positions x 4 pieces) nor the transposing ones (8 positions x 2 pieces a
 // half wave) meet on a bank.  Rows go from the cache to LDS directly: bf16
 // into a ring of four such tiles, by swizzled source addresses; MXFP8 codes
-// and scales into a ring of three, from where the wave that loaded them
-// converts them (exact) into one of two tiles.  Three tiles (two) are in
-// flight, across the requests of a workgroup's part too; positions that are
+// and scales into a ring of two, from where the wave that loaded them converts
+// them (exact) into a ring of three.  Three tiles (two) are in flight, across the requests of a workgroup's part too; positions that are
 // not seen read a row of zeros.
-// Bound by the cache's bytes for some 64 rows and by LDS reads beyond: 34 KB
-// for each wave's 34 MFMAs.
+// Measured: 64 bf16 requests of 100 .. 8100 positions, 64 heads, 127 MB: 56 us,
+// of which 12 are the join (partial results of 39 MB are a third of all
+// traffic); a tile of 32 positions takes 1.7 us against 1.5 for its bytes alone.
+// Five MXFP8 requests of 20000 .. 50000 positions, two tokens, 59 GFLOP: 135 us
+// (0.44 PFLOP/s).  There no unit is full: a turn's 4900 cycles have 1090 of
+// matrix instructions, some 2000 of LDS reads (34 KB a wave) and 1900 of vector
+// instructions, and eight waves that meet at its end overlap them by halves.
 // ---------------------------------------------------------------------------
 __device__ uint8_t attn_zero_row[2048];
 
@@ -667,10 +685,9 @@ __device__ __forceinline__ void load_to_lds(const void *src, void *lds) {
 }
 
 // A wave's scores of 16 positions: 18 steps of 32 channels, even ones from `km` and odd ones from `km1` (1 KB
-// on every second step), the last two from `kr` and `kr1`; eight operands are on their way ahead of the
-// products.  One statement, since the compiler waits for all reads wherever it needs the first of eight, and
-// for what it holds in flight there is no place in it that could be overwritten.  (v208 .. v239 hold the
-// operands; the no-ops are what a vector instruction has to stay behind a product's last.)
+// on every second step), the last two from `kr` and `kr1`.  Eight operands, in v224 .. v255, are on their way
+// ahead of the products.  One statement with its waits: the compiler waits for all eight where it needs the
+// first.  (The no-ops at the end: a vector instruction has to stay that far behind a product it reads.)
 __device__ __forceinline__ glm_f32x4 latent_scores(const glm_bf16x8 (&q)[18], uint32_t km, uint32_t km1,
                                                    uint32_t kr, uint32_t kr1) {
   glm_f32x4 even, odd;
@@ -732,7 +749,9 @@ __device__ __forceinline__ glm_f32x4 latent_scores(const glm_bf16x8 (&q)[18], ui
       "s_nop 7\n\t"
       "s_nop 7\n\t"
       : "=&v"(even), "=&v"(odd)
-      : "v"(km), "v"(km1), "v"(kr), "v"(kr1), "v"(q[0]), "v"(q[1]), "v"(q[2]), "v"(q[3]), "v"(q[4]), "v"(q[5]), "v"(q[6]), "v"(q[7]), "v"(q[8]), "v"(q[9]), "v"(q[10]), "v"(q[11]), "v"(q[12]), "v"(q[13]), "v"(q[14]), "v"(q[15]), "v"(q[16]), "v"(q[17])
+      : "v"(km), "v"(km1), "v"(kr), "v"(kr1), "v"(q[0]), "v"(q[1]), "v"(q[2]), "v"(q[3]), "v"(q[4]),
+        "v"(q[5]), "v"(q[6]), "v"(q[7]), "v"(q[8]), "v"(q[9]), "v"(q[10]), "v"(q[11]), "v"(q[12]),
+        "v"(q[13]), "v"(q[14]), "v"(q[15]), "v"(q[16]), "v"(q[17])
       : "memory", "v224", "v225", "v226", "v227", "v228", "v229", "v230", "v231", "v232", "v233",
         "v234", "v235", "v236", "v237", "v238", "v239", "v240", "v241", "v242", "v243", "v244",
         "v245", "v246", "v247", "v248", "v249", "v250", "v251", "v252", "v253", "v254", "v255");
@@ -740,7 +759,8 @@ __device__ __forceinline__ glm_f32x4 latent_scores(const glm_bf16x8 (&q)[18], ui
 }
 
 // The products with a wave's 16 channel tiles of the values: tile d's transposed operand comes from at[d % 4]
-// + 1024 (d / 4), positions 16 .. 31 from 16 KB on, six tiles ahead of the products.  One statement, as above.
+// + 1024 (d / 4), and positions 16 .. 31 from 16 KB on.  Seven tiles are on their way, in one statement as above;
+// the compiler would also wait for every load on its way to LDS, not knowing the place of a transposing read.
 __device__ __forceinline__ void latent_values(glm_f32x4 (&acc)[16], const glm_bf16x8 &prob,
                                               const uint32_t (&at)[4]) {
   asm volatile(
@@ -810,7 +830,9 @@ __device__ __forceinline__ void latent_values(glm_f32x4 (&acc)[16], const glm_bf
       "v_mfma_f32_16x16x32_bf16 %15, v[228:231], %16, %15\n\t"
       "s_nop 7\n\t"
       "s_nop 7\n\t"
-      : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]), "+v"(acc[4]), "+v"(acc[5]), "+v"(acc[6]), "+v"(acc[7]), "+v"(acc[8]), "+v"(acc[9]), "+v"(acc[10]), "+v"(acc[11]), "+v"(acc[12]), "+v"(acc[13]), "+v"(acc[14]), "+v"(acc[15])
+      : "+&v"(acc[0]), "+&v"(acc[1]), "+&v"(acc[2]), "+&v"(acc[3]), "+&v"(acc[4]), "+&v"(acc[5]),
+        "+&v"(acc[6]), "+&v"(acc[7]), "+&v"(acc[8]), "+&v"(acc[9]), "+&v"(acc[10]), "+&v"(acc[11]),
+        "+&v"(acc[12]), "+&v"(acc[13]), "+&v"(acc[14]), "+&v"(acc[15])
       : "v"(prob), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
       : "memory", "v224", "v225", "v226", "v227", "v228", "v229", "v230", "v231", "v232", "v233",
         "v234", "v235", "v236", "v237", "v238", "v239", "v240", "v241", "v242", "v243", "v244",
@@ -849,7 +871,8 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
   constexpr int kG = L::kG;
   constexpr int kD = DV / 32;  // 16-channel tiles of a wave's half
   constexpr int kLoads = kMx ? 4 : 5;  // of a wave and tile (bf16: a pair's middle block is both's)
-  static_assert(DK == 576 && DV == 512, "nine blocks of 64 channels; MXFP8: 36 pieces of 16 codes, 18 scales a row");
+  // (nine blocks of 64 channels; MXFP8: 36 pieces of 16 codes and 18 scales a row)
+  static_assert(DK == 576 && DV == 512, "widths that the lanes' shares are made for");
   // (one dynamic array: for reads of a static one the compiler waits for every load on its way to it)
   extern __shared__ __align__(16) uint8_t smem[];
   glm_f32x4(*const s_x)[4][2][64] = reinterpret_cast<glm_f32x4(*)[4][2][64]>(smem + L::kX);
@@ -1248,7 +1271,11 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
 // most one of them, so the launch goes by parts and not by requests.  A thread
 // has four channels of a row; a workgroup's four waves take every fourth piece
 // of the same 64 such quads, two in flight each, and are joined in LDS in
-// their order.
+// their order.  Bound by latency for few requests and by the pieces' bytes for
+// many (39 MB in 12 us).  Four waves a quad and not one, with eight pieces in
+// flight: 35 us for 51 (one request of 32000 positions, 63 pieces a head); two
+// in flight for four or eight: 57.8, 59.9, 64.9 us (64 latent requests, some
+// four pieces each), against 35.8, 34.1, 33.5 (the request of 32000).
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int kFlight = 2, kWaves = 4;
@@ -1384,20 +1411,31 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
   if (latent && key_dim == 576 && value_dim == 512) {
     z.form = kAttnLatent;
     z.rows = 64;
-    slots = 256;
+    slots = 256;  // (its LDS lets one workgroup on a CU)
+    // 64 requests of 100 .. 8100 positions with 1, 2, 4 units: 65.4, 58.9, 59.5 us
     z.over = 2;
-    z.min_part = z.over + 1;
+    z.min_part = 3;  // one request of 8000 with 3, 5: 32.4, 36.3 us
   } else if (group_widths(key_dim, value_dim)) {
     z.form = kAttnGroup;
+    // 32 rows share a tile's operands where there are more than 16 and the registers hold them (256 channels:
+    // not).  40 requests with 16, 32 rows a workgroup: 24 rows of 128 channels 33.1, 28.6 us, 64 rows 51.1,
+    // 38.5; 48 rows of 64 channels 41.3, 32.8 (64 rows a workgroup: 43.2); 64 rows of 192 channels 61.9, 44.6
     z.rows = R <= 16 || key_dim > 192 ? 16 : 32;
+    // workgroups a CU, as many as its registers hold: 45 requests of 64 channels with 2, 3: 33.9, 31.0 us;
+    // 32 rows of 192 channels with 2, 1: 40.7, 31.6 (one is resident)
     slots = 256 * (key_dim > 192 || (key_dim > 128 && z.rows == 32) ? 1 : key_dim == 64 && z.rows == 16 ? 3 : 2);
+    // units 1, 2, 3 beside the tiles: 57.0, 50.2, 49.1 us (96 requests, MXFP8), 33.9, 33.4, 36.1 (45 requests
+    // of 64 channels), 96.0, 95.3, 97.2 (32 ragged ones)
     z.over = 2;
+    // one request with parts of 3, 6 or more units: 12.8, 14.6 us (517 positions), 12.6, 16.0 (2000), 18.1,
+    // 17.4 (8000)
     z.min_part = 3;
   } else {
     z.form = kAttnAny;
     z.rows = 1;
-    slots = 2048;
+    slots = 2048;  // (1024: the same)
     z.over = 1;
+    // parts of 2, 5 units: 43, 82 us (one request of 517 positions), 251, 244 (32 of 100 .. 4000)
     z.min_part = 2;
   }
   z.rblocks = (R + z.rows - 1) / z.rows;
@@ -1508,7 +1546,8 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
     launch_attention<GLM_FMT_BF16>(s, grid, z.form, a);
   GLM_LAUNCH_CHECK("paged_attention");
   if (z.parts > 1) {
-    // as many workgroups as have work for few cut pairs, and no more than fill the chip for many
+    // as many workgroups as have work for few cut pairs, and for many no more than fill the chip twice: 64
+    // latent requests with 2048, 4096, 8192 in all: 61.0, 59.9, 62.3 us
     const int quads = q_len * (heads / kv_heads) * value_dim / 4;
     const int pairs = z.parts < (long long)B * kv_heads ? z.parts : B * kv_heads;
     int ways = (quads + 63) / 64;

@@ -18,8 +18,10 @@ namespace glm {
 // is then a thread's own work: it finds its request by bisection in LDS.
 // One workgroup, since a page given back may be taken in the same call and
 // only a workgroup can wait for its own writes; bound by latency: the
-// requests' loads, the pages', the tables'.  The tokens' slots ride in this
-// launch up to kStepTokens and take a launch over all CUs beyond.
+// requests' loads, the pages', the tables': 6 us for 64 requests of one token,
+// of a call's 9.4.  The tokens' slots ride in this launch up to kStepTokens and
+// take a launch over all CUs beyond: 12.7 us for 13.9 at 6748 tokens, 18.4 for
+// 13.5 at 14010.
 // ---------------------------------------------------------------------------
 constexpr int kStepThreads = 1024;
 constexpr int kStepRequests = 4096;  // three sums per request in LDS
@@ -203,7 +205,10 @@ __global__ __launch_bounds__(256) void cache_slots_kernel(
 // rounding rules of glm_mx_quantize may cut a group's largest element by up
 // to 29 %, which a softmax would see; -124, because 2^-9 2^-124 is bf16's own
 // smallest step.  An infinity or a NaN is stored as E4M3's NaN and does not
-// enter amax.  Bound by the bytes.  A slot outside the cache is skipped.
+// enter amax.  A slot outside the cache is skipped.
+// Bound by the bytes: 13.4 us for 7777 tokens of 8 heads of 128 + 128 channels
+// into MXFP8 (48 MB, 3.6 TB/s with the launch), 101 us for 60000 into bf16
+// (491 MB, 4.9 TB/s); 2.9 us for 64 tokens, which is latency.
 // ---------------------------------------------------------------------------
 struct CacheWrite {
   const uint16_t *rows[2];  // keys, values
@@ -358,7 +363,8 @@ extern "C" int glm_cache_write(void *stream, const uint16_t *keys, int64_t key_s
                     {key_scales, value_scales}, {key_dim, value_dim}, slots, N, kv_heads,
                     page_size, num_pages * page_size,
                     page_size == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / page_size)};
-  // as many workgroups as the chip holds: a thread's channels serve all its tokens
+  // as many workgroups as the chip holds, a thread's channels serve all its tokens: 7777 tokens with at most
+  // 1024, 2048, no limit: 13.6, 14.0, 15.4 us, 60000 tokens 101.5, 101.4, 112.5
   const int pieces = kv_heads * (key_dim + value_dim) / 8, tokens = pieces < 256 ? 256 / pieces : 1;
   const int blocks = (N - 1) / tokens + 1;
   const dim3 grid(blocks < 2048 ? blocks : 2048);
