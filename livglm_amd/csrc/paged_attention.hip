@@ -510,7 +510,7 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
           for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
           mx = max_over_quads(mx);
           if (__any(mx > top[m] + kAttnSlack)) {
-            const float next = fmaxf(top[m], mx);
+            const float next = mx > top[m] + kAttnSlack ? mx : top[m];  // (no row depends on another)
             const float keep = __builtin_amdgcn_exp2f(top[m] - (next == -INFINITY ? 0.0f : next));
             top[m] = next;
             sum[m] *= keep;
@@ -1146,7 +1146,7 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
         for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
         mx = max_over_quads(mx);
         if (__any(mx > top + kAttnSlack)) {
-          const float next = fmaxf(top, mx);
+          const float next = mx > top + kAttnSlack ? mx : top;  // (no row depends on another)
           const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.0f : next));
           top = next;
           sum *= keep;

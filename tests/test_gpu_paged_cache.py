@@ -68,7 +68,7 @@ def random_state(rng, B, page, width, pool):
 
 @pytest.mark.parametrize("B, page, width, tokens", [
     (1, 16, 4, 10), (1, 1, 1, 0), (3, 5, 9, 40), (64, 16, 64, 70), (65, 7, 30, 4096), (300, 16, 20, 4097),
-    (1000, 1, 8, 2000), (1025, 64, 3, 9000), (4096, 16, 6, 20001),
+    (1000, 1, 8, 2000), (1025, 64, 3, 9000), (4096, 16, 6, 20001), (70, 16, 20, 8192), (70, 16, 20, 8193),
 ])
 @pytest.mark.parametrize("alias", [False, True])
 def test_step(C, B, page, width, tokens, alias):
@@ -337,6 +337,76 @@ def test_attend_scores(C, latent, spread, scale):
     rng = np.random.default_rng(13)
     shape = (16, 1, 576, 512) if latent else (8, 2, 128, 128)
     attend_case(C, rng, 2, 1, *shape, [700, 33], 16, "bf16", latent, spread=spread, scale=scale)
+
+
+@pytest.mark.parametrize("latent", [False, True])
+@pytest.mark.parametrize("step", [0.02, 0.3, 5.0, -0.3])
+def test_attend_rising_scores(C, latent, step):
+    """Scores that rise by `step` powers of two from position to position, in small steps and in large ones, beside
+    rows whose scores fall: a running maximum lags behind, leaps, or stays, row by row."""
+    rng = np.random.default_rng(15)
+    n, page, heads = 1000, 16, 16
+    dk, dv = (576, 512) if latent else (128, 128)
+    kc, _, kv = make_cache(rng, 63, 1, page, dk, "bf16")
+    vc, vv = (None, kv[..., :dv]) if latent else make_cache(rng, 63, 1, page, dv, "bf16")[::2]
+    tables = np.arange(63, dtype=np.int32).reshape(1, -1)
+    at = torch.arange(63 * page, device="cuda").view(63, 1, page)
+    kc[..., dk - 1] = (at % 256).to(torch.bfloat16)  # (integers to 256 are exact)
+    kc[..., dk - 2] = (at // 256).to(torch.bfloat16)
+    q = torch.from_numpy(rng.standard_normal((1, 1, heads, dk), np.float32)).to(torch.bfloat16).cuda()
+    for h in range(heads):
+        sign = 1.0 if h % 2 else -1.0
+        q[0, 0, h, dk - 1] = sign * step * 0.6931 * dk ** 0.5
+        q[0, 0, h, dk - 2] = sign * step * 0.6931 * dk ** 0.5 * 256
+    lens = np.array([n])
+    got = f64(C.paged_attention(q, kc, vc, dev(tables), dev(lens), scale=dk ** -0.5, value_dim=dv))
+    kv = f64(kc)
+    want, size, reach = P.attend(f64(q), kv, kv[..., :dv] if latent else vv, tables, lens, dk ** -0.5)
+    delta = (dk + 4) * 2.0 ** -24 * reach + 2.0 ** -22 * (1 + reach)
+    tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2 * delta[..., None] + (n + 64) * 2.0 ** -24) * 1.01 * size + 1e-30
+    assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_attend_rows_do_not_depend_on_others(C, latent):
+    """A head's result is the same bits whatever the other heads of its kv head ask."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    dk, dv = (576, 512) if latent else (128, 128)
+    kc = torch.randn((60, 1, 16, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    vc = None if latent else torch.randn((60, 1, 16, dv), generator=gen, device="cuda", dtype=torch.bfloat16)
+    table = torch.randperm(60, generator=gen, device="cuda").int().view(2, 30)
+    q = torch.randn((2, 16, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    lens = dev([471, 333])
+    want = C.paged_attention(q, kc, vc, table, lens, scale=0.5, value_dim=dv)
+    q[:, 3:] *= -7
+    got = C.paged_attention(q, kc, vc, table, lens, scale=0.5, value_dim=dv)
+    assert torch.equal(got[:, :3], want[:, :3])
+
+
+@pytest.mark.parametrize("latent", [False, True])
+def test_attend_on_two_streams_at_once(C, latent):
+    """Calls that run beside each other share no workspace."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    dk, dv = (576, 512) if latent else (128, 128)
+    kc = torch.randn((600, 1, 64, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    vc = None if latent else torch.randn((600, 1, 64, dv), generator=gen, device="cuda", dtype=torch.bfloat16)
+    calls = []
+    for i in range(2):
+        table = torch.randperm(600, generator=gen, device="cuda").int().view(4, 150)
+        q = torch.randn((4, 32, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+        lens = dev([9600, 5000 + i, 1, 7777])
+        calls.append((q, kc, vc, table, lens))
+    want = [C.paged_attention(*c, scale=0.05, value_dim=dv) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for s, c, g in zip(streams, calls, got):
+            with torch.cuda.stream(s):
+                g.append(C.paged_attention(*c, scale=0.05, value_dim=dv))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        assert all(torch.equal(w, g) for g in gs)
 
 
 def test_attend_many_requests(C):
