@@ -306,6 +306,8 @@ extern "C" int glm_cache_step(void *stream, const int32_t *new_lens, int B, int 
               GLM_ERR_INVALID_ARGUMENT, "cache_step: invalid sizes");
   GLM_REQUIRE(B <= glm::kStepRequests, GLM_ERR_UNSUPPORTED_SHAPE,
               "cache_step: %d requests, at most %d", B, glm::kStepRequests);
+  GLM_REQUIRE(max_tokens <= 1 << 30, GLM_ERR_UNSUPPORTED_SHAPE,
+              "cache_step: %d tokens, at most 2^30", max_tokens);
   GLM_REQUIRE((long long)num_pages * page_size <= INT_MAX &&
                   (long long)max_blocks * page_size <= INT_MAX,
               GLM_ERR_UNSUPPORTED_SHAPE,

@@ -13,7 +13,9 @@ then, for a sparse layer, this FFN block on the hyper-connection streams
 hyper-connection, the norm and its bf16 cast run as one library call
 (``glm_hc_pre``), the MoE layer and the residual update as another
 (``glm_moe_forward_hc``; at a few tokens the update rides in the layer's last
-kernel): two kernels before the MoE's own, no host synchronisation.  Attention is not part of this package.
+kernel): two kernels before the MoE's own, no host synchronisation.  Of the
+attention before it, this package has the cache and the products over it
+(``paged_cache``), not its projections.
 """
 
 from __future__ import annotations

@@ -1,9 +1,10 @@
 """GLM text configuration (subset that the routed-MoE layer reads).
 
 Mirrors ``GLMTextConfig`` of the reference (``model_config.py:11-54``): the
-MoE fields keep their names and meaning; the attention/mHC fields are kept with
-neutral defaults so that configurations written for the reference construct
-unchanged, but nothing here reads them.
+MoE fields keep their names and meaning; the others are kept with neutral
+defaults so that configurations written for the reference construct unchanged.
+Of those, the FFN site reads the mHC and norm fields, and
+``paged_cache.PagedKVCache.from_config`` the attention's head sizes.
 """
 
 from __future__ import annotations
@@ -100,6 +101,13 @@ class GLMTextConfig:
             hc_mult=int(text.get("hc_mult", 1)),
             hc_sinkhorn_iters=int(text.get("hc_sinkhorn_iters", 1)),
             hc_eps=float(text.get("hc_eps", 1e-6)),
+            # the attention's head sizes, for its cache; optional too, and null where a model has none
+            num_attention_heads=int(text.get("num_attention_heads") or 1),
+            num_key_value_heads=int(text.get("num_key_value_heads") or 1),
+            kv_lora_rank=int(text.get("kv_lora_rank") or 0),
+            qk_nope_head_dim=int(text.get("qk_nope_head_dim") or 0),
+            qk_rope_head_dim=int(text.get("qk_rope_head_dim") or 0),
+            v_head_dim=int(text.get("v_head_dim") or 0),
         )
         result.validate()
         return result

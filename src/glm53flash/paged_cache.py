@@ -142,8 +142,8 @@ def cache_step(new_lens: torch.Tensor, lens: torch.Tensor, blocks: torch.Tensor,
                             f"{lens.numel()} lens and {blocks.numel()} blocks")
     if num_free.numel() != 1:
         raise ContractError("cache_step: num_free must have one element")
-    if max_tokens < 0:
-        raise ContractError("cache_step: max_tokens is negative")
+    if not 0 <= max_tokens <= 1 << 30 or not 1 <= page_size < 1 << 31:
+        raise ContractError(f"cache_step: max_tokens {max_tokens} or page_size {page_size}")
     if kv_lens is not None:
         _check(kv_lens, "kv_lens", _I32, dev)
         if kv_lens.numel() < B:
@@ -169,7 +169,8 @@ def cache_write(keys: torch.Tensor, values: torch.Tensor | None, slots: torch.Te
                 value_scales: torch.Tensor | None = None) -> None:
     """Writes rows ``keys`` ``[N, kv_heads, key_dim]`` and ``values`` ``[N,
     kv_heads, value_dim]`` (bf16; slices of a fused projection are taken as they
-    are) to ``slots`` i32 ``[N]``; a slot outside the cache is skipped.
+    are) to ``slots`` i32 ``[N]``; a slot outside the cache is skipped.  Two
+    tokens with one slot leave a mixture of both rows there.
     ``values`` and ``value_cache`` are None for a latent cache.  With scales the
     caches are MXFP8."""
     key_stride = _token_rows(keys, "keys")

@@ -88,6 +88,7 @@ INVALID, SHAPE, WORKSPACE = (native.GLM_ERR_INVALID_ARGUMENT, native.GLM_ERR_UNS
                                      "positions", "status")],
     (INVALID, {"B": 0}), (INVALID, {"B": -1}), (SHAPE, {"B": 4097}), (INVALID, {"num_pages": 0}),
     (INVALID, {"page": 0}), (INVALID, {"max_blocks": 0}), (INVALID, {"max_tokens": -1}),
+    (SHAPE, {"max_tokens": (1 << 30) + 1}),
     (SHAPE, {"num_pages": 1 << 27}), (SHAPE, {"max_blocks": 1 << 27}),
 ])
 def test_step_refusals(code, change):
@@ -171,6 +172,16 @@ def test_python_objects():
     assert cache.keys.shape == (8, 2, 16, 128) and cache.values.shape == (8, 2, 16, 96)
     with pytest.raises(ContractError):
         C.PagedKVCache.from_config(GLMTextConfig(), table)
+    moe = {"hidden_size": 64, "moe_intermediate_size": 64, "n_routed_experts": 8, "num_experts_per_tok": 2,
+           "n_shared_experts": 1, "n_group": 1, "topk_group": 1, "routed_scaling_factor": 1.0}
+    read = GLMTextConfig.from_model_dict
+    cache = C.PagedKVCache.from_config(read({**moe, "kv_lora_rank": 256, "qk_rope_head_dim": 64}), table)
+    assert cache.latent and cache.keys.shape == (8, 1, 16, 320) and cache.value_dim == 256
+    cache = C.PagedKVCache.from_config(read({**moe, "kv_lora_rank": None, "num_key_value_heads": 4,
+                                             "qk_nope_head_dim": 96, "qk_rope_head_dim": 32, "v_head_dim": 64}), table)
+    assert cache.keys.shape == (8, 4, 16, 128) and cache.values.shape == (8, 4, 16, 64)
+    with pytest.raises(ContractError):
+        C.PagedKVCache.from_config(read(moe), table)
     with pytest.raises(ContractError):
         C.PagedKVCache(table, 1, 64, 128, latent=True)
     with pytest.raises(ContractError):
