@@ -712,7 +712,7 @@ size_t glm_paged_attention_workspace_bytes(int B, int q_len, int heads, int kv_h
  * value_cache NULL: a latent cache (value_dim <= key_dim).
  * Limits: heads % kv_heads == 0, heads <= 1024, q_len <= 16, B <= 65535, widths
  * multiples of 8 (MXFP8: 32) up to 1024, num_pages * page_size * kv_heads and
- * max_blocks * page_size + 64 < 2^31.  The workspace needs no clearing; calls
+ * max_blocks * page_size + 1024 < 2^31.  The workspace needs no clearing; calls
  * that may overlap need their own.
  */
 int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_stride, int B, int q_len,

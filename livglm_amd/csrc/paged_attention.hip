@@ -664,9 +664,13 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
 // of which 12 are the join (partial results of 39 MB are a third of all
 // traffic); a tile of 32 positions takes 1.7 us against 1.5 for its bytes alone.
 // Five MXFP8 requests of 20000 .. 50000 positions, two tokens, 59 GFLOP: 135 us
-// (0.44 PFLOP/s).  There no unit is full: a turn's 4900 cycles have 1090 of
-// matrix instructions, some 2000 of LDS reads (34 KB a wave) and 1900 of vector
-// instructions, and eight waves that meet at its end overlap them by halves.
+// (0.44 PFLOP/s).  There no unit is full: of a tile's 2.2 us a SIMD has matrix
+// instructions for a fifth and vector ones for less than half, and LDS reads
+// (34 KB a wave) take as much.  Without products and conversion the launches
+// take 94 us, without loads too 83: what bounds it is the issue of some 500
+// instructions a tile by two waves a SIMD that meet at its end (softmax,
+// exchange, addresses, conversion).  Half of the waves with the next tile's
+// scores behind the values: 139 us; with the conversion first: 157 for 154.
 // ---------------------------------------------------------------------------
 __device__ uint8_t attn_zero_row[2048];
 
@@ -1404,7 +1408,8 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
   if (B < 0 || q_len < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || key_dim < 1 ||
       value_dim < 1 || page_size < 1 || max_blocks < 1)
     return false;
-  if (B > 65535 || q_len > 16 || heads > 1024 || (long long)max_blocks * page_size > INT_MAX - glm::kAttnTile)
+  // (positions a turn ahead of the last, 256 at most, are formed in 32 bits)
+  if (B > 65535 || q_len > 16 || heads > 1024 || (long long)max_blocks * page_size > INT_MAX - 1024)
     return false;
   const int R = q_len * (heads / kv_heads);
   int slots;  // workgroups that the chip holds at once

@@ -120,6 +120,7 @@ def test_write_refusals(code, change):
     (INVALID, {"qs": 1028}), (INVALID, {"scale": float("nan")}), (INVALID, {"scale": float("inf")}),
     (INVALID, {"q": ODD}), (INVALID, {"out": ODD}), (INVALID, {"ws": ODD}), (WORKSPACE, {"nbytes": 16}),
     (SHAPE, {"num_pages": 1 << 27}), (SHAPE, {"max_blocks": 1 << 27}), (INVALID, {"max_blocks": 0}),
+    (SHAPE, {"max_blocks": (1 << 27) - 64}),
 ])
 def test_attend_refusals(code, change):
     assert native.load().glm_paged_attention(*_attend_args(**change)) == code
@@ -132,6 +133,7 @@ def test_attend_workspace():
     assert need > 0
     assert native.load().glm_paged_attention(*_attend_args(nbytes=need - 1 - 256)) == WORKSPACE
     assert size(2, 1, 7, 2, 128, 128, 0, 16, 4) == 0 and size(-1, 1, 8, 2, 128, 128, 0, 16, 4) == 0
+    assert size(1, 1, 8, 2, 128, 128, 0, 16, (1 << 27) - 64) == 0 < size(1, 1, 8, 2, 128, 128, 0, 16, (1 << 27) - 65)
     # bounded by the work that the chip takes at once, not by the batch
     assert 0 < size(4096, 1, 128, 8, 128, 128, 0, 16, 8192) < 512 << 20
     assert 0 < size(4096, 2, 128, 1, 576, 512, 1, 64, 2048) < 512 << 20
