@@ -416,6 +416,18 @@ def test_attend_many_requests(C):
     lens[5], lens[200] = 3000, 1500
     attend_case(C, rng, 261, 1, 4, 2, 64, 64, lens, 16)
     attend_case(C, rng, 70, 2, 16, 1, 576, 512, rng.integers(0, 150, 70), 32, latent=True)
+    attend_case(C, rng, 1500, 1, 2, 2, 64, 64, rng.integers(0, 20, 1500), 4)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads, kv_heads, dk, dv, latent", [
+    (8, 1, 128, 128, False), (3, 3, 64, 64, False), (4, 2, 256, 256, False), (6, 2, 192, 128, False), (2, 1, 32, 64, False),
+    (4, 1, 576, 512, True), (20, 1, 576, 512, True)])
+@pytest.mark.parametrize("q_len", [7, 16])
+def test_attend_many_new_tokens(C, fmt, heads, kv_heads, dk, dv, latent, q_len):
+    """More new tokens than a request has, as many, and tiles that end among them."""
+    rng = np.random.default_rng(heads + q_len)
+    attend_case(C, rng, 7, q_len, heads, kv_heads, dk, dv, [1, 16, 17, 40, 0, 70, 200], 16, fmt, latent)
 
 
 def long_case(C, kv_heads, group, dk, dv, n, latent, fmt, q_len=1, page=64):
