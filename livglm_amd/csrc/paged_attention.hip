@@ -667,10 +667,10 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
 // (0.44 PFLOP/s).  There no unit is full: of a tile's 2.2 us a SIMD has matrix
 // instructions for a fifth and vector ones for less than half, and LDS reads
 // (34 KB a wave) take as much.  Without products and conversion the launches
-// take 94 us, without loads too 83: what bounds it is the issue of some 500
-// instructions a tile by two waves a SIMD that meet at its end (softmax,
-// exchange, addresses, conversion).  Half of the waves with the next tile's
-// scores behind the values: 139 us; with the conversion first: 157 for 154.
+// take 94 us, without loads too 83, the join's 12 among them: softmax, exchange,
+// addresses and the meeting at a tile's end are the larger part.  Half of the
+// waves with the next tile's scores behind the values: 139 us for 135; with the
+// conversion first: 157 for 154; waits for two operands at once: 136 for 134.
 // ---------------------------------------------------------------------------
 __device__ uint8_t attn_zero_row[2048];
 
