@@ -63,7 +63,8 @@ def _token_rows(t: torch.Tensor, name: str) -> int:
     if t.dtype is not _BF16:
         raise ContractError(f"{name} has dtype {t.dtype}, expected {_BF16}")
     shape = t.shape
-    if len(shape) not in (3, 4):
+    dims = len(shape)
+    if dims != 3 and dims != 4:
         raise ContractError(f"{name} must be [tokens, heads, dim] rows, got {tuple(shape)}")
     row = shape[-1] * shape[-2]
     if t.is_contiguous():
@@ -129,15 +130,18 @@ def cache_step(new_lens: torch.Tensor, lens: torch.Tensor, blocks: torch.Tensor,
     place.  ``kv_lens`` (allocated when not given; may be ``lens``) receives the
     lengths after the step.  Slots and positions have ``max_tokens`` rows.
     """
-    N.require_device(new_lens, "new_lens", (_I32,))
-    dev = new_lens.get_device()
+    dev = new_lens.get_device() if isinstance(new_lens, torch.Tensor) else -1
+    if dev < 0:
+        N.require_device(new_lens, "new_lens", (_I32,))
+    _check(new_lens, "new_lens", _I32, dev)
     _check(lens, "lens", _I32, dev)
     _check(blocks, "blocks", _I32, dev)
     _check(tables, "tables", _I32, dev)
     _check(free_pages, "free_pages", _I32, dev)
     _check(num_free, "num_free", _I32, dev)
     B = new_lens.numel()
-    if tables.ndim != 2 or tables.shape[0] < B or lens.numel() < B or blocks.numel() < B:
+    shape = tables.shape
+    if len(shape) != 2 or shape[0] < B or lens.numel() < B or blocks.numel() < B:
         raise ContractError(f"cache_step: {B} requests, tables {tuple(tables.shape)}, "
                             f"{lens.numel()} lens and {blocks.numel()} blocks")
     if num_free.numel() != 1:
@@ -149,14 +153,16 @@ def cache_step(new_lens: torch.Tensor, lens: torch.Tensor, blocks: torch.Tensor,
         if kv_lens.numel() < B:
             raise ContractError(f"cache_step: kv_lens for {kv_lens.numel()} of {B} requests")
     # one allocation: cu_new | status | slots | positions | kv_lens
-    buf = _empty(2 * B + 2 + 2 * max_tokens, dtype=_I32, device=new_lens.device)
-    cu, status, slots, positions, after = buf.split_with_sizes(
-        (B + 1, 1, max_tokens, max_tokens, B))
     if kv_lens is None:
-        kv_lens = after
+        buf = _empty(2 * B + 2 + 2 * max_tokens, dtype=_I32, device=new_lens.device)
+        cu, status, slots, positions, kv_lens = buf.split_with_sizes(
+            (B + 1, 1, max_tokens, max_tokens, B))
+    else:
+        buf = _empty(B + 2 + 2 * max_tokens, dtype=_I32, device=new_lens.device)
+        cu, status, slots, positions = buf.split_with_sizes((B + 1, 1, max_tokens, max_tokens))
     base = buf.data_ptr()
     _run(dev, "glm_cache_step", N.native.load().glm_cache_step, new_lens.data_ptr(), B,
-         free_pages.numel(), page_size, tables.shape[1], max_tokens, lens.data_ptr(),
+         free_pages.numel(), page_size, shape[1], max_tokens, lens.data_ptr(),
          blocks.data_ptr(), tables.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
          kv_lens.data_ptr(), base, base + 4 * (B + 2), base + 4 * (B + 2 + max_tokens),
          base + 4 * (B + 1))
@@ -233,7 +239,8 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
     pages, kv_heads, page, key_dim = key_cache.shape
     if shape[-1] != key_dim:
         raise ContractError(f"query rows of {shape[-1]} channels, keys of {key_dim}")
-    if tables.ndim != 2 or tables.shape[0] < B or lens.numel() < B:
+    rows = tables.shape
+    if len(rows) != 2 or rows[0] < B or lens.numel() < B:
         raise ContractError(f"{B} requests, tables {tuple(tables.shape)} and {lens.numel()} lens")
     if value_cache is not None:
         if _cache_format(value_cache, value_scales, "value_cache", dev) != fmt:
@@ -253,7 +260,7 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
             raise ContractError(f"out {tuple(out.shape)}, expected {(*shape[:-1], value_dim)}")
     if B == 0 or q_len == 0:
         return out
-    max_blocks = tables.shape[1]
+    max_blocks = rows[1]
     need = _attention_workspace(B, q_len, heads, kv_heads, key_dim, value_dim,
                                 int(value_cache is None), page, max_blocks)
     ws = _empty(need, dtype=_U8, device=query.device)
