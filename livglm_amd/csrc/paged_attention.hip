@@ -1426,7 +1426,8 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
     // not).  40 requests with 16, 32 rows a workgroup: 24 rows of 128 channels 33.1, 28.6 us, 64 rows 51.1,
     // 38.5; 48 rows of 64 channels 41.3, 32.8 (64 rows a workgroup: 43.2); 64 rows of 192 channels 61.9, 44.6
     z.rows = R <= 16 || key_dim > 192 ? 16 : 32;
-    // workgroups a CU, as many as its registers hold: 45 requests of 64 channels with 2, 3: 33.9, 31.0 us;
+    // workgroups a CU, as many as its registers hold: 45 requests of 64 channels with 2, 3, 4: 33.9, 30.8, 29.9
+    // us, but 60 longer ones 44.6, 45.4 with 3, 4; 32 ragged ones of 128 channels with 2, 3: 91, 115 (spills);
     // 32 rows of 192 channels with 2, 1: 40.7, 31.6 (one is resident)
     slots = 256 * (key_dim > 192 || (key_dim > 128 && z.rows == 32) ? 1 : key_dim == 64 && z.rows == 16 ? 3 : 2);
     // units 1, 2, 3 beside the tiles: 57.0, 50.2, 49.1 us (96 requests, MXFP8), 33.9, 33.4, 36.1 (45 requests
