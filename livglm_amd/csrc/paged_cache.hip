@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kStepThreads) void cache_step_kernel(
     const bool gone = nb < 0;
     const int n = gone ? -1 - nb : nb, have = gone ? 0 : blocks[b];
     const int total = (gone ? 0 : lens[b]) + n;
-    const int need = max(0, (total + page - 1) / page - have);
+    const int need = max(0, total / page + (total % page != 0) - have);  // (total + page may pass 32 bits)
     s_given[b] = (int)at.given;
     s_need[b] = (int)at.need;
     s_cu[b] = (int)at.tokens;

@@ -126,6 +126,23 @@ def test_step_refuses_and_changes_nothing(C, what, bits, tokens):
     assert (want["tables"] == tables).all() and want["num_free"] == top
 
 
+@pytest.mark.parametrize("B", [2, 1025])  # (1025: two requests a thread)
+@pytest.mark.parametrize("page, width", [(2 ** 31 - 1, 1), (2 ** 30 - 1, 2)])
+def test_step_lengths_within_a_page_of_32_bits(C, B, page, width):
+    """A length and a page together pass 32 bits: the last page goes to the request that needs it."""
+    for who in (0, B - 2, B - 1):
+        lens, blocks = np.zeros(B, int), np.zeros(B, int)
+        tables, free = np.full((B, width), -1, np.int32), np.arange(width, dtype=np.int32)
+        blocks[who] = width - 1
+        lens[who] = (width - 1) * page
+        tables[who, :width - 1] = width - 1
+        new = np.zeros(B, int)
+        new[who] = 5
+        want = P.step(new, lens, blocks, tables, free, 1, page, 8)
+        assert want["status"] == 0 and want["blocks"][who] == width and want["num_free"] == 0
+        same_step(run_step(C, new, lens, blocks, tables, free, 1, page, 8), want, B)
+
+
 def test_step_captured_and_replayed(C):
     """A graph of steps over the table's own state, replayed with new inputs in between."""
     table = C.PageTable(40, 4, 3, 12)
