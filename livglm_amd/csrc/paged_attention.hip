@@ -26,8 +26,10 @@ namespace glm {
 
 constexpr int kAttnTile = 64;  // positions; parts are cut between tiles
 constexpr float kLog2e = 1.44269504088896341f;
-// A running maximum is raised where a score passes it by more than this (in powers of two), so that the sums
-// are seldom rescaled: weights then lie up to 2^8, which costs neither bf16 nor the sums in 32 bits any digit.
+// Weights are 2^(s - top): where a score passes top it is raised to that score and this many powers of two more,
+// so that the sums are seldom rescaled.  None passes 1, so the sums of values near the type's largest stay finite
+// (with top the maximum itself and weights up to 2^8 they did not), and neither bf16 nor the sums in 32 bits lose a
+// digit.  A row's pieces are joined by their tops, whatever they lie above.
 constexpr float kAttnSlack = 8.0f;
 
 // Sums over the wave by DPP: row_shr 1, 2, 4, 8, then a row's last lane to the next rows.
@@ -452,7 +454,7 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
         q[m][s] = *reinterpret_cast<const glm_bf16x8 *>(p + KRow::channel(s, quad));
     }
     glm_f32x4 acc[DV / 16][MT];
-    float top[MT], sum[MT];  // running maximum; this lane's part of the running sum
+    float top[MT], sum[MT];  // what weights are formed below; this lane's part of the running sum
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       top[m] = -INFINITY;
@@ -509,8 +511,8 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
 #pragma unroll
           for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
           mx = max_over_quads(mx);
-          if (__any(mx > top[m] + kAttnSlack)) {
-            const float next = mx > top[m] + kAttnSlack ? mx : top[m];  // (no row depends on another)
+          if (__any(mx > top[m])) {
+            const float next = mx > top[m] ? mx + kAttnSlack : top[m];  // (no row depends on another)
             const float keep = __builtin_amdgcn_exp2f(top[m] - (next == -INFINITY ? 0.0f : next));
             top[m] = next;
             sum[m] *= keep;
@@ -1149,8 +1151,8 @@ __global__ __launch_bounds__(512, 1) void attn_latent_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
         mx = max_over_quads(mx);
-        if (__any(mx > top + kAttnSlack)) {
-          const float next = mx > top + kAttnSlack ? mx : top;  // (no row depends on another)
+        if (__any(mx > top)) {
+          const float next = mx > top ? mx + kAttnSlack : top;  // (no row depends on another)
           const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.0f : next));
           top = next;
           sum *= keep;

@@ -384,6 +384,35 @@ def test_attend_rising_scores(C, latent, step):
     assert (np.abs(got - want) <= tol).all()
 
 
+@pytest.mark.parametrize("dk, dv, latent", [(128, 128, False), (96, 96, False), (576, 512, True)])
+@pytest.mark.parametrize("step, leap, n", [(0.02, 0, 300), (0.0, 7, 300), (0.0, 7, 5000)])
+def test_attend_largest_values(C, dk, dv, latent, step, leap, n):
+    """Values near the largest of the type, whose weighted mean is finite: weights are held at 1 at most, also where a
+    running maximum lags behind scores that rise by `step` powers of two a position, or by `leap` at the last one."""
+    rng = np.random.default_rng(n + leap)
+    page, heads = 16, 16
+    pages = -(-n // page)
+    kc, _, _ = make_cache(rng, pages, 1, page, dk, "bf16")
+    vc = None if latent else make_cache(rng, pages, 1, page, dv, "bf16")[0]
+    at = torch.arange(pages * page, device="cuda").view(pages, 1, page)
+    kc[..., dk - 1] = (at % 256).to(torch.bfloat16)  # (integers to 256 are exact)
+    kc[..., dk - 2] = (at // 256).to(torch.bfloat16)
+    kc[..., dk - 3] = (at == n - 1).to(torch.bfloat16)
+    values = kc[..., :dv] if latent else vc
+    values *= 2.0 ** 116 if leap else 2.0 ** 120
+    if leap:
+        values[(n - 1) // page, 0, (n - 1) % page] = 2.0 ** 126
+    q = torch.zeros((1, 1, heads, dk), dtype=torch.bfloat16, device="cuda")  # (nothing of the values' channels)
+    share = (torch.arange(heads, device="cuda") + 1) / heads * 0.6931 * dk ** 0.5
+    q[0, 0, :, dk - 1], q[0, 0, :, dk - 2], q[0, 0, :, dk - 3] = share * step, share * step * 256, share * leap
+    tables, lens = np.arange(pages, dtype=np.int32).reshape(1, -1), np.array([n])
+    got = f64(C.paged_attention(q, kc, vc, dev(tables), dev(lens), scale=dk ** -0.5, value_dim=dv))
+    want, size, reach = P.attend(f64(q), f64(kc), f64(values), tables, lens, dk ** -0.5)
+    delta = (dk + 4) * 2.0 ** -24 * reach + 2.0 ** -22 * (1 + reach)
+    tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2 * delta[..., None] + (n + 64) * 2.0 ** -24) * 1.01 * size
+    assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all()
+
+
 @pytest.mark.parametrize("latent", [False, True])
 def test_attend_rows_do_not_depend_on_others(C, latent):
     """A head's result is the same bits whatever the other heads of its kv head ask."""
