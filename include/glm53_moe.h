@@ -657,10 +657,11 @@ int glm_scalex_decode(void *stream, const uint8_t *staging, int64_t staging_byte
  * are taken from the top, requests in order.
  * Written: kv_lens i32 [B], the lengths after the step (may be lens itself);
  * cu_new i32 [B + 1], exclusive sums of the new tokens; for each of the
- * max_tokens token rows slots i32 (where it goes in the cache, -1 past the
- * last token) and positions i32 (in its request, 0 past the last); status i32
- * [1], 0 or GLM_CACHE_* bits.  Where a bit is set, the state stays as it was,
- * kv_lens = lens, cu_new = 0 and every slot is -1.
+ * max_tokens token rows slots i32 (where it goes in the cache; -1 past the
+ * last token, and where its table entry is not in [0, num_pages)) and positions
+ * i32 (in its request, 0 past the last); status i32 [1], 0 or GLM_CACHE_* bits.
+ * Where a bit is set, the state stays as it was, kv_lens = lens, cu_new = 0 and
+ * every slot is -1.
  * Limits: B <= 4096; max_tokens <= 2^30; num_pages * page_size and
  * max_blocks * page_size below 2^31.  Calls on one state must be ordered.
  */

@@ -52,15 +52,18 @@ __device__ __forceinline__ int owner_of(const int *first, int B, int i) {
 }
 
 // Token t of a step: its slot and position, from the sums of the requests'
-// tokens and their new lengths.  tables as this step left them.
+// tokens and their new lengths.  tables as this step left them; an entry that
+// is no page of the cache gives no slot (times page, it might name another's).
 __device__ __forceinline__ void token_slot(int t, int B, const int *cu, const int32_t *kv_lens,
-                                           const int32_t *tables, int max_blocks, int page,
-                                           int32_t *slots, int32_t *positions) {
+                                           const int32_t *tables, int max_blocks,
+                                           int num_pages, int page, int32_t *slots,
+                                           int32_t *positions) {
   int slot = -1, pos = 0;
   if (t < cu[B]) {
     const int r = owner_of(cu, B, t);
     pos = kv_lens[r] - cu[r + 1] + t;
-    slot = tables[(long long)r * max_blocks + pos / page] * page + pos % page;
+    const int id = tables[(long long)r * max_blocks + pos / page];
+    if ((uint32_t)id < (uint32_t)num_pages) slot = id * page + pos % page;
   }
   slots[t] = slot;
   positions[t] = pos;
@@ -177,19 +180,19 @@ __global__ __launch_bounds__(kStepThreads) void cache_step_kernel(
   if (!own_slots) return;
   __syncthreads();
   for (int t = tid; t < max_tokens; t += nt)
-    token_slot(t, B, s_cu, kv_lens, tables, max_blocks, page, slots, positions);
+    token_slot(t, B, s_cu, kv_lens, tables, max_blocks, num_pages, page, slots, positions);
 }
 
 // The tokens' slots of a large step, over all CUs.
 __global__ __launch_bounds__(256) void cache_slots_kernel(
-    const int32_t *cu_new, const int32_t *kv_lens, const int32_t *tables, int B, int page,
-    int max_blocks, int max_tokens, int32_t *slots, int32_t *positions) {
+    const int32_t *cu_new, const int32_t *kv_lens, const int32_t *tables, int B, int num_pages,
+    int page, int max_blocks, int max_tokens, int32_t *slots, int32_t *positions) {
   __shared__ int s_cu[kStepRequests + 1];
   for (int b = threadIdx.x; b <= B; b += blockDim.x) s_cu[b] = cu_new[b];
   __syncthreads();
   const int t = blockIdx.x * blockDim.x + threadIdx.x;
   if (t < max_tokens)
-    token_slot(t, B, s_cu, kv_lens, tables, max_blocks, page, slots, positions);
+    token_slot(t, B, s_cu, kv_lens, tables, max_blocks, num_pages, page, slots, positions);
 }
 
 // ---------------------------------------------------------------------------
@@ -321,8 +324,8 @@ extern "C" int glm_cache_step(void *stream, const int32_t *new_lens, int B, int 
   GLM_LAUNCH_CHECK("cache_step_kernel");
   if (!own) {
     hipLaunchKernelGGL(glm::cache_slots_kernel, dim3((max_tokens + 255) / 256), dim3(256), 0, s,
-                       cu_new, kv_lens, tables, B, page_size, max_blocks, max_tokens, slots,
-                       positions);
+                       cu_new, kv_lens, tables, B, num_pages, page_size, max_blocks, max_tokens,
+                       slots, positions);
     GLM_LAUNCH_CHECK("cache_slots_kernel");
   }
   return GLM_OK;

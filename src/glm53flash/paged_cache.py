@@ -108,8 +108,9 @@ def _cache_format(cache: torch.Tensor, scales: torch.Tensor | None, name: str, d
 
 class CacheStep(NamedTuple):
     """What a step gives: lengths after it, sums of the new tokens, each token
-    row's slot (-1 past the last) and position, and the status (0, or the
-    ``OUT_OF_PAGES`` ... bits, with which nothing has changed)."""
+    row's slot (-1 past the last, and where its table entry is no page of the
+    cache) and position, and the status (0, or the ``OUT_OF_PAGES`` ... bits,
+    with which nothing has changed)."""
 
     kv_lens: torch.Tensor
     cu_new: torch.Tensor

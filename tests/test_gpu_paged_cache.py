@@ -143,6 +143,21 @@ def test_step_lengths_within_a_page_of_32_bits(C, B, page, width):
         same_step(run_step(C, new, lens, blocks, tables, free, 1, page, 8), want, B)
 
 
+@pytest.mark.parametrize("tokens", [8, 9000])
+def test_step_of_pages_outside_the_cache(C, tokens):
+    """A token whose table entry is no page of the cache has no slot, also where entry times page passes 32 bits."""
+    page, pool = 16, 12
+    wild = [pool, -1, 2 ** 28, 2 ** 28 + 3, -2 ** 31, 2 ** 31 - 1, -2 ** 28]
+    B = len(wild) + 1
+    tables = np.array([[w, -1] for w in wild] + [[5, -1]], np.int32)
+    lens, blocks = np.full(B, 10), np.ones(B, int)
+    got = run_step(C, np.ones(B, int), lens, blocks, tables, np.arange(pool, dtype=np.int32), 4, page, tokens)
+    assert got["status"] == 0
+    np.testing.assert_array_equal(got["slots"], [-1] * len(wild) + [5 * page + 10] + [-1] * (tokens - B))
+    np.testing.assert_array_equal(got["positions"], [10] * B + [0] * (tokens - B))
+    np.testing.assert_array_equal(got["tables"], tables)
+
+
 def test_step_captured_and_replayed(C):
     """A graph of steps over the table's own state, replayed with new inputs in between."""
     table = C.PageTable(40, 4, 3, 12)
