@@ -690,7 +690,7 @@ int glm_cache_write(void *stream, const uint16_t *keys, int64_t key_stride,
 
 /*
  * Workspace bytes of glm_paged_attention (latent: value_cache is NULL); 0 for
- * sizes that it refuses.
+ * sizes that it refuses in either format.
  */
 size_t glm_paged_attention_workspace_bytes(int B, int q_len, int heads, int kv_heads, int key_dim,
                                            int value_dim, int latent, int page_size,
@@ -713,8 +713,9 @@ size_t glm_paged_attention_workspace_bytes(int B, int q_len, int heads, int kv_h
  * value_cache NULL: a latent cache (value_dim <= key_dim).
  * Limits: heads % kv_heads == 0, heads <= 1024, q_len <= 16, B <= 65535, widths
  * multiples of 8 (MXFP8: 32) up to 1024, num_pages * page_size * kv_heads and
- * max_blocks * page_size + 1024 < 2^31.  The workspace needs no clearing; calls
- * that may overlap need their own.
+ * max_blocks * page_size + 1024 < 2^31, B * kv_heads * (max_blocks * page_size /
+ * 64 + 3) < 2^30 (the tables' width, whatever the lengths).  The workspace needs
+ * no clearing; calls that may overlap need their own.
  */
 int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_stride, int B, int q_len,
                         int heads, int kv_heads, int key_dim, int value_dim,

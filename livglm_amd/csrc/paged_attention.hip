@@ -1404,15 +1404,21 @@ void launch_attention(hipStream_t s, dim3 grid, AttnForm form, const glm::AttnAr
     launch_group<256, 256, FMT>(s, grid, a);
 }
 
-// Sizes that follow from a call's shape; false for shapes that are refused.
-bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int value_dim, bool latent,
-                int page_size, int max_blocks, AttnSizes &z) {
-  if (B < 0 || q_len < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || key_dim < 1 ||
-      value_dim < 1 || page_size < 1 || max_blocks < 1)
-    return false;
+// Sizes that follow from a call's shape; for shapes that are refused in either format, why.
+const char *attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int value_dim, bool latent,
+                       int page_size, int max_blocks, AttnSizes &z) {
+  if (B < 0 || q_len < 1 || heads < 1 || kv_heads < 1 || key_dim < 1 || value_dim < 1 || page_size < 1 ||
+      max_blocks < 1)
+    return "invalid sizes";
+  if (heads % kv_heads) return "the heads are no multiple of the kv heads";
+  if (key_dim % 8 || value_dim % 8 || key_dim > glm::kAnyDim || value_dim > glm::kAnyDim)
+    return "widths must be multiples of 8 up to 1024";
+  if (latent && value_dim > key_dim) return "more value channels than a latent row has";
+  if (B > 65535) return "at most 65535 requests";
+  if (q_len > 16) return "at most 16 new tokens";
+  if (heads > 1024) return "at most 1024 heads";
   // (positions a turn ahead of the last, 256 at most, are formed in 32 bits)
-  if (B > 65535 || q_len > 16 || heads > 1024 || (long long)max_blocks * page_size > INT_MAX - 1024)
-    return false;
+  if ((long long)max_blocks * page_size > INT_MAX - 1024) return "the tables' positions pass 32 bits";
   const int R = q_len * (heads / kv_heads);
   int slots;  // workgroups that the chip holds at once
   if (latent && key_dim == 576 && value_dim == 512) {
@@ -1450,7 +1456,7 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
   z.parts = slots / z.rblocks > 1 ? slots / z.rblocks : 1;
   const long long tiles = ((long long)max_blocks * page_size + glm::kAttnTile - 1) / glm::kAttnTile;
   const long long units = (tiles + z.over) * B * kv_heads;
-  if (units > INT_MAX / 2) return false;
+  if (units > INT_MAX / 2) return "the tables' tiles of all requests and kv heads pass 2^30";
   const long long most_parts = (units + z.min_part - 1) / z.min_part;
   if (z.parts > most_parts) z.parts = most_parts > 1 ? (int)most_parts : 1;
   z.grid = z.rblocks > 1 ? (unsigned)((z.parts + 7) / 8 * 8 * z.rblocks) : (unsigned)z.parts;
@@ -1458,7 +1464,7 @@ bool attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, int valu
   z.plan_bytes = up256((size_t)z.parts * sizeof(int4));
   z.part_bytes = up256(results * value_dim * sizeof(float));
   z.ml_bytes = up256(results * 2 * sizeof(float));
-  return true;
+  return nullptr;
 }
 
 }  // namespace
@@ -1467,7 +1473,7 @@ extern "C" size_t glm_paged_attention_workspace_bytes(int B, int q_len, int head
                                                       int key_dim, int value_dim, int latent,
                                                       int page_size, int max_blocks) {
   AttnSizes z;
-  if (!attn_sizes(B, q_len, heads, kv_heads, key_dim, value_dim, latent != 0, page_size, max_blocks, z))
+  if (attn_sizes(B, q_len, heads, kv_heads, key_dim, value_dim, latent != 0, page_size, max_blocks, z))
     return 0;
   return z.plan_bytes + z.part_bytes + z.ml_bytes + 256;
 }
@@ -1483,30 +1489,23 @@ extern "C" int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_st
   const bool mx = fmt == GLM_FMT_MXFP8, shared = value_cache == nullptr;
   GLM_REQUIRE(fmt == GLM_FMT_BF16 || mx, GLM_ERR_INVALID_ARGUMENT,
               "paged_attention: unsupported format %d", fmt);
-  GLM_REQUIRE(q && key_cache && tables && lens && workspace && out && (!mx || key_scales) &&
-                  (!mx || shared || value_scales),
-              GLM_ERR_INVALID_ARGUMENT, "paged_attention: null pointer");
   GLM_REQUIRE(B >= 0 && q_len >= 1 && heads >= 1 && kv_heads >= 1 && key_dim >= 1 &&
                   value_dim >= 1 && num_pages >= 1 && page_size >= 1 && max_blocks >= 1,
               GLM_ERR_INVALID_ARGUMENT, "paged_attention: invalid sizes");
-  GLM_REQUIRE(heads % kv_heads == 0, GLM_ERR_UNSUPPORTED_SHAPE,
-              "paged_attention: %d heads over %d kv heads", heads, kv_heads);
-  const int unit = mx ? 32 : 8;
-  GLM_REQUIRE(key_dim % unit == 0 && value_dim % unit == 0 && key_dim <= glm::kAnyDim &&
-                  value_dim <= glm::kAnyDim,
-              GLM_ERR_UNSUPPORTED_SHAPE,
-              "paged_attention: widths %d and %d must be multiples of %d up to %d", key_dim,
-              value_dim, unit, glm::kAnyDim);
-  GLM_REQUIRE(!shared || value_dim <= key_dim, GLM_ERR_UNSUPPORTED_SHAPE,
-              "paged_attention: values of %d channels in rows of %d", value_dim, key_dim);
+  // (sizes first: a refused size has no workspace, whose pointer may then be null)
+  AttnSizes z;
+  const char *why = attn_sizes(B, q_len, heads, kv_heads, key_dim, value_dim, shared, page_size, max_blocks, z);
+  GLM_REQUIRE(!why, GLM_ERR_UNSUPPORTED_SHAPE,
+              "paged_attention: %s (%d requests, %d tokens, %d heads over %d, widths %d and %d, %d blocks of %d)",
+              why, B, q_len, heads, kv_heads, key_dim, value_dim, max_blocks, page_size);
+  GLM_REQUIRE(!mx || (key_dim % 32 == 0 && value_dim % 32 == 0), GLM_ERR_UNSUPPORTED_SHAPE,
+              "paged_attention: MXFP8 widths %d and %d must be multiples of 32", key_dim, value_dim);
   GLM_REQUIRE((long long)num_pages * page_size * kv_heads <= INT_MAX, GLM_ERR_UNSUPPORTED_SHAPE,
               "paged_attention: %d pages of %d x %d rows pass 32 bits", num_pages, kv_heads,
               page_size);
-  AttnSizes z;
-  GLM_REQUIRE(attn_sizes(B, q_len, heads, kv_heads, key_dim, value_dim, shared, page_size, max_blocks, z),
-              GLM_ERR_UNSUPPORTED_SHAPE,
-              "paged_attention: batch %d, %d tokens, %d heads or %d blocks of %d are too many", B,
-              q_len, heads, max_blocks, page_size);
+  GLM_REQUIRE(q && key_cache && tables && lens && workspace && out && (!mx || key_scales) &&
+                  (!mx || shared || value_scales),
+              GLM_ERR_INVALID_ARGUMENT, "paged_attention: null pointer");
   GLM_REQUIRE(q_stride >= (int64_t)heads * key_dim && q_stride % 8 == 0, GLM_ERR_INVALID_ARGUMENT,
               "paged_attention: the query's token stride must cover the heads and be a multiple of 8");
   GLM_REQUIRE(std::isfinite(scale * glm::kLog2e), GLM_ERR_INVALID_ARGUMENT, "paged_attention: scale is not finite");

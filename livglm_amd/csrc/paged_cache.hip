@@ -302,9 +302,6 @@ extern "C" int glm_cache_step(void *stream, const int32_t *new_lens, int B, int 
                               int32_t *num_free, int32_t *kv_lens, int32_t *cu_new,
                               int32_t *slots, int32_t *positions, int32_t *status) {
   glm::clear_error();
-  GLM_REQUIRE(new_lens && lens && blocks && tables && free_pages && num_free && kv_lens && cu_new &&
-                  status && (max_tokens == 0 || (slots && positions)),
-              GLM_ERR_INVALID_ARGUMENT, "cache_step: null pointer");
   GLM_REQUIRE(B >= 1 && num_pages >= 1 && page_size >= 1 && max_blocks >= 1 && max_tokens >= 0,
               GLM_ERR_INVALID_ARGUMENT, "cache_step: invalid sizes");
   GLM_REQUIRE(B <= glm::kStepRequests, GLM_ERR_UNSUPPORTED_SHAPE,
@@ -316,6 +313,9 @@ extern "C" int glm_cache_step(void *stream, const int32_t *new_lens, int B, int 
               GLM_ERR_UNSUPPORTED_SHAPE,
               "cache_step: %d pages (%d a request) of %d tokens pass 32 bits", num_pages,
               max_blocks, page_size);
+  GLM_REQUIRE(new_lens && lens && blocks && tables && free_pages && num_free && kv_lens && cu_new &&
+                  status && (max_tokens == 0 || (slots && positions)),
+              GLM_ERR_INVALID_ARGUMENT, "cache_step: null pointer");
   hipStream_t s = (hipStream_t)stream;
   const bool own = max_tokens <= glm::kStepTokens;
   hipLaunchKernelGGL(glm::cache_step_kernel, dim3(1), dim3(glm::kStepThreads), 0, s, new_lens, B,

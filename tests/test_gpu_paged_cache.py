@@ -763,3 +763,15 @@ def test_python_refusals(C, change):
         kc, kw["key_scales"] = codes, torch.zeros((4, 2, 16, 1), device="cuda", dtype=torch.uint8)
     with pytest.raises(ContractError):
         C.paged_attention(q, kc, vc, table, lens, **kw)
+
+
+@pytest.mark.parametrize("q_len, heads, kv_heads, dim, width, why", [
+    (17, 8, 2, 64, 2, "16 new tokens"), (1, 7, 2, 64, 2, "multiple of the kv heads"), (1, 8, 2, 60, 2, "multiples of 8"),
+    (1, 2, 1, 64, 1 << 27, "pass 32 bits")])
+def test_python_refusals_say_why(C, q_len, heads, kv_heads, dim, width, why):
+    from glm53flash.contract import ContractError
+    kc = torch.zeros((4, kv_heads, 16, dim), device="cuda", dtype=torch.bfloat16)
+    q = torch.zeros((1, q_len, heads, dim), device="cuda", dtype=torch.bfloat16)
+    table = torch.zeros((1, width), device="cuda", dtype=torch.int32)
+    with pytest.raises(ContractError, match=why):
+        C.paged_attention(q, kc, kc, table, dev([3]), scale=1.0)

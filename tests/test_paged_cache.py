@@ -127,6 +127,43 @@ def test_attend_refusals(code, change):
     assert native.load().glm_last_error()
 
 
+REASONS = [({"q_len": 17}, "16 new tokens"), ({"heads": 7}, "multiple of the kv heads"),
+           ({"heads": 2048, "qs": 1 << 18}, "1024 heads"), ({"B": 65536}, "65535 requests"), ({"dk": 100}, "multiples of 8"),
+           ({"dv": 1032}, "up to 1024"), ({"vc": None, "dv": 136}, "value channels"),
+           ({"max_blocks": 1 << 27}, "pass 32 bits"), ({"B": 4096, "heads": 128, "kv_heads": 128, "qs": 1 << 14,
+                                                        "max_blocks": 8192}, "tiles of all requests")]
+
+
+@pytest.mark.parametrize("change, why", REASONS)
+def test_attend_says_why(change, why):
+    """A refused size has no workspace, and its reason comes before the workspace's null pointer."""
+    a = _attend_args(**change)
+    size = native.load().glm_paged_attention_workspace_bytes
+    latent = int(change.get("vc", FAKE) is None)
+    assert size(*a[3:9], latent, a[15], a[18]) == 0
+    for ws in (FAKE, None):
+        assert native.load().glm_paged_attention(*_attend_args(**{**change, "ws": ws, "nbytes": 0})) == SHAPE
+        assert why in native.load().glm_last_error().decode()
+
+
+def test_step_says_why():
+    for change, why in (({"num_pages": 0, "free": None}, "sizes"), ({"max_blocks": 0, "tables": None}, "sizes"),
+                        ({"B": 4097, "new": None}, "4096")):
+        assert native.load().glm_cache_step(*_step_args(**change)) in (INVALID, SHAPE)
+        assert why in native.load().glm_last_error().decode()
+
+
+def test_attend_table_limit():
+    """Requests x kv heads x tiles of the tables' width: the documented bound is taken, just beyond it is not."""
+    size = native.load().glm_paged_attention_workspace_bytes
+    for heads, dk, dv, latent in ((128, 128, 128, 0), (128, 96, 96, 0), (1, 576, 512, 1)):
+        kv = 1 if latent else heads
+        B = 65535 if latent else 4096
+        tiles = (1 << 30) // (B * kv)
+        assert size(B, 1, heads, kv, dk, dv, latent, 64, tiles - 4) > 0  # B kv (tiles - 4 + 3) < 2^30
+        assert size(B, 1, heads, kv, dk, dv, latent, 64, tiles + 1) == 0
+
+
 def test_attend_workspace():
     size = native.load().glm_paged_attention_workspace_bytes
     need = size(2, 1, 8, 2, 128, 128, 0, 16, 4)
