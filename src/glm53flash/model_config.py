@@ -81,6 +81,14 @@ class GLMTextConfig:
                 raise ContractError(f"configuration field must be numeric: {key}")
             return float(value)
 
+        def size(key: str, neutral: int) -> int:
+            # a size that the FFN site does not read: what is no integer is kept as -1,
+            # which what reads the size refuses
+            value = text.get(key)
+            if value is None:
+                return neutral
+            return value if isinstance(value, int) and not isinstance(value, bool) else -1
+
         result = cls(
             hidden_size=integer("hidden_size"),
             moe_intermediate_size=integer("moe_intermediate_size"),
@@ -102,12 +110,12 @@ class GLMTextConfig:
             hc_sinkhorn_iters=int(text.get("hc_sinkhorn_iters", 1)),
             hc_eps=float(text.get("hc_eps", 1e-6)),
             # the attention's head sizes, for its cache; optional too, and null where a model has none
-            num_attention_heads=int(text.get("num_attention_heads") or 1),
-            num_key_value_heads=int(text.get("num_key_value_heads") or 1),
-            kv_lora_rank=int(text.get("kv_lora_rank") or 0),
-            qk_nope_head_dim=int(text.get("qk_nope_head_dim") or 0),
-            qk_rope_head_dim=int(text.get("qk_rope_head_dim") or 0),
-            v_head_dim=int(text.get("v_head_dim") or 0),
+            num_attention_heads=size("num_attention_heads", 1),
+            num_key_value_heads=size("num_key_value_heads", 1),
+            kv_lora_rank=size("kv_lora_rank", 0),
+            qk_nope_head_dim=size("qk_nope_head_dim", 0),
+            qk_rope_head_dim=size("qk_rope_head_dim", 0),
+            v_head_dim=size("v_head_dim", 0),
         )
         result.validate()
         return result

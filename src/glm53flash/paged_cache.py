@@ -334,11 +334,16 @@ class PagedKVCache:
         """The cache of the configuration's attention: latent rows of
         ``kv_lora_rank + qk_rope_head_dim`` channels where it compresses keys
         and values, else ``num_key_value_heads`` heads."""
+        for name in ("kv_lora_rank", "num_key_value_heads", "qk_nope_head_dim", "qk_rope_head_dim",
+                     "v_head_dim"):
+            value = getattr(config, name)
+            if isinstance(value, bool) or not isinstance(value, int) or value < 0:
+                raise ContractError(f"configuration field must be a size: {name}")
         if config.kv_lora_rank > 0:
             return cls(table, 1, config.kv_lora_rank + config.qk_rope_head_dim,
                        config.kv_lora_rank, latent=True, quantization_mode=quantization_mode)
         key_dim = config.qk_nope_head_dim + config.qk_rope_head_dim
-        if key_dim < 1 or config.v_head_dim < 1:
+        if key_dim < 1 or config.v_head_dim < 1 or config.num_key_value_heads < 1:
             raise ContractError("the configuration has no attention head sizes")
         return cls(table, config.num_key_value_heads, key_dim, config.v_head_dim,
                    quantization_mode=quantization_mode)

@@ -258,3 +258,35 @@ def test_token_rows_strides():
     for bad in (qkv.transpose(1, 2), qkv[:, ::2], qkv.view(2, 3, 10, 64)[:, :2], qkv[0]):
         with pytest.raises(ContractError):
             rows(bad)
+
+
+MOE = {"hidden_size": 64, "moe_intermediate_size": 64, "n_routed_experts": 8, "num_experts_per_tok": 2,
+       "n_shared_experts": 1, "n_group": 1, "topk_group": 1, "routed_scaling_factor": 1.0}
+HEADS = {"num_attention_heads": 8, "num_key_value_heads": 2, "qk_nope_head_dim": 64, "qk_rope_head_dim": 64,
+         "v_head_dim": 96}
+
+
+@pytest.mark.parametrize("value", ["4", "auto", [4, 8], True, 4.0, 1.5, -4, {}, float("nan")])
+@pytest.mark.parametrize("key", ["num_key_value_heads", "qk_nope_head_dim", "qk_rope_head_dim", "v_head_dim",
+                                 "kv_lora_rank"])
+def test_mistyped_head_sizes(key, value):
+    """The FFN site's configuration does not depend on the attention's sizes; the cache refuses what is no size."""
+    from glm53flash import paged_cache as C
+    from glm53flash.contract import ContractError
+    from glm53flash.model_config import GLMTextConfig
+    cfg = GLMTextConfig.from_model_dict({**MOE, **HEADS, key: value})
+    assert cfg.hidden_size == 64 and hash(cfg) == hash(cfg)
+    table = C.PageTable(8, 16, 4, 6, device="cpu")
+    with pytest.raises(ContractError, match=key):
+        C.PagedKVCache.from_config(cfg, table)
+    with pytest.raises(ContractError):
+        C.PagedKVCache.from_config(GLMTextConfig(**{**HEADS, key: value}), table)
+
+
+def test_head_counts_of_none():
+    from glm53flash import paged_cache as C
+    from glm53flash.contract import ContractError
+    from glm53flash.model_config import GLMTextConfig
+    with pytest.raises(ContractError):
+        C.PagedKVCache.from_config(GLMTextConfig.from_model_dict({**MOE, **HEADS, "num_key_value_heads": 0}),
+                                   C.PageTable(8, 16, 4, 6, device="cpu"))
