@@ -111,7 +111,8 @@ class GLMTextConfig:
             hc_eps=float(text.get("hc_eps", 1e-6)),
             # the attention's head sizes, for its cache; optional too, and null where a model has none
             num_attention_heads=size("num_attention_heads", 1),
-            num_key_value_heads=size("num_key_value_heads", 1),
+            # (unstated: a kv head for each head; 0 where that is unstated too)
+            num_key_value_heads=size("num_key_value_heads", size("num_attention_heads", 0)),
             kv_lora_rank=size("kv_lora_rank", 0),
             qk_nope_head_dim=size("qk_nope_head_dim", 0),
             qk_rope_head_dim=size("qk_rope_head_dim", 0),

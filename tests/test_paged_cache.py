@@ -290,3 +290,28 @@ def test_head_counts_of_none():
     with pytest.raises(ContractError):
         C.PagedKVCache.from_config(GLMTextConfig.from_model_dict({**MOE, **HEADS, "num_key_value_heads": 0}),
                                    C.PageTable(8, 16, 4, 6, device="cpu"))
+
+
+@pytest.mark.parametrize("change, heads", [({}, 2), ({"num_key_value_heads": None}, 8), ({"num_key_value_heads": 8}, 8),
+                                           ({"num_key_value_heads": None, "num_attention_heads": 12}, 12)])
+def test_unstated_kv_heads(change, heads):
+    """A configuration without a kv head count has one kv head for each head."""
+    from glm53flash import paged_cache as C
+    from glm53flash.model_config import GLMTextConfig
+    table = C.PageTable(8, 16, 4, 6, device="cpu")
+    text = {**MOE, **HEADS, **change}
+    cache = C.PagedKVCache.from_config(GLMTextConfig.from_model_dict(text), table)
+    assert cache.keys.shape == (8, heads, 16, 128) and cache.values.shape == (8, heads, 16, 96)
+    if text["num_key_value_heads"] is None:
+        del text["num_key_value_heads"]
+        assert C.PagedKVCache.from_config(GLMTextConfig.from_model_dict(text), table).kv_heads == heads
+
+
+@pytest.mark.parametrize("heads", ["8", None])
+def test_no_head_count_for_kv_heads(heads):
+    from glm53flash import paged_cache as C
+    from glm53flash.contract import ContractError
+    from glm53flash.model_config import GLMTextConfig
+    text = {**MOE, **HEADS, "num_key_value_heads": None, "num_attention_heads": heads}
+    with pytest.raises(ContractError):
+        C.PagedKVCache.from_config(GLMTextConfig.from_model_dict(text), C.PageTable(8, 16, 4, 6, device="cpu"))
