@@ -699,11 +699,13 @@ size_t glm_paged_attention_workspace_bytes(int B, int q_len, int heads, int kv_h
 /*
  * Attention of the newest q_len tokens of B requests over their cached
  * history (one token of a decode step, a few of a verify step; the reference's
- * dense-equivalent attention, dsa.py:41-56).  q bf16, token (b, t) at
- * (b * q_len + t) * q_stride elements, heads x key_dim; query head h reads kv
- * head h / (heads / kv_heads).  lens i32 [B]: positions in the cache, the new
- * tokens' own among them (glm_cache_step's kv_lens; clamped to [0, max_blocks
- * * page_size]).  Token t sees the positions j < lens[b] - (q_len - 1 - t):
+ * dense-equivalent attention, dsa.py:41-56: every position is seen, so for a
+ * model that selects index_topk of them the result is its own up to that many).
+ * q bf16, token (b, t) at (b * q_len + t) * q_stride elements, heads x key_dim;
+ * query head h reads kv head h / (heads / kv_heads).  lens i32 [B]: positions
+ * in the cache, the new tokens' own among them (glm_cache_step's kv_lens;
+ * clamped to [0, max_blocks * page_size]).  Token t sees the positions
+ * j < lens[b] - (q_len - 1 - t):
  *   s_j = scale q . k_j,  out[b][t][h] = sum_j softmax(s)_j v_j
  * in f32, the probabilities rounded to bf16 for their product with the values
  * (the denominator is their f32 sum); out bf16 [B * q_len][heads][value_dim].

@@ -117,6 +117,8 @@ class GLMTextConfig:
             qk_nope_head_dim=size("qk_nope_head_dim", 0),
             qk_rope_head_dim=size("qk_rope_head_dim", 0),
             v_head_dim=size("v_head_dim", 0),
+            # up to so many positions its attention is dense; 1 where unstated
+            index_topk=size("index_topk", 1),
         )
         result.validate()
         return result

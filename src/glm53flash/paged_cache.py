@@ -224,8 +224,9 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
     """Attention of ``query`` ``[B, heads, key_dim]`` (one new token a request)
     or ``[B, q_len, heads, key_dim]`` (its ``q_len`` newest) over the first
     ``lens`` i32 ``[B]`` positions that ``tables`` i32 ``[>= B, max_blocks]``
-    names; the newest tokens' own rows are in the cache and counted in ``lens``,
-    and token ``t`` sees the positions below ``lens - (q_len - 1 - t)``.
+    names (all of them: no selection of positions is made); the newest tokens'
+    own rows are in the cache and counted in ``lens``, and token ``t`` sees the
+    positions below ``lens - (q_len - 1 - t)``.
     ``value_cache`` None: the values are the first ``value_dim`` channels of the
     key rows.  Returns bf16 of the query's shape with ``value_dim`` channels; a
     row that sees nothing gives zeros."""
@@ -333,12 +334,19 @@ class PagedKVCache:
                     quantization_mode: str | None = None) -> "PagedKVCache":
         """The cache of the configuration's attention: latent rows of
         ``kv_lora_rank + qk_rope_head_dim`` channels where it compresses keys
-        and values, else ``num_key_value_heads`` heads."""
+        and values, else ``num_key_value_heads`` heads.  Where the model selects
+        ``index_topk`` positions (more than 1), the dense attention here is its
+        own up to that many (``dsa.py:41-56``), and a table whose requests may
+        grow longer is refused; the constructor takes any."""
         for name in ("kv_lora_rank", "num_key_value_heads", "qk_nope_head_dim", "qk_rope_head_dim",
-                     "v_head_dim"):
+                     "v_head_dim", "index_topk"):
             value = getattr(config, name)
             if isinstance(value, bool) or not isinstance(value, int) or value < 0:
                 raise ContractError(f"configuration field must be a size: {name}")
+        longest = table.tables.shape[1] * table.page_size
+        if 1 < config.index_topk < longest:
+            raise ContractError(f"requests of up to {longest} positions: beyond index_topk "
+                                f"{config.index_topk} the model's attention is not dense")
         if config.kv_lora_rank > 0:
             return cls(table, 1, config.kv_lora_rank + config.qk_rope_head_dim,
                        config.kv_lora_rank, latent=True, quantization_mode=quantization_mode)

@@ -315,3 +315,21 @@ def test_no_head_count_for_kv_heads(heads):
     text = {**MOE, **HEADS, "num_key_value_heads": None, "num_attention_heads": heads}
     with pytest.raises(ContractError):
         C.PagedKVCache.from_config(GLMTextConfig.from_model_dict(text), C.PageTable(8, 16, 4, 6, device="cpu"))
+
+
+@pytest.mark.parametrize("topk, taken", [(None, True), (1, True), (96, True), (2048, True), (95, False), (64, False),
+                                         ("96", False), (-1, False)])
+@pytest.mark.parametrize("latent", [False, True])
+def test_dense_up_to_index_topk(topk, taken, latent):
+    """A table of 96 positions a request, and models that select as many, more or fewer."""
+    from glm53flash import paged_cache as C
+    from glm53flash.contract import ContractError
+    from glm53flash.model_config import GLMTextConfig
+    table = C.PageTable(8, 16, 4, 6, device="cpu")
+    text = {**MOE, **HEADS, "kv_lora_rank": 256 if latent else None, "index_topk": topk}
+    cfg = GLMTextConfig.from_model_dict(text)
+    if taken:
+        assert C.PagedKVCache.from_config(cfg, table).latent == latent
+    else:
+        with pytest.raises(ContractError, match="index_topk"):
+            C.PagedKVCache.from_config(cfg, table)
