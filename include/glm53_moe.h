@@ -662,7 +662,7 @@ int glm_scalex_decode(void *stream, const uint8_t *staging, int64_t staging_byte
  * i32 (in its request, 0 past the last); status i32 [1], 0 or GLM_CACHE_* bits.
  * Where a bit is set, the state stays as it was, kv_lens = lens, cu_new = 0 and
  * every slot is -1.
- * Limits: B <= 4096; max_tokens <= 2^30; num_pages * page_size and
+ * Limits: 1 <= B <= 4096; max_tokens <= 2^30; num_pages * page_size and
  * max_blocks * page_size below 2^31.  Calls on one state must be ordered.
  */
 int glm_cache_step(void *stream, const int32_t *new_lens, int B, int num_pages, int page_size,

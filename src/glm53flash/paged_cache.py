@@ -161,6 +161,10 @@ def cache_step(new_lens: torch.Tensor, lens: torch.Tensor, blocks: torch.Tensor,
     else:
         buf = _empty(B + 2 + 2 * max_tokens, dtype=_I32, device=new_lens.device)
         cu, status, slots, positions = buf.split_with_sizes((B + 1, 1, max_tokens, max_tokens))
+    if B == 0:  # no request: no token either, and the state stays as it is
+        buf.zero_()
+        slots.fill_(-1)
+        return CacheStep(kv_lens, cu, slots, positions, status)
     base = buf.data_ptr()
     _run(dev, "glm_cache_step", N.native.load().glm_cache_step, new_lens.data_ptr(), B,
          free_pages.numel(), page_size, shape[1], max_tokens, lens.data_ptr(),

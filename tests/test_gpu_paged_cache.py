@@ -158,6 +158,26 @@ def test_step_of_pages_outside_the_cache(C, tokens):
     np.testing.assert_array_equal(got["tables"], tables)
 
 
+@pytest.mark.parametrize("tokens", [0, 5])
+def test_step_of_no_requests(C, tokens):
+    """An empty batch goes through step, write and attention, and leaves the table as it was."""
+    table = C.PageTable(6, 4, 3, 2)
+    cache = C.PagedKVCache(table, 2, 64, 64)
+    table.step(dev([3, 0, 5]), 8)
+    before = [t.clone() for t in (table.lens, table.blocks, table.tables, table.free_pages, table.num_free, cache.keys)]
+    step = table.step(dev(np.zeros(0)), tokens)
+    assert step.cu_new.tolist() == [0] and int(step.status) == 0
+    assert step.slots.tolist() == [-1] * tokens and step.positions.tolist() == [0] * tokens
+    rows = torch.ones((tokens, 2, 64), device="cuda", dtype=torch.bfloat16)
+    cache.write(rows, rows, step.slots)
+    assert cache.attend(torch.ones((0, 4, 64), device="cuda", dtype=torch.bfloat16), 1.0).shape == (0, 4, 64)
+    after = (table.lens, table.blocks, table.tables, table.free_pages, table.num_free, cache.keys)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(after, before))
+    empty = C.cache_step(dev(np.zeros(0)), table.lens, table.blocks, table.tables, table.free_pages, table.num_free,
+                         page_size=4, max_tokens=tokens)
+    assert empty.kv_lens.numel() == 0 and empty.cu_new.tolist() == [0] and empty.slots.tolist() == [-1] * tokens
+
+
 def test_step_captured_and_replayed(C):
     """A graph of steps over the table's own state, replayed with new inputs in between."""
     table = C.PageTable(40, 4, 3, 12)
