@@ -48,7 +48,11 @@ _empty = torch.empty
 
 def _check(t: torch.Tensor, name: str, dtype: torch.dtype, device: int) -> None:
     """A contiguous tensor of the call's device and the dtype it has to have."""
-    if t is None or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+    try:  # (no call beside those that a tensor needs)
+        fine = t.dtype is dtype and t.get_device() == device and t.is_contiguous()
+    except AttributeError:  # no tensor
+        fine = False
+    if not fine:
         N.require_device(t, name, (dtype,))
         raise ContractError(f"{name} is on {t.device}, the call's tensors on device {device}")
 

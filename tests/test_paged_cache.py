@@ -333,3 +333,13 @@ def test_dense_up_to_index_topk(topk, taken, latent):
     else:
         with pytest.raises(ContractError, match="index_topk"):
             C.PagedKVCache.from_config(cfg, table)
+
+
+@pytest.mark.parametrize("thing", [None, [1, 2], np.zeros(4, np.int32), 5, torch.int32, torch.zeros(4, dtype=torch.int32)])
+def test_python_refuses_what_is_no_tensor(thing):
+    from glm53flash import paged_cache as C
+    from glm53flash.contract import ContractError
+    with pytest.raises(ContractError, match="lens"):
+        C._check(thing, "lens", torch.int32, 0)
+    with pytest.raises(ContractError, match="key_cache"):
+        C._cache_format(thing, None, "key_cache", 0)
