@@ -13,9 +13,9 @@
 // Three forms, by the widths alone: the grouped one for heads of 64, 128, 256
 // or 192 / 128 channels, the latent one for rows of 576 channels whose first
 // 512 are the values, and one for all other widths.  The last form on the
-// others' cases: 3554 us for 93 (32 ragged requests, 32 heads over 8 of 128),
-// 328 for 31 (45 requests, 16 heads of 64), 93 for 13 (one request of 517),
-// 15.9 ms for 58 us (64 latent requests).
+// others' cases: 3513 us for 90 (32 ragged requests, 32 heads over 8 of 128),
+// 387 for 26 (45 requests, 16 heads of 64), 49 for 13 (one request of 517),
+// 15.9 ms for 57 us (64 latent requests).
 #include <climits>
 #include <cmath>
 
@@ -293,18 +293,23 @@ __global__ __launch_bounds__(256) void attn_any_kernel(AttnArgs a) {
 // as soon as the products with this one's are formed, its values as soon as
 // these are in LDS, its page numbers a tile earlier.
 // Bound by the cache's bytes; a wave holds 32 positions of keys and values in
-// flight.  Measured, 128 channels in bf16: 91 us for 461 MB of 32 ragged
-// requests (5.1 TB/s), 197 us for 1.07 GB of two requests of 131000 positions
-// (5.4 TB/s; a large copy moves 4.9 TB/s, counting both ways).  96 requests of
-// two tokens on an MXFP8 cache, 164 MB: 46 us, where conversion and rescaling
-// show; 45 requests of 16 heads of 64 channels, 102 MB: 30 us.
+// flight.  Measured, 128 channels in bf16: 90 us for 461 MB of 32 ragged
+// requests (5.1 TB/s), 195 us for 1.07 GB of two requests of 131000 positions
+// (5.5 TB/s; a large copy moves 4.9 TB/s, counting both ways).  96 requests of
+// two tokens on an MXFP8 cache, 164 MB: 48 us, where conversion and rescaling
+// show; 45 requests of 16 heads of 64 channels, 102 MB: 26 us.
 // Masks: rows of a tile see the same positions but where it ends, so only
 // tiles with a position that some row does not see take the masked form.
 // ---------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 
 // One cache row's channels as lane (n, quad) holds them: pieces of 16 bytes,
-// 64 bytes of four quads in turn, and the scales of its pieces.
+// 64 bytes of four quads in turn, and the scales of its pieces.  Plain loads: a
+// non-temporal hint kept a head's row blocks from sharing their tiles in an
+// XCD's cache (40 requests of 64 rows: 38.4 us for 32.7 with 128 channels, 44.2
+// for 39.8 with 192) and gained little or lost where there is one block (32
+// ragged requests 91.2 for 89.5, 64-wide heads 30.8 for 26.5, 40 requests of 256
+// channels 58.8 for 55.2; 96 MXFP8 requests 47.4 for 48.0).
 template <int FMT, int D>
 struct CacheRow {
   static constexpr int kPieces = FMT == GLM_FMT_BF16 ? D / 32 : D / 64;
@@ -316,7 +321,7 @@ struct CacheRow {
     const uint8_t *p = (const uint8_t *)cache + row * (FMT == GLM_FMT_BF16 ? 2 * dim : dim) + 16 * quad;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
-      v[i] = __builtin_nontemporal_load(reinterpret_cast<const glm_u32x4 *>(p + 64 * i));
+      v[i] = *reinterpret_cast<const glm_u32x4 *>(p + 64 * i);
     if constexpr (FMT != GLM_FMT_BF16) {
       const uint8_t *s = scales + row * (dim / 32);
 #pragma unroll
@@ -1431,18 +1436,18 @@ const char *attn_sizes(int B, int q_len, int heads, int kv_heads, int key_dim, i
   } else if (group_widths(key_dim, value_dim)) {
     z.form = kAttnGroup;
     // 32 rows share a tile's operands where there are more than 16 and the registers hold them (256 channels:
-    // not).  40 requests with 16, 32 rows a workgroup: 24 rows of 128 channels 33.1, 28.6 us, 64 rows 51.1,
-    // 38.5; 48 rows of 64 channels 41.3, 32.8 (64 rows a workgroup: 43.2); 64 rows of 192 channels 61.9, 44.6
+    // not).  40 requests with 16, 32 rows a workgroup: 24 rows of 128 channels 26.8, 24.0 us, 64 rows 41.3,
+    // 32.7; 48 rows of 64 channels 32.8, 28.1; 64 rows of 192 channels 49.8, 40.0
     z.rows = R <= 16 || key_dim > 192 ? 16 : 32;
-    // workgroups a CU, as many as its registers hold: 45 requests of 64 channels with 2, 3, 4: 33.9, 30.8, 29.9
-    // us, but 60 longer ones 44.6, 45.4 with 3, 4; 32 ragged ones of 128 channels with 2, 3: 91, 115 (spills);
-    // 32 rows of 192 channels with 2, 1: 40.7, 31.6 (one is resident)
+    // workgroups a CU, as many as its registers hold: 45 requests of 64 channels with 2, 3, 4: 27.9, 26.7, 27.1
+    // us, in MXFP8 23.6, 20.4, 19.4, but 60 longer ones 129, 133, 135; 32 ragged ones of 128 channels with 2, 3: 90,
+    // 110 (spills); 32 rows of 192 channels with 2, 1: 35.1, 28.7 (one is resident)
     slots = 256 * (key_dim > 192 || (key_dim > 128 && z.rows == 32) ? 1 : key_dim == 64 && z.rows == 16 ? 3 : 2);
-    // units 1, 2, 3 beside the tiles: 57.0, 50.2, 49.1 us (96 requests, MXFP8), 33.9, 33.4, 36.1 (45 requests
-    // of 64 channels), 96.0, 95.3, 97.2 (32 ragged ones)
+    // units 1, 2, 3 beside the tiles: 55.0, 48.0, 46.7 us (96 requests, MXFP8), 26.3, 26.5, 27.1 (45 requests
+    // of 64 channels), 90.3, 90.2, 89.9 (32 ragged ones)
     z.over = 2;
-    // one request with parts of 3, 6 or more units: 12.8, 14.6 us (517 positions), 12.6, 16.0 (2000), 18.1,
-    // 17.4 (8000)
+    // one request with parts of 3, 6 or more units: 12.5, 13.2 us (517 positions), 12.4, 13.9 (2000), 16.9,
+    // 15.9 (8000)
     z.min_part = 3;
   } else {
     z.form = kAttnAny;
