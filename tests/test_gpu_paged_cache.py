@@ -795,3 +795,231 @@ def test_python_refusals_say_why(C, q_len, heads, kv_heads, dim, width, why):
     table = torch.zeros((1, width), device="cuda", dtype=torch.int32)
     with pytest.raises(ContractError, match=why):
         C.paged_attention(q, kc, kc, table, dev([3]), scale=1.0)
+
+
+# ---------------------------------------------------------------- edges of the attention, in all forms
+
+FORMS = [(8, 2, 128, 128, False), (16, 1, 576, 512, True), (6, 2, 96, 96, False)]  # grouped, latent, any widths
+
+
+def score_tolerance(want, size, reach, n):
+    """For scores that are exact integers times a power of two: log2 e and one product are rounded (2^-24 of a
+    score each, at the position and at the maximum), beside exp2, the probabilities, the sums and the output."""
+    delta = 2 * 1.45 * 2.0 ** -24 * reach + 2.0 ** -22
+    tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2 * delta[..., None] + (n + 64) * 2.0 ** -24) * 1.01 * size
+    assert (tol <= 0.1 * size).all(), "the bound says nothing"
+    return tol + 1e-30  # (weights below 2^-126 are none in 32 bits)
+
+
+@pytest.mark.parametrize("heads, kv_heads, dk, dv, latent", FORMS)
+@pytest.mark.parametrize("q_len", [1, 3])
+@pytest.mark.parametrize("scale", [1.0, 0.25, -1.0])
+def test_attend_huge_scores(C, heads, kv_heads, dk, dv, latent, q_len, scale):
+    """Scores of thousands, exact in 32 bits, with ties for the largest: small whole numbers as keys and queries."""
+    rng = np.random.default_rng(heads + q_len)
+    page, lens = 16, np.array([700, 33, 130])
+    width = 44
+    tables = rng.permutation(3 * width).reshape(3, width).astype(np.int32)
+
+    def whole(*shape):
+        return torch.from_numpy(rng.integers(-8, 9, shape).astype(np.float32)).to(torch.bfloat16)
+    kc = whole(3 * width, kv_heads, page, dk)
+    for b in range(3):  # every row's largest score has a twin, further on or behind
+        for _ in range(lens[b] // 3):
+            i, j = rng.integers(0, lens[b], 2)
+            tail = slice(dv, None) if latent else slice(None)
+            kc[tables[b, i // page], :, i % page, tail] = kc[tables[b, j // page], :, j % page, tail]
+            if latent:  # (values of its own)
+                kc[tables[b, i // page], :, i % page, :dv] = kc[tables[b, j // page], :, j % page, :dv]
+    vc = None if latent else torch.from_numpy(rng.standard_normal((3 * width, kv_heads, page, dv), np.float32)).to(torch.bfloat16)
+    q = whole(3, q_len, heads, dk)
+    values = kc[..., :dv] if latent else vc
+    want, size, reach = P.attend(f64(q), f64(kc), f64(values), tables, lens, scale)
+    got = f64(C.paged_attention(q.cuda(), kc.cuda(), None if latent else vc.cuda(), dev(tables), dev(lens), scale=scale,
+                                value_dim=dv))
+    assert reach.max() > 2000 * abs(scale)
+    assert (np.abs(got - want) <= score_tolerance(want, size, reach, 700)).all()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads, kv_heads, dk, dv, latent", FORMS)
+def test_attend_lengths_beyond_the_table(C, fmt, heads, kv_heads, dk, dv, latent):
+    """Lengths below none and past the table are those of none and of the whole table; rows of the table and of
+    the lengths behind the batch are not read."""
+    rng = np.random.default_rng(dk)
+    page, width = 16, 5
+    kc, ks, kv = make_cache(rng, 8 * width, kv_heads, page, dk, fmt)
+    vc, vs, vv = (None, None, kv[..., :dv]) if latent else make_cache(rng, 8 * width, kv_heads, page, dv, fmt)
+    tables = rng.permutation(8 * width).reshape(8, width).astype(np.int32)
+    tables[6:] = 2 ** 31 - 1
+    lens = np.array([-1, -2 ** 31, 81, 2 ** 31 - 1, 80, 3, 2 ** 31 - 1, -7])
+    q = torch.from_numpy(rng.standard_normal((6, 2, heads, dk), np.float32)).to(torch.bfloat16).cuda()
+    got = f64(C.paged_attention(q, kc, vc, dev(tables), dev(lens), scale=dk ** -0.5, value_dim=dv, key_scales=ks,
+                                value_scales=vs))
+    want, size, reach = P.attend(f64(q), kv, vv, tables[:6], lens, dk ** -0.5)
+    delta = (dk + 4) * 2.0 ** -24 * reach + 2.0 ** -22 * (1 + reach)
+    tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2 * delta[..., None] + 144 * 2.0 ** -24) * 1.01 * size
+    assert (np.abs(got - want) <= tol).all() and (got[:2] == 0).all()
+
+
+@pytest.mark.parametrize("heads, kv_heads, dk, dv, latent", FORMS)
+def test_attend_not_finite_queries_and_keys(C, heads, kv_heads, dk, dv, latent):
+    """A NaN in a query row reaches that row alone.  An infinite key channel of a seen position: a score of -infinity
+    takes nothing from the row, one of +infinity makes it NaN, as in the formula."""
+    gen = torch.Generator(device="cuda").manual_seed(dk)
+    pages, n = 40, 600
+    kc = torch.randn((pages, kv_heads, 16, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    vc = None if latent else torch.randn((pages, kv_heads, 16, dv), generator=gen, device="cuda", dtype=torch.bfloat16)
+    table = torch.randperm(pages, generator=gen, device="cuda").int().view(1, -1)
+    q = torch.randn((1, 2, heads, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    q[..., dk - 1] = 1.0
+    q[:, :, 1::2, dk - 1] = -1.0
+    lens = dev([n])
+
+    def attend(query):
+        return C.paged_attention(query, kc, vc, table, lens, scale=0.05, value_dim=dv)
+    want = attend(q)
+    bad = q.clone()
+    bad[0, 0, 2, 3] = float("nan")
+    got = attend(bad)
+    assert got[0, 0, 2].isnan().all()
+    got[0, 0, 2] = want[0, 0, 2]
+    assert torch.equal(got, want)
+    # channel dk - 1 is none of the latent form's values
+    kc[table[0, 17].long(), :, 4, dk - 1] = float("inf")
+    got = attend(q)
+    assert got[:, :, ::2].isnan().all() and got[:, :, 1::2].isfinite().all()
+    shorter = [x for x in range(n) if x != 17 * 16 + 4]
+    flat = (lambda t: t[table[0].long()].double().transpose(0, 1).flatten(1, 2)[:, shorter])
+    k = flat(kc)
+    v = k[..., :dv] if latent else flat(vc)
+    group = heads // kv_heads
+    for h in range(1, heads, 2):  # (the last token sees all n positions)
+        kh, vh, qh = k[h // group], v[h // group], q[0, 1, h].double()
+        p = torch.softmax(kh @ qh * 0.05, 0)
+        reach = 0.05 * (kh.abs() @ qh.abs()).max()
+        delta = (dk + 4) * 2.0 ** -24 * reach + 2.0 ** -22 * (1 + reach)
+        tol = 2.0 ** -8 * (p @ vh).abs() + (2.0 ** -8 + 2 * delta + (n + 64) * 2.0 ** -24) * 1.01 * (p @ vh.abs())
+        assert ((got[0, 1, h].double() - p @ vh).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("heads, kv_heads, dk, dv, latent", FORMS)
+def test_attend_scale_bytes_of_unowned_rows(C, heads, kv_heads, dk, dv, latent):
+    """MXFP8 rows that no request holds: NaN codes and scales of any byte there change nothing."""
+    rng = np.random.default_rng(dv)
+    page, lens = 16, np.array([70, 0, 129, 16])
+    kc, ks, kv = make_cache(rng, 20, kv_heads, page, dk, "mxfp8")
+    vc, vs, vv = (None, None, kv[..., :dv]) if latent else make_cache(rng, 20, kv_heads, page, dv, "mxfp8")
+    tables = np.full((4, 9), -1, np.int32)
+    order, held = rng.permutation(20), np.zeros((20, page), bool)
+    for b, n in enumerate(lens):
+        for j in range(-(-n // page)):
+            tables[b, j], order = order[0], order[1:]
+            held[tables[b, j], :min(page, n - j * page)] = True
+    q = torch.from_numpy(rng.standard_normal((4, 2, heads, dk), np.float32)).to(torch.bfloat16).cuda()
+
+    def attend(k, ks, v, vs):
+        return C.paged_attention(q, k, v, dev(tables), dev(lens), scale=0.1, value_dim=dv, key_scales=ks, value_scales=vs)
+    want = attend(kc, ks, vc, vs)
+    gone = torch.from_numpy(~held).cuda()[:, None, :, None]
+    for code, byte in ((0x7f, 255), (0xff, 0), (0x7e, 255), (0x7e, 254)):
+        k, s = kc.masked_fill(gone, code), ks.masked_fill(gone, byte)
+        v, t = (None, None) if latent else (vc.masked_fill(gone, code), vs.masked_fill(gone, byte))
+        assert torch.equal(attend(k, s, v, t), want)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("heads, kv_heads, dk, dv, latent", FORMS)
+def test_attend_captured(C, fmt, heads, kv_heads, dk, dv, latent):
+    """Every form in a graph, replayed with other lengths, tables and queries, eager calls between."""
+    rng = np.random.default_rng(heads)
+    page, width, B = 16, 40, 5
+    kc, ks, _ = make_cache(rng, B * width, kv_heads, page, dk, fmt)
+    vc, vs, _ = (None, None, None) if latent else make_cache(rng, B * width, kv_heads, page, dv, fmt)
+    q = torch.zeros((B, 2, heads, dk), device="cuda", dtype=torch.bfloat16)
+    tables, lens = dev(np.zeros((B, width))), dev(np.zeros(B))
+
+    def attend():
+        return C.paged_attention(q, kc, vc, tables, lens, scale=0.1, value_dim=dv, key_scales=ks, value_scales=vs)
+    attend()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend()
+    for turn in range(6):
+        q.copy_(torch.from_numpy(rng.standard_normal(q.shape, np.float32)))
+        tables.copy_(dev(rng.permutation(B * width).reshape(B, width)))
+        lens.copy_(dev(rng.integers(0, [1, 20, width * page + 1, 300, 2][turn % 5], B)))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, attend())
+
+
+@pytest.mark.parametrize("kv_heads, group, dk, dv, n", [(1, 8, 128, 128, 30001), (2, 4, 64, 64, 20000), (1, 4, 192, 128, 9000),
+                                                        (1, 4, 256, 256, 9000), (1, 2, 96, 96, 5000)])
+def test_attend_long_mxfp8(C, kv_heads, group, dk, dv, n):
+    """Long histories of keys and values apart in MXFP8, against 64-bit torch on the GPU."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    page = 64
+    pages = -(-n // page)
+    slots = torch.arange(pages * page, device="cuda", dtype=torch.int32)
+    caches, values = [], []
+    for d in (dk, dv):
+        rows = torch.randn((pages * page, kv_heads, d), generator=gen, device="cuda", dtype=torch.bfloat16)
+        codes = torch.empty((pages, kv_heads, page, d), dtype=torch.uint8, device="cuda")
+        scales = torch.empty((pages, kv_heads, page, d // 32), dtype=torch.uint8, device="cuda")
+        C.cache_write(rows, None, slots, codes, None, key_scales=scales)
+        caches.append((codes, scales))
+        values.append((codes.view(torch.float8_e4m3fn).double().unflatten(-1, (-1, 32))
+                       * torch.exp2(scales.double() - 127)[..., None]).flatten(-2))
+    q = torch.randn((1, kv_heads * group, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    table = torch.randperm(pages, generator=gen, device="cuda").int().view(1, -1)
+    got = C.paged_attention(q, caches[0][0], caches[1][0], table, dev([n]), scale=dk ** -0.5, key_scales=caches[0][1],
+                            value_scales=caches[1][1])
+    k, v = (x[table[0].long()].transpose(0, 1).flatten(1, 2)[:, :n].contiguous() for x in values)
+    scores = torch.bmm(k, q[0].double().view(kv_heads, group, dk).transpose(1, 2).contiguous()) * dk ** -0.5
+    p = torch.softmax(scores, 1).transpose(1, 2).contiguous()
+    want, size = torch.bmm(p, v).view(-1, dv), torch.bmm(p, v.abs()).view(-1, dv)
+    reach = (k.abs().amax(1) * 1.0) @ torch.ones(dk, device="cuda", dtype=torch.float64)  # sum of largest |k| ..
+    reach = (reach.max() * q.double().abs().max() * dk ** -0.5).item()  # .. times the largest |q|: above every sum |q k|
+    delta = (dk + 4) * 2.0 ** -24 * reach + 2.0 ** -22 * (1 + reach)
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * delta + (n + 64) * 2.0 ** -24) * 1.01 * size
+    assert ((got[0].double() - want).abs() <= tol).all() and (tol < 0.1 * size).all()
+
+
+@pytest.mark.parametrize("heads, kv_heads, dk, dv, latent, fmt", [
+    (8, 1, 576, 512, True, "bf16"), (8, 1, 576, 512, True, "mxfp8"), (8, 2, 128, 128, False, "mxfp8"),
+    (4, 2, 96, 96, False, "bf16"), (4, 2, 96, 96, False, "mxfp8")])
+def test_every_form_beyond_32_bits(C, heads, kv_heads, dk, dv, latent, fmt):
+    """Caches of more than 2^32 elements (and bytes), in all forms and both formats; the pages used lie at their end."""
+    page, n = 64, 150
+    pages = (1 << 32) // (kv_heads * page * dk) + 40
+    kind = torch.bfloat16 if fmt == "bf16" else torch.uint8
+
+    def empty(d):
+        shape = (pages, kv_heads, page, d)
+        return (torch.zeros(shape, dtype=kind, device="cuda"),
+                None if fmt == "bf16" else torch.zeros((*shape[:3], d // 32), dtype=torch.uint8, device="cuda"))
+    kc, ks = empty(dk)
+    vc, vs = (None, None) if latent else empty(dv)
+    gen = torch.Generator(device="cuda").manual_seed(dk)
+    keys = torch.randn((3 * page, kv_heads, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    values = None if latent else torch.randn((3 * page, kv_heads, dv), generator=gen, device="cuda", dtype=torch.bfloat16)
+    slots = torch.arange((pages - 3) * page, pages * page, dtype=torch.int32, device="cuda")
+    C.cache_write(keys, values, slots, kc, vc, key_scales=ks, value_scales=vs)
+
+    def small(t):
+        return None if t is None else t[-3:].clone()
+    q = torch.randn((1, 2, heads, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    order = [2, 0, 1]
+    got = C.paged_attention(q, kc, vc, dev([[pages - 3 + i for i in order]]), dev([n]), scale=0.1, value_dim=dv,
+                            key_scales=ks, value_scales=vs)
+    # the same rows in a cache of three pages: the same bits
+    k3, v3, ks3, vs3 = small(kc), small(vc), small(ks), small(vs)
+    want = C.paged_attention(q, k3, v3, dev([order]), dev([n]), scale=0.1, value_dim=dv, key_scales=ks3, value_scales=vs3)
+    assert torch.equal(got, want) and got.isfinite().all()
+    rows = f64(keys) if fmt == "bf16" else P.mx_values(*P.mx_rows(f64(keys)))
+    k64 = f64(k3) if fmt == "bf16" else P.mx_values(k3.cpu().numpy(), ks3.cpu().numpy())
+    np.testing.assert_array_equal(k64.transpose(0, 2, 1, 3).reshape(3 * page, kv_heads, dk), rows)
+    assert not kc[:-3].any() and (vc is None or not vc[:-3].any())
