@@ -157,6 +157,9 @@ def cache_step(new_lens: torch.Tensor, lens: torch.Tensor, blocks: torch.Tensor,
         _check(kv_lens, "kv_lens", _I32, dev)
         if kv_lens.numel() < B:
             raise ContractError(f"cache_step: kv_lens for {kv_lens.numel()} of {B} requests")
+    if (B | shape[1] | free_pages.numel()) >> 31:  # (the library's sizes are 32-bit: none may wrap)
+        raise ContractError(f"cache_step: {free_pages.numel()} pages or {shape[1]} blocks a request "
+                            "pass 32 bits")
     # one allocation: cu_new | status | slots | positions | kv_lens
     if kv_lens is None:
         buf = _empty(2 * B + 2 + 2 * max_tokens, dtype=_I32, device=new_lens.device)
@@ -211,6 +214,8 @@ def cache_write(keys: torch.Tensor, values: torch.Tensor | None, slots: torch.Te
                                 f"{tuple(value_cache.shape)} do not fit the keys")
     if n == 0:
         return
+    if (n | pages | heads | page | key_dim | value_dim) >> 31:
+        raise ContractError(f"cache_write: {n} slots or a cache {tuple(key_cache.shape)} pass 32 bits")
     _run(dev, "glm_cache_write", N.native.load().glm_cache_write, keys.data_ptr(), key_stride,
          N.ptr(values), value_stride, slots.data_ptr(), n, pages, page, heads, key_dim, value_dim,
          fmt, key_cache.data_ptr(), N.ptr(key_scales), N.ptr(value_cache), N.ptr(value_scales))
@@ -218,7 +223,11 @@ def cache_write(keys: torch.Tensor, values: torch.Tensor | None, slots: torch.Te
 
 @lru_cache(maxsize=256)  # a function of the sizes alone
 def _attention_workspace(B: int, q_len: int, heads: int, kv_heads: int, key_dim: int,
-                         value_dim: int, latent: int, page: int, max_blocks: int) -> int:
+                         value_dim: int, latent: int, page: int, max_blocks: int,
+                         pages: int) -> int:
+    if (B | q_len | heads | kv_heads | key_dim | value_dim | page | max_blocks | pages) >> 31:
+        raise ContractError(f"paged_attention: {B} requests, {pages} pages of {page}, {max_blocks} "
+                            "blocks a request or their widths pass 32 bits")
     return int(N.native.load().glm_paged_attention_workspace_bytes(
         B, q_len, heads, kv_heads, key_dim, value_dim, latent, page, max_blocks))
 
@@ -272,7 +281,7 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor,
         return out
     max_blocks = rows[1]
     need = _attention_workspace(B, q_len, heads, kv_heads, key_dim, value_dim,
-                                int(value_cache is None), page, max_blocks)
+                                int(value_cache is None), page, max_blocks, pages)
     ws = _empty(need, dtype=_U8, device=query.device)
     _run(dev, "glm_paged_attention", N.native.load().glm_paged_attention, query.data_ptr(),
          q_stride, B, q_len, heads, kv_heads, key_dim, value_dim, key_cache.data_ptr(),

@@ -1023,3 +1023,32 @@ def test_every_form_beyond_32_bits(C, heads, kv_heads, dk, dv, latent, fmt):
     k64 = f64(k3) if fmt == "bf16" else P.mx_values(k3.cpu().numpy(), ks3.cpu().numpy())
     np.testing.assert_array_equal(k64.transpose(0, 2, 1, 3).reshape(3 * page, kv_heads, dk), rows)
     assert not kc[:-3].any() and (vc is None or not vc[:-3].any())
+
+
+@pytest.mark.parametrize("what", ["pages", "page", "blocks", "free"])
+def test_sizes_that_pass_32_bits(C, what):
+    """Tensors with an axis beyond 2^32, whose low bits alone would be a size that fits: refused by all."""
+    from glm53flash.contract import ContractError
+    long = (1 << 32) + 8
+    lens = dev([3])
+    q = torch.zeros((1, 2, 8), device="cuda", dtype=torch.bfloat16)
+    try:
+        if what in ("pages", "page"):
+            shape = (long, 1, 1, 8) if what == "pages" else (1, 1, long, 8)
+            kc = torch.empty(shape, device="cuda", dtype=torch.bfloat16)  # 69 GB, never touched
+            with pytest.raises(ContractError, match="32 bits"):
+                C.paged_attention(q, kc, None, dev([[0]]), lens, scale=1.0, value_dim=8)
+            with pytest.raises(ContractError, match="32 bits"):
+                C.cache_write(q[:, :1], None, dev([-1]), kc, None)
+        else:
+            wide = torch.zeros((1, long), device="cuda", dtype=torch.int32)  # 17 GB
+            if what == "blocks":
+                kc = torch.zeros((1, 1, 1, 8), device="cuda", dtype=torch.bfloat16)
+                with pytest.raises(ContractError, match="32 bits"):
+                    C.paged_attention(q, kc, None, wide, lens, scale=1.0, value_dim=8)
+            tables, free = (wide, dev([0])) if what == "blocks" else (dev([[0]]), wide.view(-1))
+            with pytest.raises(ContractError, match="32 bits"):
+                C.cache_step(dev([0]), dev([0]), dev([0]), tables, free, dev([1]), page_size=1, max_tokens=1)
+    finally:
+        kc = wide = tables = free = None
+        torch.cuda.empty_cache()
