@@ -1052,3 +1052,42 @@ def test_sizes_that_pass_32_bits(C, what):
     finally:
         kc = wide = tables = free = None
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("N, heads, page, dk, dv, fmt, pad", [
+    (5, 33, 4, 96, 64, "bf16", 8), (5, 33, 4, 96, 64, "mxfp8", 0), (70, 64, 16, 128, 128, "mxfp8", 8),
+    (2, 65536, 1, 8, 0, "bf16", 0), (3, 1, 1, 1024, 1024, "mxfp8", 0), (2500, 1, 16, 8, 8, "bf16", 8)])
+def test_write_wide_and_narrow_tokens(C, N, heads, page, dk, dv, fmt, pad):
+    """Tokens of more pieces than a workgroup has threads, of as few as two, and the widest rows."""
+    test_write(C, N, heads, page, dk, dv, fmt, pad)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("dk, dv", [(64, 64), (192, 128), (256, 256), (320, 256), (576, 64)])
+def test_attend_latents_of_other_forms(C, fmt, dk, dv):
+    """Values that are the keys' first channels, at the grouped form's widths and at others."""
+    attend_case(C, np.random.default_rng(dk), 3, 2, 8, 2, dk, dv, [70, 200, 1], 16, fmt, latent=True)
+
+
+@pytest.mark.parametrize("dk, dv, latent", [(64, 64, False), (576, 512, True), (32, 32, False)])
+def test_attend_most_rows(C, dk, dv, latent):
+    """1024 heads of one kv head and 16 new tokens: 16384 rows share every position."""
+    attend_case(C, np.random.default_rng(dk), 1, 16, 1024, 1, dk, dv, [70], 16, latent=latent)
+
+
+@pytest.mark.parametrize("heads, dk, dv, latent", [(2, 64, 64, False), (1, 576, 512, True), (1, 32, 32, False)])
+def test_attend_most_requests(C, heads, dk, dv, latent):
+    """65535 short requests: the same bits as in batches of 5000, since no request here is cut."""
+    gen = torch.Generator(device="cuda").manual_seed(dk)
+    B, page, pages = 65535, 4, 3000
+    kc = torch.randn((pages, 1, page, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    vc = None if latent else torch.randn((pages, 1, page, dv), generator=gen, device="cuda", dtype=torch.bfloat16)
+    table = torch.randint(0, pages, (B, 2), generator=gen, device="cuda", dtype=torch.int32)
+    lens = torch.randint(0, 9, (B,), generator=gen, device="cuda", dtype=torch.int32)
+    q = torch.randn((B, heads, dk), generator=gen, device="cuda", dtype=torch.bfloat16)
+    got = C.paged_attention(q, kc, vc, table, lens, scale=0.1, value_dim=dv)
+    for b in range(0, B, 5000):
+        some = slice(b, b + 5000)
+        want = C.paged_attention(q[some], kc, vc, table[some], lens[some], scale=0.1, value_dim=dv)
+        assert torch.equal(got[some], want)
+    assert (got[lens == 0] == 0).all() and not (got[lens > 0] == 0).all(-1).any()
