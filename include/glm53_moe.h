@@ -678,7 +678,8 @@ int glm_cache_step(void *stream, const int32_t *new_lens, int B, int num_pages, 
  * 2^-124 on) that keeps the largest finite magnitude within 448, codes rounded
  * to nearest even; an infinity or a NaN is stored as NaN.
  * A token whose slot is not in [0, num_pages * page_size) is skipped.  Slots
- * named twice in one call hold pieces of either row.
+ * named twice in one call hold pieces of either row.  The rows lie outside the
+ * caches.
  * Limits: N <= 2^30, kv_heads <= 65536, widths multiples of 8 (MXFP8: 32) up to
  * 1024, strides multiples of 8, num_pages * page_size * kv_heads < 2^31.
  */
@@ -709,9 +710,10 @@ size_t glm_paged_attention_workspace_bytes(int B, int q_len, int heads, int kv_h
  *   s_j = scale q . k_j,  out[b][t][h] = sum_j softmax(s)_j v_j
  * in f32, the probabilities rounded to bf16 for their product with the values
  * (the denominator is their f32 sum); out bf16 [B * q_len][heads][value_dim].
- * A row that sees no position gives zeros.  A position whose table entry is
- * not in [0, num_pages) is not seen; cache rows past a request's length are
- * never used, whatever they hold.
+ * A row that sees no position, or none with a score above -infinity, gives
+ * zeros.  A position whose table entry is not in [0, num_pages) is not seen;
+ * cache rows past a request's length are never used, whatever they hold.  out
+ * overlaps no input.
  * value_cache NULL: a latent cache (value_dim <= key_dim).
  * Limits: heads % kv_heads == 0, heads <= 1024, q_len <= 16, B <= 65535, widths
  * multiples of 8 (MXFP8: 32) up to 1024, num_pages * page_size * kv_heads and

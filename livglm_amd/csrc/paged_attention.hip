@@ -529,7 +529,8 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
           for (int i = 0; i < 8; ++i) {
             const float e = __builtin_amdgcn_exp2f(x[i] - from);
             sum[m] += e;
-            // bf16 for the matrix product: 2^-9 of each weight, as the output's own rounding
+            // bf16 for the matrix product: off by 2^-8 of each weight at most, as the output's own rounding
+            // is of the output; together 1.7e-3 to 2.4e-3 from 64 bits, 1.65e-3 of it the output's (2-norm)
             prob[m][i] = (__bf16)e;
           }
         }
@@ -667,9 +668,10 @@ __global__ __launch_bounds__(256, OCC) void attn_group_kernel(AttnArgs a) {
 // and scales into a ring of two, from where the wave that loaded them converts
 // them (exact) into a ring of three.  Three tiles (two) are in flight, across the requests of a workgroup's part too; positions that are
 // not seen read a row of zeros.
-// Measured: 64 bf16 requests of 100 .. 8100 positions, 64 heads, 127 MB: 56 us,
-// of which 12 are the join (partial results of 39 MB are a third of all
-// traffic); a tile of 32 positions takes 1.7 us against 1.5 for its bytes alone.
+// Measured: 64 bf16 requests of 100 .. 8100 positions, 64 heads, 127 MB: 56 us:
+// a part's 14 tiles at 1.74 us are 24, its start and end 17 with one request (11
+// with 16 heads), and the join 14 (54 requests are cut into 282 pieces, whose 37
+// MB are written and read beside the cache's bytes).
 // Five MXFP8 requests of 20000 .. 50000 positions, two tokens, 59 GFLOP: 135 us
 // (0.44 PFLOP/s).  There no unit is full: of a tile's 2.2 us a SIMD has matrix
 // instructions for a fifth and vector ones for less than half, and LDS reads

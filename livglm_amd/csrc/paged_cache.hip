@@ -19,7 +19,7 @@ namespace glm {
 // One workgroup, since a page given back may be taken in the same call and
 // only a workgroup can wait for its own writes; bound by latency: the
 // requests' loads, the pages', the tables': 6 us for 64 requests of one token,
-// of a call's 9.0.  The tokens' slots ride in this launch up to kStepTokens and
+// of a call's 9.5.  The tokens' slots ride in this launch up to kStepTokens and
 // take a launch over all CUs beyond: 12.7 us for 13.9 at 6748 tokens, 18.4 for
 // 13.5 at 14010.
 // ---------------------------------------------------------------------------
