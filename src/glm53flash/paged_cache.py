@@ -22,6 +22,7 @@ page_size + offset``.
 from __future__ import annotations
 
 from functools import lru_cache
+from numbers import Integral
 from typing import NamedTuple
 
 import torch
@@ -358,7 +359,7 @@ class PagedKVCache:
         for name in ("kv_lora_rank", "num_key_value_heads", "qk_nope_head_dim", "qk_rope_head_dim",
                      "v_head_dim", "index_topk"):
             value = getattr(config, name)
-            if isinstance(value, bool) or not isinstance(value, int) or value < 0:
+            if isinstance(value, bool) or not isinstance(value, Integral) or value < 0:
                 raise ContractError(f"configuration field must be a size: {name}")
         longest = table.tables.shape[1] * table.page_size
         if 1 < config.index_topk < longest:

@@ -343,3 +343,11 @@ def test_python_refuses_what_is_no_tensor(thing):
         C._check(thing, "lens", torch.int32, 0)
     with pytest.raises(ContractError, match="key_cache"):
         C._cache_format(thing, None, "key_cache", 0)
+
+
+def test_head_sizes_of_other_integer_types():
+    from glm53flash import paged_cache as C
+    from glm53flash.model_config import GLMTextConfig
+    table = C.PageTable(8, 16, 4, 6, device="cpu")
+    cfg = GLMTextConfig(num_key_value_heads=np.int64(2), qk_nope_head_dim=np.int32(64), v_head_dim=np.int64(32))
+    assert C.PagedKVCache.from_config(cfg, table).values.shape == (8, 2, 16, 32)
