@@ -27,9 +27,9 @@ namespace glm {
 constexpr int kAttnTile = 64;  // positions; parts are cut between tiles
 constexpr float kLog2e = 1.44269504088896341f;
 // Weights are 2^(s - top): where a score passes top it is raised to that score and this many powers of two more,
-// so that the sums are seldom rescaled.  None passes 1, so the sums of values near the type's largest stay finite
-// (with top the maximum itself and weights up to 2^8 they did not), and neither bf16 nor the sums in 32 bits lose a
-// digit.  A row's pieces are joined by their tops, whatever they lie above.
+// so that the sums are seldom rescaled.  None passes 1, and neither bf16 nor the sums in 32 bits lose a digit.  (With
+// top the score itself and weights up to 2^8 one value near the type's largest made its sum infinite; now it takes
+// 2^8 equal ones.)  A row's pieces are joined by their tops, whatever they lie above.
 constexpr float kAttnSlack = 8.0f;
 
 // Sums over the wave by DPP: row_shr 1, 2, 4, 8, then a row's last lane to the next rows.
