@@ -728,6 +728,75 @@ int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_stride, int B
                         const int32_t *tables, const int32_t *lens, int max_blocks, float scale,
                         void *workspace, size_t workspace_bytes, uint16_t *out);
 
+/* ------------------------------------------------------------ block-scaled 8-bit products */
+
+/*
+ * Rows and weights in E4M3 with f32 scales.  The reference's resident weights
+ * are group-32 MXFP8 and its rows bf16 (DeferredLinear, layers.py:38-99); here
+ * both sides of a product are 8-bit, as checkpoints with a scale for each
+ * 128 x 128 block of a weight hold them:
+ *   rows     codes u8 [T][K], scales f32 [T][ceil(K / 128)]
+ *   weights  codes u8 [N][K], scales f32 [ceil(N / 128)][ceil(K / 128)]
+ * A code times its scale is the value.  Quantising takes amax, the largest
+ * finite magnitude of the group or block (448 2^-126 at least):
+ *   scale = amax / 448,  code = e4m3(value * (448 / amax)), nearest even,
+ * all in f32; an infinity or a NaN becomes E4M3's NaN.  Scales that a caller
+ * brings may be any f32.  Every buffer is 16-byte aligned; outputs overlap no
+ * input except where said.
+ */
+#define GLM_ROWS_BF16 0 /* bf16 [T][K] */
+#define GLM_ROWS_F32 1  /* f32 [T][K] */
+#define GLM_ROWS_FP8 2  /* codes and scales as above */
+
+/* Rows x (bf16 or f32) to codes and scales.  Limits: K % 8 == 0. */
+int glm_fp8_quantize_rows(void *stream, const void *x, int x_type, int T, int K, uint8_t *codes,
+                          float *scales);
+
+/* A weight bf16 [N][K] to codes and scales.  Limits: K % 8 == 0, N <= 65535 * 128. */
+int glm_fp8_quantize_weight(void *stream, const uint16_t *w, int N, int K, uint8_t *codes,
+                            float *scales);
+
+/*
+ * The residual's addition, RMSNorm (layers.py:119-131) and the quantisation of
+ * its result: h = x + residual, residual_out = h (in the residual's type),
+ * y = h * (1 / sqrt(mean(h^2) + eps)) * weight from the unrounded h, and y's
+ * codes and scales.  x and residual each GLM_ROWS_BF16 or GLM_ROWS_F32;
+ * residual and residual_out may be the same buffer, and both NULL (h = x);
+ * weight f32 [d] or NULL.  Limits: d % 8 == 0, d <= 32768.
+ */
+int glm_add_rms_norm_fp8(void *stream, const void *x, int x_type, const void *residual,
+                         int residual_type, int T, int d, const float *weight, float eps,
+                         void *residual_out, uint8_t *codes, float *scales);
+
+/*
+ * Workspace bytes of glm_fp8_linear (gated 0), glm_fp8_gate_up (gated 1); 0
+ * where none is needed and for sizes that they refuse.
+ */
+size_t glm_fp8_workspace_bytes(int x_type, int T, int K, int N, int gated);
+
+/*
+ * y = bf16(x W^T), f32 sums of f32 products of the codes' sums and the scales
+ * (DeferredLinear.__call__, layers.py:38-70, in this format).  Rows in bf16 or
+ * f32 are quantised as glm_fp8_quantize_rows does.  y bf16 [T][N].  The
+ * workspace needs no clearing; calls that may overlap need their own.
+ * Limits: K % 16 == 0, K and N <= 2^20, T <= 2^21.
+ */
+int glm_fp8_linear(void *stream, const void *x, int x_type, const float *x_scales, int T, int K,
+                   const uint8_t *weight, const float *scales, int N, void *workspace,
+                   size_t workspace_bytes, uint16_t *out);
+
+/*
+ * The first half of DenseMLP (layers.py:160-171) in this format: g = x Wg^T,
+ * u = x Wu^T (each weight [N][K]), with limit > 0 g = min(g, limit) and u
+ * clipped to [-limit, limit], h = g / (1 + e^-g) * u, all in f32 without
+ * rounding in between, and h's codes u8 [T][N] and scales f32 [T][ceil(N /
+ * 128)].  Limits as glm_fp8_linear, N % 16 == 0.
+ */
+int glm_fp8_gate_up(void *stream, const void *x, int x_type, const float *x_scales, int T, int K,
+                    const uint8_t *gate, const float *gate_scales, const uint8_t *up,
+                    const float *up_scales, int N, float limit, void *workspace,
+                    size_t workspace_bytes, uint8_t *codes, float *scales);
+
 #ifdef __cplusplus
 }
 #endif

@@ -42,6 +42,10 @@ GLM_READ_DROP_CACHE = 1
 GLM_HC_BF16_STREAMS = 1
 GLM_NOALLOC_SCRATCH_BYTES = 64 << 20
 
+GLM_ROWS_BF16 = 0
+GLM_ROWS_F32 = 1
+GLM_ROWS_FP8 = 2
+
 GLM_CACHE_OUT_OF_PAGES = 1
 GLM_CACHE_TABLE_FULL = 2
 GLM_CACHE_TOO_MANY_TOKENS = 4
@@ -115,6 +119,12 @@ SIGNATURES = {
     "glm_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "glm_paged_attention": (_i, [_p, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _i, _i, _i,
                                  _p, _p, _i, _f, _p, _sz, _p]),
+    "glm_fp8_quantize_rows": (_i, [_p, _p, _i, _i, _i, _p, _p]),
+    "glm_fp8_quantize_weight": (_i, [_p, _p, _i, _i, _p, _p]),
+    "glm_add_rms_norm_fp8": (_i, [_p, _p, _i, _p, _i, _i, _i, _p, _f, _p, _p, _p]),
+    "glm_fp8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "glm_fp8_linear": (_i, [_p, _p, _i, _p, _i, _i, _p, _p, _i, _p, _sz, _p]),
+    "glm_fp8_gate_up": (_i, [_p, _p, _i, _p, _i, _i, _p, _p, _p, _p, _i, _f, _p, _sz, _p, _p]),
 }
 
 

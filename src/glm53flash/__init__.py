@@ -6,7 +6,8 @@ of its checkpoint side (the safetensors index, the bank load plan, ScaleX
 scale coding and layer containers) on torch tensors, computed by the HIP library
 ``libglm53moe.so`` (``livglm_amd``).  Every expert is resident in HBM.  Beside
 the FFN site, ``paged_cache`` has the attention's cache for a batch of requests:
-pages, writes and the attention of the newest tokens over it.
+pages, writes and the attention of the newest tokens over it; ``fp8_block`` has
+the products of 8-bit rows and weights with block scales, and what quantises them.
 """
 
 __all__ = [
@@ -15,6 +16,7 @@ __all__ = [
     "checkpoint",
     "contract",
     "expert_ssd",
+    "fp8_block",
     "layers",
     "mhc",
     "model",

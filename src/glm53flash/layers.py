@@ -2,7 +2,7 @@
 
 Mirrors ``layers.py:12-105,160-171`` of the reference on torch tensors; the
 arithmetic runs in libglm53moe (``glm_linear``, ``glm_dense_mlp``,
-``glm_mx_quantize``).
+``glm_mx_quantize``; ``fp8_block`` for weights in that format).
 """
 
 from __future__ import annotations
@@ -10,6 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
+from . import fp8_block
 from .contract import ContractError
 from .expert_ssd import limited_swiglu
 
@@ -27,7 +28,12 @@ class DeferredLinear:
     ``weight`` is bf16 ``[out, in]`` until ``quantize_to_mxfp`` replaces it by
     MX codes (u8 ``[out, in]`` for MXFP8, ``[out, in/2]`` for MXFP4) and
     ``scales`` (u8 ``[out, in/32]``).  Inputs are bf16 ``[..., in]``; outputs
-    bf16 ``[..., out]`` (``layers.py:38-70``)."""
+    bf16 ``[..., out]`` (``layers.py:38-70``).
+
+    With ``quantization_mode`` "fp8_block" ``weight`` holds E4M3 codes ``[out,
+    in]`` and ``scales`` f32 ``[ceil(out/128), ceil(in/128)]``, converted by
+    ``quantize_to_fp8_block`` or attached as a checkpoint has them, and the
+    inputs are multiplied in 8 bits: bf16, f32 or ``fp8_block.Fp8Rows``."""
 
     def __init__(self, input_dims: int, output_dims: int, *, bias: bool = False,
                  quantize_resident: bool = True):
@@ -41,12 +47,16 @@ class DeferredLinear:
 
     @property
     def fmt(self) -> int:
+        if self.quantization_mode == "fp8_block":
+            raise ContractError("block-scaled weights have no format of the bf16-row kernels")
         return N.FORMAT_OF_MODE[self.quantization_mode]
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         weight = require_weight(self.weight, "linear.weight")
         if self.bias is not False:
             raise ContractError("biased deferred linears are not part of the MoE path")
+        if self.quantization_mode == "fp8_block":
+            return fp8_block.linear(x, weight, require_weight(self.scales, "linear.scales"))
         N.require_device(x, "x", (torch.bfloat16,))
         if x.shape[-1] != self.input_dims:
             raise ContractError(f"linear input width {x.shape[-1]} != {self.input_dims}")
@@ -87,6 +97,20 @@ class DeferredLinear:
         self.quantization_mode = mode
         return source_bytes, codes.numel() + scales.numel()
 
+    def quantize_to_fp8_block(self) -> tuple[int, int]:
+        """Startup conversion to E4M3 with an f32 scale for each 128 x 128 block
+        (the reference's conversion is ``layers.py:72-99``, to MX groups).
+        Returns ``(source_bytes, destination_bytes)``."""
+        if not self.quantize_resident:
+            raise ContractError("this deferred linear is excluded from resident FP8")
+        if self.quantization_mode is not None:
+            raise ContractError("deferred linear was already quantized")
+        weight = require_weight(self.weight, "linear.weight")
+        source_bytes = weight.numel() * weight.element_size()
+        self.weight, self.scales = fp8_block.quantize_weight(weight)
+        self.quantization_mode = "fp8_block"
+        return source_bytes, self.weight.numel() + 4 * self.scales.numel()
+
     def quantize_to_mxfp8(self) -> tuple[int, int]:
         return self.quantize_to_mxfp(8)
 
@@ -111,9 +135,27 @@ class DenseMLP:
                  self.down_proj.quantization_mode}
         if len(modes) != 1:
             return None
-        return N.FORMAT_OF_MODE[modes.pop()]
+        return N.FORMAT_OF_MODE.get(modes.pop())
+
+    @property
+    def block_scaled(self) -> bool:
+        """All three projections hold block-scaled E4M3: 8-bit products
+        throughout, the SwiGLU in f32 (``fp8_block.gate_up``)."""
+        return all(p.quantization_mode == "fp8_block"
+                   for p in (self.gate_proj, self.up_proj, self.down_proj))
+
+    def _block_scaled(self, x) -> torch.Tensor:
+        g, u, d = self.gate_proj, self.up_proj, self.down_proj
+        h = fp8_block.gate_up(x, require_weight(g.weight, "gate_proj.weight"),
+                              require_weight(g.scales, "gate_proj.scales"),
+                              require_weight(u.weight, "up_proj.weight"),
+                              require_weight(u.scales, "up_proj.scales"), self.swiglu_limit)
+        return fp8_block.linear(h, require_weight(d.weight, "down_proj.weight"),
+                                require_weight(d.scales, "down_proj.scales"))
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        if self.block_scaled:
+            return self._block_scaled(x)
         fmt = self.fused_format()
         if fmt is None:
             return self.down_proj(limited_swiglu(self.gate_proj(x), self.up_proj(x),
@@ -164,6 +206,17 @@ class RMSNorm:
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         return _rms_norm(x, self.dims, self.weight_f32(), self.eps)
+
+    def quantized(self, x: torch.Tensor, residual: torch.Tensor | None = None, *,
+                  residual_out: torch.Tensor | None = None):
+        """``(rows, h)`` for block-scaled linears: the norm of ``h = x +
+        residual`` (of ``x`` without one) as ``fp8_block.Fp8Rows``, and h in the
+        residual's type (None without one)."""
+        if isinstance(x, torch.Tensor) and x.shape[-1:] != (self.dims,):
+            raise ContractError(f"rms_norm over {self.dims} features got rows of "
+                                f"{tuple(x.shape)}")
+        return fp8_block.add_rms_norm(x, self.weight_f32(), self.eps, residual=residual,
+                                      residual_out=residual_out)
 
 
 class UnweightedRMSNorm:

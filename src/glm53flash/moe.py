@@ -127,12 +127,21 @@ class ExpertSSDMoE:
         bank = self.experts
         bank._require_active()
         shared = self.shared_experts
-        fmt = shared.fused_format()
-        if fmt is None:
-            raise ContractError("shared expert projections must share one storage format")
-        sg = require_weight(shared.gate_proj.weight, "shared gate_proj.weight")
-        su = require_weight(shared.up_proj.weight, "shared up_proj.weight")
-        sd = require_weight(shared.down_proj.weight, "shared down_proj.weight")
+        # a block-scaled shared expert runs first, by itself; the layer adds its output
+        ready = shared(rows) if shared.block_scaled else None
+        if ready is None:
+            fmt = shared.fused_format()
+            if fmt is None:
+                raise ContractError("shared expert projections must share one storage format")
+            sg, su, sd = (require_weight(p.weight, f"shared {name}.weight") for name, p in (
+                ("gate_proj", shared.gate_proj), ("up_proj", shared.up_proj),
+                ("down_proj", shared.down_proj)))
+            shared_args = (shared.intermediate_size, fmt, sg.data_ptr(),
+                           N.ptr(shared.gate_proj.scales), su.data_ptr(),
+                           N.ptr(shared.up_proj.scales), sd.data_ptr(),
+                           N.ptr(shared.down_proj.scales), None)
+        else:
+            shared_args = (0, N.FMT_BF16, None, None, None, None, None, None, ready.data_ptr())
         k = cfg.num_experts_per_tok
         out = torch.empty((T, d), dtype=torch.float32, device=dev)
         weights = torch.empty((T, k), dtype=torch.float32, device=dev)
@@ -163,9 +172,7 @@ class ExpertSSDMoE:
                rb.data_ptr(), cfg.n_routed_experts, k, cfg.n_group, cfg.topk_group,
                int(cfg.norm_topk_prob), float(cfg.routed_scaling_factor),
                cfg.moe_intermediate_size, gw.data_ptr(), gs.data_ptr(), uw.data_ptr(),
-               us.data_ptr(), dw.data_ptr(), ds.data_ptr(), shared.intermediate_size, fmt,
-               sg.data_ptr(), N.ptr(shared.gate_proj.scales), su.data_ptr(),
-               N.ptr(shared.up_proj.scales), sd.data_ptr(), N.ptr(shared.down_proj.scales), None,
+               us.data_ptr(), dw.data_ptr(), ds.data_ptr(), *shared_args,
                float(cfg.swiglu_limit), ws.data_ptr(), ws.numel(), out.data_ptr(),
                weights.data_ptr(), indices.data_ptr(), *hc_args)
         self.last_weights = weights
