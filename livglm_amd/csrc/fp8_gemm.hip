@@ -19,6 +19,7 @@
 // to bf16 (1.7e-3) and whose time the matrix cores set.
 #include "fp8_rows.h"
 #include "lds_stage.h"
+#include "mfma_tile.h"
 
 #include <climits>
 
@@ -28,7 +29,6 @@ typedef int fp8_frag __attribute__((ext_vector_type(8)));
 
 constexpr int kStreamWaves = 8;
 constexpr int kStreamThreads = 64 * kStreamWaves;
-constexpr int kStreamAhead = 4;  // groups whose weights a wave has in flight
 constexpr int kFusedTokens = 16; // rows that the product quantises itself, up to so many
 
 struct Fp8Args {
@@ -52,45 +52,36 @@ template <bool FAST>
 struct Fp8Operand;
 template <>
 struct Fp8Operand<false> {
+  static constexpr int kSteps = 4;
   glm_bf16x8 v[4];
   __device__ __forceinline__ explicit Fp8Operand(const fp8_frag &f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = mxfp8_words_to_bf16x8((uint32_t)f[2 * i], (uint32_t)f[2 * i + 1], 1.0f);
+    for (int i = 0; i < 4; ++i) part(f, i);
+  }
+  __device__ __forceinline__ void part(const fp8_frag &f, int i) {
+    v[i] = mxfp8_words_to_bf16x8((uint32_t)f[2 * i], (uint32_t)f[2 * i + 1], 1.0f);
   }
   Fp8Operand() = default;
 };
 template <>
 struct Fp8Operand<true> {
+  static constexpr int kSteps = 1;
   fp8_frag v;
   __device__ __forceinline__ explicit Fp8Operand(const fp8_frag &f) : v(f) {}
   Fp8Operand() = default;
 };
 
-// c[t] = a b[t] over the group's 128 channels
-template <int TB>
-__device__ __forceinline__ void group_sums(const Fp8Operand<false> &a,
-                                           const Fp8Operand<false> (&b)[TB], glm_f32x4 (&c)[TB]) {
-#pragma unroll
-  for (int t = 0; t < TB; ++t) c[t] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int t = 0; t < TB; ++t)
-      c[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b[t].v[i], c[t], 0, 0, 0);
+// Step i of a b over the group's 128 channels, from zero in the first.
+__device__ __forceinline__ glm_f32x4 step_sum(const Fp8Operand<false> &a,
+                                              const Fp8Operand<false> &b, int i, glm_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      a.v[i], b.v[i], i == 0 ? glm_f32x4{0.f, 0.f, 0.f, 0.f} : c, 0, 0, 0);
 }
-template <int TB>
-__device__ __forceinline__ void group_sums(const Fp8Operand<true> &a,
-                                           const Fp8Operand<true> (&b)[TB], glm_f32x4 (&c)[TB]) {
-#pragma unroll
-  for (int t = 0; t < TB; ++t)  // (scale operands of zero: the unscaled instruction)
-    c[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-        a.v, b[t].v, glm_f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-}
-
-// 16 codes at k of a row, zeros behind its end (K % 16 == 0).
-__device__ __forceinline__ glm_u32x4 codes16(const uint8_t *row, int k, int K) {
-  return k < K ? *reinterpret_cast<const glm_u32x4 *>(row + k) : glm_u32x4{0, 0, 0, 0};
+__device__ __forceinline__ glm_f32x4 step_sum(const Fp8Operand<true> &a, const Fp8Operand<true> &b,
+                                              int, glm_f32x4) {
+  // (scale operands of zero: the unscaled instruction)
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      a.v, b.v, glm_f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
 }
 
 // silu(min(g, limit)) * clip(u, limit) in f32; NaN passes through the clamps.
@@ -105,51 +96,65 @@ __device__ __forceinline__ float gated(float g, float u, float limit) {
 // ---------------------------------------------------------------------------
 // Few tokens: the weights are streamed once for up to 16 TB tokens.  A
 // workgroup has 16 weight rows (of each projection); its eight waves take the
-// groups of K in turn and add up their f32 results in LDS.  ROWS says what x
-// holds: bf16 and f32 rows are quantised in registers, where the four lanes of
-// a token hold its group.
+// groups of K in turn and add up their f32 results in LDS.  A wave asks for
+// the weights and the rows of AHEAD groups before it works on the first: what
+// it waits for is then one latency for as many groups.  ROWS says what x holds:
+// bf16 and f32 rows are quantised in registers, where the four lanes of a token
+// hold its group.
 // ---------------------------------------------------------------------------
 template <int ROWS>
-struct StreamRow {
-  fp8_frag b;
+struct StreamRow;  // a lane's 32 channels of a group, as they are stored
+template <>
+struct StreamRow<GLM_ROWS_FP8> {
+  glm_u32x4 v[2];
   float scale;
-  __device__ __forceinline__ void load(const Fp8Args &a, int t, int g, int q) {
-    const int k = g * kFp8Group + 32 * q;
-    if constexpr (ROWS == GLM_ROWS_FP8) {
-      const uint8_t *row = (const uint8_t *)a.x + (long long)t * a.K;
-      b = join16(codes16(row, k, a.K), codes16(row, k + 16, a.K));
-      scale = a.xs[(long long)t * a.groups + g];
-    } else {
-      float v[32];
+  __device__ __forceinline__ void load(const Fp8Args &a, long long t, int g, int k0, int k1) {
+    const uint8_t *row = (const uint8_t *)a.x + t * a.K;
+    v[0] = *reinterpret_cast<const glm_u32x4 *>(row + k0);
+    v[1] = *reinterpret_cast<const glm_u32x4 *>(row + k1);
+    scale = a.xs[t * a.groups + g];
+  }
+  __device__ __forceinline__ fp8_frag codes(bool in0, bool in1, float &s) {
+    s = scale;
+    return join16(in0 ? v[0] : glm_u32x4{0, 0, 0, 0}, in1 ? v[1] : glm_u32x4{0, 0, 0, 0});
+  }
+};
+template <int ROWS>
+struct StreamRow {
+  static constexpr bool kF32 = ROWS == GLM_ROWS_F32;
+  float v[4][8];
+  __device__ __forceinline__ void load(const Fp8Args &a, long long t, int, int k0, int k1) {
+    load8<kF32>(a.x, t * a.K + k0, v[0]);
+    load8<kF32>(a.x, t * a.K + k0 + 8, v[1]);
+    load8<kF32>(a.x, t * a.K + k1, v[2]);
+    load8<kF32>(a.x, t * a.K + k1 + 8, v[3]);
+  }
+  __device__ __forceinline__ static float over_lanes(float m) {
+    m = fmaxf(m, __shfl_xor(m, 16, kWave));
+    return fmaxf(m, __shfl_xor(m, 32, kWave));
+  }
+  __device__ __forceinline__ fp8_frag codes(bool in0, bool in1, float &s) {
+    float (&f)[32] = reinterpret_cast<float (&)[32]>(v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float (&p)[8] = *reinterpret_cast<float (*)[8]>(v + 8 * i);
+    for (int j = 0; j < 32; ++j) f[j] = (j < 16 ? in0 : in1) ? f[j] : 0.f;
+    float m = over_lanes(abs_max(f));
+    if (__builtin_expect(__any(isinf(m)), 0)) m = over_lanes(finite_abs_max(f));
+    m = fmaxf(m, kFp8Tiny);
+    const float up = kFp8Max / m;
+    fp8_frag b;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = 0.f;
-        if (k + 8 * i < a.K) load8<ROWS == GLM_ROWS_F32>(a.x, (long long)t * a.K + k + 8 * i, p);
-      }
-      float m = abs_max(v);
-      m = fmaxf(m, __shfl_xor(m, 16, kWave));
-      m = fmaxf(m, __shfl_xor(m, 32, kWave));
-      if (__builtin_expect(__any(isinf(m)), 0)) {
-        m = finite_abs_max(v);
-        m = fmaxf(m, __shfl_xor(m, 16, kWave));
-        m = fmaxf(m, __shfl_xor(m, 32, kWave));
-      }
-      m = fmaxf(m, kFp8Tiny);
-      const float up = kFp8Max / m;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        b[j] = (int)fp8_codes4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], up);
-      scale = m / kFp8Max;
-    }
+    for (int j = 0; j < 8; ++j)
+      b[j] = (int)fp8_codes4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3], up);
+    s = m / kFp8Max;
+    return b;
   }
 };
 
-template <int NPROJ, int TB, int ROWS>
+template <int NPROJ, int TB, int ROWS, int AHEAD>
 __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
   __shared__ glm_f32x4 part[kStreamWaves][NPROJ * TB][kWave];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
   const int n0 = 16 * blockIdx.x, t0 = 16 * TB * blockIdx.y;
   const uint8_t *wrow[NPROJ];
   const float *wscale[NPROJ];
@@ -164,39 +169,45 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
 #pragma unroll
     for (int b = 0; b < TB; ++b) acc[p][b] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int g0 = wave; g0 < a.groups; g0 += kStreamWaves * kStreamAhead) {
-    glm_u32x4 wv[kStreamAhead][NPROJ][2];
-    float sw[kStreamAhead][NPROJ];
+  for (int g0 = wave; g0 < a.groups; g0 += kStreamWaves * AHEAD) {
+    glm_u32x4 wv[AHEAD][NPROJ][2];
+    float sw[AHEAD][NPROJ];
+    StreamRow<ROWS> row[AHEAD][TB];
 #pragma unroll
-    for (int i = 0; i < kStreamAhead; ++i) {
+    for (int i = 0; i < AHEAD; ++i) {  // (past the last group or channel: the last again)
       const int g = min(g0 + i * kStreamWaves, a.groups - 1), k = g * kFp8Group + 32 * q;
+      const int k0 = min(k, a.K - 16), k1 = min(k + 16, a.K - 16);
 #pragma unroll
       for (int p = 0; p < NPROJ; ++p) {
-        wv[i][p][0] = codes16(wrow[p], k, a.K);
-        wv[i][p][1] = codes16(wrow[p], k + 16, a.K);
+        wv[i][p][0] = load_stream(wrow[p] + k0);
+        wv[i][p][1] = load_stream(wrow[p] + k1);
         sw[i][p] = wscale[p][g];
       }
+#pragma unroll
+      for (int b = 0; b < TB; ++b) row[i][b].load(a, min(t0 + 16 * b + r, a.T - 1), g, k0, k1);
     }
 #pragma unroll
-    for (int i = 0; i < kStreamAhead; ++i) {
-      const int g = g0 + i * kStreamWaves;
-      if (g >= a.groups) break;
+    for (int i = 0; i < AHEAD; ++i) {
+      const int g = g0 + i * kStreamWaves, k = g * kFp8Group + 32 * q;
+      // (a branch around a group past the last would let its loads sink behind it;
+      // both sides are zeroed: a NaN behind the end would pass through a zero)
+      const bool in0 = k < a.K, in1 = k + 16 < a.K;
       Fp8Operand<false> x[TB];
       float sx[TB];
 #pragma unroll
-      for (int b = 0; b < TB; ++b) {
-        StreamRow<ROWS> row;
-        row.load(a, min(t0 + 16 * b + r, a.T - 1), g, q);
-        x[b] = Fp8Operand<false>(row.b);
-        sx[b] = row.scale;
-      }
+      for (int b = 0; b < TB; ++b) x[b] = Fp8Operand<false>(row[i][b].codes(in0, in1, sx[b]));
 #pragma unroll
       for (int p = 0; p < NPROJ; ++p) {
+        const glm_u32x4 zero{0, 0, 0, 0};
+        const Fp8Operand<false> w(join16(in0 ? wv[i][p][0] : zero, in1 ? wv[i][p][1] : zero));
         glm_f32x4 c[TB];
-        group_sums(Fp8Operand<false>(join16(wv[i][p][0], wv[i][p][1])), x, c);
+#pragma unroll
+        for (int j = 0; j < Fp8Operand<false>::kSteps; ++j)
+#pragma unroll
+          for (int b = 0; b < TB; ++b) c[b] = step_sum(w, x[b], j, c[b]);
 #pragma unroll
         for (int b = 0; b < TB; ++b) {
-          const float s = sx[b] * sw[i][p];
+          const float s = g < a.groups ? sx[b] * sw[i][p] : 0.f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[p][b][j] += c[b][j] * s;
         }
@@ -242,19 +253,15 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// Many tokens: a workgroup computes 32 BN weight rows (NPROJ 2: half of them
-// from each projection) x 64 BT tokens.  Eight waves, two along the weight rows
-// x four along the tokens; a wave holds BN x BT blocks of 16 x 16.  Both
+// Many tokens: a workgroup computes weight rows (NPROJ 2: half of them
+// from each projection) x tokens with WN x WT waves of BN x BT blocks of 16 x 16.  Both
 // operands come into LDS a group of K at a time by direct loads of 16-byte
-// pieces, a ring of groups deep, with the rows' scales behind them.  Piece p of
+// pieces, a ring of groups deep.  Piece p of
 // row R lies at p ^ ((R >> 1) & 7): the 16 rows that a quarter of a wave reads
 // are then on 16 different pieces of 256 bytes.  Rows past the last and pieces
 // past K are out of the buffers' range, which gives zeros.
 // ---------------------------------------------------------------------------
-constexpr int kTileWN = 2, kTileWT = 4, kTileWaves = kTileWN * kTileWT;
-constexpr int kTileThreads = 64 * kTileWaves;
 constexpr int kTileXcds = 8;
-constexpr int kTileKB = 156;  // LDS of a workgroup
 constexpr uint32_t kOutOfRange = 0x40000000u;  // past any tile's operand (256 rows of 2^20 bytes)
 
 struct Fp8TileArgs {
@@ -265,18 +272,22 @@ struct Fp8TileArgs {
   int rows_outer;   // consecutive items walk the tokens of one row tile, else the reverse
 };
 
-template <int BN, int BT>
+// WN x WT waves of BN x BT blocks; KB of LDS for a workgroup.
+template <int WN_, int WT_, int BN_, int BT_, int KB = 156>
 struct Fp8Tile {
-  static constexpr int kRows = 16 * BN * kTileWN, kTok = 16 * BT * kTileWT;
-  static constexpr int kX = kTok * kFp8Group, kW = kRows * kFp8Group, kS = kTileThreads * 4;
-  static constexpr int kStage = kX + kW + kS;
-  static constexpr int kXLoads = kX / (1024 * kTileWaves), kWLoads = kW / (1024 * kTileWaves);
-  static constexpr int kLoads = kXLoads + kWLoads + 1;
-  static constexpr int kFit = kTileKB * 1024 / kStage;
+  static constexpr int WN = WN_, WT = WT_, BN = BN_, BT = BT_;
+  static constexpr int kWaves = WN * WT, kThreads = 64 * kWaves;
+  static constexpr int kRows = 16 * BN * WN, kTok = 16 * BT * WT;
+  static constexpr int kX = kTok * kFp8Group, kW = kRows * kFp8Group;
+  static constexpr int kStage = kX + kW;
+  static constexpr int kS = 2 * kTok * 16;  // the rows' scales, four groups at a time, twice
+  static constexpr int kXLoads = kX / (1024 * kWaves), kWLoads = kW / (1024 * kWaves);
+  static constexpr int kLoads = kXLoads + kWLoads;
+  static constexpr int kFit = (KB * 1024 - kS) / kStage;
   static constexpr int kStages = kFit < 6 ? kFit : 6;
-  static constexpr int kBytes = kStages * kStage;
-  static_assert(kX % (1024 * kTileWaves) == 0 && kW % (1024 * kTileWaves) == 0, "whole loads");
-  static_assert(kTok <= kTileThreads, "one load of scales");
+  static constexpr int kBytes = kStages * kStage + kS;
+  static_assert(kX % (1024 * kWaves) == 0 && kW % (1024 * kWaves) == 0, "whole loads");
+  static_assert(kTok <= kThreads, "a thread has one token's scales");
   static_assert(kStages >= 2, "a ring");
   __device__ static int swz(int row) { return (row >> 1) & 7; }
 };
@@ -301,9 +312,9 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 enum { kOutBf16, kOutF32, kOutCodes };
 
-template <int NPROJ, bool FAST, int BN, int BT, int OUT>
-__global__ __launch_bounds__(kTileThreads) void fp8_tile_kernel(Fp8TileArgs a) {
-  using L = Fp8Tile<BN, BT>;
+template <int NPROJ, bool FAST, class L, int OUT>
+__global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
+  constexpr int BN = L::BN, BT = L::BT, kWaves = L::kWaves;
   constexpr int kS = L::kStages;
   constexpr int kFeat = L::kRows / NPROJ;  // features of a workgroup
   constexpr int HB = BN / NPROJ;           // 16-row blocks of a wave and projection
@@ -319,61 +330,81 @@ __global__ __launch_bounds__(kTileThreads) void fp8_tile_kernel(Fp8TileArgs a) {
   const int tt = a.rows_outer ? item % a.tok_tiles : item / a.row_tiles;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int wn = wave % kTileWN, wt = wave / kTileWN;
+  const int wn = wave % L::WN, wt = wave / L::WN;
   const int K = a.p.K, N = a.p.N, T = a.p.T, groups = a.p.groups;
   const int f0 = rt * kFeat, t0 = tt * L::kTok;
   const int toks = min(T - t0, L::kTok), feats = min(N - f0, kFeat);
 
   const __amdgpu_buffer_rsrc_t xres =
       make_rsrc((const uint8_t *)a.p.x + (long long)t0 * K, (uint32_t)toks * (uint32_t)K);
-  const __amdgpu_buffer_rsrc_t sres =
-      make_rsrc(a.p.xs + (long long)t0 * groups, (uint32_t)toks * (uint32_t)groups * 4u);
   __amdgpu_buffer_rsrc_t wres[NPROJ];
 #pragma unroll
   for (int p = 0; p < NPROJ; ++p)
     wres[p] = make_rsrc(a.p.w[p] + (long long)f0 * K, (uint32_t)feats * (uint32_t)K);
-  // load j of wave w fills the (kTileWaves j + w)-th 1 KB of the tokens, then of the weight rows
+  // load j of wave w fills the (kWaves j + w)-th 1 KB of the tokens, then of the weight rows
   uint32_t xoff[L::kXLoads], woff[L::kWLoads];
 #pragma unroll
   for (int j = 0; j < L::kXLoads; ++j) {
-    const int slot = (j * kTileWaves + wave) * 64 + lane, row = slot / 8;
+    const int slot = (j * kWaves + wave) * 64 + lane, row = slot / 8;
     xoff[j] = (uint32_t)row * (uint32_t)K + 16 * ((slot % 8) ^ L::swz(row));
   }
 #pragma unroll
   for (int j = 0; j < L::kWLoads; ++j) {
-    const int slot = (j * kTileWaves + wave) * 64 + lane, row = slot / 8;
+    const int slot = (j * kWaves + wave) * 64 + lane, row = slot / 8;
     woff[j] = (uint32_t)(row % kFeat) * (uint32_t)K + 16 * ((slot % 8) ^ L::swz(row));
   }
-  const uint32_t soff = (uint32_t)((wave * 64 + lane) % L::kTok) * (uint32_t)groups * 4u;
   const int tail = K % kFp8Group;  // codes of a last group that is not whole
   auto issue = [&](int c, int stage) {
     uint8_t *base = smem + stage * L::kStage;
-    const bool cut = tail != 0 && c == groups - 1;
+    if (tail != 0 && c == groups - 1) {  // (the last use of the offsets)
+      auto outside = [&](int j) {
+        const int slot = (j * kWaves + wave) * 64 + lane;
+        return 16 * ((slot % 8) ^ L::swz(slot / 8)) >= tail;
+      };
 #pragma unroll
-    for (int j = 0; j < L::kXLoads; ++j) {
-      const int slot = (j * kTileWaves + wave) * 64 + lane;
-      const bool in = !cut || 16 * ((slot % 8) ^ L::swz(slot / 8)) < tail;
-      buf16_to_lds(xres, base + (j * kTileWaves + wave) * 1024, in ? xoff[j] : kOutOfRange,
-                   (uint32_t)c * kFp8Group);
+      for (int j = 0; j < L::kXLoads; ++j)
+        if (outside(j)) xoff[j] = kOutOfRange;
+#pragma unroll
+      for (int j = 0; j < L::kWLoads; ++j)
+        if (outside(j)) woff[j] = kOutOfRange;
     }
+#pragma unroll
+    for (int j = 0; j < L::kXLoads; ++j)
+      buf16_to_lds(xres, base + (j * kWaves + wave) * 1024, xoff[j], (uint32_t)c * kFp8Group);
 #pragma unroll
     for (int j = 0; j < L::kWLoads; ++j) {
-      const int slot = (j * kTileWaves + wave) * 64 + lane;
-      const bool in = !cut || 16 * ((slot % 8) ^ L::swz(slot / 8)) < tail;
       // (a 1 KB block of rows lies in one projection)
-      const int p = NPROJ == 2 && (j * kTileWaves + wave) * 8 >= kFeat;
+      const int p = NPROJ == 2 && (j * kWaves + wave) * 8 >= kFeat;
       buf16_to_lds(NPROJ == 2 && p ? wres[NPROJ - 1] : wres[0],
-                   base + L::kX + (j * kTileWaves + wave) * 1024, in ? woff[j] : kOutOfRange,
+                   base + L::kX + (j * kWaves + wave) * 1024, woff[j],
                    (uint32_t)c * kFp8Group);
     }
-    buf4_to_lds(sres, base + L::kX + L::kW + wave * 256, soff, (uint32_t)c * 4);
+  };
+  // The rows' scales: a thread has one token's, loads four groups of them four
+  // groups ahead and puts them into LDS where the last four are done with.  (One
+  // group at a time they were 64 cache lines a wave and group.)
+  float *slds = reinterpret_cast<float *>(smem + kS * L::kStage);
+  const float *srow = a.p.xs + (long long)(t0 + min(tid, toks - 1)) * groups;
+  glm_f32x4 squad;
+  auto load_scales = [&](int g) {
+    if (groups % 4 == 0) {  // (the rows of scales lie on 16 bytes)
+      squad = *reinterpret_cast<const glm_f32x4 *>(srow + g);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) squad[j] = srow[min(g + j, groups - 1)];
+    }
   };
 
-  // the block scales of the wave's features (its rows lie in one block of 128)
+  // The block scales of the wave's features (its rows lie in one block of 128):
+  // lane l has group c0 + l's, c0 a multiple of 64.  A load a group would be
+  // waited for with the direct loads, whose counter it shares.
   const float *sw[NPROJ];
+  float held[NPROJ];
 #pragma unroll
-  for (int p = 0; p < NPROJ; ++p)
+  for (int p = 0; p < NPROJ; ++p) {
     sw[p] = a.p.ws[p] + (long long)min((f0 + wn * HB * 16) / kFp8Group, (N - 1) / kFp8Group) * groups;
+    held[p] = sw[p][min(lane, groups - 1)];
+  }
 
   glm_f32x4 acc[BN][BT];
 #pragma unroll
@@ -386,45 +417,102 @@ __global__ __launch_bounds__(kTileThreads) void fp8_tile_kernel(Fp8TileArgs a) {
     return join16(*reinterpret_cast<const glm_u32x4 *>(p + 16 * ((2 * q) ^ L::swz(row))),
                   *reinterpret_cast<const glm_u32x4 *>(p + 16 * ((2 * q + 1) ^ L::swz(row))));
   };
-  auto compute = [&](int stage, const float (&ws)[NPROJ]) {
+  // Row block b's products run beside the scaling of block b - 1's and the
+  // reads (and the conversion) of block b + 1.  The order is written out: left
+  // to itself the compiler scales a result right behind its product and waits
+  // for it there.
+  auto compute = [&](int stage, int g, const float (&ws)[NPROJ]) {
     const uint8_t *base = smem + stage * L::kStage;
-    const float *sx = reinterpret_cast<const float *>(base + L::kX + L::kW) + wt * BT * 16 + r;
-    Fp8Operand<FAST> x[BT];
+    const float *sx = slds + ((g >> 2) & 1) * (4 * L::kTok) + 4 * (wt * BT * 16 + r) + (g & 3);
+    constexpr int kSteps = Fp8Operand<FAST>::kSteps;
+    auto wfrag = [&](int b) {
+      return frag(base + L::kX, (b / HB) * kFeat + wn * HB * 16 + (b % HB) * 16 + r);
+    };
+    fp8_frag w = wfrag(0), xf[BT];
+#pragma unroll
+    for (int t = 0; t < BT; ++t) xf[t] = frag(base, (wt * BT + t) * 16 + r);
     float s[NPROJ][BT];
 #pragma unroll
-    for (int t = 0; t < BT; ++t) {
-      x[t] = Fp8Operand<FAST>(frag(base, (wt * BT + t) * 16 + r));
+    for (int t = 0; t < BT; ++t) s[0][t] = sx[64 * t];
+    glm_f32x4 c[2][BT];
+    Fp8Operand<FAST> x[BT], now(w), next;
+    w = wfrag(BN > 1 ? 1 : 0);
+    // block 0: token blocks in turn, so that the first products do not wait for the last's operands
 #pragma unroll
-      for (int p = 0; p < NPROJ; ++p) s[p][t] = sx[16 * t] * ws[p];
+    for (int t = 0; t < BT; ++t) {
+      x[t] = Fp8Operand<FAST>(xf[t]);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) c[0][t] = step_sum(now, x[t], i, c[0][t]);
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int b = 0; b < BN; ++b) {
-      const int row = (b / HB) * kFeat + wn * HB * 16 + (b % HB) * 16 + r;
-      glm_f32x4 c[BT];
-      group_sums(Fp8Operand<FAST>(frag(base + L::kX, row)), x, c);
+    for (int t = 0; t < BT; ++t)
 #pragma unroll
-      for (int t = 0; t < BT; ++t)
+      for (int p = NPROJ - 1; p >= 0; --p) s[p][t] = s[0][t] * ws[p];
+    next = Fp8Operand<FAST>(w);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[b][t][j] += c[t][j] * s[b / HB][t];
+    for (int b = 1; b <= BN; ++b) {
+      now = next;
+      if (b + 1 < BN) w = wfrag(b + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+        for (int t = 0; t < BT; ++t) {
+          if (b < BN) {
+            c[b & 1][t] = step_sum(now, x[t], i, c[b & 1][t]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          constexpr int kEach = 4 / kSteps;  // of a block's four values
+#pragma unroll
+          for (int j = i * kEach; j < (i + 1) * kEach; ++j)
+            acc[b - 1][t][j] += c[(b - 1) & 1][t][j] * s[(b - 1) / HB][t];
+          if constexpr (!FAST) {  // block b + 1, in the second half of this one
+            if (b + 1 < BN && i >= 2 && t < 2) next.part(w, 2 * (i - 2) + t);
+            if (b + 1 < BN && i >= 2 && BT == 1) next.part(w, 2 * (i - 2) + 1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if constexpr (FAST) next = Fp8Operand<FAST>(w);
     }
   };
   // The loads of the next kS - 1 groups are in flight while one is multiplied.
   // The barrier of group c also says that every wave is done with group c - 1,
   // whose stage the loads of group c + kS - 1 overwrite.
+  if (tid < L::kTok) load_scales(0);
 #pragma unroll
-  for (int c = 0; c < kS - 1; ++c)
-    if (c < groups) issue(c, c);
+  for (int g = 0; g < kS - 1; ++g)
+    if (g < groups) issue(g, g);
   int stage = 0;
-  for (int c = 0; c < groups; ++c) {
+  auto group = [&](int c, bool more) {
     float ws[NPROJ];
 #pragma unroll
-    for (int p = 0; p < NPROJ; ++p) ws[p] = sw[p][c];
-    wait_groups_ahead<kS - 2, L::kLoads>(min(kS - 2, groups - 1 - c));
+    for (int p = 0; p < NPROJ; ++p) {
+      if (c != 0 && c % 64 == 0) held[p] = sw[p][min(c + lane, groups - 1)];
+      ws[p] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(held[p]), c & 63));
+    }
+    if ((c & 3) == 0 && tid < L::kTok) {
+      // (this half was last read four groups ago)
+      *reinterpret_cast<glm_f32x4 *>(slds + ((c >> 2) & 1) * (4 * L::kTok) + 4 * tid) = squad;
+      if (c + 4 < groups) load_scales(c + 4);
+    }
+    if (more) {
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm((kS - 2) * L::kLoads));
+    } else {
+      wait_groups_ahead<kS - 2, L::kLoads>(min(kS - 2, groups - 1 - c));
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's scales are in LDS
     ring_barrier();
-    if (c + kS - 1 < groups) issue(c + kS - 1, stage == 0 ? kS - 1 : stage - 1);
-    compute(stage, ws);
+    if (more) issue(c + kS - 1, stage == 0 ? kS - 1 : stage - 1);
+    compute(stage, c, ws);
     stage = stage + 1 == kS ? 0 : stage + 1;
-  }
+  };
+  int c = 0;
+#pragma clang loop unroll(disable)
+  for (; c < groups - (kS - 1); ++c) group(c, true);
+#pragma clang loop unroll(disable)
+  for (; c < groups; ++c) group(c, false);
 
   const int fw = f0 + wn * HB * 16, tw = t0 + wt * BT * 16;  // the wave's first feature and token
   if constexpr (OUT == kOutBf16) {
@@ -446,7 +534,7 @@ __global__ __launch_bounds__(kTileThreads) void fp8_tile_kernel(Fp8TileArgs a) {
     // each 16-token block through the wave's own LDS: a token's features leave in whole pieces
     ring_barrier();
     constexpr int kSegs = 2 * BN, kStride = 16 * kSegs + 16;
-    static_assert(kTileWaves * 16 * kStride <= L::kBytes, "output staging");
+    static_assert(kWaves * 16 * kStride <= L::kBytes, "output staging");
     uint8_t *st = smem + wave * 16 * kStride;
 #pragma unroll
     for (int t = 0; t < BT; ++t) {
@@ -491,10 +579,10 @@ __global__ __launch_bounds__(kTileThreads) void fp8_tile_kernel(Fp8TileArgs a) {
       // a token's largest finite magnitude over the 128 features: the lane's 4 HB, the four lanes of
       // the token, the waves along the features
       ring_barrier();
-      float *red = reinterpret_cast<float *>(smem);  // [kTileWN][kTok]
-      uint8_t *st = smem + kTileWN * L::kTok * 4;    // [kTok][128 codes, 16 bytes of padding]
+      float *red = reinterpret_cast<float *>(smem);  // [L::WN][kTok]
+      uint8_t *st = smem + L::WN * L::kTok * 4;    // [kTok][128 codes, 16 bytes of padding]
       constexpr int kStride = kFp8Group + 16;
-      static_assert(kTileWN * L::kTok * 4 + L::kTok * kStride <= L::kBytes, "output staging");
+      static_assert(L::WN * L::kTok * 4 + L::kTok * kStride <= L::kBytes, "output staging");
 #pragma unroll
       for (int t = 0; t < BT; ++t) {
         float m = 0.f;
@@ -513,7 +601,7 @@ __global__ __launch_bounds__(kTileThreads) void fp8_tile_kernel(Fp8TileArgs a) {
         const int tok = (wt * BT + t) * 16 + r;
         float m = kFp8Tiny;
 #pragma unroll
-        for (int w = 0; w < kTileWN; ++w) m = fmaxf(m, red[w * L::kTok + tok]);
+        for (int w = 0; w < L::WN; ++w) m = fmaxf(m, red[w * L::kTok + tok]);
         const float up = kFp8Max / m;
 #pragma unroll
         for (int b = 0; b < HB; ++b)
@@ -524,8 +612,8 @@ __global__ __launch_bounds__(kTileThreads) void fp8_tile_kernel(Fp8TileArgs a) {
       }
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < L::kTok * 8 / kTileThreads; ++i) {
-        const int slot = i * kTileThreads + tid, tok = slot / 8, n = f0 + 16 * (slot % 8);
+      for (int i = 0; i < L::kTok * 8 / L::kThreads; ++i) {
+        const int slot = i * L::kThreads + tid, tok = slot / 8, n = f0 + 16 * (slot % 8);
         if (t0 + tok < T && n < N)
           *reinterpret_cast<glm_u32x4 *>(a.codes + (long long)(t0 + tok) * N + n) =
               *reinterpret_cast<const glm_u32x4 *>(st + tok * kStride + 16 * (slot % 8));
@@ -540,17 +628,27 @@ using namespace glm;
 
 static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+template <int NPROJ, int TB, int ROWS>
+static void launch_stream_tokens(hipStream_t stream, const Fp8Args &a) {
+  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.T + 16 * TB - 1) / (16 * TB)));
+  const dim3 block(kStreamThreads);
+  if (a.groups <= kStreamWaves)
+    hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, TB, ROWS, 1>), grid, block, 0, stream, a);
+  else if (TB >= 4 || a.groups <= 2 * kStreamWaves)
+    hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, TB, ROWS, 2>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, TB, ROWS, TB >= 4 ? 2 : 4>), grid, block, 0, stream, a);
+}
+
 template <int NPROJ, int ROWS>
 static int launch_stream(hipStream_t stream, const Fp8Args &a) {
-  const unsigned n = (unsigned)((a.N + 15) / 16);
   if (a.T <= 16) {
-    hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, 1, ROWS>), dim3(n), dim3(kStreamThreads), 0, stream, a);
+    launch_stream_tokens<NPROJ, 1, ROWS>(stream, a);
   } else if constexpr (ROWS == GLM_ROWS_FP8) {
     if (a.T <= 32)
-      hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, 2, ROWS>), dim3(n), dim3(kStreamThreads), 0, stream, a);
+      launch_stream_tokens<NPROJ, 2, ROWS>(stream, a);
     else
-      hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, 4, ROWS>), dim3(n, (unsigned)((a.T + 63) / 64)),
-                         dim3(kStreamThreads), 0, stream, a);
+      launch_stream_tokens<NPROJ, 4, ROWS>(stream, a);
   }
   GLM_LAUNCH_CHECK("fp8_stream_kernel");
   return GLM_OK;
@@ -575,17 +673,16 @@ static size_t rows_bytes(int T, int K, int type) {
   return round256((size_t)T * K) + round256((size_t)T * fp8_groups(K) * 4);
 }
 
-template <int NPROJ, bool FAST, int BN, int BT, int OUT>
+template <int NPROJ, bool FAST, class L, int OUT>
 static int launch_tile(hipStream_t stream, Fp8TileArgs a) {
-  using L = Fp8Tile<BN, BT>;
   constexpr int feat = L::kRows / NPROJ;
   a.row_tiles = (a.p.N + feat - 1) / feat;
   a.tok_tiles = (a.p.T + L::kTok - 1) / L::kTok;
   a.rows_outer = NPROJ * a.p.N >= a.p.T;
   const int items = a.row_tiles * a.tok_tiles;
-  hipLaunchKernelGGL((fp8_tile_kernel<NPROJ, FAST, BN, BT, OUT>),
+  hipLaunchKernelGGL((fp8_tile_kernel<NPROJ, FAST, L, OUT>),
                      dim3((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds)),
-                     dim3(kTileThreads), (size_t)L::kBytes, stream, a);
+                     dim3(L::kThreads), (size_t)L::kBytes, stream, a);
   GLM_LAUNCH_CHECK("fp8_tile_kernel");
   return GLM_OK;
 }
@@ -597,16 +694,16 @@ static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
   if (type == GLM_ROWS_F32) return launch_stream<1, GLM_ROWS_F32>(stream, a);
   if (a.T <= kStreamTokens) return launch_stream<1, GLM_ROWS_FP8>(stream, a);
   const Fp8TileArgs t{a, nullptr, nullptr, 0, 0, 0};
-  if (a.T <= 512) return launch_tile<1, true, 4, 1, kOutBf16>(stream, t);
-  return launch_tile<1, true, 8, 4, kOutBf16>(stream, t);
+  if (a.T <= 512) return launch_tile<1, true, Fp8Tile<2, 4, 4, 1>, kOutBf16>(stream, t);
+  return launch_tile<1, true, Fp8Tile<2, 4, 8, 4>, kOutBf16>(stream, t);
 }
 
 static int gated_product(hipStream_t stream, const Fp8Args &a, int type, uint8_t *codes,
                          float *scales) {
   if (a.T > kStreamTokens) {
     const Fp8TileArgs t{a, codes, scales, 0, 0, 0};
-    if (a.T <= 1024) return launch_tile<2, false, 8, 1, kOutCodes>(stream, t);
-    return launch_tile<2, false, 8, 4, kOutCodes>(stream, t);
+    if (a.T <= 1024) return launch_tile<2, false, Fp8Tile<2, 4, 8, 1>, kOutCodes>(stream, t);
+    return launch_tile<2, false, Fp8Tile<4, 2, 4, 4>, kOutCodes>(stream, t);
   }
   const int rc = type == GLM_ROWS_BF16  ? launch_stream<2, GLM_ROWS_BF16>(stream, a)
                  : type == GLM_ROWS_F32 ? launch_stream<2, GLM_ROWS_F32>(stream, a)
