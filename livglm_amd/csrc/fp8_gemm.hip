@@ -287,8 +287,8 @@ struct Fp8Tile {
   static constexpr int kStages = kFit < 6 ? kFit : 6;
   static constexpr int kBytes = kStages * kStage + kS;
   static_assert(kX % (1024 * kWaves) == 0 && kW % (1024 * kWaves) == 0, "whole loads");
-  static_assert(kTok <= kThreads, "a thread has one token's scales");
-  static_assert(kStages >= 2, "a ring");
+  static_assert(kTok <= kThreads && kTok % 64 == 0, "a lane has one token's scales");
+  static_assert(kStages >= 2 && BN >= 2, "a ring, blocks in turn");
   __device__ static int swz(int row) { return (row >> 1) & 7; }
 };
 
@@ -354,56 +354,60 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
     woff[j] = (uint32_t)(row % kFeat) * (uint32_t)K + 16 * ((slot % 8) ^ L::swz(row));
   }
   const int tail = K % kFp8Group;  // codes of a last group that is not whole
-  auto issue = [&](int c, int stage) {
+  // Load j of group c into its stage; the x loads come first.
+  auto issue = [&](int c, int stage, int j) {
     uint8_t *base = smem + stage * L::kStage;
-    if (tail != 0 && c == groups - 1) {  // (the last use of the offsets)
-      auto outside = [&](int j) {
-        const int slot = (j * kWaves + wave) * 64 + lane;
+    if (j == 0 && tail != 0 && c == groups - 1) {  // (the last use of the offsets)
+      auto outside = [&](int i) {
+        const int slot = (i * kWaves + wave) * 64 + lane;
         return 16 * ((slot % 8) ^ L::swz(slot / 8)) >= tail;
       };
 #pragma unroll
-      for (int j = 0; j < L::kXLoads; ++j)
-        if (outside(j)) xoff[j] = kOutOfRange;
+      for (int i = 0; i < L::kXLoads; ++i)
+        if (outside(i)) xoff[i] = kOutOfRange;
 #pragma unroll
-      for (int j = 0; j < L::kWLoads; ++j)
-        if (outside(j)) woff[j] = kOutOfRange;
+      for (int i = 0; i < L::kWLoads; ++i)
+        if (outside(i)) woff[i] = kOutOfRange;
     }
-#pragma unroll
-    for (int j = 0; j < L::kXLoads; ++j)
+    if (j < L::kXLoads) {
       buf16_to_lds(xres, base + (j * kWaves + wave) * 1024, xoff[j], (uint32_t)c * kFp8Group);
-#pragma unroll
-    for (int j = 0; j < L::kWLoads; ++j) {
+    } else {
+      const int i = j - L::kXLoads;
       // (a 1 KB block of rows lies in one projection)
-      const int p = NPROJ == 2 && (j * kWaves + wave) * 8 >= kFeat;
+      const int p = NPROJ == 2 && (i * kWaves + wave) * 8 >= kFeat;
       buf16_to_lds(NPROJ == 2 && p ? wres[NPROJ - 1] : wres[0],
-                   base + L::kX + (j * kWaves + wave) * 1024, woff[j],
-                   (uint32_t)c * kFp8Group);
+                   base + L::kX + (i * kWaves + wave) * 1024, woff[i], (uint32_t)c * kFp8Group);
     }
   };
-  // The rows' scales: a thread has one token's, loads four groups of them four
-  // groups ahead and puts them into LDS where the last four are done with.  (One
-  // group at a time they were 64 cache lines a wave and group.)
+  // The rows' scales come the same way, four groups at a time and up to eight
+  // ahead, the first waves' lanes a token each: 16 bytes a token where the rows
+  // of scales lie on 16 bytes ([token][4 groups] in LDS), else a group at a time
+  // ([4 groups][token]).
+  const bool quads = groups % 4 == 0;
   float *slds = reinterpret_cast<float *>(smem + kS * L::kStage);
-  const float *srow = a.p.xs + (long long)(t0 + min(tid, toks - 1)) * groups;
-  glm_f32x4 squad;
-  auto load_scales = [&](int g) {
-    if (groups % 4 == 0) {  // (the rows of scales lie on 16 bytes)
-      squad = *reinterpret_cast<const glm_f32x4 *>(srow + g);
+  const __amdgpu_buffer_rsrc_t sres =
+      make_rsrc(a.p.xs + (long long)t0 * groups, (uint32_t)toks * (uint32_t)groups * 4u);
+  auto issue_scales = [&](int g) {  // of groups g .. g + 3, g a multiple of 4
+    if (wave * 64 >= L::kTok) return;
+    float *to = slds + ((g >> 2) & 1) * (4 * L::kTok);
+    const uint32_t off = (uint32_t)tid * (uint32_t)groups * 4u;
+    if (quads) {
+      buf16_to_lds(sres, to + wave * 256, off, (uint32_t)g * 4);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) squad[j] = srow[min(g + j, groups - 1)];
+      for (int j = 0; j < 4; ++j)
+        buf4_to_lds(sres, to + j * L::kTok + wave * 64, off, (uint32_t)(g + j) * 4);
     }
   };
 
   // The block scales of the wave's features (its rows lie in one block of 128):
-  // lane l has group c0 + l's, c0 a multiple of 64.  A load a group would be
-  // waited for with the direct loads, whose counter it shares.
+  // lane l has the l-th group's of each 64.  No load into a register is within
+  // the loop over these: it would share its counter with the direct loads, and
+  // the compiler would wait for all of them in every group.
   const float *sw[NPROJ];
-  float held[NPROJ];
 #pragma unroll
   for (int p = 0; p < NPROJ; ++p) {
     sw[p] = a.p.ws[p] + (long long)min((f0 + wn * HB * 16) / kFp8Group, (N - 1) / kFp8Group) * groups;
-    held[p] = sw[p][min(lane, groups - 1)];
   }
 
   glm_f32x4 acc[BN][BT];
@@ -412,31 +416,45 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
 #pragma unroll
     for (int t = 0; t < BT; ++t) acc[b][t] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
 
+  const int p0 = 4 * (q & 1) + 2 * (q >> 1);  // the lane's pieces of a row: p0, p0 + 1
   auto frag = [&](const uint8_t *row0, int row) {
     const uint8_t *p = row0 + row * kFp8Group;
-    return join16(*reinterpret_cast<const glm_u32x4 *>(p + 16 * ((2 * q) ^ L::swz(row))),
-                  *reinterpret_cast<const glm_u32x4 *>(p + 16 * ((2 * q + 1) ^ L::swz(row))));
+    return join16(*reinterpret_cast<const glm_u32x4 *>(p + 16 * (p0 ^ L::swz(row))),
+                  *reinterpret_cast<const glm_u32x4 *>(p + 16 * ((p0 + 1) ^ L::swz(row))));
   };
   // Row block b's products run beside the scaling of block b - 1's and the
   // reads (and the conversion) of block b + 1.  The order is written out: left
   // to itself the compiler scales a result right behind its product and waits
   // for it there.
-  auto compute = [&](int stage, int g, const float (&ws)[NPROJ]) {
+  // side() is done beside block 0's products.
+  auto compute = [&](int stage, int g, const float (&wsc)[2], auto side) {
     const uint8_t *base = smem + stage * L::kStage;
-    const float *sx = slds + ((g >> 2) & 1) * (4 * L::kTok) + 4 * (wt * BT * 16 + r) + (g & 3);
+    const int tstep = quads ? 4 : 1, gstep = quads ? 1 : L::kTok;
+    const float *sx = slds + ((g >> 2) & 1) * (4 * L::kTok) + (wt * BT * 16 + r) * tstep + (g & 3) * gstep;
     constexpr int kSteps = Fp8Operand<FAST>::kSteps;
     auto wfrag = [&](int b) {
       return frag(base + L::kX, (b / HB) * kFeat + wn * HB * 16 + (b % HB) * 16 + r);
     };
-    fp8_frag w = wfrag(0), xf[BT];
+    // two blocks' reads ahead of the products (all of them ahead: 8 % more time at BT 1)
+    constexpr int kAhead = 2;
+    fp8_frag w[BN], xf[BT];
+    w[0] = wfrag(0);
 #pragma unroll
     for (int t = 0; t < BT; ++t) xf[t] = frag(base, (wt * BT + t) * 16 + r);
     float s[NPROJ][BT];
 #pragma unroll
-    for (int t = 0; t < BT; ++t) s[0][t] = sx[64 * t];
-    glm_f32x4 c[2][BT];
-    Fp8Operand<FAST> x[BT], now(w), next;
-    w = wfrag(BN > 1 ? 1 : 0);
+    for (int t = 0; t < BT; ++t) s[0][t] = sx[16 * t * tstep];
+    // One result a token block, scaled before the next block's first step
+    // overwrites it, or two in turn where too few blocks lie between.
+    constexpr int kBuf = BT >= 4 ? 1 : 2;
+    glm_f32x4 c[kBuf][BT];
+    auto scale = [&](int b, int t) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[b][t][j] += c[b % kBuf][t][j] * s[b / HB][t];
+    };
+#pragma unroll
+    for (int b = 1; b < kAhead; ++b) w[b] = wfrag(b);
+    Fp8Operand<FAST> x[BT], now(w[0]);
     // block 0: token blocks in turn, so that the first products do not wait for the last's operands
 #pragma unroll
     for (int t = 0; t < BT; ++t) {
@@ -448,71 +466,85 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
 #pragma unroll
     for (int t = 0; t < BT; ++t)
 #pragma unroll
-      for (int p = NPROJ - 1; p >= 0; --p) s[p][t] = s[0][t] * ws[p];
-    next = Fp8Operand<FAST>(w);
+      for (int p = NPROJ - 1; p >= 0; --p) s[p][t] = s[0][t] * wsc[p];
+    side();
+    now = Fp8Operand<FAST>(w[1]);
+    if (kAhead < BN) w[kAhead] = wfrag(kAhead);
 #pragma unroll
     for (int b = 1; b <= BN; ++b) {
-      now = next;
-      if (b + 1 < BN) w = wfrag(b + 1);
+      Fp8Operand<FAST> next = now;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
+        if constexpr (!FAST) {
+          if (i > 0 && b + 1 < BN) next.part(w[b + 1], i - 1);
+        }
 #pragma unroll
         for (int t = 0; t < BT; ++t) {
-          if (b < BN) {
-            c[b & 1][t] = step_sum(now, x[t], i, c[b & 1][t]);
+          if (i == 0 && (kBuf == 1 || b == BN)) scale(b - 1, t);
+          if (b < BN) c[b % kBuf][t] = step_sum(now, x[t], i, c[b % kBuf][t]);
+          if (i == 0 && kBuf == 2 && b < BN) {
             __builtin_amdgcn_sched_barrier(0);
-          }
-          constexpr int kEach = 4 / kSteps;  // of a block's four values
-#pragma unroll
-          for (int j = i * kEach; j < (i + 1) * kEach; ++j)
-            acc[b - 1][t][j] += c[(b - 1) & 1][t][j] * s[(b - 1) / HB][t];
-          if constexpr (!FAST) {  // block b + 1, in the second half of this one
-            if (b + 1 < BN && i >= 2 && t < 2) next.part(w, 2 * (i - 2) + t);
-            if (b + 1 < BN && i >= 2 && BT == 1) next.part(w, 2 * (i - 2) + 1);
+            scale(b - 1, t);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+        if (b == BN) break;
       }
-      if constexpr (FAST) next = Fp8Operand<FAST>(w);
+      if constexpr (FAST) {
+        if (b + 1 < BN) now = Fp8Operand<FAST>(w[b + 1]);
+      } else {
+        if (b + 1 < BN) next.part(w[b + 1], kSteps - 1);
+        now = next;
+      }
+      if (b + kAhead < BN) w[b + kAhead] = wfrag(b + kAhead);
     }
   };
-  // The loads of the next kS - 1 groups are in flight while one is multiplied.
-  // The barrier of group c also says that every wave is done with group c - 1,
-  // whose stage the loads of group c + kS - 1 overwrite.
-  if (tid < L::kTok) load_scales(0);
+  issue_scales(0);
 #pragma unroll
   for (int g = 0; g < kS - 1; ++g)
-    if (g < groups) issue(g, g);
-  int stage = 0;
-  auto group = [&](int c, bool more) {
-    float ws[NPROJ];
+    if (g < groups)
 #pragma unroll
-    for (int p = 0; p < NPROJ; ++p) {
-      if (c != 0 && c % 64 == 0) held[p] = sw[p][min(c + lane, groups - 1)];
-      ws[p] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(held[p]), c & 63));
-    }
-    if ((c & 3) == 0 && tid < L::kTok) {
-      // (this half was last read four groups ago)
-      *reinterpret_cast<glm_f32x4 *>(slds + ((c >> 2) & 1) * (4 * L::kTok) + 4 * tid) = squad;
-      if (c + 4 < groups) load_scales(c + 4);
-    }
+      for (int j = 0; j < L::kLoads; ++j) issue(g, g, j);
+  // The loads are asked for behind the first products: the address unit takes 16
+  // cycles for one, and a wave stands still meanwhile.  Scales asked for in group
+  // c are there in group c + 4: as many groups' loads as may be outstanding then
+  // (kS - 2) were asked for behind them.
+  static_assert(kS <= 6, "the scales' loads are older than those that may be outstanding");
+  int stage = 0;
+  auto group = [&](int c, bool more, const float (&held)[NPROJ]) {
+    float ws[2];
+    ws[0] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(held[0]), c & 63));
+    ws[1] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(held[NPROJ - 1]), c & 63));
     if (more) {
       __builtin_amdgcn_s_waitcnt(vmcnt_imm((kS - 2) * L::kLoads));
     } else {
       wait_groups_ahead<kS - 2, L::kLoads>(min(kS - 2, groups - 1 - c));
     }
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's scales are in LDS
     ring_barrier();
-    if (more) issue(c + kS - 1, stage == 0 ? kS - 1 : stage - 1);
-    compute(stage, c, ws);
+    const int into = stage == 0 ? kS - 1 : stage - 1;
+    compute(stage, c, ws, [&] {
+      if ((c & 3) == 0 && c + 4 < groups) issue_scales(c + 4);
+      if (more) {
+#pragma unroll
+        for (int j = 0; j < L::kLoads; ++j) issue(c + kS - 1, into, j);
+      }
+    });
     stage = stage + 1 == kS ? 0 : stage + 1;
   };
-  int c = 0;
+  for (int c = 0; c < groups;) {
+    const int end = min(c + 64, groups), whole = min(end, groups - (kS - 1));
+    float held[NPROJ];
+#pragma unroll
+    for (int p = 0; p < NPROJ; ++p) {
+      held[p] = sw[p][min(c + lane, groups - 1)];
+      asm volatile("" ::"v"(held[p]));  // (waited for here, not within the loops)
+    }
 #pragma clang loop unroll(disable)
-  for (; c < groups - (kS - 1); ++c) group(c, true);
+    for (; c < whole; ++c) group(c, true, held);
 #pragma clang loop unroll(disable)
-  for (; c < groups; ++c) group(c, false);
+    for (; c < end; ++c) group(c, false, held);
+  }
 
   const int fw = f0 + wn * HB * 16, tw = t0 + wt * BT * 16;  // the wave's first feature and token
   if constexpr (OUT == kOutBf16) {
@@ -694,7 +726,7 @@ static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
   if (type == GLM_ROWS_F32) return launch_stream<1, GLM_ROWS_F32>(stream, a);
   if (a.T <= kStreamTokens) return launch_stream<1, GLM_ROWS_FP8>(stream, a);
   const Fp8TileArgs t{a, nullptr, nullptr, 0, 0, 0};
-  if (a.T <= 512) return launch_tile<1, true, Fp8Tile<2, 4, 4, 1>, kOutBf16>(stream, t);
+  if (a.T <= 512) return launch_tile<1, true, Fp8Tile<2, 2, 2, 2, 52>, kOutBf16>(stream, t);
   return launch_tile<1, true, Fp8Tile<2, 4, 8, 4>, kOutBf16>(stream, t);
 }
 
@@ -703,7 +735,7 @@ static int gated_product(hipStream_t stream, const Fp8Args &a, int type, uint8_t
   if (a.T > kStreamTokens) {
     const Fp8TileArgs t{a, codes, scales, 0, 0, 0};
     if (a.T <= 1024) return launch_tile<2, false, Fp8Tile<2, 4, 8, 1>, kOutCodes>(stream, t);
-    return launch_tile<2, false, Fp8Tile<4, 2, 4, 4>, kOutCodes>(stream, t);
+    return launch_tile<2, false, Fp8Tile<2, 4, 8, 4>, kOutCodes>(stream, t);
   }
   const int rc = type == GLM_ROWS_BF16  ? launch_stream<2, GLM_ROWS_BF16>(stream, a)
                  : type == GLM_ROWS_F32 ? launch_stream<2, GLM_ROWS_F32>(stream, a)
