@@ -29,7 +29,10 @@ typedef int fp8_frag __attribute__((ext_vector_type(8)));
 
 constexpr int kStreamWaves = 8;
 constexpr int kStreamThreads = 64 * kStreamWaves;
-constexpr int kFusedTokens = 16; // rows that the product quantises itself, up to so many
+// Rows that the product quantises itself: up to so many, and so many codes, which
+// have to fit its LDS.  (Each workgroup does it for itself: at K and N 4096 1, 4
+// and 16 rows so take 7.0, 7.6 and 13.1 us, quantised before 8.5 to 8.8.)
+constexpr int kFusedTokens = 4, kFusedCodes = 1 << 16;
 
 struct Fp8Args {
   const void *x;          // codes, or bf16 / f32 rows
@@ -38,8 +41,12 @@ struct Fp8Args {
   const float *ws[2];     // [ceil(N / 128)][groups]
   int T, K, N, groups;
   float limit;
+  int ahead;              // fp8_stream_kernel: groups that a wave has in flight
+  uint32_t per_token;     // and 2^32 / T upwards, T from 2 to kFusedTokens, for quotients below 2^16
   uint16_t *out;          // NPROJ 1: bf16 [T][N]
-  float *h;               // NPROJ 2: f32 [T][N]
+  float *h;               // NPROJ 2, few tokens: f32 [split][2][T][N]; else f32 [T][N]
+  uint8_t *codes;         // gated and quantised
+  float *scales;
 };
 
 __device__ __forceinline__ fp8_frag join16(const glm_u32x4 &a, const glm_u32x4 &b) {
@@ -93,163 +100,297 @@ __device__ __forceinline__ float gated(float g, float u, float limit) {
   return g / (1.0f + expf(-g)) * u;
 }
 
+constexpr uint32_t kOutOfRange = 0x40000000u;  // past any tile's operand (256 rows of 2^20 codes)
+
+// Waits until at most `ahead` (0 .. MAX, uniform) groups of LOADS loads are
+// outstanding.
+template <int MAX, int LOADS>
+__device__ __forceinline__ void wait_groups_ahead(int ahead) {
+  static_assert(MAX * LOADS < 64, "the wait counter's range");
+  if (ahead >= MAX) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(MAX * LOADS));
+  } else if constexpr (MAX > 0) {
+    wait_groups_ahead<MAX - 1, LOADS>(ahead);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Few tokens: the weights are streamed once for up to 16 TB tokens.  A
 // workgroup has 16 weight rows (of each projection); its eight waves take the
-// groups of K in turn and add up their f32 results in LDS.  A wave asks for
-// the weights and the rows of AHEAD groups before it works on the first: what
-// it waits for is then one latency for as many groups.  ROWS says what x holds:
-// bf16 and f32 rows are quantised in registers, where the four lanes of a token
-// hold its group.
+// groups of K in turn, each through LDS of its own, and add up their f32
+// results at the end: no wave waits for another before that.  Gated pairs of
+// few row tiles are split along K too (blockIdx.z); what reads their sums joins
+// them.
+//
+// Operands come by direct loads, 16 bytes a lane, whose lanes walk along a
+// row: an operand's own lanes lie in 16 rows, and loads into registers took 64
+// address cycles instead of 16 (64 tokens of the pair, K 4096, 2 x 2048
+// features: 20 us).  The group behind is asked for as soon as a group's
+// operands are in registers.  ROWS says what x holds: bf16 and f32 rows are
+// quantised by the workgroup into LDS while the first weights are on their way,
+// four lanes a group (by each wave for its own groups, 16 columns whatever the
+// tokens are, one token at K 4096 took 2 us more).
 // ---------------------------------------------------------------------------
-template <int ROWS>
-struct StreamRow;  // a lane's 32 channels of a group, as they are stored
-template <>
-struct StreamRow<GLM_ROWS_FP8> {
-  glm_u32x4 v[2];
-  float scale;
-  __device__ __forceinline__ void load(const Fp8Args &a, long long t, int g, int k0, int k1) {
-    const uint8_t *row = (const uint8_t *)a.x + t * a.K;
-    v[0] = *reinterpret_cast<const glm_u32x4 *>(row + k0);
-    v[1] = *reinterpret_cast<const glm_u32x4 *>(row + k1);
-    scale = a.xs[t * a.groups + g];
+constexpr int kStreamKB = 152;  // LDS of a workgroup where the CUs have one each
+constexpr int kStreamPairKB = 78;  // else
+
+// FEW: up to 8 tokens, one load's.
+template <int NPROJ, int TB, int ROWS, bool FEW>
+struct Fp8Stream {
+  static constexpr bool kCoded = ROWS == GLM_ROWS_FP8;
+  static constexpr int kTok = !kCoded ? kFusedTokens : FEW ? 8 : 16 * TB;
+  static constexpr int kW = NPROJ * 16 * kFp8Group;          // one group in LDS: the weight rows,
+  static constexpr int kX = kCoded ? kTok * kFp8Group : 0;   // the tokens' codes
+  static constexpr int kS = kCoded ? 256 : 0;                // and scales, a lane each
+  static constexpr int kSlot = kW + kX + kS;
+  static constexpr int kLoads = (kW + kX) / 1024 + (kS ? 1 : 0);
+  static constexpr int kMost = 4;                            // groups a wave has in flight at most
+  static constexpr int kPart = kStreamWaves * NPROJ * TB * kWave * 16;
+  static_assert(kLoads * (kMost - 1) < 64 && TB * 16 <= kWave, "the wait counter, a lane a token's scale");
+  // piece p of row R lies at p ^ swz(R)
+  __host__ __device__ static int swz(int row) { return (row >> 1) & 7; }
+  // rows that the workgroup quantises: codes [group][token][128] and scales [group][token] behind
+  // the ring, of so many groups
+  __host__ __device__ static int coded_groups(int groups, int splits) {
+    return kCoded ? 0 : kStreamWaves * ((groups + kStreamWaves * splits - 1) / (kStreamWaves * splits));
   }
-  __device__ __forceinline__ fp8_frag codes(bool in0, bool in1, float &s) {
-    s = scale;
-    return join16(in0 ? v[0] : glm_u32x4{0, 0, 0, 0}, in1 ? v[1] : glm_u32x4{0, 0, 0, 0});
-  }
-};
-template <int ROWS>
-struct StreamRow {
-  static constexpr bool kF32 = ROWS == GLM_ROWS_F32;
-  float v[4][8];
-  __device__ __forceinline__ void load(const Fp8Args &a, long long t, int, int k0, int k1) {
-    load8<kF32>(a.x, t * a.K + k0, v[0]);
-    load8<kF32>(a.x, t * a.K + k0 + 8, v[1]);
-    load8<kF32>(a.x, t * a.K + k1, v[2]);
-    load8<kF32>(a.x, t * a.K + k1 + 8, v[3]);
-  }
-  __device__ __forceinline__ static float over_lanes(float m) {
-    m = fmaxf(m, __shfl_xor(m, 16, kWave));
-    return fmaxf(m, __shfl_xor(m, 32, kWave));
-  }
-  __device__ __forceinline__ fp8_frag codes(bool in0, bool in1, float &s) {
-    float (&f)[32] = reinterpret_cast<float (&)[32]>(v);
-#pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = (j < 16 ? in0 : in1) ? f[j] : 0.f;
-    float m = over_lanes(abs_max(f));
-    if (__builtin_expect(__any(isinf(m)), 0)) m = over_lanes(finite_abs_max(f));
-    m = fmaxf(m, kFp8Tiny);
-    const float up = kFp8Max / m;
-    fp8_frag b;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      b[j] = (int)fp8_codes4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3], up);
-    s = m / kFp8Max;
-    return b;
+  static int coded_bytes(int groups, int splits) {
+    return coded_groups(groups, splits) * kTok * (kFp8Group + 4);
   }
 };
 
-template <int NPROJ, int TB, int ROWS, int AHEAD>
+template <int NPROJ, int TB, int ROWS, bool FEW>
 __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
-  __shared__ glm_f32x4 part[kStreamWaves][NPROJ * TB][kWave];
+  using L = Fp8Stream<NPROJ, TB, ROWS, FEW>;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int n0 = 16 * blockIdx.x, t0 = 16 * TB * blockIdx.y;
-  const uint8_t *wrow[NPROJ];
-  const float *wscale[NPROJ];
+  const int K = a.K, groups = a.groups, ahead = a.ahead;
+  const int first = wave + kStreamWaves * blockIdx.z, step = kStreamWaves * gridDim.z;
+  const int mine = first < groups ? (groups - first + step - 1) / step : 0;  // groups of this wave
+  uint8_t *ring = smem + wave * (ahead * L::kSlot);
+  uint8_t *coded = smem + kStreamWaves * ahead * L::kSlot;  // the workgroup's own codes and scales
+  const int ncoded = L::coded_groups(groups, gridDim.z);
+  float *coded_scales = reinterpret_cast<float *>(coded + ncoded * L::kTok * kFp8Group);
+
+  const uint32_t feats = (uint32_t)min(a.N - n0, 16), toks = (uint32_t)min(a.T - t0, L::kTok);
+  const __amdgpu_buffer_rsrc_t xres =
+      make_rsrc((const uint8_t *)a.x + (long long)t0 * K, toks * (uint32_t)K);
+  const __amdgpu_buffer_rsrc_t sres =
+      make_rsrc(L::kCoded ? a.xs + (long long)t0 * groups : a.ws[0], toks * (uint32_t)groups * 4u);
+  __amdgpu_buffer_rsrc_t wres[NPROJ];
 #pragma unroll
-  for (int p = 0; p < NPROJ; ++p) {
-    wrow[p] = a.w[p] + (long long)min(n0 + r, a.N - 1) * a.K;
-    wscale[p] = a.ws[p] + (long long)(n0 / kFp8Group) * a.groups;
+  for (int p = 0; p < NPROJ; ++p)
+    wres[p] = make_rsrc(a.w[p] + (long long)n0 * K, feats * (uint32_t)K);
+  // rows past the last and channels past K are out of the buffers' range, which gives zeros
+  auto issue = [&](int i, int slot) {  // the wave's i-th group
+    const int g = first + i * step;
+    uint8_t *to = ring + slot * L::kSlot;
+    const int left = K - g * kFp8Group;
+#pragma unroll
+    for (int j = 0; j < (L::kW + L::kX) / 1024; ++j) {
+      const bool isw = j < L::kW / 1024;
+      const int row = (isw ? (j & 1) : j - L::kW / 1024) * 8 + lane / 8;
+      const int piece = (lane % 8) ^ L::swz(row);
+      buf16_to_lds(isw ? wres[isw ? j / 2 : 0] : xres, to + j * 1024,
+                   16 * piece < left ? (uint32_t)row * (uint32_t)K + 16 * piece : kOutOfRange,
+                   (uint32_t)g * kFp8Group);
+    }
+    if constexpr (L::kCoded)
+      buf4_to_lds(sres, to + L::kW + L::kX,
+                  lane < L::kTok ? (uint32_t)lane * (uint32_t)groups * 4u : kOutOfRange,
+                  (uint32_t)g * 4);
+  };
+  // lane l holds the block scales of the wave's l-th group of each 64
+  float held[NPROJ];
+  auto hold = [&](int i) {
+#pragma unroll
+    for (int p = 0; p < NPROJ; ++p)
+      held[p] = a.ws[p][(long long)(n0 / kFp8Group) * groups + min(first + (i + lane) * step, groups - 1)];
+  };
+  hold(0);
+  if constexpr (L::kCoded) {
+    for (int i = 0; i < ahead; ++i)
+      if (i < mine) issue(i, i);
+  } else {
+    // item: token item % toks of the workgroup's group item / toks; four lanes, of which each
+    // has every fourth eight channels
+    constexpr int kPer = kStreamThreads / 4;
+    const int items = ncoded * (int)toks, l4 = threadIdx.x & 3;
+    auto place = [&](int item, int &li, int &t) {
+      li = toks == 1 ? item : (int)__umulhi((uint32_t)item, a.per_token);
+      t = item - li * (int)toks;
+    };
+    float v[32], ahead_v[32];
+    auto load = [&](int item, float (&to)[32]) {
+      int li, t;
+      place(item, li, t);
+      const int g = (li / kStreamWaves) * step + kStreamWaves * blockIdx.z + li % kStreamWaves;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = g * kFp8Group + 8 * (4 * j + l4);
+        float (&e)[8] = *reinterpret_cast<float (*)[8]>(to + 8 * j);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = 0.f;
+        if (item < items && k < K) load8<ROWS == GLM_ROWS_F32>(a.x, (long long)(t0 + t) * K + k, e);
+      }
+    };
+    load(threadIdx.x >> 2, v);
+    for (int i = 0; i < ahead; ++i)
+      if (i < mine) issue(i, i);
+    for (int item = threadIdx.x >> 2; item < items; item += kPer) {
+      load(item + kPer, ahead_v);
+      int li, t;
+      place(item, li, t);
+      auto over_lanes = [](float m) {
+        m = fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0xB1, 0xf, 0xf, true)));
+        return fmaxf(m, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0x4E, 0xf, 0xf, true)));
+      };
+      float m = over_lanes(abs_max(v));
+      if (__builtin_expect(isinf(m), 0)) m = over_lanes(finite_abs_max(v));  // (one answer in the four)
+      m = fmaxf(m, kFp8Tiny);
+      const float up = kFp8Max / m;
+      uint8_t *row = coded + (li * L::kTok + t) * kFp8Group + 8 * (l4 & 1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint2 *>(row + 16 * ((2 * j + (l4 >> 1)) ^ L::swz(t))) =
+            uint2{fp8_codes4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3], up),
+                  fp8_codes4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7], up)};
+      if (l4 == 0) coded_scales[li * L::kTok + t] = m / kFp8Max;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = ahead_v[i];
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's codes are in LDS
+    ring_barrier();
   }
+
   glm_f32x4 acc[NPROJ][TB];
 #pragma unroll
   for (int p = 0; p < NPROJ; ++p)
 #pragma unroll
     for (int b = 0; b < TB; ++b) acc[p][b] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
-
-  for (int g0 = wave; g0 < a.groups; g0 += kStreamWaves * AHEAD) {
-    glm_u32x4 wv[AHEAD][NPROJ][2];
-    float sw[AHEAD][NPROJ];
-    StreamRow<ROWS> row[AHEAD][TB];
+  // the lane's pieces of a row of codes, p0 and p0 + 1 (fp8_tile_kernel): channels 16 p0 .. + 31
+  const int p0 = 4 * (q & 1) + 2 * (q >> 1);
+  auto frag = [&](const uint8_t *rows, int row) {
+    const glm_u32x4 *p = reinterpret_cast<const glm_u32x4 *>(rows + row * kFp8Group);
+    return join16(p[p0 ^ L::swz(row)], p[(p0 + 1) ^ L::swz(row)]);
+  };
+  int slot = 0;
+  auto group = [&](int i) {
+    wait_groups_ahead<L::kMost - 1, L::kLoads>(min(ahead - 1, mine - 1 - i));
+    asm volatile("" ::: "memory");
+    const uint8_t *from = ring + slot * L::kSlot;
+    fp8_frag w[NPROJ];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {  // (past the last group or channel: the last again)
-      const int g = min(g0 + i * kStreamWaves, a.groups - 1), k = g * kFp8Group + 32 * q;
-      const int k0 = min(k, a.K - 16), k1 = min(k + 16, a.K - 16);
+    for (int p = 0; p < NPROJ; ++p) w[p] = frag(from + p * 16 * kFp8Group, r);
+    // (columns past the tokens repeat one)
+    const int li = i * kStreamWaves + wave;
+    const uint8_t *xrows = L::kCoded ? from + L::kW : coded + li * L::kTok * kFp8Group;
+    const float *xscales = L::kCoded ? reinterpret_cast<const float *>(from + L::kW + L::kX)
+                                     : coded_scales + li * L::kTok;
+    Fp8Operand<false> x[TB];
+    float sx[TB];
 #pragma unroll
-      for (int p = 0; p < NPROJ; ++p) {
-        wv[i][p][0] = load_stream(wrow[p] + k0);
-        wv[i][p][1] = load_stream(wrow[p] + k1);
-        sw[i][p] = wscale[p][g];
-      }
-#pragma unroll
-      for (int b = 0; b < TB; ++b) row[i][b].load(a, min(t0 + 16 * b + r, a.T - 1), g, k0, k1);
+    for (int b = 0; b < TB; ++b) {
+      const int t = min(b * 16 + r, L::kCoded ? L::kTok - 1 : (int)toks - 1);
+      x[b] = Fp8Operand<false>(frag(xrows, t));
+      sx[b] = xscales[t];
     }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // the slot's reads are done
+    asm volatile("" ::: "memory");
+    if (i + ahead < mine) issue(i + ahead, slot);
+    slot = slot + 1 == ahead ? 0 : slot + 1;
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int g = g0 + i * kStreamWaves, k = g * kFp8Group + 32 * q;
-      // (a branch around a group past the last would let its loads sink behind it;
-      // both sides are zeroed: a NaN behind the end would pass through a zero)
-      const bool in0 = k < a.K, in1 = k + 16 < a.K;
-      Fp8Operand<false> x[TB];
-      float sx[TB];
+    for (int p = 0; p < NPROJ; ++p) {
+      const float sw = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(held[p]), i & 63));
+      const Fp8Operand<false> wo(w[p]);
+      glm_f32x4 c[TB];
 #pragma unroll
-      for (int b = 0; b < TB; ++b) x[b] = Fp8Operand<false>(row[i][b].codes(in0, in1, sx[b]));
+      for (int j = 0; j < Fp8Operand<false>::kSteps; ++j)
 #pragma unroll
-      for (int p = 0; p < NPROJ; ++p) {
-        const glm_u32x4 zero{0, 0, 0, 0};
-        const Fp8Operand<false> w(join16(in0 ? wv[i][p][0] : zero, in1 ? wv[i][p][1] : zero));
-        glm_f32x4 c[TB];
+        for (int b = 0; b < TB; ++b) c[b] = step_sum(wo, x[b], j, c[b]);
 #pragma unroll
-        for (int j = 0; j < Fp8Operand<false>::kSteps; ++j)
+      for (int b = 0; b < TB; ++b) {
+        const float s = sx[b] * sw;
 #pragma unroll
-          for (int b = 0; b < TB; ++b) c[b] = step_sum(w, x[b], j, c[b]);
-#pragma unroll
-        for (int b = 0; b < TB; ++b) {
-          const float s = g < a.groups ? sx[b] * sw[i][p] : 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[p][b][j] += c[b][j] * s;
-        }
+        for (int j = 0; j < 4; ++j) acc[p][b][j] += c[b][j] * s;
       }
     }
+  };
+  for (int i = 0; i < mine;) {
+    const int end = min(i + 64, mine);
+    if (i != 0) hold(i);
+#pragma unroll
+    for (int p = 0; p < NPROJ; ++p) asm volatile("" ::"v"(held[p]));  // (waited for here, not within the loop)
+#pragma clang loop unroll(disable)
+    for (; i < end; ++i) group(i);
   }
+
+  __syncthreads();  // (the ring is done with)
+  glm_f32x4 *part = reinterpret_cast<glm_f32x4 *>(smem);  // [wave][NPROJ * TB][lane]
 #pragma unroll
   for (int p = 0; p < NPROJ; ++p)
 #pragma unroll
-    for (int b = 0; b < TB; ++b) part[wave][p * TB + b][lane] = acc[p][b];
+    for (int b = 0; b < TB; ++b) part[(wave * NPROJ * TB + p * TB + b) * kWave + lane] = acc[p][b];
   __syncthreads();
-  if (wave >= TB) return;
-  const int t = t0 + 16 * wave + r, n = n0 + 4 * q;
-  glm_f32x4 sum[NPROJ];
+  constexpr int kJobs = NPROJ * TB;  // blocks of 16 x 16 to add up, a wave each
+  static_assert(kJobs <= kStreamWaves, "a wave a block");
+  if (wave >= kJobs) return;
+  const int t = t0 + 16 * (wave % TB) + r, n = n0 + 4 * q, p = wave / TB;
+  glm_f32x4 sum = part[wave * kWave + lane];
 #pragma unroll
-  for (int p = 0; p < NPROJ; ++p) {
-    sum[p] = part[0][p * TB + wave][lane];
+  for (int w = 1; w < kStreamWaves; ++w) {
+    const glm_f32x4 o = part[(w * kJobs + wave) * kWave + lane];
 #pragma unroll
-    for (int w = 1; w < kStreamWaves; ++w) {
-      const glm_f32x4 o = part[w][p * TB + wave][lane];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum[p][j] += o[j];
-    }
+    for (int j = 0; j < 4; ++j) sum[j] += o[j];
   }
   if (t >= a.T || n >= a.N) return;
-  if constexpr (NPROJ == 2) {
-    glm_f32x4 h;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = gated(sum[0][j], sum[1][j], a.limit);
-    *reinterpret_cast<glm_f32x4 *>(a.h + (long long)t * a.N + n) = h;  // (N % 16 == 0)
+  if constexpr (NPROJ == 2) {  // (N % 16 == 0)
+    *reinterpret_cast<glm_f32x4 *>(a.h + (((long long)blockIdx.z * 2 + p) * a.T + t) * a.N + n) = sum;
   } else {
     uint16_t *out = a.out + (long long)t * a.N + n;
     if (a.N % 4 == 0) {
-      *reinterpret_cast<uint2 *>(out) =
-          uint2{f32_to_bf16(sum[0][0]) | (f32_to_bf16(sum[0][1]) << 16),
-                f32_to_bf16(sum[0][2]) | (f32_to_bf16(sum[0][3]) << 16)};
+      *reinterpret_cast<uint2 *>(out) = uint2{f32_to_bf16(sum[0]) | (f32_to_bf16(sum[1]) << 16),
+                                              f32_to_bf16(sum[2]) | (f32_to_bf16(sum[3]) << 16)};
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (n + j < a.N) out[j] = (uint16_t)f32_to_bf16(sum[0][j]);
+        if (n + j < a.N) out[j] = (uint16_t)f32_to_bf16(sum[j]);
     }
   }
+}
+
+// The gated pair's sums [split][projection][T][N] joined, gated and quantised:
+// sixteen lanes a group of features.
+__global__ __launch_bounds__(256) void fp8_gate_kernel(const float *h, int splits, int T, int N,
+                                                       float limit, uint8_t *codes, float *scales) {
+  const int groups = fp8_groups(N), lane = threadIdx.x & 15;
+  const long long item = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (item >= (long long)T * groups) return;
+  const int t = (int)(item / groups), n = (int)(item - (long long)t * groups) * kFp8Group + 8 * lane;
+  float v[8] = {};
+  if (n < N) {
+    float sum[2][8];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      load8<true>(h, ((long long)p * T + t) * N + n, sum[p]);
+      for (int z = 1; z < splits; ++z) {
+        float o[8];
+        load8<true>(h, ((long long)(2 * z + p) * T + t) * N + n, o);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[p][j] += o[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = gated(sum[0][j], sum[1][j], limit);
+  }
+  const float amax = group_amax(v);
+  const float up = kFp8Max / amax;
+  if (n < N)
+    *reinterpret_cast<uint2 *>(codes + (long long)t * N + n) =
+        uint2{fp8_codes4(v[0], v[1], v[2], v[3], up), fp8_codes4(v[4], v[5], v[6], v[7], up)};
+  if (lane == 0) scales[item] = amax / kFp8Max;
 }
 
 // ---------------------------------------------------------------------------
@@ -262,12 +403,9 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
 // past K are out of the buffers' range, which gives zeros.
 // ---------------------------------------------------------------------------
 constexpr int kTileXcds = 8;
-constexpr uint32_t kOutOfRange = 0x40000000u;  // past any tile's operand (256 rows of 2^20 bytes)
 
 struct Fp8TileArgs {
   Fp8Args p;
-  uint8_t *codes;   // gated and quantised
-  float *scales;
   int row_tiles, tok_tiles;
   int rows_outer;   // consecutive items walk the tokens of one row tile, else the reverse
 };
@@ -291,18 +429,6 @@ struct Fp8Tile {
   static_assert(kStages >= 2 && BN >= 2, "a ring, blocks in turn");
   __device__ static int swz(int row) { return (row >> 1) & 7; }
 };
-
-// Waits until at most `ahead` (0 .. MAX, uniform) groups of LOADS loads are
-// outstanding.
-template <int MAX, int LOADS>
-__device__ __forceinline__ void wait_groups_ahead(int ahead) {
-  static_assert(MAX * LOADS < 64, "the wait counter's range");
-  if (ahead >= MAX) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(MAX * LOADS));
-  } else if constexpr (MAX > 0) {
-    wait_groups_ahead<MAX - 1, LOADS>(ahead);
-  }
-}
 
 __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -640,14 +766,14 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
           *reinterpret_cast<uint32_t *>(st + tok * kStride + wn * HB * 16 + 16 * b + 4 * q) =
               fp8_codes4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3], up);
         if (wn == 0 && q == 0 && t0 + tok < T)
-          a.scales[(long long)(t0 + tok) * fp8_groups(N) + f0 / kFp8Group] = m / kFp8Max;
+          a.p.scales[(long long)(t0 + tok) * fp8_groups(N) + f0 / kFp8Group] = m / kFp8Max;
       }
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < L::kTok * 8 / L::kThreads; ++i) {
         const int slot = i * L::kThreads + tid, tok = slot / 8, n = f0 + 16 * (slot % 8);
         if (t0 + tok < T && n < N)
-          *reinterpret_cast<glm_u32x4 *>(a.codes + (long long)(t0 + tok) * N + n) =
+          *reinterpret_cast<glm_u32x4 *>(a.p.codes + (long long)(t0 + tok) * N + n) =
               *reinterpret_cast<const glm_u32x4 *>(st + tok * kStride + 16 * (slot % 8));
       }
     }
@@ -660,36 +786,69 @@ using namespace glm;
 
 static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-template <int NPROJ, int TB, int ROWS>
-static void launch_stream_tokens(hipStream_t stream, const Fp8Args &a) {
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.T + 16 * TB - 1) / (16 * TB)));
-  const dim3 block(kStreamThreads);
-  if (a.groups <= kStreamWaves)
-    hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, TB, ROWS, 1>), grid, block, 0, stream, a);
-  else if (TB >= 4 || a.groups <= 2 * kStreamWaves)
-    hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, TB, ROWS, 2>), grid, block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, TB, ROWS, TB >= 4 ? 2 : 4>), grid, block, 0, stream, a);
+// splits: the workgroups along K.
+template <int NPROJ, int TB, int ROWS, bool FEW>
+static void launch_stream_tokens(hipStream_t stream, Fp8Args a, int splits) {
+  using L = Fp8Stream<NPROJ, TB, ROWS, FEW>;
+  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.T + 16 * TB - 1) / (16 * TB)),
+                  (unsigned)splits);
+  // a workgroup a CU takes all the LDS for its groups in flight, else two share it
+  const int coded = L::coded_bytes(a.groups, splits);
+  const long long wgs = (long long)grid.x * grid.y * grid.z;
+  const int room = (wgs <= 256 ? kStreamKB : kStreamPairKB) * 1024 - coded;
+  int ahead = room / (kStreamWaves * L::kSlot);
+  const int per_wave = (a.groups + kStreamWaves * splits - 1) / (kStreamWaves * splits);
+  ahead = ahead < L::kMost ? ahead : L::kMost;
+  ahead = ahead < per_wave ? ahead : per_wave;
+  a.ahead = ahead < 1 ? 1 : ahead;
+  a.per_token = a.T > 1 && a.T <= kFusedTokens ? (uint32_t)(((1ull << 32) + a.T - 1) / a.T) : 0;
+  const int bytes = kStreamWaves * a.ahead * L::kSlot + coded;
+  hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, TB, ROWS, FEW>), grid, dim3(kStreamThreads),
+                     (size_t)(bytes > L::kPart ? bytes : L::kPart), stream, a);
 }
 
-template <int NPROJ, int ROWS>
-static int launch_stream(hipStream_t stream, const Fp8Args &a) {
-  if (a.T <= 16) {
-    launch_stream_tokens<NPROJ, 1, ROWS>(stream, a);
-  } else if constexpr (ROWS == GLM_ROWS_FP8) {
-    if (a.T <= 32)
-      launch_stream_tokens<NPROJ, 2, ROWS>(stream, a);
-    else
-      launch_stream_tokens<NPROJ, 4, ROWS>(stream, a);
-  }
+template <int NPROJ>
+static int launch_stream(hipStream_t stream, const Fp8Args &a, int type, int splits) {
+  if (type == GLM_ROWS_BF16)
+    launch_stream_tokens<NPROJ, 1, GLM_ROWS_BF16, true>(stream, a, splits);
+  else if (type == GLM_ROWS_F32)
+    launch_stream_tokens<NPROJ, 1, GLM_ROWS_F32, true>(stream, a, splits);
+  else if (a.T <= 8)
+    launch_stream_tokens<NPROJ, 1, GLM_ROWS_FP8, true>(stream, a, splits);
+  else if (a.T <= 16)
+    launch_stream_tokens<NPROJ, 1, GLM_ROWS_FP8, false>(stream, a, splits);
+  else if (a.T <= 32)
+    launch_stream_tokens<NPROJ, 2, GLM_ROWS_FP8, false>(stream, a, splits);
+  else if (a.T <= 48)
+    launch_stream_tokens<NPROJ, 3, GLM_ROWS_FP8, false>(stream, a, splits);
+  else
+    launch_stream_tokens<NPROJ, 4, GLM_ROWS_FP8, false>(stream, a, splits);
   GLM_LAUNCH_CHECK("fp8_stream_kernel");
   return GLM_OK;
 }
 
-// Rows as the kernels take them: up to kFusedTokens as they are, more of them
-// quantised into the workspace first.
+constexpr int kStreamTokens = 64;  // up to so many the weights are streamed
+
+// Ways that a gated pair's K is split where its row tiles are fewer than the
+// CUs: as many as leave every wave a group.
+static int stream_splits(int K, int N) {
+  const int tiles = N / 16, most = fp8_groups(K) / kStreamWaves;
+  int s = 256 / (tiles > 0 ? tiles : 1);
+  s = s < most ? s : most;
+  return s < 1 ? 1 : s < 8 ? s : 8;
+}
+
+// Workspace of rows that the product does not take as they are.
+static size_t rows_bytes(int T, int K, int type) {
+  const long long codes = (long long)kFusedTokens * fp8_groups(K) * kFp8Group;
+  if (type == GLM_ROWS_FP8 || (T <= kFusedTokens && codes <= kFusedCodes)) return 0;
+  return round256((size_t)T * K) + round256((size_t)T * fp8_groups(K) * 4);
+}
+
+// Rows as the kernels take them: few as they are, more of them quantised into
+// the workspace first.
 static int rows_for(hipStream_t stream, Fp8Args &a, int &type, uint8_t *&ws) {
-  if (type == GLM_ROWS_FP8 || a.T <= kFusedTokens) return GLM_OK;
+  if (!rows_bytes(a.T, a.K, type)) return GLM_OK;
   uint8_t *codes = ws;
   ws += round256((size_t)a.T * a.K);
   float *scales = reinterpret_cast<float *>(ws);
@@ -699,10 +858,6 @@ static int rows_for(hipStream_t stream, Fp8Args &a, int &type, uint8_t *&ws) {
   a.xs = scales;
   type = GLM_ROWS_FP8;
   return rc;
-}
-static size_t rows_bytes(int T, int K, int type) {
-  if (type == GLM_ROWS_FP8 || T <= kFusedTokens) return 0;
-  return round256((size_t)T * K) + round256((size_t)T * fp8_groups(K) * 4);
 }
 
 template <int NPROJ, bool FAST, class L, int OUT>
@@ -719,28 +874,27 @@ static int launch_tile(hipStream_t stream, Fp8TileArgs a) {
   return GLM_OK;
 }
 
-constexpr int kStreamTokens = 64;  // up to so many the weights are streamed
-
 static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
-  if (type == GLM_ROWS_BF16) return launch_stream<1, GLM_ROWS_BF16>(stream, a);
-  if (type == GLM_ROWS_F32) return launch_stream<1, GLM_ROWS_F32>(stream, a);
-  if (a.T <= kStreamTokens) return launch_stream<1, GLM_ROWS_FP8>(stream, a);
-  const Fp8TileArgs t{a, nullptr, nullptr, 0, 0, 0};
+  if (a.T <= kStreamTokens) return launch_stream<1>(stream, a, type, 1);
+  const Fp8TileArgs t{a, 0, 0, 0};
   if (a.T <= 512) return launch_tile<1, true, Fp8Tile<2, 2, 2, 2, 52>, kOutBf16>(stream, t);
   return launch_tile<1, true, Fp8Tile<2, 4, 8, 4>, kOutBf16>(stream, t);
 }
 
-static int gated_product(hipStream_t stream, const Fp8Args &a, int type, uint8_t *codes,
-                         float *scales) {
+static int gated_product(hipStream_t stream, const Fp8Args &a, int type) {
   if (a.T > kStreamTokens) {
-    const Fp8TileArgs t{a, codes, scales, 0, 0, 0};
+    const Fp8TileArgs t{a, 0, 0, 0};
     if (a.T <= 1024) return launch_tile<2, false, Fp8Tile<2, 4, 8, 1>, kOutCodes>(stream, t);
     return launch_tile<2, false, Fp8Tile<2, 4, 8, 4>, kOutCodes>(stream, t);
   }
-  const int rc = type == GLM_ROWS_BF16  ? launch_stream<2, GLM_ROWS_BF16>(stream, a)
-                 : type == GLM_ROWS_F32 ? launch_stream<2, GLM_ROWS_F32>(stream, a)
-                                        : launch_stream<2, GLM_ROWS_FP8>(stream, a);
-  return rc ? rc : glm_fp8_quantize_rows(stream, a.h, GLM_ROWS_F32, a.T, a.N, codes, scales);
+  const int splits = stream_splits(a.K, a.N);
+  const int rc = launch_stream<2>(stream, a, type, splits);
+  if (rc) return rc;
+  const long long items = (long long)a.T * fp8_groups(a.N);
+  hipLaunchKernelGGL(fp8_gate_kernel, dim3((unsigned)((items + 15) / 16)), dim3(256), 0, stream,
+                     a.h, splits, a.T, a.N, a.limit, a.codes, a.scales);
+  GLM_LAUNCH_CHECK("fp8_gate_kernel");
+  return GLM_OK;
 }
 
 static bool sizes_fit(int T, int K, int N) {
@@ -765,7 +919,9 @@ static int check_product(const char *name, const void *x, int x_type, const floa
 
 extern "C" size_t glm_fp8_workspace_bytes(int x_type, int T, int K, int N, int gated) {
   if (!sizes_fit(T, K, N) || x_type < GLM_ROWS_BF16 || x_type > GLM_ROWS_FP8) return 0;
-  return rows_bytes(T, K, x_type) + (gated && T <= kStreamTokens ? round256((size_t)T * N * 4) : 0);
+  size_t sums = 0;  // of a gated pair of few rows
+  if (gated && T <= kStreamTokens) sums = round256((size_t)stream_splits(K, N) * 2 * T * N * 4);
+  return rows_bytes(T, K, x_type) + sums;
 }
 
 extern "C" int glm_fp8_linear(void *stream, const void *x, int x_type, const float *x_scales, int T,
@@ -779,8 +935,8 @@ extern "C" int glm_fp8_linear(void *stream, const void *x, int x_type, const flo
   GLM_REQUIRE(glm_aligned16({weight, scales, out}), GLM_ERR_INVALID_ARGUMENT,
               "fp8_linear: buffers must be 16-byte aligned");
   if (T == 0) return GLM_OK;
-  Fp8Args a{x, x_scales, {weight, nullptr}, {scales, nullptr}, T, K, N, fp8_groups(K), 0.f, out,
-            nullptr};
+  Fp8Args a{x, x_scales, {weight, nullptr}, {scales, nullptr}, T, K, N, fp8_groups(K), 0.f, 0,
+            0, out, nullptr, nullptr, nullptr};
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   hipStream_t s = (hipStream_t)stream;
   const int rc = rows_for(s, a, x_type, ws);
@@ -804,11 +960,11 @@ extern "C" int glm_fp8_gate_up(void *stream, const void *x, int x_type, const fl
               GLM_ERR_INVALID_ARGUMENT, "fp8_gate_up: buffers must be 16-byte aligned");
   if (T == 0) return GLM_OK;
   Fp8Args a{x, x_scales, {gate, up}, {gate_scales, up_scales}, T, K, N, fp8_groups(K), limit,
-            nullptr, nullptr};
+            0, 0, nullptr, nullptr, codes, scales};
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   hipStream_t s = (hipStream_t)stream;
   int rc = rows_for(s, a, x_type, ws);
   if (rc) return rc;
   a.h = reinterpret_cast<float *>(ws);
-  return gated_product(s, a, x_type, codes, scales);
+  return gated_product(s, a, x_type);
 }

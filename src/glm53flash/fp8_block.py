@@ -33,9 +33,11 @@ GROUP = 128
 
 _BF16, _F32, _U8, _F8 = torch.bfloat16, torch.float32, torch.uint8, torch.float8_e4m3fn
 _ROWS = {_BF16: N.native.GLM_ROWS_BF16, _F32: N.native.GLM_ROWS_F32}
+_CODED = N.native.GLM_ROWS_FP8
+_CODES, _SCALES = (_U8, _F8), (_F32,)
 _getDevice = torch._C._cuda_getDevice
 _getStream = torch._C._cuda_getCurrentRawStream
-_empty = torch.empty
+_empty, _empty_like = torch.empty, torch.empty_like
 
 
 class Fp8Rows(NamedTuple):
@@ -46,14 +48,14 @@ class Fp8Rows(NamedTuple):
     scales: torch.Tensor
 
 
-def _groups(n: int) -> int:
-    return -(-n // GROUP)
+# The calls of a decode step are a few microseconds of GPU work each, so what
+# the host does before them counts: what is right is recognised with a few
+# attributes, and only what is not is looked at again for the message.
 
 
-def _run(device: int, name: str, *args) -> None:
+def _run(device: int, name: str, function, *args) -> None:
     """A native call on the current stream of the tensors' device, which is the
     current one meanwhile, as a launch needs it."""
-    function = getattr(N.native.load(), name)
     if device == _getDevice():
         code = function(_getStream(device), *args)
     else:
@@ -65,90 +67,110 @@ def _run(device: int, name: str, *args) -> None:
 
 def _check(t, name: str, dtypes: tuple, device: int) -> None:
     """A contiguous tensor of the call's device and one of the dtypes."""
-    N.require_device(t, name, dtypes)
-    if t.get_device() != device:
+    try:
+        fine = t.dtype in dtypes and t.get_device() == device and t.is_contiguous()
+    except AttributeError:  # no tensor
+        fine = False
+    if not fine:
+        N.require_device(t, name, dtypes)
         raise ContractError(f"{name} is on {t.device}, the call's rows on device {device}")
 
 
-def _out(out, name: str, shape: tuple, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return _empty(shape, dtype=dtype, device=like.device)
-    _check(out, name, (dtype,), like.get_device())
-    if tuple(out.shape) != tuple(shape):
+def _given(out, name: str, shape, dtype: torch.dtype, device: int) -> torch.Tensor:
+    """An output that the caller brings."""
+    _check(out, name, (dtype,), device)
+    if out.shape != shape:
         raise ContractError(f"{name} {tuple(out.shape)}, expected {tuple(shape)}")
     return out
 
 
-def _plain_rows(x, name: str) -> tuple[int, int, int]:
-    """Device, rows and channels of bf16 or f32 rows ``[..., K]``."""
-    N.require_device(x, name, (_BF16, _F32))
-    if x.dim() < 1 or x.shape[-1] < 1:
+def _plain_rows(x, name: str = "x") -> tuple[int, int, int, int]:
+    """Device, native type, rows and channels of bf16 or f32 rows ``[..., K]``."""
+    try:
+        kind, dev, shape = _ROWS.get(x.dtype), x.get_device(), x.shape
+        K = shape[-1] if len(shape) else 0
+        fine = kind is not None and dev >= 0 and K > 0 and x.is_contiguous()
+    except AttributeError:  # no tensor
+        fine = False
+    if not fine:
+        N.require_device(x, name, (_BF16, _F32))
         raise ContractError(f"{name} must be [..., K] rows, got {tuple(x.shape)}")
-    K = x.shape[-1]
-    return x.get_device(), x.numel() // K, K
+    T = shape[0] if len(shape) == 2 else x.numel() // K
+    if (T | K) >> 31:  # (the library's sizes are 32-bit: none may wrap)
+        raise ContractError(f"{name}: {T} rows of {K} channels pass 32 bits")
+    return dev, kind, T, K
 
 
 def _rows(x) -> tuple:
-    """Device, rows, channels, leading shape and the native (pointer, type,
-    scales) of a product's rows: bf16, f32 or ``Fp8Rows``."""
-    if isinstance(x, tuple):
-        if len(x) != 2:
-            raise ContractError("quantised rows are (codes, scales)")
-        codes, scales = x
-        N.require_device(codes, "codes", (_U8, _F8))
-        dev = codes.get_device()
-        _check(scales, "scales", (_F32,), dev)
-        if codes.dim() < 1 or codes.shape[-1] < 1 or \
-                tuple(scales.shape) != (*codes.shape[:-1], _groups(codes.shape[-1])):
-            raise ContractError(f"scales {tuple(scales.shape)} do not fit codes "
-                                f"{tuple(codes.shape)}")
-        K = codes.shape[-1]
-        return dev, codes.numel() // K, K, codes.shape[:-1], codes.device, \
-            (codes.data_ptr(), N.native.GLM_ROWS_FP8, scales.data_ptr())
-    dev, T, K = _plain_rows(x, "x")
-    return dev, T, K, x.shape[:-1], x.device, (x.data_ptr(), _ROWS[x.dtype], None)
+    """Device, native type, rows, channels, pointers of the rows and their
+    scales, and the tensor whose leading shape they have, of a product's rows:
+    bf16, f32 or ``Fp8Rows``."""
+    if not isinstance(x, tuple):
+        return *_plain_rows(x), x.data_ptr(), None, x
+    if len(x) != 2:
+        raise ContractError("quantised rows are (codes, scales)")
+    codes, scales = x
+    try:
+        dev, shape = codes.get_device(), codes.shape
+        K = shape[-1] if len(shape) else 0
+        fine = codes.dtype in _CODES and dev >= 0 and K > 0 and codes.is_contiguous()
+    except AttributeError:  # no tensor
+        fine = False
+    if not fine:
+        N.require_device(codes, "codes", _CODES)
+        raise ContractError(f"codes must be [..., K] rows, got {tuple(codes.shape)}")
+    _check(scales, "scales", _SCALES, dev)
+    if scales.shape != (*shape[:-1], (K + 127) >> 7):
+        raise ContractError(f"scales {tuple(scales.shape)} do not fit codes {tuple(shape)}")
+    T = shape[0] if len(shape) == 2 else codes.numel() // K
+    if (T | K) >> 31:
+        raise ContractError(f"codes: {T} rows of {K} channels pass 32 bits")
+    return dev, _CODED, T, K, codes.data_ptr(), scales.data_ptr(), codes
 
 
 def _weight(w, scales, name: str, K: int, dev: int) -> int:
     """The output features of a weight that fits rows of K channels."""
-    _check(w, name, (_U8, _F8), dev)
-    _check(scales, f"{name} scales", (_F32,), dev)
-    if w.dim() != 2 or w.shape[1] != K or w.shape[0] < 1 or \
-            tuple(scales.shape) != (_groups(w.shape[0]), _groups(K)):
-        raise ContractError(f"{name} {tuple(w.shape)} with scales {tuple(scales.shape)} does not "
+    _check(w, name, _CODES, dev)
+    _check(scales, f"{name} scales", _SCALES, dev)
+    shape = w.shape
+    n = shape[0] if len(shape) == 2 else 0
+    if n < 1 or n >> 31 or shape[1] != K or scales.shape != ((n + 127) >> 7, (K + 127) >> 7):
+        raise ContractError(f"{name} {tuple(shape)} with scales {tuple(scales.shape)} does not "
                             f"fit rows of {K} channels")
-    return w.shape[0]
+    return n
 
 
 @lru_cache(maxsize=256)  # a function of the sizes alone
-def _workspace_bytes(name: str, *sizes: int) -> int:
-    if any(s >> 31 for s in sizes):
-        raise ContractError(f"sizes {sizes} pass 32 bits")
-    return int(getattr(N.native.load(), name)(*sizes))
+def _workspace_bytes(*sizes: int) -> int:
+    return int(N.native.load().glm_fp8_workspace_bytes(*sizes))
 
 
-def _workspace(device, name: str, *sizes: int) -> tuple:
-    need = _workspace_bytes(name, *sizes)
-    ws = _empty(need, dtype=_U8, device=device) if need else None
-    return ws, need
-
-
-def _sizes(name: str, *sizes: int) -> None:
-    if any(s >> 31 for s in sizes):  # (the library's sizes are 32-bit: none may wrap)
-        raise ContractError(f"{name}: sizes {sizes} pass 32 bits")
+def _coded_out(out, like: torch.Tensor, T: int, n: int, dev: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes ``[..., n]`` of a tensor's leading shape and their scales."""
+    groups = (n + 127) >> 7
+    shape = like.shape
+    if out is None:
+        device = like.device
+        if len(shape) == 2:  # (sizes one by one: a tuple of them takes a third longer)
+            return (_empty(T, n, dtype=_U8, device=device),
+                    _empty(T, groups, dtype=_F32, device=device))
+        return (_empty((*shape[:-1], n), dtype=_U8, device=device),
+                _empty((*shape[:-1], groups), dtype=_F32, device=device))
+    if not isinstance(out, tuple) or len(out) != 2:
+        raise ContractError("quantised rows are (codes, scales)")
+    return (_given(out[0], "codes", (*shape[:-1], n), _U8, dev),
+            _given(out[1], "scales", (*shape[:-1], groups), _F32, dev))
 
 
 def quantize_rows(x: torch.Tensor, *, out: Fp8Rows | None = None) -> Fp8Rows:
     """Codes and scales of bf16 or f32 rows ``[..., K]``, K a multiple of 8:
     per 128 channels ``scale = amax / 448``, ``code = e4m3(x * (448 / amax))``
     with amax the largest finite magnitude; an infinity or a NaN becomes NaN."""
-    dev, T, K = _plain_rows(x, "x")
-    _sizes("quantize_rows", T, K)
-    codes = _out(out and out[0], "codes", x.shape, _U8, x)
-    scales = _out(out and out[1], "scales", (*x.shape[:-1], _groups(K)), _F32, x)
+    dev, kind, T, K = _plain_rows(x)
+    codes, scales = _coded_out(out, x, T, K, dev)
     if T:
-        _run(dev, "glm_fp8_quantize_rows", x.data_ptr(), _ROWS[x.dtype], T, K, codes.data_ptr(),
-             scales.data_ptr())
+        _run(dev, "glm_fp8_quantize_rows", N.native.load().glm_fp8_quantize_rows, x.data_ptr(),
+             kind, T, K, codes.data_ptr(), scales.data_ptr())
     return Fp8Rows(codes, scales)
 
 
@@ -158,11 +180,12 @@ def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if weight.dim() != 2 or not weight.numel():
         raise ContractError(f"weight must be [N, K], got {tuple(weight.shape)}")
     n, K = weight.shape
-    _sizes("quantize_weight", n, K)
+    if (n | K) >> 31:
+        raise ContractError(f"a weight {tuple(weight.shape)} passes 32 bits")
     codes = _empty((n, K), dtype=_U8, device=weight.device)
-    scales = _empty((_groups(n), _groups(K)), dtype=_F32, device=weight.device)
-    _run(weight.get_device(), "glm_fp8_quantize_weight", weight.data_ptr(), n, K, codes.data_ptr(),
-         scales.data_ptr())
+    scales = _empty(((n + 127) >> 7, (K + 127) >> 7), dtype=_F32, device=weight.device)
+    _run(weight.get_device(), "glm_fp8_quantize_weight", N.native.load().glm_fp8_quantize_weight,
+         weight.data_ptr(), n, K, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -174,26 +197,30 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor | None, eps: float, *,
     ``x`` and ``residual`` bf16 or f32 ``[..., d]``, ``weight`` f32 ``[d]`` or
     None; ``residual_out`` may be ``residual`` itself.  Without a residual h is
     x, and None is returned for it."""
-    dev, T, d = _plain_rows(x, "x")
-    _sizes("add_rms_norm", T, d)
+    dev, kind, T, d = _plain_rows(x)
+    shape = x.shape
     if weight is not None:
-        _check(weight, "weight", (_F32,), dev)
+        _check(weight, "weight", _SCALES, dev)
         if weight.numel() != d:
             raise ContractError(f"a weight of {weight.numel()} for rows of {d} channels")
-    kind = N.native.GLM_ROWS_BF16
+    rkind = kind
     if residual is not None:
         _check(residual, "residual", (_BF16, _F32), dev)
-        if residual.shape != x.shape:
-            raise ContractError(f"residual {tuple(residual.shape)}, rows {tuple(x.shape)}")
-        kind = _ROWS[residual.dtype]
-        residual_out = _out(residual_out, "residual_out", x.shape, residual.dtype, x)
+        if residual.shape != shape:
+            raise ContractError(f"residual {tuple(residual.shape)}, rows {tuple(shape)}")
+        rkind = _ROWS[residual.dtype]
+        if residual_out is None:
+            residual_out = _empty_like(residual)
+        else:
+            _given(residual_out, "residual_out", shape, residual.dtype, dev)
     elif residual_out is not None:
         raise ContractError("residual_out comes with a residual")
-    codes = _out(out and out[0], "codes", x.shape, _U8, x)
-    scales = _out(out and out[1], "scales", (*x.shape[:-1], _groups(d)), _F32, x)
+    codes, scales = _coded_out(out, x, T, d, dev)
     if T:
-        _run(dev, "glm_add_rms_norm_fp8", x.data_ptr(), _ROWS[x.dtype], N.ptr(residual), kind, T,
-             d, N.ptr(weight), float(eps), N.ptr(residual_out), codes.data_ptr(),
+        _run(dev, "glm_add_rms_norm_fp8", N.native.load().glm_add_rms_norm_fp8, x.data_ptr(), kind,
+             None if residual is None else residual.data_ptr(), rkind, T, d,
+             None if weight is None else weight.data_ptr(), eps,
+             None if residual is None else residual_out.data_ptr(), codes.data_ptr(),
              scales.data_ptr())
     return Fp8Rows(codes, scales), residual_out
 
@@ -202,14 +229,20 @@ def linear(x: torch.Tensor | Fp8Rows, weight: torch.Tensor, scales: torch.Tensor
            out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 ``[..., N]`` of ``x @ weight.T``; bf16 and f32 rows are quantised as
     ``quantize_rows`` does.  K is a multiple of 16."""
-    dev, T, K, lead, device, rows = _rows(x)
+    dev, kind, T, K, rows, row_scales, lead = _rows(x)
     n = _weight(weight, scales, "weight", K, dev)
-    _sizes("linear", T, K, n)
-    out = _out(out, "out", (*lead, n), _BF16, weight)
+    if out is not None:
+        _given(out, "out", (*lead.shape[:-1], n), _BF16, dev)
+    elif len(lead.shape) == 2:
+        out = _empty(T, n, dtype=_BF16, device=lead.device)
+    else:
+        out = _empty((*lead.shape[:-1], n), dtype=_BF16, device=lead.device)
     if T:
-        ws, need = _workspace(device, "glm_fp8_workspace_bytes", rows[1], T, K, n, 0)
-        _run(dev, "glm_fp8_linear", *rows, T, K, weight.data_ptr(), scales.data_ptr(), n,
-             N.ptr(ws), need, out.data_ptr())
+        need = _workspace_bytes(kind, T, K, n, 0)
+        ws = _empty(need, dtype=_U8, device=lead.device) if need else None
+        _run(dev, "glm_fp8_linear", N.native.load().glm_fp8_linear, rows, kind, row_scales, T, K,
+             weight.data_ptr(), scales.data_ptr(), n, ws.data_ptr() if need else None, need,
+             out.data_ptr())
     return out
 
 
@@ -219,19 +252,18 @@ def gate_up(x: torch.Tensor | Fp8Rows, gate: torch.Tensor, gate_scales: torch.Te
     """Quantised ``silu(g) * u`` of ``g = x @ gate.T`` and ``u = x @ up.T``,
     both weights ``[I, K]``, I a multiple of 16; with ``limit > 0`` g is cut at
     ``limit`` and u at both ends.  f32 until the codes."""
-    dev, T, K, lead, device, rows = _rows(x)
+    dev, kind, T, K, rows, row_scales, lead = _rows(x)
     n = _weight(gate, gate_scales, "gate", K, dev)
     if _weight(up, up_scales, "up", K, dev) != n:
         raise ContractError(f"gate {tuple(gate.shape)} and up {tuple(up.shape)} differ")
-    _sizes("gate_up", T, K, n)
-    codes = _out(out and out[0], "codes", (*lead, n), _U8, gate)
-    codes_scales = _out(out and out[1], "scales", (*lead, _groups(n)), _F32, gate)
+    codes, scales = _coded_out(out, lead, T, n, dev)
     if T:
-        ws, need = _workspace(device, "glm_fp8_workspace_bytes", rows[1], T, K, n, 1)
-        _run(dev, "glm_fp8_gate_up", *rows, T, K, gate.data_ptr(), gate_scales.data_ptr(),
-             up.data_ptr(), up_scales.data_ptr(), n, float(limit), N.ptr(ws), need,
-             codes.data_ptr(), codes_scales.data_ptr())
-    return Fp8Rows(codes, codes_scales)
+        need = _workspace_bytes(kind, T, K, n, 1)
+        ws = _empty(need, dtype=_U8, device=lead.device) if need else None
+        _run(dev, "glm_fp8_gate_up", N.native.load().glm_fp8_gate_up, rows, kind, row_scales, T, K,
+             gate.data_ptr(), gate_scales.data_ptr(), up.data_ptr(), up_scales.data_ptr(), n,
+             limit, ws.data_ptr() if need else None, need, codes.data_ptr(), scales.data_ptr())
+    return Fp8Rows(codes, scales)
 
 
 __all__ = ["Fp8Rows", "GROUP", "add_rms_norm", "gate_up", "linear", "quantize_rows",
