@@ -779,7 +779,7 @@ size_t glm_fp8_workspace_bytes(int x_type, int T, int K, int N, int gated);
  * (DeferredLinear.__call__, layers.py:38-70, in this format).  Rows in bf16 or
  * f32 are quantised as glm_fp8_quantize_rows does.  y bf16 [T][N].  The
  * workspace needs no clearing; calls that may overlap need their own.
- * Limits: K % 16 == 0, K and N <= 2^20, T <= 2^21.
+ * Limits: K % 16 == 0, K, N and T <= 2^20.
  */
 int glm_fp8_linear(void *stream, const void *x, int x_type, const float *x_scales, int T, int K,
                    const uint8_t *weight, const float *scales, int N, void *workspace,

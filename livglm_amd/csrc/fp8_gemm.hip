@@ -28,7 +28,6 @@ namespace glm {
 typedef int fp8_frag __attribute__((ext_vector_type(8)));
 
 constexpr int kStreamWaves = 8;
-constexpr int kStreamThreads = 64 * kStreamWaves;
 // Rows that the product quantises itself: up to so many, and so many codes, which
 // have to fit its LDS.  (Each workgroup does it for itself: at K and N 4096 1, 4
 // and 16 rows so take 7.0, 7.6 and 13.1 us, quantised before 8.5 to 8.8.)
@@ -44,7 +43,7 @@ struct Fp8Args {
   int ahead;              // fp8_stream_kernel: groups that a wave has in flight
   uint32_t per_token;     // and 2^32 / T upwards, T from 2 to kFusedTokens, for quotients below 2^16
   uint16_t *out;          // NPROJ 1: bf16 [T][N]
-  float *h;               // NPROJ 2, few tokens: f32 [split][2][T][N]; else f32 [T][N]
+  float *h;               // NPROJ 2, streamed: the sums, f32 [split][2][T][N]
   uint8_t *codes;         // gated and quantised
   float *scales;
 };
@@ -134,47 +133,54 @@ __device__ __forceinline__ void wait_groups_ahead(int ahead) {
 constexpr int kStreamKB = 152;  // LDS of a workgroup where the CUs have one each
 constexpr int kStreamPairKB = 78;  // else
 
-// FEW: up to 8 tokens, one load's.
-template <int NPROJ, int TB, int ROWS, bool FEW>
+// WAVES waves, RB blocks of 16 weight rows of each projection, TB of 16 tokens;
+// FEW: up to 8 tokens, one load's; FAST: which of the two forms of the sum.
+template <int WAVES, int NPROJ_, int RB_, int TB_, int ROWS_, bool FEW = false, bool FAST_ = false>
 struct Fp8Stream {
+  static constexpr int NPROJ = NPROJ_, RB = RB_, TB = TB_, ROWS = ROWS_;
+  static constexpr bool FAST = FAST_;
+  static constexpr int kWaves = WAVES, kThreads = 64 * WAVES;
+  static constexpr int kRowBlocks = NPROJ * RB;
   static constexpr bool kCoded = ROWS == GLM_ROWS_FP8;
   static constexpr int kTok = !kCoded ? kFusedTokens : FEW ? 8 : 16 * TB;
-  static constexpr int kW = NPROJ * 16 * kFp8Group;          // one group in LDS: the weight rows,
+  static constexpr int kW = kRowBlocks * 16 * kFp8Group;     // one group in LDS: the weight rows,
   static constexpr int kX = kCoded ? kTok * kFp8Group : 0;   // the tokens' codes
-  static constexpr int kS = kCoded ? 256 : 0;                // and scales, a lane each
+  static constexpr int kSLoads = kCoded ? (kTok + 63) / 64 : 0;
+  static constexpr int kS = 256 * kSLoads;                   // and scales, a lane each
   static constexpr int kSlot = kW + kX + kS;
-  static constexpr int kLoads = (kW + kX) / 1024 + (kS ? 1 : 0);
-  static constexpr int kMost = 4;                            // groups a wave has in flight at most
-  static constexpr int kPart = kStreamWaves * NPROJ * TB * kWave * 16;
-  static_assert(kLoads * (kMost - 1) < 64 && TB * 16 <= kWave, "the wait counter, a lane a token's scale");
+  static constexpr int kLoads = (kW + kX) / 1024 + kSLoads;
+  static constexpr int kMost = kLoads <= 12 ? 4 : 2;         // groups a wave has in flight at most
+  static constexpr int kPart = WAVES * kRowBlocks * TB * kWave * 16;
+  static_assert(kLoads * (kMost - 1) < 64, "the wait counter's range");
   // piece p of row R lies at p ^ swz(R)
   __host__ __device__ static int swz(int row) { return (row >> 1) & 7; }
   // rows that the workgroup quantises: codes [group][token][128] and scales [group][token] behind
   // the ring, of so many groups
   __host__ __device__ static int coded_groups(int groups, int splits) {
-    return kCoded ? 0 : kStreamWaves * ((groups + kStreamWaves * splits - 1) / (kStreamWaves * splits));
+    return kCoded ? 0 : WAVES * ((groups + WAVES * splits - 1) / (WAVES * splits));
   }
   static int coded_bytes(int groups, int splits) {
     return coded_groups(groups, splits) * kTok * (kFp8Group + 4);
   }
 };
 
-template <int NPROJ, int TB, int ROWS, bool FEW>
-__global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
-  using L = Fp8Stream<NPROJ, TB, ROWS, FEW>;
+template <class L>
+__global__ __launch_bounds__(L::kThreads) void fp8_stream_kernel(Fp8Args a) {
+  constexpr int NPROJ = L::NPROJ, RB = L::RB, TB = L::TB, ROWS = L::ROWS, kWaves = L::kWaves;
+  constexpr bool FAST = L::FAST;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int n0 = 16 * blockIdx.x, t0 = 16 * TB * blockIdx.y;
+  const int n0 = 16 * RB * blockIdx.x, t0 = 16 * TB * blockIdx.y;
   const int K = a.K, groups = a.groups, ahead = a.ahead;
-  const int first = wave + kStreamWaves * blockIdx.z, step = kStreamWaves * gridDim.z;
+  const int first = wave + kWaves * blockIdx.z, step = kWaves * gridDim.z;
   const int mine = first < groups ? (groups - first + step - 1) / step : 0;  // groups of this wave
   uint8_t *ring = smem + wave * (ahead * L::kSlot);
-  uint8_t *coded = smem + kStreamWaves * ahead * L::kSlot;  // the workgroup's own codes and scales
+  uint8_t *coded = smem + kWaves * ahead * L::kSlot;  // the workgroup's own codes and scales
   const int ncoded = L::coded_groups(groups, gridDim.z);
   float *coded_scales = reinterpret_cast<float *>(coded + ncoded * L::kTok * kFp8Group);
 
-  const uint32_t feats = (uint32_t)min(a.N - n0, 16), toks = (uint32_t)min(a.T - t0, L::kTok);
+  const uint32_t feats = (uint32_t)min(a.N - n0, 16 * RB), toks = (uint32_t)min(a.T - t0, L::kTok);
   const __amdgpu_buffer_rsrc_t xres =
       make_rsrc((const uint8_t *)a.x + (long long)t0 * K, toks * (uint32_t)K);
   const __amdgpu_buffer_rsrc_t sres =
@@ -191,15 +197,16 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
 #pragma unroll
     for (int j = 0; j < (L::kW + L::kX) / 1024; ++j) {
       const bool isw = j < L::kW / 1024;
-      const int row = (isw ? (j & 1) : j - L::kW / 1024) * 8 + lane / 8;
+      const int row = (isw ? j % (2 * RB) : j - L::kW / 1024) * 8 + lane / 8;
       const int piece = (lane % 8) ^ L::swz(row);
-      buf16_to_lds(isw ? wres[isw ? j / 2 : 0] : xres, to + j * 1024,
+      buf16_to_lds(isw ? wres[isw ? j / (2 * RB) : 0] : xres, to + j * 1024,
                    16 * piece < left ? (uint32_t)row * (uint32_t)K + 16 * piece : kOutOfRange,
                    (uint32_t)g * kFp8Group);
     }
-    if constexpr (L::kCoded)
-      buf4_to_lds(sres, to + L::kW + L::kX,
-                  lane < L::kTok ? (uint32_t)lane * (uint32_t)groups * 4u : kOutOfRange,
+#pragma unroll
+    for (int j = 0; j < L::kSLoads; ++j)
+      buf4_to_lds(sres, to + L::kW + L::kX + j * 256,
+                  64 * j + lane < L::kTok ? (uint32_t)(64 * j + lane) * (uint32_t)groups * 4u : kOutOfRange,
                   (uint32_t)g * 4);
   };
   // lane l holds the block scales of the wave's l-th group of each 64
@@ -216,7 +223,7 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
   } else {
     // item: token item % toks of the workgroup's group item / toks; four lanes, of which each
     // has every fourth eight channels
-    constexpr int kPer = kStreamThreads / 4;
+    constexpr int kPer = L::kThreads / 4;
     const int items = ncoded * (int)toks, l4 = threadIdx.x & 3;
     auto place = [&](int item, int &li, int &t) {
       li = toks == 1 ? item : (int)__umulhi((uint32_t)item, a.per_token);
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
     auto load = [&](int item, float (&to)[32]) {
       int li, t;
       place(item, li, t);
-      const int g = (li / kStreamWaves) * step + kStreamWaves * blockIdx.z + li % kStreamWaves;
+      const int g = (li / kWaves) * step + kWaves * blockIdx.z + li % kWaves;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int k = g * kFp8Group + 8 * (4 * j + l4);
@@ -265,11 +272,11 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
     ring_barrier();
   }
 
-  glm_f32x4 acc[NPROJ][TB];
+  glm_f32x4 acc[L::kRowBlocks][TB];
 #pragma unroll
-  for (int p = 0; p < NPROJ; ++p)
+  for (int b = 0; b < L::kRowBlocks; ++b)
 #pragma unroll
-    for (int b = 0; b < TB; ++b) acc[p][b] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < TB; ++t) acc[b][t] = glm_f32x4{0.f, 0.f, 0.f, 0.f};
   // the lane's pieces of a row of codes, p0 and p0 + 1 (fp8_tile_kernel): channels 16 p0 .. + 31
   const int p0 = 4 * (q & 1) + 2 * (q >> 1);
   auto frag = [&](const uint8_t *rows, int row) {
@@ -281,40 +288,53 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
     wait_groups_ahead<L::kMost - 1, L::kLoads>(min(ahead - 1, mine - 1 - i));
     asm volatile("" ::: "memory");
     const uint8_t *from = ring + slot * L::kSlot;
-    fp8_frag w[NPROJ];
+    fp8_frag w[L::kRowBlocks];
 #pragma unroll
-    for (int p = 0; p < NPROJ; ++p) w[p] = frag(from + p * 16 * kFp8Group, r);
+    for (int b = 0; b < L::kRowBlocks; ++b) w[b] = frag(from + b * 16 * kFp8Group, r);
     // (columns past the tokens repeat one)
-    const int li = i * kStreamWaves + wave;
+    const int li = i * kWaves + wave;
     const uint8_t *xrows = L::kCoded ? from + L::kW : coded + li * L::kTok * kFp8Group;
     const float *xscales = L::kCoded ? reinterpret_cast<const float *>(from + L::kW + L::kX)
                                      : coded_scales + li * L::kTok;
-    Fp8Operand<false> x[TB];
+    fp8_frag xf[TB];
     float sx[TB];
 #pragma unroll
     for (int b = 0; b < TB; ++b) {
       const int t = min(b * 16 + r, L::kCoded ? L::kTok - 1 : (int)toks - 1);
-      x[b] = Fp8Operand<false>(frag(xrows, t));
+      xf[b] = frag(xrows, t);
       sx[b] = xscales[t];
     }
     __builtin_amdgcn_s_waitcnt(0xc07f);  // the slot's reads are done
     asm volatile("" ::: "memory");
     if (i + ahead < mine) issue(i + ahead, slot);
     slot = slot + 1 == ahead ? 0 : slot + 1;
+    float s[NPROJ][TB];
 #pragma unroll
     for (int p = 0; p < NPROJ; ++p) {
       const float sw = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(held[p]), i & 63));
-      const Fp8Operand<false> wo(w[p]);
-      glm_f32x4 c[TB];
 #pragma unroll
-      for (int j = 0; j < Fp8Operand<false>::kSteps; ++j)
+      for (int t = 0; t < TB; ++t) s[p][t] = sx[t] * sw;
+    }
+    Fp8Operand<FAST> x[TB];
 #pragma unroll
-        for (int b = 0; b < TB; ++b) c[b] = step_sum(wo, x[b], j, c[b]);
+    for (int t = 0; t < TB; ++t) x[t] = Fp8Operand<FAST>(xf[t]);
+    // a block's sums are scaled beside the next block's products
+    glm_f32x4 c[2][TB];
 #pragma unroll
-      for (int b = 0; b < TB; ++b) {
-        const float s = sx[b] * sw;
+    for (int b = 0; b <= L::kRowBlocks; ++b) {
+      if (b < L::kRowBlocks) {
+        const Fp8Operand<FAST> now(w[b]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[p][b][j] += c[b][j] * s;
+        for (int j = 0; j < Fp8Operand<FAST>::kSteps; ++j)
+#pragma unroll
+          for (int t = 0; t < TB; ++t) c[b & 1][t] = step_sum(now, x[t], j, c[b & 1][t]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (b > 0) {
+#pragma unroll
+        for (int t = 0; t < TB; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[b - 1][t][j] += c[(b - 1) & 1][t][j] * s[(b - 1) / RB][t];
       }
     }
   };
@@ -328,35 +348,47 @@ __global__ __launch_bounds__(kStreamThreads) void fp8_stream_kernel(Fp8Args a) {
   }
 
   __syncthreads();  // (the ring is done with)
-  glm_f32x4 *part = reinterpret_cast<glm_f32x4 *>(smem);  // [wave][NPROJ * TB][lane]
+  glm_f32x4 *part = reinterpret_cast<glm_f32x4 *>(smem);  // [wave][row block][token block][lane]
+  constexpr int kBlocks = L::kRowBlocks * TB;
 #pragma unroll
-  for (int p = 0; p < NPROJ; ++p)
+  for (int b = 0; b < L::kRowBlocks; ++b)
 #pragma unroll
-    for (int b = 0; b < TB; ++b) part[(wave * NPROJ * TB + p * TB + b) * kWave + lane] = acc[p][b];
+    for (int t = 0; t < TB; ++t) part[(wave * kBlocks + b * TB + t) * kWave + lane] = acc[b][t];
   __syncthreads();
-  constexpr int kJobs = NPROJ * TB;  // blocks of 16 x 16 to add up, a wave each
-  static_assert(kJobs <= kStreamWaves, "a wave a block");
-  if (wave >= kJobs) return;
-  const int t = t0 + 16 * (wave % TB) + r, n = n0 + 4 * q, p = wave / TB;
-  glm_f32x4 sum = part[wave * kWave + lane];
+  // eight features of a token a thread, so that a row leaves in whole pieces
+  constexpr int kPieces = 2 * RB;
+  for (int i = threadIdx.x; i < kPieces * NPROJ * 16 * TB; i += L::kThreads) {
+    const int piece = i % kPieces, p = i / kPieces % NPROJ, tok = i / (kPieces * NPROJ);
+    const int t = t0 + tok, n = n0 + 8 * piece;
+    if (t >= a.T || n >= a.N) continue;
+    const glm_f32x4 *from = part + ((p * RB + piece / 2) * TB + tok / 16) * kWave + tok % 16 + 32 * (piece & 1);
+    float v[8] = {};
 #pragma unroll
-  for (int w = 1; w < kStreamWaves; ++w) {
-    const glm_f32x4 o = part[(w * kJobs + wave) * kWave + lane];
+    for (int w = 0; w < kWaves; ++w) {
+      const glm_f32x4 lo = from[w * kBlocks * kWave], hi = from[w * kBlocks * kWave + 16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] += o[j];
-  }
-  if (t >= a.T || n >= a.N) return;
-  if constexpr (NPROJ == 2) {  // (N % 16 == 0)
-    *reinterpret_cast<glm_f32x4 *>(a.h + (((long long)blockIdx.z * 2 + p) * a.T + t) * a.N + n) = sum;
-  } else {
-    uint16_t *out = a.out + (long long)t * a.N + n;
-    if (a.N % 4 == 0) {
-      *reinterpret_cast<uint2 *>(out) = uint2{f32_to_bf16(sum[0]) | (f32_to_bf16(sum[1]) << 16),
-                                              f32_to_bf16(sum[2]) | (f32_to_bf16(sum[3]) << 16)};
+      for (int j = 0; j < 4; ++j) {
+        v[j] += lo[j];
+        v[4 + j] += hi[j];
+      }
+    }
+    if constexpr (NPROJ == 2) {  // (N % 16 == 0)
+      glm_f32x4 *o = reinterpret_cast<glm_f32x4 *>(
+          a.h + (((long long)blockIdx.z * 2 + p) * a.T + t) * a.N + n);
+      o[0] = glm_f32x4{v[0], v[1], v[2], v[3]};
+      o[1] = glm_f32x4{v[4], v[5], v[6], v[7]};
     } else {
+      uint16_t *out = a.out + (long long)t * a.N + n;
+      if (a.N % 8 == 0) {
+        glm_u32x4 o;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < a.N) out[j] = (uint16_t)f32_to_bf16(sum[j]);
+        for (int j = 0; j < 4; ++j) o[j] = f32_to_bf16(v[2 * j]) | (f32_to_bf16(v[2 * j + 1]) << 16);
+        *reinterpret_cast<glm_u32x4 *>(out) = o;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (n + j < a.N) out[j] = (uint16_t)f32_to_bf16(v[j]);
+      }
     }
   }
 }
@@ -436,15 +468,15 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-enum { kOutBf16, kOutF32, kOutCodes };
-
-template <int NPROJ, bool FAST, class L, int OUT>
+// NPROJ 1: bf16 products by the 8-bit instruction; 2: the gated pair, quantised, exact products.
+template <int NPROJ, class L>
 __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
   constexpr int BN = L::BN, BT = L::BT, kWaves = L::kWaves;
   constexpr int kS = L::kStages;
   constexpr int kFeat = L::kRows / NPROJ;  // features of a workgroup
   constexpr int HB = BN / NPROJ;           // 16-row blocks of a wave and projection
-  static_assert(OUT != kOutCodes || kFeat == kFp8Group, "a group of features");
+  constexpr bool FAST = NPROJ == 1;
+  static_assert(NPROJ == 1 || kFeat == kFp8Group, "a group of features");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   // workgroups are dealt to the XCDs in turn: each takes a contiguous share of the items
   const int items = a.row_tiles * a.tok_tiles;
@@ -673,7 +705,7 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
   }
 
   const int fw = f0 + wn * HB * 16, tw = t0 + wt * BT * 16;  // the wave's first feature and token
-  if constexpr (OUT == kOutBf16) {
+  if constexpr (NPROJ == 1) {
     if (N % 8 != 0) {  // rows of no 16-byte pieces: element by element
 #pragma unroll
       for (int b = 0; b < BN; ++b)
@@ -724,58 +756,47 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           acc[b][t][j] = gated(acc[b][t][j], acc[HB + b][t][j], a.p.limit);
-    if constexpr (OUT == kOutF32) {
+    // a token's largest finite magnitude over the 128 features: the lane's 4 HB, the four lanes of
+    // the token, the waves along the features
+    ring_barrier();
+    float *red = reinterpret_cast<float *>(smem);  // [L::WN][kTok]
+    uint8_t *st = smem + L::WN * L::kTok * 4;    // [kTok][128 codes, 16 bytes of padding]
+    constexpr int kStride = kFp8Group + 16;
+    static_assert(L::WN * L::kTok * 4 + L::kTok * kStride <= L::kBytes, "output staging");
+#pragma unroll
+    for (int t = 0; t < BT; ++t) {
+      float m = 0.f;
+#pragma unroll
+      for (int b = 0; b < HB; ++b) {
+        float (&v)[4] = reinterpret_cast<float (&)[4]>(acc[b][t]);
+        if (fw + 16 * b + 4 * q < N) m = fmaxf(m, finite_abs_max(v));
+      }
+      m = fmaxf(m, __shfl_xor(m, 16, kWave));
+      m = fmaxf(m, __shfl_xor(m, 32, kWave));
+      if (q == 0) red[wn * L::kTok + (wt * BT + t) * 16 + r] = m;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < BT; ++t) {
+      const int tok = (wt * BT + t) * 16 + r;
+      float m = kFp8Tiny;
+#pragma unroll
+      for (int w = 0; w < L::WN; ++w) m = fmaxf(m, red[w * L::kTok + tok]);
+      const float up = kFp8Max / m;
 #pragma unroll
       for (int b = 0; b < HB; ++b)
+        *reinterpret_cast<uint32_t *>(st + tok * kStride + wn * HB * 16 + 16 * b + 4 * q) =
+            fp8_codes4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3], up);
+      if (wn == 0 && q == 0 && t0 + tok < T)
+        a.p.scales[(long long)(t0 + tok) * fp8_groups(N) + f0 / kFp8Group] = m / kFp8Max;
+    }
+    __syncthreads();
 #pragma unroll
-        for (int t = 0; t < BT; ++t) {
-          const int tok = tw + 16 * t + r, n = fw + 16 * b + 4 * q;
-          if (tok < T && n < N)  // (N % 16 == 0)
-            *reinterpret_cast<glm_f32x4 *>(a.p.h + (long long)tok * N + n) = acc[b][t];
-        }
-    } else {
-      // a token's largest finite magnitude over the 128 features: the lane's 4 HB, the four lanes of
-      // the token, the waves along the features
-      ring_barrier();
-      float *red = reinterpret_cast<float *>(smem);  // [L::WN][kTok]
-      uint8_t *st = smem + L::WN * L::kTok * 4;    // [kTok][128 codes, 16 bytes of padding]
-      constexpr int kStride = kFp8Group + 16;
-      static_assert(L::WN * L::kTok * 4 + L::kTok * kStride <= L::kBytes, "output staging");
-#pragma unroll
-      for (int t = 0; t < BT; ++t) {
-        float m = 0.f;
-#pragma unroll
-        for (int b = 0; b < HB; ++b) {
-          float (&v)[4] = reinterpret_cast<float (&)[4]>(acc[b][t]);
-          if (fw + 16 * b + 4 * q < N) m = fmaxf(m, finite_abs_max(v));
-        }
-        m = fmaxf(m, __shfl_xor(m, 16, kWave));
-        m = fmaxf(m, __shfl_xor(m, 32, kWave));
-        if (q == 0) red[wn * L::kTok + (wt * BT + t) * 16 + r] = m;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int t = 0; t < BT; ++t) {
-        const int tok = (wt * BT + t) * 16 + r;
-        float m = kFp8Tiny;
-#pragma unroll
-        for (int w = 0; w < L::WN; ++w) m = fmaxf(m, red[w * L::kTok + tok]);
-        const float up = kFp8Max / m;
-#pragma unroll
-        for (int b = 0; b < HB; ++b)
-          *reinterpret_cast<uint32_t *>(st + tok * kStride + wn * HB * 16 + 16 * b + 4 * q) =
-              fp8_codes4(acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3], up);
-        if (wn == 0 && q == 0 && t0 + tok < T)
-          a.p.scales[(long long)(t0 + tok) * fp8_groups(N) + f0 / kFp8Group] = m / kFp8Max;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < L::kTok * 8 / L::kThreads; ++i) {
-        const int slot = i * L::kThreads + tid, tok = slot / 8, n = f0 + 16 * (slot % 8);
-        if (t0 + tok < T && n < N)
-          *reinterpret_cast<glm_u32x4 *>(a.p.codes + (long long)(t0 + tok) * N + n) =
-              *reinterpret_cast<const glm_u32x4 *>(st + tok * kStride + 16 * (slot % 8));
-      }
+    for (int i = 0; i < L::kTok * 8 / L::kThreads; ++i) {
+      const int slot = i * L::kThreads + tid, tok = slot / 8, n = f0 + 16 * (slot % 8);
+      if (t0 + tok < T && n < N)
+        *reinterpret_cast<glm_u32x4 *>(a.p.codes + (long long)(t0 + tok) * N + n) =
+            *reinterpret_cast<const glm_u32x4 *>(st + tok * kStride + 16 * (slot % 8));
     }
   }
 }
@@ -787,44 +808,39 @@ using namespace glm;
 static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // splits: the workgroups along K.
-template <int NPROJ, int TB, int ROWS, bool FEW>
-static void launch_stream_tokens(hipStream_t stream, Fp8Args a, int splits) {
-  using L = Fp8Stream<NPROJ, TB, ROWS, FEW>;
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.T + 16 * TB - 1) / (16 * TB)),
-                  (unsigned)splits);
+template <class L>
+static int launch_stream(hipStream_t stream, Fp8Args a, int splits = 1) {
+  const dim3 grid((unsigned)((a.N + 16 * L::RB - 1) / (16 * L::RB)),
+                  (unsigned)((a.T + 16 * L::TB - 1) / (16 * L::TB)), (unsigned)splits);
   // a workgroup a CU takes all the LDS for its groups in flight, else two share it
   const int coded = L::coded_bytes(a.groups, splits);
   const long long wgs = (long long)grid.x * grid.y * grid.z;
   const int room = (wgs <= 256 ? kStreamKB : kStreamPairKB) * 1024 - coded;
-  int ahead = room / (kStreamWaves * L::kSlot);
-  const int per_wave = (a.groups + kStreamWaves * splits - 1) / (kStreamWaves * splits);
+  int ahead = room / (L::kWaves * L::kSlot);
+  const int per_wave = (a.groups + L::kWaves * splits - 1) / (L::kWaves * splits);
   ahead = ahead < L::kMost ? ahead : L::kMost;
   ahead = ahead < per_wave ? ahead : per_wave;
   a.ahead = ahead < 1 ? 1 : ahead;
   a.per_token = a.T > 1 && a.T <= kFusedTokens ? (uint32_t)(((1ull << 32) + a.T - 1) / a.T) : 0;
-  const int bytes = kStreamWaves * a.ahead * L::kSlot + coded;
-  hipLaunchKernelGGL((fp8_stream_kernel<NPROJ, TB, ROWS, FEW>), grid, dim3(kStreamThreads),
+  const int bytes = L::kWaves * a.ahead * L::kSlot + coded;
+  hipLaunchKernelGGL((fp8_stream_kernel<L>), grid, dim3(L::kThreads),
                      (size_t)(bytes > L::kPart ? bytes : L::kPart), stream, a);
+  GLM_LAUNCH_CHECK("fp8_stream_kernel");
+  return GLM_OK;
 }
 
 template <int NPROJ>
-static int launch_stream(hipStream_t stream, const Fp8Args &a, int type, int splits) {
+static int stream_few(hipStream_t stream, const Fp8Args &a, int type, int splits) {
+  constexpr int W = kStreamWaves;
   if (type == GLM_ROWS_BF16)
-    launch_stream_tokens<NPROJ, 1, GLM_ROWS_BF16, true>(stream, a, splits);
-  else if (type == GLM_ROWS_F32)
-    launch_stream_tokens<NPROJ, 1, GLM_ROWS_F32, true>(stream, a, splits);
-  else if (a.T <= 8)
-    launch_stream_tokens<NPROJ, 1, GLM_ROWS_FP8, true>(stream, a, splits);
-  else if (a.T <= 16)
-    launch_stream_tokens<NPROJ, 1, GLM_ROWS_FP8, false>(stream, a, splits);
-  else if (a.T <= 32)
-    launch_stream_tokens<NPROJ, 2, GLM_ROWS_FP8, false>(stream, a, splits);
-  else if (a.T <= 48)
-    launch_stream_tokens<NPROJ, 3, GLM_ROWS_FP8, false>(stream, a, splits);
-  else
-    launch_stream_tokens<NPROJ, 4, GLM_ROWS_FP8, false>(stream, a, splits);
-  GLM_LAUNCH_CHECK("fp8_stream_kernel");
-  return GLM_OK;
+    return launch_stream<Fp8Stream<W, NPROJ, 1, 1, GLM_ROWS_BF16, true>>(stream, a, splits);
+  if (type == GLM_ROWS_F32)
+    return launch_stream<Fp8Stream<W, NPROJ, 1, 1, GLM_ROWS_F32, true>>(stream, a, splits);
+  if (a.T <= 8) return launch_stream<Fp8Stream<W, NPROJ, 1, 1, GLM_ROWS_FP8, true>>(stream, a, splits);
+  if (a.T <= 16) return launch_stream<Fp8Stream<W, NPROJ, 1, 1, GLM_ROWS_FP8>>(stream, a, splits);
+  if (a.T <= 32) return launch_stream<Fp8Stream<W, NPROJ, 1, 2, GLM_ROWS_FP8>>(stream, a, splits);
+  if (a.T <= 48) return launch_stream<Fp8Stream<W, NPROJ, 1, 3, GLM_ROWS_FP8>>(stream, a, splits);
+  return launch_stream<Fp8Stream<W, NPROJ, 1, 4, GLM_ROWS_FP8>>(stream, a, splits);
 }
 
 constexpr int kStreamTokens = 64;  // up to so many the weights are streamed
@@ -860,35 +876,94 @@ static int rows_for(hipStream_t stream, Fp8Args &a, int &type, uint8_t *&ws) {
   return rc;
 }
 
-template <int NPROJ, bool FAST, class L, int OUT>
-static int launch_tile(hipStream_t stream, Fp8TileArgs a) {
+template <int NPROJ, class L>
+static int launch_tile(hipStream_t stream, const Fp8Args &p) {
   constexpr int feat = L::kRows / NPROJ;
-  a.row_tiles = (a.p.N + feat - 1) / feat;
-  a.tok_tiles = (a.p.T + L::kTok - 1) / L::kTok;
-  a.rows_outer = NPROJ * a.p.N >= a.p.T;
+  Fp8TileArgs a{p, (p.N + feat - 1) / feat, (p.T + L::kTok - 1) / L::kTok, NPROJ * p.N >= p.T};
   const int items = a.row_tiles * a.tok_tiles;
-  hipLaunchKernelGGL((fp8_tile_kernel<NPROJ, FAST, L, OUT>),
+  hipLaunchKernelGGL((fp8_tile_kernel<NPROJ, L>),
                      dim3((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds)),
                      dim3(L::kThreads), (size_t)L::kBytes, stream, a);
   GLM_LAUNCH_CHECK("fp8_tile_kernel");
   return GLM_OK;
 }
 
+// A way to cut a product of more than 64 rows: features and tokens of a
+// workgroup, and its time in tenths of a us at K 4096, base + each for every 256
+// workgroups begun (one a CU), which goes with K.
+struct Fp8Cut {
+  int feat, tok, base, each;
+  long long cost(int T, int N) const {
+    const long long wgs = (long long)((N + feat - 1) / feat) * ((T + tok - 1) / tok);
+    return base + each * ((wgs + 255) / 256);
+  }
+};
+template <int M>
+static int cheapest(const Fp8Cut (&cuts)[M], int T, int N) {
+  int best = 0;
+  for (int i = 1; i < M; ++i)
+    if (cuts[i].cost(T, N) < cuts[best].cost(T, N)) best = i;
+  return best;
+}
+
+// Products by the streaming kernel (whose waves need not wait for each other, but
+// read all operands of a tile) and by the tiles, at N 4096, K 4096: 80 rows 8.1
+// us where the 64 x 64 tile takes 14.7 and the 256 x 256 one 46.8; 333 rows 15.5,
+// 17.7, 47.7; 600 rows 26.7, 22.9, 47.9; 1600 rows 54.2, 52.8 (256 x 128: 36.1),
+// 49.5; 4096 rows 124.6, 151.3 (81.6), 61.9.
 static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
-  if (a.T <= kStreamTokens) return launch_stream<1>(stream, a, type, 1);
-  const Fp8TileArgs t{a, 0, 0, 0};
-  if (a.T <= 512) return launch_tile<1, true, Fp8Tile<2, 2, 2, 2, 52>, kOutBf16>(stream, t);
-  return launch_tile<1, true, Fp8Tile<2, 4, 8, 4>, kOutBf16>(stream, t);
+  if (a.T <= kStreamTokens) return stream_few<1>(stream, a, type, 1);
+  static const Fp8Cut cuts[] = {{32, 48, 30, 52},  {64, 32, 40, 46},   {64, 48, 45, 57}, {64, 64, 90, 54},
+                                {128, 64, 100, 90}, {256, 128, 10, 330}, {256, 256, 0, 500}};
+  switch (cheapest(cuts, a.T, a.N)) {
+    case 0: return launch_stream<Fp8Stream<8, 1, 2, 3, GLM_ROWS_FP8, false, true>>(stream, a);
+    case 1: return launch_stream<Fp8Stream<4, 1, 4, 2, GLM_ROWS_FP8, false, true>>(stream, a);
+    case 2: return launch_stream<Fp8Stream<4, 1, 4, 3, GLM_ROWS_FP8, false, true>>(stream, a);
+    case 3: return launch_tile<1, Fp8Tile<2, 2, 2, 2, 52>>(stream, a);
+    case 4: return launch_tile<1, Fp8Tile<2, 2, 4, 2, 79>>(stream, a);
+    case 5: return launch_tile<1, Fp8Tile<2, 4, 8, 2>>(stream, a);
+    default: return launch_tile<1, Fp8Tile<2, 4, 8, 4>>(stream, a);
+  }
+}
+
+// Gated pairs: up to 64 rows split along K; more of them streamed, their sums
+// gated by a second launch, or in tiles that gate and quantise by themselves.  At
+// 2 x 2048 features, K 4096 (without the second launch's 2.5 us and more): 80 rows
+// 9.2 us where the 256 x 128 tile takes 60.5 and the 256 x 256 one 100; 333 rows
+// 19.0, 60.8, 100; 850 rows 41.5, 61.9, 101; 1600 rows 67.9, 64.5, 103; 3000 rows
+// 118.8, 121.4, 104.
+constexpr Fp8Cut kGatedCuts[] = {{16, 48, 30, 62}, {32, 32, 55, 51}, {32, 48, 60, 67}, {32, 64, 60, 90},
+                                 {128, 128, 0, 630}, {128, 256, 0, 1030}};
+constexpr int kGatedStreams = 4;
+static int gated_cut(int T, int K, int N) {
+  int best = 0;
+  double cost = 0;
+  for (int i = 0; i < 6; ++i) {
+    double c = (double)kGatedCuts[i].cost(T, N) * fp8_groups(K) / 32;
+    if (i < kGatedStreams) c += 25 + (double)T * N * 2e-5;  // the second launch: 8 bytes a feature
+    if (i == 0 || c < cost) {
+      best = i;
+      cost = c;
+    }
+  }
+  return best;
 }
 
 static int gated_product(hipStream_t stream, const Fp8Args &a, int type) {
-  if (a.T > kStreamTokens) {
-    const Fp8TileArgs t{a, 0, 0, 0};
-    if (a.T <= 1024) return launch_tile<2, false, Fp8Tile<2, 4, 8, 1>, kOutCodes>(stream, t);
-    return launch_tile<2, false, Fp8Tile<2, 4, 8, 4>, kOutCodes>(stream, t);
+  int splits = 1, rc;
+  if (a.T <= kStreamTokens) {
+    splits = stream_splits(a.K, a.N);
+    rc = stream_few<2>(stream, a, type, splits);
+  } else {
+    switch (gated_cut(a.T, a.K, a.N)) {
+      case 0: rc = launch_stream<Fp8Stream<8, 2, 1, 3, GLM_ROWS_FP8>>(stream, a); break;
+      case 1: rc = launch_stream<Fp8Stream<4, 2, 2, 2, GLM_ROWS_FP8>>(stream, a); break;
+      case 2: rc = launch_stream<Fp8Stream<4, 2, 2, 3, GLM_ROWS_FP8>>(stream, a); break;
+      case 3: rc = launch_stream<Fp8Stream<4, 2, 2, 4, GLM_ROWS_FP8>>(stream, a); break;
+      case 4: return launch_tile<2, Fp8Tile<2, 4, 8, 2>>(stream, a);
+      default: return launch_tile<2, Fp8Tile<2, 4, 8, 4>>(stream, a);
+    }
   }
-  const int splits = stream_splits(a.K, a.N);
-  const int rc = launch_stream<2>(stream, a, type, splits);
   if (rc) return rc;
   const long long items = (long long)a.T * fp8_groups(a.N);
   hipLaunchKernelGGL(fp8_gate_kernel, dim3((unsigned)((items + 15) / 16)), dim3(256), 0, stream,
@@ -897,8 +972,14 @@ static int gated_product(hipStream_t stream, const Fp8Args &a, int type) {
   return GLM_OK;
 }
 
+// The pair's f32 sums, where a second launch gates them.
+static size_t gated_bytes(int T, int K, int N) {
+  if (T > kStreamTokens && gated_cut(T, K, N) >= kGatedStreams) return 0;
+  return round256((size_t)(T > kStreamTokens ? 1 : stream_splits(K, N)) * 2 * T * N * 4);
+}
+
 static bool sizes_fit(int T, int K, int N) {
-  return T >= 0 && K >= 16 && N >= 1 && K % 16 == 0 && K <= 1 << 20 && N <= 1 << 20 && T <= 1 << 21;
+  return T >= 0 && K >= 16 && N >= 1 && K % 16 == 0 && K <= 1 << 20 && N <= 1 << 20 && T <= 1 << 20;
 }
 
 static int check_product(const char *name, const void *x, int x_type, const float *x_scales, int T,
@@ -906,7 +987,7 @@ static int check_product(const char *name, const void *x, int x_type, const floa
   GLM_REQUIRE(T >= 0 && K >= 1 && N >= 1 && x_type >= GLM_ROWS_BF16 && x_type <= GLM_ROWS_FP8,
               GLM_ERR_INVALID_ARGUMENT, "%s: invalid sizes or row type", name);
   GLM_REQUIRE(sizes_fit(T, K, N), GLM_ERR_UNSUPPORTED_SHAPE,
-              "%s: %d rows of %d channels (a multiple of 16) into %d: up to 2^21 rows and 2^20 "
+              "%s: %d rows of %d channels (a multiple of 16) into %d: up to 2^20 rows and 2^20 "
               "channels", name, T, K, N);
   GLM_REQUIRE(x && (x_type != GLM_ROWS_FP8 || x_scales), GLM_ERR_INVALID_ARGUMENT,
               "%s: null pointer", name);
@@ -919,9 +1000,7 @@ static int check_product(const char *name, const void *x, int x_type, const floa
 
 extern "C" size_t glm_fp8_workspace_bytes(int x_type, int T, int K, int N, int gated) {
   if (!sizes_fit(T, K, N) || x_type < GLM_ROWS_BF16 || x_type > GLM_ROWS_FP8) return 0;
-  size_t sums = 0;  // of a gated pair of few rows
-  if (gated && T <= kStreamTokens) sums = round256((size_t)stream_splits(K, N) * 2 * T * N * 4);
-  return rows_bytes(T, K, x_type) + sums;
+  return rows_bytes(T, K, x_type) + (gated ? gated_bytes(T, K, N) : 0);
 }
 
 extern "C" int glm_fp8_linear(void *stream, const void *x, int x_type, const float *x_scales, int T,
