@@ -27,7 +27,7 @@ namespace glm {
 
 typedef int fp8_frag __attribute__((ext_vector_type(8)));
 
-constexpr int kStreamWaves = 8;
+constexpr int kExactTokens = 64;  // rows whose products are summed exactly in any case
 // Rows that the product quantises itself: up to so many, and so many codes, which
 // have to fit its LDS.  (Each workgroup does it for itself: at K and N 4096 1, 4
 // and 16 rows so take 7.0, 7.6 and 13.1 us, quantised before 8.5 to 8.8.)
@@ -829,31 +829,6 @@ static int launch_stream(hipStream_t stream, Fp8Args a, int splits = 1) {
   return GLM_OK;
 }
 
-template <int NPROJ>
-static int stream_few(hipStream_t stream, const Fp8Args &a, int type, int splits) {
-  constexpr int W = kStreamWaves;
-  if (type == GLM_ROWS_BF16)
-    return launch_stream<Fp8Stream<W, NPROJ, 1, 1, GLM_ROWS_BF16, true>>(stream, a, splits);
-  if (type == GLM_ROWS_F32)
-    return launch_stream<Fp8Stream<W, NPROJ, 1, 1, GLM_ROWS_F32, true>>(stream, a, splits);
-  if (a.T <= 8) return launch_stream<Fp8Stream<W, NPROJ, 1, 1, GLM_ROWS_FP8, true>>(stream, a, splits);
-  if (a.T <= 16) return launch_stream<Fp8Stream<W, NPROJ, 1, 1, GLM_ROWS_FP8>>(stream, a, splits);
-  if (a.T <= 32) return launch_stream<Fp8Stream<W, NPROJ, 1, 2, GLM_ROWS_FP8>>(stream, a, splits);
-  if (a.T <= 48) return launch_stream<Fp8Stream<W, NPROJ, 1, 3, GLM_ROWS_FP8>>(stream, a, splits);
-  return launch_stream<Fp8Stream<W, NPROJ, 1, 4, GLM_ROWS_FP8>>(stream, a, splits);
-}
-
-constexpr int kStreamTokens = 64;  // up to so many the weights are streamed
-
-// Ways that a gated pair's K is split where its row tiles are fewer than the
-// CUs: as many as leave every wave a group.
-static int stream_splits(int K, int N) {
-  const int tiles = N / 16, most = fp8_groups(K) / kStreamWaves;
-  int s = 256 / (tiles > 0 ? tiles : 1);
-  s = s < most ? s : most;
-  return s < 1 ? 1 : s < 8 ? s : 8;
-}
-
 // Workspace of rows that the product does not take as they are.
 static size_t rows_bytes(int T, int K, int type) {
   const long long codes = (long long)kFusedTokens * fp8_groups(K) * kFp8Group;
@@ -888,15 +863,14 @@ static int launch_tile(hipStream_t stream, const Fp8Args &p) {
   return GLM_OK;
 }
 
-// A way to cut a product of more than 64 rows: features and tokens of a
-// workgroup, and its time in tenths of a us at K 4096, base + each for every 256
-// workgroups begun (one a CU), which goes with K.
+// A way to cut a product: features and tokens of a workgroup, and its time in
+// tenths of a us at K 4096, base + each for every 256 workgroups begun (one a CU).
 struct Fp8Cut {
   int feat, tok, base, each;
-  long long cost(int T, int N) const {
-    const long long wgs = (long long)((N + feat - 1) / feat) * ((T + tok - 1) / tok);
-    return base + each * ((wgs + 255) / 256);
+  long long workgroups(int T, int N) const {
+    return (long long)((N + feat - 1) / feat) * ((T + tok - 1) / tok);
   }
+  long long cost(int T, int N) const { return base + each * ((workgroups(T, N) + 255) / 256); }
 };
 template <int M>
 static int cheapest(const Fp8Cut (&cuts)[M], int T, int N) {
@@ -906,19 +880,44 @@ static int cheapest(const Fp8Cut (&cuts)[M], int T, int N) {
   return best;
 }
 
-// Products by the streaming kernel (whose waves need not wait for each other, but
-// read all operands of a tile) and by the tiles, at N 4096, K 4096: 80 rows 8.1
-// us where the 64 x 64 tile takes 14.7 and the 256 x 256 one 46.8; 333 rows 15.5,
-// 17.7, 47.7; 600 rows 26.7, 22.9, 47.9; 1600 rows 54.2, 52.8 (256 x 128: 36.1),
-// 49.5; 4096 rows 124.6, 151.3 (81.6), 61.9.
+template <int WAVES, int NPROJ, int RB, int TB, bool FAST = false>
+using CodedStream = Fp8Stream<WAVES, NPROJ, RB, TB, GLM_ROWS_FP8, false, FAST>;
+
+// Rows that come as bf16 or f32, and up to 8 coded ones: 16 features a workgroup.
+template <int NPROJ>
+static int stream_few(hipStream_t stream, const Fp8Args &a, int type, int splits) {
+  if (type == GLM_ROWS_BF16)
+    return launch_stream<Fp8Stream<8, NPROJ, 1, 1, GLM_ROWS_BF16, true>>(stream, a, splits);
+  if (type == GLM_ROWS_F32)
+    return launch_stream<Fp8Stream<8, NPROJ, 1, 1, GLM_ROWS_F32, true>>(stream, a, splits);
+  return launch_stream<Fp8Stream<8, NPROJ, 1, 1, GLM_ROWS_FP8, true>>(stream, a, splits);
+}
+static bool few(int T, int type) { return type != GLM_ROWS_FP8 || T <= 8; }
+
+// Products: up to 64 rows by the exact sum, whose time the weights' bytes set, more
+// by the 8-bit instruction; by the streaming kernel, whose waves do not wait for
+// each other but read all operands of their tile, or in larger tiles.  At N 4096,
+// K 4096, us by tile: 64 rows 16 x 32 9.6, 32 x 32 8.5, 16 x 64 9.0; 80 rows 32 x 48
+// 8.1, 64 x 32 8.8, 256 x 256 46.8; 333 rows 64 x 48 15.5, 64 x 64 17.7; 600 rows 26.7,
+// 22.9; 1600 rows 54.2, 52.8, 256 x 128 36.1, 256 x 256 49.5; 4096 rows 124.6, 151.3,
+// 81.6, 61.9.
 static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
-  if (a.T <= kStreamTokens) return stream_few<1>(stream, a, type, 1);
+  if (few(a.T, type)) return stream_few<1>(stream, a, type, 1);
+  if (a.T <= kExactTokens) {
+    static const Fp8Cut cuts[] = {{16, 16, 45, 20}, {16, 32, 51, 24}, {32, 32, 30, 56}, {16, 64, 35, 50}};
+    switch (cheapest(cuts, a.T, a.N)) {
+      case 0: return launch_stream<CodedStream<8, 1, 1, 1>>(stream, a);
+      case 1: return launch_stream<CodedStream<8, 1, 1, 2>>(stream, a);
+      case 2: return launch_stream<CodedStream<8, 1, 2, 2>>(stream, a);
+      default: return launch_stream<CodedStream<8, 1, 1, 4>>(stream, a);
+    }
+  }
   static const Fp8Cut cuts[] = {{32, 48, 30, 52},  {64, 32, 40, 46},   {64, 48, 45, 57}, {64, 64, 90, 54},
                                 {128, 64, 100, 90}, {256, 128, 10, 330}, {256, 256, 0, 500}};
   switch (cheapest(cuts, a.T, a.N)) {
-    case 0: return launch_stream<Fp8Stream<8, 1, 2, 3, GLM_ROWS_FP8, false, true>>(stream, a);
-    case 1: return launch_stream<Fp8Stream<4, 1, 4, 2, GLM_ROWS_FP8, false, true>>(stream, a);
-    case 2: return launch_stream<Fp8Stream<4, 1, 4, 3, GLM_ROWS_FP8, false, true>>(stream, a);
+    case 0: return launch_stream<CodedStream<8, 1, 2, 3, true>>(stream, a);
+    case 1: return launch_stream<CodedStream<4, 1, 4, 2, true>>(stream, a);
+    case 2: return launch_stream<CodedStream<4, 1, 4, 3, true>>(stream, a);
     case 3: return launch_tile<1, Fp8Tile<2, 2, 2, 2, 52>>(stream, a);
     case 4: return launch_tile<1, Fp8Tile<2, 2, 4, 2, 79>>(stream, a);
     case 5: return launch_tile<1, Fp8Tile<2, 4, 8, 2>>(stream, a);
@@ -926,41 +925,52 @@ static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
   }
 }
 
-// Gated pairs: up to 64 rows split along K; more of them streamed, their sums
-// gated by a second launch, or in tiles that gate and quantise by themselves.  At
-// 2 x 2048 features, K 4096 (without the second launch's 2.5 us and more): 80 rows
-// 9.2 us where the 256 x 128 tile takes 60.5 and the 256 x 256 one 100; 333 rows
-// 19.0, 60.8, 100; 850 rows 41.5, 61.9, 101; 1600 rows 67.9, 64.5, 103; 3000 rows
-// 118.8, 121.4, 104.
-constexpr Fp8Cut kGatedCuts[] = {{16, 48, 30, 62}, {32, 32, 55, 51}, {32, 48, 60, 67}, {32, 64, 60, 90},
-                                 {128, 128, 0, 630}, {128, 256, 0, 1030}};
-constexpr int kGatedStreams = 4;
-static int gated_cut(int T, int K, int N) {
-  int best = 0;
-  double cost = 0;
-  for (int i = 0; i < 6; ++i) {
+// Gated pairs: streamed, their sums gated by a second launch, or in tiles that gate
+// and quantise by themselves.  At 2 x 2048 features, K 4096, us by tile (streamed
+// ones without the second launch's 2.5 us and more): 64 rows 16 x 16 9.7, 16 x 32 8.7,
+// 16 x 48 9.2; 333 rows 32 x 32 21.7, 32 x 48 19.0, 32 x 64 23.2, 128 x 128 60.8,
+// 128 x 256 100; 850 rows 42.7, 41.6, 41.5, 61.9, 101; 1600 rows 74.9, 72.3, 67.9,
+// 64.5, 103; 3000 rows 134.6, 126.4, 118.8, 121.4, 104.
+constexpr Fp8Cut kGatedCuts[] = {{16, 16, 44, 26}, {16, 32, 50, 35}, {16, 48, 30, 62},   {32, 32, 55, 51},
+                                 {32, 48, 60, 67}, {32, 64, 60, 90}, {128, 128, 0, 630}, {128, 256, 0, 1030}};
+constexpr int kGatedStreams = 6, kGatedWays = 8;
+struct GatedPlan {
+  int cut, splits;  // of K, where the workgroups are fewer than the CUs: as many as leave every wave a group
+};
+static GatedPlan gated_plan(int T, int K, int N, int type) {
+  GatedPlan plan{0, 1};
+  double best = 0;
+  for (int i = 0; i < (few(T, type) ? 1 : kGatedWays); ++i) {
     double c = (double)kGatedCuts[i].cost(T, N) * fp8_groups(K) / 32;
     if (i < kGatedStreams) c += 25 + (double)T * N * 2e-5;  // the second launch: 8 bytes a feature
-    if (i == 0 || c < cost) {
-      best = i;
-      cost = c;
+    if (i == 0 || c < best) {
+      plan.cut = i;
+      best = c;
     }
   }
-  return best;
+  if (plan.cut >= kGatedStreams) return plan;
+  const int waves = plan.cut < 3 ? 8 : 4, most = fp8_groups(K) / waves;
+  long long s = 256 / kGatedCuts[plan.cut].workgroups(T, N);
+  s = s < most ? s : most;
+  plan.splits = s < 1 ? 1 : s < 8 ? (int)s : 8;
+  return plan;
 }
 
 static int gated_product(hipStream_t stream, const Fp8Args &a, int type) {
-  int splits = 1, rc;
-  if (a.T <= kStreamTokens) {
-    splits = stream_splits(a.K, a.N);
+  const GatedPlan plan = gated_plan(a.T, a.K, a.N, type);
+  const int splits = plan.splits;
+  int rc;
+  if (few(a.T, type)) {
     rc = stream_few<2>(stream, a, type, splits);
   } else {
-    switch (gated_cut(a.T, a.K, a.N)) {
-      case 0: rc = launch_stream<Fp8Stream<8, 2, 1, 3, GLM_ROWS_FP8>>(stream, a); break;
-      case 1: rc = launch_stream<Fp8Stream<4, 2, 2, 2, GLM_ROWS_FP8>>(stream, a); break;
-      case 2: rc = launch_stream<Fp8Stream<4, 2, 2, 3, GLM_ROWS_FP8>>(stream, a); break;
-      case 3: rc = launch_stream<Fp8Stream<4, 2, 2, 4, GLM_ROWS_FP8>>(stream, a); break;
-      case 4: return launch_tile<2, Fp8Tile<2, 4, 8, 2>>(stream, a);
+    switch (plan.cut) {
+      case 0: rc = launch_stream<CodedStream<8, 2, 1, 1>>(stream, a, splits); break;
+      case 1: rc = launch_stream<CodedStream<8, 2, 1, 2>>(stream, a, splits); break;
+      case 2: rc = launch_stream<CodedStream<8, 2, 1, 3>>(stream, a, splits); break;
+      case 3: rc = launch_stream<CodedStream<4, 2, 2, 2>>(stream, a, splits); break;
+      case 4: rc = launch_stream<CodedStream<4, 2, 2, 3>>(stream, a, splits); break;
+      case 5: rc = launch_stream<CodedStream<4, 2, 2, 4>>(stream, a, splits); break;
+      case 6: return launch_tile<2, Fp8Tile<2, 4, 8, 2>>(stream, a);
       default: return launch_tile<2, Fp8Tile<2, 4, 8, 4>>(stream, a);
     }
   }
@@ -972,10 +982,11 @@ static int gated_product(hipStream_t stream, const Fp8Args &a, int type) {
   return GLM_OK;
 }
 
-// The pair's f32 sums, where a second launch gates them.
-static size_t gated_bytes(int T, int K, int N) {
-  if (T > kStreamTokens && gated_cut(T, K, N) >= kGatedStreams) return 0;
-  return round256((size_t)(T > kStreamTokens ? 1 : stream_splits(K, N)) * 2 * T * N * 4);
+// The pair's f32 sums, where a second launch gates them.  Rows that the workspace
+// holds as codes are coded for the plan.
+static size_t gated_bytes(int T, int K, int N, int type) {
+  const GatedPlan plan = gated_plan(T, K, N, rows_bytes(T, K, type) ? GLM_ROWS_FP8 : type);
+  return plan.cut < kGatedStreams ? round256((size_t)plan.splits * 2 * T * N * 4) : 0;
 }
 
 static bool sizes_fit(int T, int K, int N) {
@@ -1000,7 +1011,7 @@ static int check_product(const char *name, const void *x, int x_type, const floa
 
 extern "C" size_t glm_fp8_workspace_bytes(int x_type, int T, int K, int N, int gated) {
   if (!sizes_fit(T, K, N) || x_type < GLM_ROWS_BF16 || x_type > GLM_ROWS_FP8) return 0;
-  return rows_bytes(T, K, x_type) + (gated ? gated_bytes(T, K, N) : 0);
+  return rows_bytes(T, K, x_type) + (gated && T > 0 ? gated_bytes(T, K, N, x_type) : 0);
 }
 
 extern "C" int glm_fp8_linear(void *stream, const void *x, int x_type, const float *x_scales, int T,
