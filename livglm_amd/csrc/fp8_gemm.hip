@@ -493,49 +493,32 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
   const int f0 = rt * kFeat, t0 = tt * L::kTok;
   const int toks = min(T - t0, L::kTok), feats = min(N - f0, kFeat);
 
-  const __amdgpu_buffer_rsrc_t xres =
-      make_rsrc((const uint8_t *)a.p.x + (long long)t0 * K, (uint32_t)toks * (uint32_t)K);
-  __amdgpu_buffer_rsrc_t wres[NPROJ];
+  // Load j fills the (kWaves j + wave)-th 1 KB of the tokens, then of the weight rows.
+  // Every load has a descriptor of its own that begins at its first row, so that one
+  // register holds the lane's offset in all of them (one each: 8 registers spilled at
+  // 128 x 256 gated, and a reload in every group).
+  constexpr int kStep = 8 * kWaves;  // rows of a load
+  static_assert(kStep % 16 == 0 && kFeat % kStep == 0, "the same order of pieces, one projection");
+  auto rows_from = [&](const uint8_t *rows, int first, int there) {
+    return make_rsrc(rows + (long long)first * K, (uint32_t)max(there - first, 0) * (uint32_t)K);
+  };
+  __amdgpu_buffer_rsrc_t res[L::kLoads];
 #pragma unroll
-  for (int p = 0; p < NPROJ; ++p)
-    wres[p] = make_rsrc(a.p.w[p] + (long long)f0 * K, (uint32_t)feats * (uint32_t)K);
-  // load j of wave w fills the (kWaves j + w)-th 1 KB of the tokens, then of the weight rows
-  uint32_t xoff[L::kXLoads], woff[L::kWLoads];
+  for (int j = 0; j < L::kXLoads; ++j)
+    res[j] = rows_from((const uint8_t *)a.p.x + (long long)t0 * K, j * kStep, toks);
 #pragma unroll
-  for (int j = 0; j < L::kXLoads; ++j) {
-    const int slot = (j * kWaves + wave) * 64 + lane, row = slot / 8;
-    xoff[j] = (uint32_t)row * (uint32_t)K + 16 * ((slot % 8) ^ L::swz(row));
-  }
-#pragma unroll
-  for (int j = 0; j < L::kWLoads; ++j) {
-    const int slot = (j * kWaves + wave) * 64 + lane, row = slot / 8;
-    woff[j] = (uint32_t)(row % kFeat) * (uint32_t)K + 16 * ((slot % 8) ^ L::swz(row));
-  }
+  for (int j = 0; j < L::kWLoads; ++j)
+    res[L::kXLoads + j] =
+        rows_from(a.p.w[j * kStep / kFeat] + (long long)f0 * K, j * kStep % kFeat, feats);
+  const int piece = 16 * ((lane % 8) ^ L::swz(wave * 8 + lane / 8));
+  uint32_t off = (uint32_t)(wave * 8 + lane / 8) * (uint32_t)K + piece;
   const int tail = K % kFp8Group;  // codes of a last group that is not whole
   // Load j of group c into its stage; the x loads come first.
   auto issue = [&](int c, int stage, int j) {
-    uint8_t *base = smem + stage * L::kStage;
-    if (j == 0 && tail != 0 && c == groups - 1) {  // (the last use of the offsets)
-      auto outside = [&](int i) {
-        const int slot = (i * kWaves + wave) * 64 + lane;
-        return 16 * ((slot % 8) ^ L::swz(slot / 8)) >= tail;
-      };
-#pragma unroll
-      for (int i = 0; i < L::kXLoads; ++i)
-        if (outside(i)) xoff[i] = kOutOfRange;
-#pragma unroll
-      for (int i = 0; i < L::kWLoads; ++i)
-        if (outside(i)) woff[i] = kOutOfRange;
-    }
-    if (j < L::kXLoads) {
-      buf16_to_lds(xres, base + (j * kWaves + wave) * 1024, xoff[j], (uint32_t)c * kFp8Group);
-    } else {
-      const int i = j - L::kXLoads;
-      // (a 1 KB block of rows lies in one projection)
-      const int p = NPROJ == 2 && (i * kWaves + wave) * 8 >= kFeat;
-      buf16_to_lds(NPROJ == 2 && p ? wres[NPROJ - 1] : wres[0],
-                   base + L::kX + (i * kWaves + wave) * 1024, woff[i], (uint32_t)c * kFp8Group);
-    }
+    if (j == 0 && tail != 0 && c == groups - 1 && piece >= tail)
+      off = kOutOfRange;  // (the last use of the offset)
+    buf16_to_lds(res[j], smem + stage * L::kStage + (j * kWaves + wave) * 1024, off,
+                 (uint32_t)c * kFp8Group);
   };
   // The rows' scales come the same way, four groups at a time and up to eight
   // ahead, the first waves' lanes a token each: 16 bytes a token where the rows
@@ -898,9 +881,12 @@ static bool few(int T, int type) { return type != GLM_ROWS_FP8 || T <= 8; }
 // by the 8-bit instruction; by the streaming kernel, whose waves do not wait for
 // each other but read all operands of their tile, or in larger tiles.  At N 4096,
 // K 4096, us by tile: 64 rows 16 x 32 9.6, 32 x 32 8.5, 16 x 64 9.0; 80 rows 32 x 48
-// 8.1, 64 x 32 8.8, 256 x 256 46.8; 333 rows 64 x 48 15.5, 64 x 64 17.7; 600 rows 26.7,
-// 22.9; 1600 rows 54.2, 52.8, 256 x 128 36.1, 256 x 256 49.5; 4096 rows 124.6, 151.3,
-// 81.6, 61.9.
+// 8.1, 64 x 32 8.8, 256 x 256 46.8; 600 rows 64 x 48 26.7, tiles of 64 x 64 22.9;
+// 1600 rows 54.2, 52.8, 256 x 128 36.1, 256 x 256 49.5; 4096 rows 124.6, 151.3, 81.6,
+// 61.9.  A workgroup a CU has all its LDS: five or six waves there, each with a group
+// in flight: 150 rows 64 x 48 of four waves 11.3, six 9.8; 256 rows 64 x 64 of six 11.9,
+// eight 11.9, the tile 15.1; 333 rows 64 x 96 of four 15.8, five 15.0, six 15.5, 64 x 48 of
+// four 16.2; but 512 rows 64 x 64 of six 20.8, the tile 18.5.
 static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
   if (few(a.T, type)) return stream_few<1>(stream, a, type, 1);
   if (a.T <= kExactTokens) {
@@ -913,7 +899,8 @@ static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
     }
   }
   static const Fp8Cut cuts[] = {{32, 48, 30, 52},  {64, 32, 40, 46},   {64, 48, 45, 57}, {64, 64, 90, 54},
-                                {128, 64, 100, 90}, {256, 128, 10, 330}, {256, 256, 0, 500}};
+                                {128, 64, 100, 90}, {256, 128, 10, 330}, {256, 256, 0, 500},
+                                {64, 48, 28, 70}, {64, 64, 30, 87}, {64, 96, 36, 113}};
   switch (cheapest(cuts, a.T, a.N)) {
     case 0: return launch_stream<CodedStream<8, 1, 2, 3, true>>(stream, a);
     case 1: return launch_stream<CodedStream<4, 1, 4, 2, true>>(stream, a);
@@ -921,7 +908,10 @@ static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
     case 3: return launch_tile<1, Fp8Tile<2, 2, 2, 2, 52>>(stream, a);
     case 4: return launch_tile<1, Fp8Tile<2, 2, 4, 2, 79>>(stream, a);
     case 5: return launch_tile<1, Fp8Tile<2, 4, 8, 2>>(stream, a);
-    default: return launch_tile<1, Fp8Tile<2, 4, 8, 4>>(stream, a);
+    case 6: return launch_tile<1, Fp8Tile<2, 4, 8, 4>>(stream, a);
+    case 7: return launch_stream<CodedStream<6, 1, 4, 3, true>>(stream, a);
+    case 8: return launch_stream<CodedStream<6, 1, 4, 4, true>>(stream, a);
+    default: return launch_stream<CodedStream<5, 1, 4, 6, true>>(stream, a);
   }
 }
 

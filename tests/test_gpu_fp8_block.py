@@ -226,8 +226,9 @@ SHAPES = [
     (17, 1408, 255), (31, 112, 129), (32, 4112, 96), (33, 272, 100), (48, 2048, 576), (64, 1024, 384), (65, 1040, 513),
     (100, 256, 1000), (128, 384, 128), (129, 400, 144), (200, 4096, 300), (256, 2048, 2048), (257, 528, 515),
     (333, 1536, 640), (700, 656, 1100), (1025, 896, 2047), (2000, 512, 4096),
-    # each way to cut a product of more than 64 rows, beside the above
-    (140, 272, 4100), (620, 272, 4095), (850, 144, 4096), (1600, 144, 4096), (3000, 144, 4096), (2900, 528, 4090),
+    # each way to cut a product, beside the above
+    (24, 272, 4096), (30, 144, 8000), (56, 400, 4100),
+    (140, 272, 4100), (250, 272, 4090), (370, 272, 4095), (230, 272, 6000), (450, 272, 4096), (620, 272, 4095), (850, 144, 4096), (1600, 144, 4096), (3000, 144, 4096), (2900, 528, 4090),
     (70, 9008, 40), (4, 9008, 40), (40, 16400, 24),
 ]
 
@@ -257,7 +258,7 @@ def test_linear(F, T, K, N, kind):
 
 
 GATED = [(1, 128, 16), (2, 2048, 768), (5, 144, 144), (16, 1408, 240), (17, 272, 128), (48, 2048, 512), (64, 4096, 2048),
-         (65, 528, 400), (129, 512, 256), (256, 1024, 1408), (333, 656, 272), (1030, 384, 768), (2000, 512, 2048), (100, 272, 1024), (333, 272, 1408), (150, 1040, 2048),
+         (65, 528, 400), (129, 512, 256), (256, 1024, 1408), (333, 656, 272), (1030, 384, 768), (2000, 512, 2048), (100, 272, 1024), (333, 272, 1408), (150, 1040, 2048), (96, 272, 2048),
          (500, 4112, 2048), (3000, 400, 2048), (2950, 272, 2032), (70, 9008, 48), (3, 9008, 48)]
 
 
