@@ -21,7 +21,7 @@
 #include "lds_stage.h"
 #include "mfma_tile.h"
 
-#include <climits>
+#include <algorithm>
 
 namespace glm {
 
@@ -439,7 +439,7 @@ constexpr int kTileXcds = 8;
 struct Fp8TileArgs {
   Fp8Args p;
   int row_tiles, tok_tiles;
-  int rows_outer;   // consecutive items walk the tokens of one row tile, else the reverse
+  int strip;        // row tiles of a strip: consecutive items walk across it, then along the tokens
 };
 
 // WN x WT waves of BN x BT blocks; KB of LDS for a workgroup.
@@ -484,8 +484,9 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
   const int on_xcd = (int)blockIdx.x / kTileXcds;
   const int item = ((int)blockIdx.x % kTileXcds) * per_xcd + on_xcd;
   if (on_xcd >= per_xcd || item >= items) return;
-  const int rt = a.rows_outer ? item / a.tok_tiles : item % a.row_tiles;
-  const int tt = a.rows_outer ? item % a.tok_tiles : item / a.row_tiles;
+  const int above = item / (a.strip * a.tok_tiles) * a.strip;  // row tiles of the strips before
+  const int wide = min(a.strip, a.row_tiles - above), in_strip = item - above * a.tok_tiles;
+  const int rt = above + in_strip % wide, tt = in_strip / wide;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int wn = wave % L::WN, wt = wave / L::WN;
@@ -837,8 +838,14 @@ static int rows_for(hipStream_t stream, Fp8Args &a, int &type, uint8_t *&ws) {
 template <int NPROJ, class L>
 static int launch_tile(hipStream_t stream, const Fp8Args &p) {
   constexpr int feat = L::kRows / NPROJ;
-  Fp8TileArgs a{p, (p.N + feat - 1) / feat, (p.T + L::kTok - 1) / L::kTok, NPROJ * p.N >= p.T};
+  Fp8TileArgs a{p, (p.N + feat - 1) / feat, (p.T + L::kTok - 1) / L::kTok, 1};
   const int items = a.row_tiles * a.tok_tiles;
+  // What an XCD's 32 CUs work on at once as square as it goes: the fewest rows and
+  // tokens for its L2 to fetch.  (8192 rows, K and N 8192: 511 us along the tokens, 463
+  // in strips; 4096, 256 x 128 tiles: 84 and 79.5.)
+  const int square = std::min((items + kTileXcds - 1) / kTileXcds, 32);
+  while (a.strip * a.strip * L::kRows < square * L::kTok) ++a.strip;
+  a.strip = std::min(a.strip, a.row_tiles);
   hipLaunchKernelGGL((fp8_tile_kernel<NPROJ, L>),
                      dim3((unsigned)((items + kTileXcds - 1) / kTileXcds * kTileXcds)),
                      dim3(L::kThreads), (size_t)L::kBytes, stream, a);
