@@ -752,7 +752,7 @@ int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_stride, int B
 int glm_fp8_quantize_rows(void *stream, const void *x, int x_type, int T, int K, uint8_t *codes,
                           float *scales);
 
-/* A weight bf16 [N][K] to codes and scales.  Limits: K % 8 == 0, N <= 65535 * 128. */
+/* A weight bf16 [N][K] to codes and scales.  Limits: K % 8 == 0, N and K <= 2^20. */
 int glm_fp8_quantize_weight(void *stream, const uint16_t *w, int N, int K, uint8_t *codes,
                             float *scales);
 
@@ -761,8 +761,9 @@ int glm_fp8_quantize_weight(void *stream, const uint16_t *w, int N, int K, uint8
  * its result: h = x + residual, residual_out = h (in the residual's type),
  * y = h * (1 / sqrt(mean(h^2) + eps)) * weight from the unrounded h, and y's
  * codes and scales.  x and residual each GLM_ROWS_BF16 or GLM_ROWS_F32;
- * residual and residual_out may be the same buffer, and both NULL (h = x);
- * weight f32 [d] or NULL.  Limits: d % 8 == 0, d <= 32768.
+ * residual_out may be the residual's buffer, or x's where the types are the
+ * same; residual and residual_out may be NULL (h = x); weight f32 [d] or NULL.
+ * Limits: d % 8 == 0, d <= 32768, T < 2^22.
  */
 int glm_add_rms_norm_fp8(void *stream, const void *x, int x_type, const void *residual,
                          int residual_type, int T, int d, const float *weight, float eps,
@@ -777,8 +778,11 @@ size_t glm_fp8_workspace_bytes(int x_type, int T, int K, int N, int gated);
 /*
  * y = bf16(x W^T), f32 sums of f32 products of the codes' sums and the scales
  * (DeferredLinear.__call__, layers.py:38-70, in this format).  Rows in bf16 or
- * f32 are quantised as glm_fp8_quantize_rows does.  y bf16 [T][N].  The
- * workspace needs no clearing; calls that may overlap need their own.
+ * f32 are quantised as glm_fp8_quantize_rows does.  y bf16 [T][N].  Up to 64
+ * rows the products within a group are exact and summed in f32; more rows go
+ * through the 8-bit matrix instruction, which aligns eight products at a time
+ * and drops what lies 2^-13 below the largest of them.  The workspace needs no
+ * clearing; calls that may overlap need their own.
  * Limits: K % 16 == 0, K, N and T <= 2^20.
  */
 int glm_fp8_linear(void *stream, const void *x, int x_type, const float *x_scales, int T, int K,

@@ -181,9 +181,9 @@ extern "C" int glm_fp8_quantize_weight(void *stream, const uint16_t *w, int N, i
                                        uint8_t *codes, float *scales) {
   glm::clear_error();
   GLM_REQUIRE(N >= 1 && K >= 1, GLM_ERR_INVALID_ARGUMENT, "fp8_quantize_weight: invalid sizes");
-  GLM_REQUIRE(K % 8 == 0 && fp8_groups(N) <= 65535, GLM_ERR_UNSUPPORTED_SHAPE,
-              "fp8_quantize_weight: a %d x %d weight (the columns in eights, at most 65535 x 128 "
-              "rows)", N, K);
+  GLM_REQUIRE(K % 8 == 0 && N <= 1 << 20 && K <= 1 << 20, GLM_ERR_UNSUPPORTED_SHAPE,
+              "fp8_quantize_weight: a %d x %d weight (the columns in eights, at most 2^20 of "
+              "either)", N, K);
   GLM_REQUIRE(w && codes && scales, GLM_ERR_INVALID_ARGUMENT, "fp8_quantize_weight: null pointer");
   GLM_REQUIRE(glm_aligned16({w, codes, scales}), GLM_ERR_INVALID_ARGUMENT,
               "fp8_quantize_weight: buffers must be 16-byte aligned");
@@ -208,8 +208,9 @@ extern "C" int glm_add_rms_norm_fp8(void *stream, const void *x, int x_type, con
   glm::clear_error();
   GLM_REQUIRE(T >= 0 && d >= 1 && row_type(x_type) && row_type(residual_type) && eps >= 0.f,
               GLM_ERR_INVALID_ARGUMENT, "add_rms_norm_fp8: invalid sizes, row type or eps");
-  GLM_REQUIRE(d % 8 == 0 && d <= 32768, GLM_ERR_UNSUPPORTED_SHAPE,
-              "add_rms_norm_fp8: d = %d, a multiple of 8 up to 32768", d);
+  GLM_REQUIRE(d % 8 == 0 && d <= 32768 && T < 1 << 22, GLM_ERR_UNSUPPORTED_SHAPE,
+              "add_rms_norm_fp8: %d rows of d = %d, fewer than 2^22 (a grid has 2^32 threads at "
+              "most) of a multiple of 8 up to 32768", T, d);
   GLM_REQUIRE(x && codes && scales, GLM_ERR_INVALID_ARGUMENT, "add_rms_norm_fp8: null pointer");
   GLM_REQUIRE(!residual == !residual_out, GLM_ERR_INVALID_ARGUMENT,
               "add_rms_norm_fp8: residual and residual_out come together");

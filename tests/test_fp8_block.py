@@ -88,6 +88,8 @@ def test_quantisers_refuse():
         refused(bad, "glm_fp8_quantize_rows", None, *args)
     refused(shape, "glm_fp8_quantize_weight", None, FAKE, 4, 12, FAKE, FAKE)
     refused(shape, "glm_fp8_quantize_weight", None, FAKE, 65535 * 128 + 1, 8, FAKE, FAKE)
+    # grids of 2^32 threads and more
+    refused(shape, "glm_fp8_quantize_weight", None, FAKE, 1, (1 << 31) - 8, FAKE, FAKE)
     refused(bad, "glm_fp8_quantize_weight", None, FAKE, 0, 8, FAKE, FAKE)
     refused(bad, "glm_fp8_quantize_weight", None, FAKE, 4, 8, None, FAKE)
 
@@ -99,6 +101,8 @@ def test_quantisers_refuse():
         refused(bad, "glm_add_rms_norm_fp8", *norm(**kw))
     for d in (12, 32776):
         refused(shape, "glm_add_rms_norm_fp8", *norm(d=d))
+    refused(shape, "glm_add_rms_norm_fp8", *norm(T=1 << 24, d=8))
+    refused(shape, "glm_add_rms_norm_fp8", *norm(T=1 << 22, d=8))
     assert native.load().glm_add_rms_norm_fp8(*norm(T=0)) == native.GLM_OK
 
 
@@ -111,6 +115,14 @@ def test_python_side_refuses_what_is_no_gpu_tensor():
                  lambda: F.linear("rows", w, s)):
         with pytest.raises(ContractError):
             call()
+
+
+def test_outputs_lie_apart():
+    raw = torch.zeros(64, dtype=torch.uint8)
+    for a, b in ((0, 0), (0, 8), (8, 0), (15, 0), (0, 15)):  # 16 bytes each
+        with pytest.raises(ContractError, match="overlaps"):
+            F._apart(raw[a:a + 16], "out", None, raw[40:], raw[b:b + 16])
+    F._apart(raw[:16], "out", None, raw[16:32], raw[:0])
 
 
 def test_layers_keep_their_rules():

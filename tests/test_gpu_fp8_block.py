@@ -212,6 +212,10 @@ def test_add_rms_norm_in_place_and_nan(F):
     got, same = F.add_rms_norm(x, None, 1e-6, residual=into, residual_out=into)
     assert same is into and torch.equal(into.view(torch.int32), h.view(torch.int32))
     assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    into = x.clone()  # in the rows' own place
+    got2, same = F.add_rms_norm(into, None, 1e-6, residual=r, residual_out=into)
+    assert same is into and torch.equal(into.view(torch.int32), h.view(torch.int32))
+    assert torch.equal(got2.codes, want.codes) and torch.equal(got2.scales, want.scales)
     codes = host(got.codes)
     assert ((codes[1] & 127) == 127).all()  # a NaN spreads over its row
     assert (codes[2, 9] & 127) == 127 and not (np.delete(codes[2], 9) & 127).any()
@@ -228,8 +232,11 @@ SHAPES = [
     (333, 1536, 640), (700, 656, 1100), (1025, 896, 2047), (2000, 512, 4096),
     # each way to cut a product, beside the above
     (24, 272, 4096), (30, 144, 8000), (56, 400, 4100),
-    (140, 272, 4100), (250, 272, 4090), (370, 272, 4095), (230, 272, 6000), (450, 272, 4096), (620, 272, 4095), (850, 144, 4096), (1600, 144, 4096), (3000, 144, 4096), (2900, 528, 4090),
+    (140, 272, 4100), (250, 272, 4090), (370, 272, 4095), (230, 272, 6000),
+    (450, 272, 4096), (620, 272, 4095), (850, 144, 4096), (1600, 144, 4096), (3000, 144, 4096), (2900, 528, 4090),
     (70, 9008, 40), (4, 9008, 40), (40, 16400, 24),
+    # the longest rows that a workgroup quantises, longer ones, the longest
+    (4, 16384, 40), (3, 16400, 24), (2, 1 << 20, 20), (66, 1 << 17, 33),
 ]
 
 
@@ -258,8 +265,10 @@ def test_linear(F, T, K, N, kind):
 
 
 GATED = [(1, 128, 16), (2, 2048, 768), (5, 144, 144), (16, 1408, 240), (17, 272, 128), (48, 2048, 512), (64, 4096, 2048),
-         (65, 528, 400), (129, 512, 256), (256, 1024, 1408), (333, 656, 272), (1030, 384, 768), (2000, 512, 2048), (100, 272, 1024), (333, 272, 1408), (150, 1040, 2048), (96, 272, 2048),
-         (500, 4112, 2048), (3000, 400, 2048), (2950, 272, 2032), (70, 9008, 48), (3, 9008, 48)]
+         (65, 528, 400), (129, 512, 256), (256, 1024, 1408), (333, 656, 272), (1030, 384, 768), (2000, 512, 2048), (100, 272, 1024),
+         (333, 272, 1408), (150, 1040, 2048), (96, 272, 2048),
+         (500, 4112, 2048), (3000, 400, 2048), (2950, 272, 2032), (70, 9008, 48), (3, 9008, 48),
+         (4, 16384, 48), (3, 16400, 32)]
 
 
 @pytest.mark.parametrize("T, K, N", GATED)
@@ -339,6 +348,8 @@ def test_refusals(F):
     rng = np.random.default_rng(7)
     x, (w, s) = gpu(rows(rng, 4, 256)), [gpu(a) for a in weight(rng, 48, 256)]
     q = F.quantize_rows(x)
+    big = torch.zeros(2048, device="cuda")
+    square, wide = big[:512].view(torch.bfloat16).view(4, 256), [gpu(a) for a in weight(rng, 256, 256)]
     cases = [
         lambda: F.linear(x[:, :128], w, s),                       # not contiguous
         lambda: F.linear(x.double(), w, s), lambda: F.linear(x.half(), w, s),
@@ -360,11 +371,50 @@ def test_refusals(F):
         lambda: F.add_rms_norm(x, None, 1e-6, residual_out=x.clone()),
         lambda: F.add_rms_norm(x, None, 1e-6, residual=x, residual_out=x.bfloat16()),
         lambda: F.linear(torch.zeros((), device="cuda"), w, s),
+        # outputs over what is read
+        lambda: F.linear(square, *wide, out=square),
+        lambda: F.linear((big[:256].view(torch.uint8).view(4, 256), q.scales), *wide, out=square),
+        lambda: F.gate_up(q, *wide, *wide, 0.0, out=q),
+        lambda: F.quantize_rows(x, out=F.Fp8Rows(x.view(-1)[:256].view(torch.uint8).view(4, 256), q.scales)),
+        lambda: F.add_rms_norm(square, None, 1e-6, residual=x, residual_out=big[:1024].view(4, 256)),
+        lambda: F.add_rms_norm(big[:1024].view(4, 256), None, 1e-6, residual=x, residual_out=big[8:1032].view(4, 256)),
+        lambda: F.add_rms_norm(x, None, 1e-6, residual=x.clone(), residual_out=big[:1024].view(4, 256),
+                               out=F.Fp8Rows(big[:256].view(torch.uint8).view(4, 256), q.scales)),
     ]
     for i, case in enumerate(cases):
         with pytest.raises(ContractError):
             case()
             pytest.fail(f"case {i} was taken")
+
+
+def test_offsets_past_32_bits(F):
+    # 2^20 rows of 2064 channels: codes, bf16 rows and outputs beyond 2^31 and 2^32 bytes
+    T, K = 1 << 20, 2064
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    some = torch.tensor([0, 1, 777_777, *range(T - 70, T)], device="cuda")
+    x = torch.empty((T, K), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    r = torch.empty((T, K), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    q = F.quantize_rows(x)
+    want = P.quantize_rows(host(x[some]))
+    assert np.array_equal(host(q.codes[some]), want[0]) and np.array_equal(host(q.scales[some]), want[1])
+    n, h = F.add_rms_norm(x, None, 1e-6, residual=r)
+    few, few_h = F.add_rms_norm(x[some], None, 1e-6, residual=r[some])
+    assert torch.equal(n.codes[some], few.codes) and torch.equal(n.scales[some], few.scales)
+    assert torch.equal(h[some], few_h)
+    del n, h, r, x
+    w = weight(np.random.default_rng(14), K, K)
+    y = F.linear(q, gpu(w[0]), gpu(w[1]))
+    dot, S = P.product(want, w)
+    check_bf16(y[some], dot, product_error(K, S) + dropped(want, w))
+    del y
+    short = F.Fp8Rows(q.codes[:, :144].contiguous(), q.scales[:, :2].contiguous())
+    ws = [gpu(w[0][:, :144]), gpu(w[1][:, :2])]
+    got = F.gate_up(short, *ws, *ws, 5.0)
+    few = F.gate_up(F.Fp8Rows(short.codes[some], short.scales[some]), *ws, *ws, 5.0)
+    # exact products of two groups either way: the same f32 sums but for their order, a code apart at most
+    a, b = (P.row_values(host(v.codes), host(v.scales)) for v in (F.Fp8Rows(got.codes[some], got.scales[some]), few))
+    step = np.repeat(host(few.scales).astype(np.float64), 128, 1)[:, :K]
+    assert np.all(np.abs(a - b) <= np.maximum(np.abs(b) * 2.0 ** -3, step * 2.0 ** -9) * (1 + 2.0 ** -10))
 
 
 # ---------------------------------------------------------------- as they are used
@@ -482,10 +532,20 @@ def test_a_block_scaled_shared_expert(F, T):
         p.quantize_to_fp8_block()
     out = moe(x)
     shared = moe.shared_experts(x)
+    assert moe(x[:0]).shape == (0, shape.d)
+    # with the FFN site's residual streams: the same layer, then post y + comb residual
+    from glm53flash.mhc import hyper_residual
+    streams, post, comb = (torch.from_numpy(rng.normal(0, 1, n).astype(np.float32)).cuda()
+                           for n in ((T, 4, shape.d), (T, 4), (T, 4, 4)))
+    whole = moe.with_hyper_residual(x, streams, post, comb)
+    apart = hyper_residual(streams, out, post, comb)
     moe.shared_experts = mlp_of(rng, shape.d, shape.I_shared)
     moe.shared_experts.down_proj.scales.zero_()
     rest = moe(x)
     # f32 sums of at most nine terms, the shared one last
     err = (out - (rest + shared.float())).abs()
     assert bool((err <= 2.0 ** -22 * (rest.abs() + shared.float().abs())).all())
+    # at most nine terms of y in another order, and ten roundings of the five terms
+    most = hyper_residual(streams.abs(), rest.abs() + shared.float().abs(), post.abs(), comb.abs())
+    assert bool(((whole - apart).abs() <= 2.0 ** -20 * most).all())
     assert float(shared.float().abs().max()) > 0 and out.dtype == torch.float32
