@@ -14,7 +14,7 @@
 // v_mfma_f32_16x16x32_bf16: exact products, f32 sums (1e-8 relative error on
 // normal values).  As it is in one v_mfma_f32_16x16x128_f8f6f4, at twice the
 // rate: the core aligns eight products at a time to the largest of them and
-// drops what lies 2^-14 of it below, which is 1.5e-5 of the sum on normal
+// drops what lies 2^-13 of it below, which is 1.5e-5 of the sum on normal
 // values, without a bias.  The latter serves products whose result is rounded
 // to bf16 (1.7e-3) and whose time the matrix cores set.
 #include "fp8_rows.h"
@@ -223,31 +223,43 @@ __global__ __launch_bounds__(L::kThreads) void fp8_stream_kernel(Fp8Args a) {
   } else {
     // item: token item % toks of the workgroup's group item / toks; four lanes, of which each
     // has every fourth eight channels
-    constexpr int kPer = L::kThreads / 4;
+    constexpr bool F32 = ROWS == GLM_ROWS_F32;
+    constexpr int kPer = L::kThreads / 4, kBytes = F32 ? 4 : 2, kRaw = 2 * kBytes;
+    const __amdgpu_buffer_rsrc_t rows = make_rsrc(a.x, toks * (uint32_t)K * kBytes);
     const int items = ncoded * (int)toks, l4 = threadIdx.x & 3;
     auto place = [&](int item, int &li, int &t) {
       li = toks == 1 ? item : (int)__umulhi((uint32_t)item, a.per_token);
       t = item - li * (int)toks;
     };
-    float v[32], ahead_v[32];
-    auto load = [&](int item, float (&to)[32]) {
+    glm_u32x4 raw[kRaw];
+    auto load = [&](int item, glm_u32x4 (&to)[kRaw]) {
       int li, t;
       place(item, li, t);
       const int g = (li / kWaves) * step + kWaves * blockIdx.z + li % kWaves;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; ++j) {  // (no branches between the loads)
         const int k = g * kFp8Group + 8 * (4 * j + l4);
-        float (&e)[8] = *reinterpret_cast<float (*)[8]>(to + 8 * j);
+        const uint32_t off = item < items && k < K ? (uint32_t)(t * K + k) * kBytes : kOutOfRange;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = 0.f;
-        if (item < items && k < K) load8<ROWS == GLM_ROWS_F32>(a.x, (long long)(t0 + t) * K + k, e);
+        for (int i = 0; i < kRaw / 4; ++i)
+          to[j * (kRaw / 4) + i] = __builtin_amdgcn_raw_buffer_load_b128(rows, off + 16 * i, 0, 0);
       }
     };
-    load(threadIdx.x >> 2, v);
+    load(threadIdx.x >> 2, raw);
     for (int i = 0; i < ahead; ++i)
       if (i < mine) issue(i, i);
-    for (int item = threadIdx.x >> 2; item < items; item += kPer) {
-      load(item + kPer, ahead_v);
+    auto code = [&](int item) {
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float (&e)[8] = *reinterpret_cast<float (*)[8]>(v + 8 * j);
+        if constexpr (F32) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = __uint_as_float(raw[2 * j + i / 4][i % 4]);
+        } else {
+          unpack8(raw[j], e);
+        }
+      }
       int li, t;
       place(item, li, t);
       auto over_lanes = [](float m) {
@@ -265,8 +277,18 @@ __global__ __launch_bounds__(L::kThreads) void fp8_stream_kernel(Fp8Args a) {
             uint2{fp8_codes4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3], up),
                   fp8_codes4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7], up)};
       if (l4 == 0) coded_scales[li * L::kTok + t] = m / kFp8Max;
+    };
+    int item = threadIdx.x >> 2;
+    if (items <= kPer) {  // (no loads behind the weights')
+      if (item < items) code(item);
+    } else {
+      for (; item < items; item += kPer) {
+        glm_u32x4 next[kRaw];
+        load(item + kPer, next);
+        code(item);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = ahead_v[i];
+        for (int j = 0; j < kRaw; ++j) raw[j] = next[j];
+      }
     }
     __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's codes are in LDS
     ring_barrier();
@@ -394,7 +416,10 @@ __global__ __launch_bounds__(L::kThreads) void fp8_stream_kernel(Fp8Args a) {
 }
 
 // The gated pair's sums [split][projection][T][N] joined, gated and quantised:
-// sixteen lanes a group of features.
+// sixteen lanes a group of features.  Its own launch, since a group's maximum
+// spans eight workgroups' features (a workgroup for all 128 leaves most CUs idle:
+// 2 rows, K 2048, 2 x 768 features 14.3 us, the two launches 7.1); 2.4 us for 2
+// rows of 768, 3.9 for 64 of 2048, most of it the launch.
 __global__ __launch_bounds__(256) void fp8_gate_kernel(const float *h, int splits, int T, int N,
                                                        float limit, uint8_t *codes, float *scales) {
   const int groups = fp8_groups(N), lane = threadIdx.x & 15;
@@ -433,6 +458,14 @@ __global__ __launch_bounds__(256) void fp8_gate_kernel(const float *h, int split
 // row R lies at p ^ ((R >> 1) & 7): the 16 rows that a quarter of a wave reads
 // are then on 16 different pieces of 256 bytes.  Rows past the last and pieces
 // past K are out of the buffers' range, which gives zeros.
+//
+// The largest tile is 256 x 256 (the pair: 2 x 128 x 256): 64 KB a group of K, two
+// groups in LDS, 128 of 256 registers hold sums.  4096 rows, K and N 4096: 58 to 63
+// us, 2.2 to 2.35 PFLOP/s where a library's product of plain 8-bit matrices has
+// 2.8; 8192 rows, K and N 8192: 463 us, 2.37; the pair, 4001 rows, K 4096, 2 x 2048
+// features: 104 to 111 us, 1.25 where a bf16 one has 1.45.  Matrix cores are busy for
+// 56 to 58 % of the cycles, at a clock that power limits: without the loads 68.6 us
+// are 62.6, and without the conversions the pair takes longer.
 // ---------------------------------------------------------------------------
 constexpr int kTileXcds = 8;
 

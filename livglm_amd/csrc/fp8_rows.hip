@@ -11,7 +11,10 @@ namespace glm {
 constexpr int kRowsThreads = 256;
 
 // ---------------------------------------------------------------------------
-// Rows.  Sixteen lanes hold a group, eight channels each.
+// Rows: one pass over the bytes, sixteen lanes a group with eight channels each,
+// so that a lane loads 16 bytes of bf16 and the maximum is four steps over lanes.
+// Bound by bytes: 7777 bf16 rows of 4096 (96.6 MB) 16.4 us, 5.9 TB/s (a large copy
+// has 4.9; the rest is the memory-side cache's); 64 rows 2.5, a launch.
 // ---------------------------------------------------------------------------
 template <bool F32>
 __global__ __launch_bounds__(kRowsThreads) void fp8_quantize_rows_kernel(
@@ -34,7 +37,8 @@ __global__ __launch_bounds__(kRowsThreads) void fp8_quantize_rows_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Weights: a workgroup holds one 128 x 128 block, 64 values a thread.
+// Weights: a workgroup holds one 128 x 128 block, 64 values a thread, so that the
+// block is read once.  Done once, when a weight is loaded.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kRowsThreads) void fp8_quantize_weight_kernel(
     const uint16_t *w, int N, int K, uint8_t *codes, float *scales) {
@@ -69,8 +73,12 @@ __global__ __launch_bounds__(kRowsThreads) void fp8_quantize_weight_kernel(
 
 // ---------------------------------------------------------------------------
 // h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, y quantised.  A
-// workgroup holds its row in registers, 8 STEPS channels a thread; h is not
-// rounded before the norm.
+// workgroup holds its row in registers, 8 STEPS channels a thread, so that x and
+// the residual are read once; h is not rounded before the norm.  As many threads
+// as a row needs with few steps each: the loads of all steps are on their way
+// before the sum.  Bound by bytes: 8191 bf16 rows of 4096 (236 MB) 41.8 us, 5.6
+// TB/s; 1500 f32 rows of 2048 (40 MB) 8.6, 4.6 TB/s; one row 3.5, a launch and two
+// trips to memory.
 // ---------------------------------------------------------------------------
 struct NormArgs {
   const void *x, *residual;
