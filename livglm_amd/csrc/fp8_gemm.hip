@@ -28,10 +28,12 @@ namespace glm {
 typedef int fp8_frag __attribute__((ext_vector_type(8)));
 
 constexpr int kExactTokens = 64;  // rows whose products are summed exactly in any case
-// Rows that the product quantises itself: up to so many, and so many codes, which
-// have to fit its LDS.  (Each workgroup does it for itself: at K and N 4096 1, 4
-// and 16 rows so take 7.0, 7.6 and 13.1 us, quantised before 8.5 to 8.8.)
-constexpr int kFusedTokens = 4, kFusedCodes = 1 << 16;
+// Rows that the product quantises itself: up to so many, and so many codes.  (Each
+// workgroup does it for itself: at K and N 4096 1, 4 and 8 rows so take 6.6, 7.1 and
+// 8.5 us, quantised before 8.0, 8.1 and 8.2 and a launch more for the host; 16 rows of
+// K 2048 5.8 and 5.9; 8 rows of K 8192 12.1 and 10.6; the gated pair of 16 rows, K
+// 2048, 2 x 768 features 7.2 and 8.4.)
+constexpr int kFusedTokens = 16, kFusedCodes = 1 << 15;
 
 struct Fp8Args {
   const void *x;          // codes, or bf16 / f32 rows
@@ -159,8 +161,8 @@ struct Fp8Stream {
   __host__ __device__ static int coded_groups(int groups, int splits) {
     return kCoded ? 0 : WAVES * ((groups + WAVES * splits - 1) / (WAVES * splits));
   }
-  static int coded_bytes(int groups, int splits) {
-    return coded_groups(groups, splits) * kTok * (kFp8Group + 4);
+  static int coded_bytes(int groups, int splits, int T) {
+    return coded_groups(groups, splits) * T * (kFp8Group + 4);
   }
 };
 
@@ -178,9 +180,8 @@ __global__ __launch_bounds__(L::kThreads) void fp8_stream_kernel(Fp8Args a) {
   uint8_t *ring = smem + wave * (ahead * L::kSlot);
   uint8_t *coded = smem + kWaves * ahead * L::kSlot;  // the workgroup's own codes and scales
   const int ncoded = L::coded_groups(groups, gridDim.z);
-  float *coded_scales = reinterpret_cast<float *>(coded + ncoded * L::kTok * kFp8Group);
-
   const uint32_t feats = (uint32_t)min(a.N - n0, 16 * RB), toks = (uint32_t)min(a.T - t0, L::kTok);
+  float *coded_scales = reinterpret_cast<float *>(coded + ncoded * (int)toks * kFp8Group);
   const __amdgpu_buffer_rsrc_t xres =
       make_rsrc((const uint8_t *)a.x + (long long)t0 * K, toks * (uint32_t)K);
   const __amdgpu_buffer_rsrc_t sres =
@@ -270,13 +271,13 @@ __global__ __launch_bounds__(L::kThreads) void fp8_stream_kernel(Fp8Args a) {
       if (__builtin_expect(isinf(m), 0)) m = over_lanes(finite_abs_max(v));  // (one answer in the four)
       m = fmaxf(m, kFp8Tiny);
       const float up = kFp8Max / m;
-      uint8_t *row = coded + (li * L::kTok + t) * kFp8Group + 8 * (l4 & 1);
+      uint8_t *row = coded + (li * (int)toks + t) * kFp8Group + 8 * (l4 & 1);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<uint2 *>(row + 16 * ((2 * j + (l4 >> 1)) ^ L::swz(t))) =
             uint2{fp8_codes4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3], up),
                   fp8_codes4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7], up)};
-      if (l4 == 0) coded_scales[li * L::kTok + t] = m / kFp8Max;
+      if (l4 == 0) coded_scales[li * (int)toks + t] = m / kFp8Max;
     };
     int item = threadIdx.x >> 2;
     if (items <= kPer) {  // (no loads behind the weights')
@@ -315,9 +316,9 @@ __global__ __launch_bounds__(L::kThreads) void fp8_stream_kernel(Fp8Args a) {
     for (int b = 0; b < L::kRowBlocks; ++b) w[b] = frag(from + b * 16 * kFp8Group, r);
     // (columns past the tokens repeat one)
     const int li = i * kWaves + wave;
-    const uint8_t *xrows = L::kCoded ? from + L::kW : coded + li * L::kTok * kFp8Group;
+    const uint8_t *xrows = L::kCoded ? from + L::kW : coded + li * (int)toks * kFp8Group;
     const float *xscales = L::kCoded ? reinterpret_cast<const float *>(from + L::kW + L::kX)
-                                     : coded_scales + li * L::kTok;
+                                     : coded_scales + li * (int)toks;
     fp8_frag xf[TB];
     float sx[TB];
 #pragma unroll
@@ -830,7 +831,7 @@ static int launch_stream(hipStream_t stream, Fp8Args a, int splits = 1) {
   const dim3 grid((unsigned)((a.N + 16 * L::RB - 1) / (16 * L::RB)),
                   (unsigned)((a.T + 16 * L::TB - 1) / (16 * L::TB)), (unsigned)splits);
   // a workgroup a CU takes all the LDS for its groups in flight, else two share it
-  const int coded = L::coded_bytes(a.groups, splits);
+  const int coded = L::coded_bytes(a.groups, splits, a.T);
   const long long wgs = (long long)grid.x * grid.y * grid.z;
   const int room = (wgs <= 256 ? kStreamKB : kStreamPairKB) * 1024 - coded;
   int ahead = room / (L::kWaves * L::kSlot);
@@ -848,7 +849,7 @@ static int launch_stream(hipStream_t stream, Fp8Args a, int splits = 1) {
 
 // Workspace of rows that the product does not take as they are.
 static size_t rows_bytes(int T, int K, int type) {
-  const long long codes = (long long)kFusedTokens * fp8_groups(K) * kFp8Group;
+  const long long codes = (long long)T * fp8_groups(K) * kFp8Group;
   if (type == GLM_ROWS_FP8 || (T <= kFusedTokens && codes <= kFusedCodes)) return 0;
   return round256((size_t)T * K) + round256((size_t)T * fp8_groups(K) * 4);
 }
