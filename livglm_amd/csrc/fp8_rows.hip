@@ -3,6 +3,7 @@
 // reference keeps its resident weights in group-32 MXFP8 (layers.py:72-99) and
 // multiplies bf16 rows; here both sides of a product are E4M3.
 #include "fp8_rows.h"
+#include "lds_stage.h"
 
 #include <climits>
 
@@ -75,11 +76,20 @@ __global__ __launch_bounds__(kRowsThreads) void fp8_quantize_weight_kernel(
 // h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, y quantised.  A
 // workgroup holds its row in registers, 8 STEPS channels a thread, so that x and
 // the residual are read once; h is not rounded before the norm.  As many threads
-// as a row needs with few steps each: the loads of all steps are on their way
-// before the sum.  Bound by bytes: 8191 bf16 rows of 4096 (236 MB) 41.8 us, 5.6
-// TB/s; 1500 f32 rows of 2048 (40 MB) 8.6, 4.6 TB/s; one row 3.5, a launch and two
-// trips to memory.
+// as a row needs with one step each, as far as a workgroup goes.  Bound by bytes:
+// 8191 bf16 rows of 4096 (236 MB) 41 us, 5.8 TB/s; 1500 f32 rows of 2048 (40 MB) 8.7,
+// 4.6 TB/s; one row of 4096 3.4, a launch, a trip to memory and the sum.
 // ---------------------------------------------------------------------------
+template <bool F32>
+__device__ __forceinline__ void values8(const glm_u32x4 *raw, float v[8]) {
+  if constexpr (F32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw[j / 4][j % 4]);
+  } else {
+    unpack8(raw[0], v);
+  }
+}
+
 struct NormArgs {
   const void *x, *residual;
   const float *weight;
@@ -94,22 +104,40 @@ template <int THREADS, int STEPS, bool XF32, bool RF32>
 __global__ __launch_bounds__(THREADS) void add_rms_norm_fp8_kernel(NormArgs a) {
   __shared__ float red[THREADS / 64];
   const long long row = (long long)blockIdx.x * a.d;
+  constexpr int kX = XF32 ? 4 : 2, kR = RF32 ? 4 : 2;  // bytes
+  // What a row needs is asked for at once and without branches, past d and of absent
+  // operands zeros from outside the buffers' range: a wait behind each load, and the
+  // weight's behind the sum, cost one row of 4096 0.2 us and 8191 of them 1.
+  const auto of = [&](const void *p, int bytes) {
+    return make_rsrc((const uint8_t *)p + (p ? row * bytes : 0), p ? (uint32_t)(a.d * bytes) : 0u);
+  };
+  const __amdgpu_buffer_rsrc_t xres = of(a.x, kX), rres = of(a.residual, kR),
+                               wres = make_rsrc(a.weight, a.weight ? (uint32_t)a.d * 4 : 0u);
+  const auto get = [](__amdgpu_buffer_rsrc_t res, int byte) {
+    return __builtin_amdgcn_raw_buffer_load_b128(res, byte, 0, 0);
+  };
+  glm_u32x4 x[STEPS][kX / 2], r[STEPS][kR / 2], w[STEPS][2];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int c = 8 * (i * THREADS + threadIdx.x);
+#pragma unroll
+    for (int j = 0; j < kX / 2; ++j) x[i][j] = get(xres, c * kX + 16 * j);
+#pragma unroll
+    for (int j = 0; j < kR / 2; ++j) r[i][j] = get(rres, c * kR + 16 * j);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) w[i][j] = get(wres, c * 4 + 16 * j);
+  }
   float h[STEPS][8];
   float sq = 0.f;
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     const int c = 8 * (i * THREADS + threadIdx.x);
+    float add[8];
+    values8<XF32>(x[i], h[i]);
+    values8<RF32>(r[i], add);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
-    if (c >= a.d) continue;
-    load8<XF32>(a.x, row + c, h[i]);
-    if (a.residual) {
-      float r[8];
-      load8<RF32>(a.residual, row + c, r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] += r[j];
-    }
-    if (a.residual_out) {
+    for (int j = 0; j < 8; ++j) h[i][j] = a.residual ? h[i][j] + add[j] : h[i][j];
+    if (a.residual_out && c < a.d) {
       if constexpr (RF32) {
         glm_f32x4 *o = reinterpret_cast<glm_f32x4 *>((float *)a.residual_out + row + c);
         o[0] = glm_f32x4{h[i][0], h[i][1], h[i][2], h[i][3]};
@@ -135,14 +163,10 @@ __global__ __launch_bounds__(THREADS) void add_rms_norm_fp8_kernel(NormArgs a) {
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     const int c = 8 * (i * THREADS + threadIdx.x);
-    if (c < a.d) {
-      float w[8];
-      if (a.weight) load8<true>(a.weight, c, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        h[i][j] *= inv;
-        if (a.weight) h[i][j] *= w[j];
-      }
+    for (int j = 0; j < 8; ++j) {
+      h[i][j] *= inv;
+      if (a.weight) h[i][j] *= __uint_as_float(w[i][j / 4][j % 4]);
     }
     const float amax = group_amax(h[i]);  // (all lanes of the group are here)
     const float up = kFp8Max / amax;
@@ -228,9 +252,14 @@ extern "C" int glm_add_rms_norm_fp8(void *stream, const void *x, int x_type, con
   const NormArgs a{x, residual, weight, residual_out, codes, scales, d, fp8_groups(d), eps};
   const bool xf = x_type == GLM_ROWS_F32, rf = residual_type == GLM_ROWS_F32;
   hipStream_t s = (hipStream_t)stream;
+  // One step a thread where a workgroup can.  bf16 without a weight, us: one row of 2048 by 256 x 1
+  // threads and steps 2.9 to 3.1, 128 x 2 3.4; 4096 by 512 x 1 3.1, 256 x 2 3.5; 8192
+  // by 1024 x 1 3.5, 256 x 4 5.0; many rows of 2048 23.5 and 24.9; 4096 43.8 and 46.0,
+  // 1024 x 1 54.0; 8192 42.8 and 47.9; 16384 by 1024 x 2 44.4, 1024 x 4 45.2.
   if (d <= 2048) launch_norm<256, 1>(s, T, xf, rf, a);
-  else if (d <= 4096) launch_norm<256, 2>(s, T, xf, rf, a);
-  else if (d <= 8192) launch_norm<256, 4>(s, T, xf, rf, a);
+  else if (d <= 4096) launch_norm<512, 1>(s, T, xf, rf, a);
+  else if (d <= 8192) launch_norm<1024, 1>(s, T, xf, rf, a);
+  else if (d <= 16384) launch_norm<1024, 2>(s, T, xf, rf, a);
   else launch_norm<1024, 4>(s, T, xf, rf, a);
   GLM_LAUNCH_CHECK("add_rms_norm_fp8_kernel");
   return GLM_OK;
