@@ -72,14 +72,6 @@ __global__ __launch_bounds__(kRowsThreads) void fp8_quantize_weight_kernel(
   if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = m / kFp8Max;
 }
 
-// ---------------------------------------------------------------------------
-// h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, y quantised.  A
-// workgroup holds its row in registers, 8 STEPS channels a thread, so that x and
-// the residual are read once; h is not rounded before the norm.  As many threads
-// as a row needs with one step each, as far as a workgroup goes.  Bound by bytes:
-// 8191 bf16 rows of 4096 (236 MB) 41 us, 5.8 TB/s; 1500 f32 rows of 2048 (40 MB) 8.7,
-// 4.6 TB/s; one row of 4096 3.4, a launch, a trip to memory and the sum.
-// ---------------------------------------------------------------------------
 template <bool F32>
 __device__ __forceinline__ void values8(const glm_u32x4 *raw, float v[8]) {
   if constexpr (F32) {
@@ -90,6 +82,14 @@ __device__ __forceinline__ void values8(const glm_u32x4 *raw, float v[8]) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, y quantised.  A
+// workgroup holds its row in registers, 8 STEPS channels a thread, so that x and
+// the residual are read once; h is not rounded before the norm.  As many threads
+// as a row needs with one step each, as far as a workgroup goes.  Bound by bytes:
+// 8191 bf16 rows of 4096 (236 MB) 41 us, 5.8 TB/s; 1500 f32 rows of 2048 (40 MB) 8.7,
+// 4.6 TB/s; one row of 4096 3.4, a launch, a trip to memory and the sum.
+// ---------------------------------------------------------------------------
 struct NormArgs {
   const void *x, *residual;
   const float *weight;
