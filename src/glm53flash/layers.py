@@ -106,6 +106,9 @@ class DeferredLinear:
         if self.quantization_mode is not None:
             raise ContractError("deferred linear was already quantized")
         weight = require_weight(self.weight, "linear.weight")
+        if self.input_dims % 16:  # (the weight would be gone, and no product takes its codes)
+            raise ContractError(f"block-scaled linears take a multiple of 16 channels, not "
+                                f"{self.input_dims}")
         source_bytes = weight.numel() * weight.element_size()
         self.weight, self.scales = fp8_block.quantize_weight(weight)
         self.quantization_mode = "fp8_block"

@@ -129,6 +129,11 @@ def test_layers_keep_their_rules():
     lin = DeferredLinear(128, 32, quantize_resident=False)
     with pytest.raises(ContractError, match="excluded"):
         lin.quantize_to_fp8_block()
+    lin = DeferredLinear(24, 32)
+    lin.weight = kept = torch.zeros((32, 24), dtype=torch.bfloat16)
+    with pytest.raises(ContractError, match="multiple of 16"):
+        lin.quantize_to_fp8_block()
+    assert lin.weight is kept and lin.quantization_mode is None
     lin = DeferredLinear(128, 32)
     with pytest.raises(ContractError, match="not loaded"):
         lin.quantize_to_fp8_block()

@@ -328,6 +328,26 @@ def test_products_pass_nan_and_infinity_on(F, T):
     assert np.isnan(y[:, 5]).all() and np.isfinite(np.delete(y, 5, 1)).all()
 
 
+@pytest.mark.parametrize("T", [1, 3, 8, 16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_quantised_by_the_product_are_the_quantisers(F, T, dtype):
+    # zeros of either sign, infinities and NaN, tiny and huge groups
+    rng = np.random.default_rng(T)
+    x = rows(rng, T, 656)
+    x[0, :128] = np.where(rng.random(128) < 0.5, -0.0, 0.0)
+    x[0, 128:256] *= 1e-38
+    x[0, 256:384] *= 1e30
+    x[-1, 5], x[-1, 300], x[T // 2, 655] = np.inf, -np.inf, np.nan
+    x, w, u = gpu(x, dtype), [gpu(a) for a in weight(rng, 272, 656)], [gpu(a) for a in weight(rng, 272, 656)]
+    q = F.quantize_rows(x)
+    a, b = F.linear(x, *w).float(), F.linear(q, *w).float()
+    assert bool((a.isnan() == b.isnan()).all()) and bool(a[-1].isnan().all())
+    # the same f32 products, added up in the same order
+    assert torch.equal(a.nan_to_num(0.0), b.nan_to_num(0.0))
+    a, b = F.gate_up(x, *w, *u, 7.0), F.gate_up(q, *w, *u, 7.0)
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
 def test_shapes_of_rows(F):
     rng = np.random.default_rng(6)
     x, w = gpu(rows(rng, 6, 256), torch.bfloat16), [gpu(a) for a in weight(rng, 48, 256)]
