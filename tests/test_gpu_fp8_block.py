@@ -231,7 +231,7 @@ SHAPES = [
     (100, 256, 1000), (128, 384, 128), (129, 400, 144), (200, 4096, 300), (256, 2048, 2048), (257, 528, 515),
     (333, 1536, 640), (700, 656, 1100), (1025, 896, 2047), (2000, 512, 4096),
     # each way to cut a product, beside the above
-    (24, 272, 4096), (30, 144, 8000), (56, 400, 4100),
+    (24, 272, 4096), (30, 144, 8000), (56, 400, 4100), (24, 2064, 4096), (50, 16400, 2064),
     (140, 272, 4100), (250, 272, 4090), (370, 272, 4095), (230, 272, 6000),
     (450, 272, 4096), (620, 272, 4095), (850, 144, 4096), (1600, 144, 4096), (3000, 144, 4096), (2900, 528, 4090),
     (70, 9008, 40), (4, 9008, 40), (40, 16400, 24),
