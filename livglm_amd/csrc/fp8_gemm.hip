@@ -28,12 +28,14 @@ namespace glm {
 typedef int fp8_frag __attribute__((ext_vector_type(8)));
 
 constexpr int kExactTokens = 64;  // rows whose products are summed exactly in any case
-// Rows that the product quantises itself: up to so many, and so many codes.  (Each
-// workgroup does it for itself: at K and N 4096 1, 4 and 8 rows so take 6.6, 7.1 and
-// 8.5 us, quantised before 8.0, 8.1 and 8.2 and a launch more for the host; 16 rows of
-// K 2048 5.8 and 5.9; 8 rows of K 8192 12.1 and 10.6; the gated pair of 16 rows, K
-// 2048, 2 x 768 features 7.2 and 8.4.)
-constexpr int kFusedTokens = 16, kFusedCodes = 1 << 15;
+// Rows that the product quantises itself: up to so many, and so many codes, for so
+// many features.  (Each workgroup does it for itself: at K and N 4096 1, 4 and 8 rows
+// so take 6.6, 7.1 and 8.5 us, quantised before 8.0, 8.1 and 8.2 and a launch more for
+// the host; 16 rows of K 2048 5.8 and 5.9; 8 rows of K 8192 12.1 and 10.6; the gated
+// pair of 16 rows, K 2048, 2 x 768 features 7.2 and 8.4.  At K 2048 1 and 8 rows into
+// 8192 features 6.0 and 6.7, before 7.1 and 7.3; into 16384 11.5 and 12.1, before 10.8
+// and 11.2; into 65536 32.3 and 34.8, before 25.0 and 25.3.)
+constexpr int kFusedTokens = 16, kFusedCodes = 1 << 15, kFusedFeatures = 8192;
 
 struct Fp8Args {
   const void *x;          // codes, or bf16 / f32 rows
@@ -848,16 +850,16 @@ static int launch_stream(hipStream_t stream, Fp8Args a, int splits = 1) {
 }
 
 // Workspace of rows that the product does not take as they are.
-static size_t rows_bytes(int T, int K, int type) {
+static size_t rows_bytes(int T, int K, int N, int type) {
   const long long codes = (long long)T * fp8_groups(K) * kFp8Group;
-  if (type == GLM_ROWS_FP8 || (T <= kFusedTokens && codes <= kFusedCodes)) return 0;
+  if (type == GLM_ROWS_FP8 || (T <= kFusedTokens && codes <= kFusedCodes && N <= kFusedFeatures)) return 0;
   return round256((size_t)T * K) + round256((size_t)T * fp8_groups(K) * 4);
 }
 
 // Rows as the kernels take them: few as they are, more of them quantised into
 // the workspace first.
 static int rows_for(hipStream_t stream, Fp8Args &a, int &type, uint8_t *&ws) {
-  if (!rows_bytes(a.T, a.K, type)) return GLM_OK;
+  if (!rows_bytes(a.T, a.K, a.N, type)) return GLM_OK;
   uint8_t *codes = ws;
   ws += round256((size_t)a.T * a.K);
   float *scales = reinterpret_cast<float *>(ws);
@@ -1021,7 +1023,7 @@ static int gated_product(hipStream_t stream, const Fp8Args &a, int type) {
 // The pair's f32 sums, where a second launch gates them.  Rows that the workspace
 // holds as codes are coded for the plan.
 static size_t gated_bytes(int T, int K, int N, int type) {
-  const GatedPlan plan = gated_plan(T, K, N, rows_bytes(T, K, type) ? GLM_ROWS_FP8 : type);
+  const GatedPlan plan = gated_plan(T, K, N, rows_bytes(T, K, N, type) ? GLM_ROWS_FP8 : type);
   return plan.cut < kGatedStreams ? round256((size_t)plan.splits * 2 * T * N * 4) : 0;
 }
 
@@ -1047,7 +1049,7 @@ static int check_product(const char *name, const void *x, int x_type, const floa
 
 extern "C" size_t glm_fp8_workspace_bytes(int x_type, int T, int K, int N, int gated) {
   if (!sizes_fit(T, K, N) || x_type < GLM_ROWS_BF16 || x_type > GLM_ROWS_FP8) return 0;
-  return rows_bytes(T, K, x_type) + (gated && T > 0 ? gated_bytes(T, K, N, x_type) : 0);
+  return rows_bytes(T, K, N, x_type) + (gated && T > 0 ? gated_bytes(T, K, N, x_type) : 0);
 }
 
 extern "C" int glm_fp8_linear(void *stream, const void *x, int x_type, const float *x_scales, int T,

@@ -237,7 +237,7 @@ SHAPES = [
     (70, 9008, 40), (4, 9008, 40), (40, 16400, 24),
     # the longest rows that a workgroup quantises, longer ones, the longest
     (2, 16384, 40), (8, 4096, 40), (7, 4112, 33), (1, 32784, 24), (6, 1040, 4100), (16, 2048, 70), (13, 2064, 40),
-    (11, 400, 4100), (2, 1 << 20, 20), (66, 1 << 17, 33),
+    (11, 400, 4100), (5, 272, 8192), (5, 272, 8200), (2, 1 << 20, 20), (66, 1 << 17, 33),
 ]
 
 
@@ -269,7 +269,7 @@ GATED = [(1, 128, 16), (2, 2048, 768), (5, 144, 144), (16, 1408, 240), (17, 272,
          (65, 528, 400), (129, 512, 256), (256, 1024, 1408), (333, 656, 272), (1030, 384, 768), (2000, 512, 2048), (100, 272, 1024),
          (333, 272, 1408), (150, 1040, 2048), (96, 272, 2048),
          (500, 4112, 2048), (3000, 400, 2048), (2950, 272, 2032), (70, 9008, 48), (3, 9008, 48),
-         (2, 16384, 48), (8, 4096, 1040), (16, 2048, 272), (11, 400, 1040), (3, 16400, 32), (7, 4112, 48)]
+         (2, 16384, 48), (8, 4096, 1040), (16, 2048, 272), (11, 400, 1040), (5, 144, 8208), (3, 16400, 32), (7, 4112, 48)]
 
 
 @pytest.mark.parametrize("T, K, N", GATED)
