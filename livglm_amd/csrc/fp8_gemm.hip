@@ -930,8 +930,8 @@ static bool few(int T, int type) { return type != GLM_ROWS_FP8 || T <= 8; }
 // each other but read all operands of their tile, or in larger tiles.  At N 4096,
 // K 4096, us by tile: 64 rows 16 x 32 9.6, 32 x 32 8.5, 16 x 64 9.0; 80 rows 32 x 48
 // 8.1, 64 x 32 8.8, 256 x 256 46.8; 600 rows 64 x 48 26.7, tiles of 64 x 64 22.9;
-// 1600 rows 54.2, 52.8, 256 x 128 36.1, 256 x 256 49.5; 4096 rows 124.6, 151.3, 81.6,
-// 61.9.  A workgroup a CU has all its LDS: five or six waves there, each with a group
+// 1024 rows 128 x 128 24.5, 64 x 64 34.0; 1600 rows 64 x 48 54.2, 64 x 64 52.8, 256 x
+// 128 36.1, 256 x 256 49.5; 4096 rows 124.6, 151.3, 79.5, 61.9.  A workgroup a CU has all its LDS: five or six waves there, each with a group
 // in flight: 150 rows 64 x 48 of four waves 11.3, six 9.8; 256 rows 64 x 64 of six 11.9,
 // eight 11.9, the tile 15.1; 333 rows 64 x 96 of four 15.8, five 15.0, six 15.5, 64 x 48 of
 // four 16.2; but 512 rows 64 x 64 of six 20.8, the tile 18.5.
@@ -947,14 +947,14 @@ static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
     }
   }
   static const Fp8Cut cuts[] = {{32, 48, 30, 52},  {64, 32, 40, 46},   {64, 48, 45, 62}, {64, 64, 90, 54},
-                                {128, 64, 105, 93}, {256, 128, 10, 330}, {256, 256, 0, 500},
+                                {128, 128, 25, 227}, {256, 128, 10, 331}, {256, 256, 0, 500},
                                 {64, 48, 28, 70}, {64, 64, 30, 87}, {64, 96, 36, 113}};
   switch (cheapest(cuts, a.T, a.N, 32)) {
     case 0: return launch_stream<CodedStream<8, 1, 2, 3, true>>(stream, a);
     case 1: return launch_stream<CodedStream<4, 1, 4, 2, true>>(stream, a);
     case 2: return launch_stream<CodedStream<4, 1, 4, 3, true>>(stream, a);
     case 3: return launch_tile<1, Fp8Tile<2, 2, 2, 2, 52>>(stream, a);
-    case 4: return launch_tile<1, Fp8Tile<2, 2, 4, 2, 79>>(stream, a);
+    case 4: return launch_tile<1, Fp8Tile<2, 4, 4, 2>>(stream, a);
     case 5: return launch_tile<1, Fp8Tile<2, 4, 8, 2>>(stream, a);
     case 6: return launch_tile<1, Fp8Tile<2, 4, 8, 4>>(stream, a);
     case 7: return launch_stream<CodedStream<6, 1, 4, 3, true>>(stream, a);

@@ -233,7 +233,8 @@ SHAPES = [
     # each way to cut a product, beside the above
     (24, 272, 4096), (30, 144, 8000), (56, 400, 4100), (24, 2064, 4096), (50, 16400, 2064),
     (140, 272, 4100), (250, 272, 4090), (370, 272, 4095), (230, 272, 6000),
-    (450, 272, 4096), (620, 272, 4095), (850, 144, 4096), (1600, 144, 4096), (3000, 144, 4096), (2900, 528, 4090),
+    (450, 272, 4096), (620, 272, 4095), (850, 144, 4096), (900, 1040, 4090), (1600, 144, 4096),
+    (3000, 144, 4096), (2900, 528, 4090),
     (70, 9008, 40), (4, 9008, 40), (40, 16400, 24),
     # the longest rows that a workgroup quantises, longer ones, the longest
     (2, 16384, 40), (8, 4096, 40), (7, 4112, 33), (1, 32784, 24), (6, 1040, 4100), (16, 2048, 70), (13, 2064, 40),
