@@ -893,7 +893,8 @@ static int launch_tile(hipStream_t stream, const Fp8Args &p) {
 // tenths of a us at K 4096, base + each for every 256 workgroups begun (one a CU);
 // `groups` where the second part alone goes by K.  Over 9 pairs of K from 1024 to
 // 16384 and N from 1024 to 8192, 12 to 6000 rows, what the costs choose takes 0.5 %
-// more than the fastest cut on average, 24 % at most (72 rows, K 16384, N 4096).
+// more than the fastest cut on average, 26 % at most (72 rows, K 16384, N 4096); of
+// the gated pair's 5 % at most.
 struct Fp8Cut {
   int feat, tok, base, each;
   long long workgroups(int T, int N) const {
@@ -966,12 +967,14 @@ static int linear_product(hipStream_t stream, const Fp8Args &a, int type) {
 // Gated pairs: streamed, their sums gated by a second launch, or in tiles that gate
 // and quantise by themselves.  At 2 x 2048 features, K 4096, us by tile (streamed
 // ones without the second launch's 2.5 us and more): 64 rows 16 x 16 9.7, 16 x 32 8.7,
-// 16 x 48 9.2; 333 rows 32 x 32 21.7, 32 x 48 19.0, 32 x 64 23.2, 128 x 128 60.8,
-// 128 x 256 100; 850 rows 42.7, 41.6, 41.5, 61.9, 101; 1600 rows 74.9, 72.3, 67.9,
-// 64.5, 103; 3000 rows 134.6, 126.4, 118.8, 121.4, 104.
+// 16 x 48 9.2; 333 rows 32 x 32 21.7, 32 x 48 19.0, 32 x 64 21.4, 128 x 64 38.9, 128 x 128
+// 60.9; 1000 rows 32 x 48 51.4, 32 x 64 46.7, 128 x 64 44.4, 128 x 128 64.5, 128 x 256 101;
+// 1500 rows 71.5, 65.8, 75.8, 64.7, 101; 3000 rows 128 x 128 121, 128 x 256 104.  256 rows
+// of K 2048 into 2 x 7168: 32 x 64 and its second launch take 1.4 times 128 x 64.
 constexpr Fp8Cut kGatedCuts[] = {{16, 16, 44, 26}, {16, 32, 50, 35}, {16, 48, 30, 62},   {32, 32, 55, 52},
-                                 {32, 48, 60, 71}, {32, 64, 60, 84}, {128, 128, 0, 580}, {128, 256, 0, 870}};
-constexpr int kGatedStreams = 6, kGatedWays = 8;
+                                 {32, 48, 60, 71}, {32, 64, 60, 84}, {128, 64, 30, 380}, {128, 128, 0, 520},
+                                 {128, 256, 0, 865}};
+constexpr int kGatedStreams = 6, kGatedWays = 9;
 struct GatedPlan {
   int cut, splits;  // of K, where the workgroups are fewer than the CUs: as many as leave every wave a group
 };
@@ -1008,7 +1011,8 @@ static int gated_product(hipStream_t stream, const Fp8Args &a, int type) {
       case 3: rc = launch_stream<CodedStream<4, 2, 2, 2>>(stream, a, splits); break;
       case 4: rc = launch_stream<CodedStream<4, 2, 2, 3>>(stream, a, splits); break;
       case 5: rc = launch_stream<CodedStream<4, 2, 2, 4>>(stream, a, splits); break;
-      case 6: return launch_tile<2, Fp8Tile<2, 4, 8, 2>>(stream, a);
+      case 6: return launch_tile<2, Fp8Tile<4, 2, 4, 2>>(stream, a);
+      case 7: return launch_tile<2, Fp8Tile<2, 4, 8, 2>>(stream, a);
       default: return launch_tile<2, Fp8Tile<2, 4, 8, 4>>(stream, a);
     }
   }

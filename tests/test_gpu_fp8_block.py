@@ -268,7 +268,8 @@ def test_linear(F, T, K, N, kind):
 
 GATED = [(1, 128, 16), (2, 2048, 768), (5, 144, 144), (16, 1408, 240), (17, 272, 128), (48, 2048, 512), (64, 4096, 2048),
          (65, 528, 400), (129, 512, 256), (256, 1024, 1408), (333, 656, 272), (1030, 384, 768), (2000, 512, 2048), (100, 272, 1024),
-         (333, 272, 1408), (150, 1040, 2048), (96, 272, 2048),
+         (333, 272, 1408), (150, 1040, 2048), (96, 272, 2048), (120, 528, 2032),
+         (700, 528, 2032), (250, 272, 7168),
          (500, 4112, 2048), (3000, 400, 2048), (2950, 272, 2032), (70, 9008, 48), (3, 9008, 48),
          (2, 16384, 48), (8, 4096, 1040), (16, 2048, 272), (11, 400, 1040), (5, 144, 8208), (3, 16400, 32), (7, 4112, 48)]
 
