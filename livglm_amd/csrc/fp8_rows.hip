@@ -5,8 +5,6 @@
 #include "fp8_rows.h"
 #include "lds_stage.h"
 
-#include <climits>
-
 namespace glm {
 
 constexpr int kRowsThreads = 256;
