@@ -18,6 +18,7 @@
 // values, without a bias.  The latter serves products whose result is rounded
 // to bf16 (1.7e-3) and whose time the matrix cores set.
 #include "fp8_rows.h"
+#include "fp8_span.h"
 #include "lds_stage.h"
 #include "mfma_tile.h"
 
@@ -464,8 +465,9 @@ __global__ __launch_bounds__(256) void fp8_gate_kernel(const float *h, int split
 // operands come into LDS a group of K at a time by direct loads of 16-byte
 // pieces, a ring of groups deep.  Piece p of
 // row R lies at p ^ ((R >> 1) & 7): the 16 rows that a quarter of a wave reads
-// are then on 16 different pieces of 256 bytes.  Rows past the last and pieces
-// past K are out of the buffers' range, which gives zeros.
+// are then on 16 different pieces of 256 bytes.  Pieces past K are out of the
+// buffers' range, which gives zeros; rows past the last are that or the tile's
+// first once more (fp8_span.h), and their sums are not stored.
 //
 // The largest tile is 256 x 256 (the pair: 2 x 128 x 256): 64 KB a group of K, two
 // groups in LDS, 128 of 256 registers hold sums.  4096 rows, K and N 4096: 58 to 63
@@ -542,7 +544,8 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
   constexpr int kStep = 8 * kWaves;  // rows of a load
   static_assert(kStep % 16 == 0 && kFeat % kStep == 0, "the same order of pieces, one projection");
   auto rows_from = [&](const uint8_t *rows, int first, int there) {
-    return make_rsrc(rows + (long long)first * K, (uint32_t)max(there - first, 0) * (uint32_t)K);
+    const Fp8Span span = fp8_span(first, there);
+    return make_rsrc(rows + (long long)span.first * K, (uint32_t)span.rows * (uint32_t)K);
   };
   __amdgpu_buffer_rsrc_t res[L::kLoads];
 #pragma unroll
@@ -579,7 +582,7 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        buf4_to_lds(sres, to + j * L::kTok + wave * 64, off, (uint32_t)(g + j) * 4);
+        buf4_to_lds(sres, to + j * L::kTok + wave * 64, off, (uint32_t)fp8_scale_group(g, j, groups) * 4);
     }
   };
 
