@@ -56,7 +56,7 @@ class DeferredLinear:
         if self.bias is not False:
             raise ContractError("biased deferred linears are not part of the MoE path")
         if self.quantization_mode == "fp8_block":
-            return fp8_block.linear(x, weight, require_weight(self.scales, "linear.scales"))
+            return fp8_block.linear(x, *self.block_scaled_weight("linear"))
         N.require_device(x, "x", (torch.bfloat16,))
         if x.shape[-1] != self.input_dims:
             raise ContractError(f"linear input width {x.shape[-1]} != {self.input_dims}")
@@ -68,6 +68,18 @@ class DeferredLinear:
         N.call("glm_linear", N.stream_of(x), rows.data_ptr(), rows.shape[0], self.input_dims,
                weight.data_ptr(), N.ptr(scales), self.fmt, self.output_dims, out.data_ptr())
         return out.reshape(*x.shape[:-1], self.output_dims)
+
+    def block_scaled_weight(self, name: str) -> tuple[torch.Tensor, torch.Tensor]:
+        """The codes and scales of mode "fp8_block".  A weight of another shape
+        than the layer's is refused: what follows relies on the output's width."""
+        weight = require_weight(self.weight, f"{name}.weight")
+        self._require_shape(weight, name)
+        return weight, require_weight(self.scales, f"{name}.scales")
+
+    def _require_shape(self, weight: torch.Tensor, name: str) -> None:
+        if weight.shape != (self.output_dims, self.input_dims):
+            raise ContractError(f"{name}.weight {tuple(weight.shape)}, the layer is "
+                                f"{(self.output_dims, self.input_dims)}")
 
     def quantize_to_mxfp(self, bits: int, rule: int = N.MX_RULE_NEAREST) -> tuple[int, int]:
         """Startup conversion to group-32 MXFP8/MXFP4 (``layers.py:72-99``).
@@ -106,6 +118,7 @@ class DeferredLinear:
         if self.quantization_mode is not None:
             raise ContractError("deferred linear was already quantized")
         weight = require_weight(self.weight, "linear.weight")
+        self._require_shape(weight, "linear")
         if self.input_dims % 16:  # (the weight would be gone, and no product takes its codes)
             raise ContractError(f"block-scaled linears take a multiple of 16 channels, not "
                                 f"{self.input_dims}")
@@ -148,13 +161,11 @@ class DenseMLP:
                    for p in (self.gate_proj, self.up_proj, self.down_proj))
 
     def _block_scaled(self, x) -> torch.Tensor:
-        g, u, d = self.gate_proj, self.up_proj, self.down_proj
-        h = fp8_block.gate_up(x, require_weight(g.weight, "gate_proj.weight"),
-                              require_weight(g.scales, "gate_proj.scales"),
-                              require_weight(u.weight, "up_proj.weight"),
-                              require_weight(u.scales, "up_proj.scales"), self.swiglu_limit)
-        return fp8_block.linear(h, require_weight(d.weight, "down_proj.weight"),
-                                require_weight(d.scales, "down_proj.scales"))
+        gate, gate_scales = self.gate_proj.block_scaled_weight("gate_proj")
+        up, up_scales = self.up_proj.block_scaled_weight("up_proj")
+        down, down_scales = self.down_proj.block_scaled_weight("down_proj")
+        h = fp8_block.gate_up(x, gate, gate_scales, up, up_scales, self.swiglu_limit)
+        return fp8_block.linear(h, down, down_scales)
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         if self.block_scaled:

@@ -141,6 +141,8 @@ class ExpertSSDMoE:
                            N.ptr(shared.up_proj.scales), sd.data_ptr(),
                            N.ptr(shared.down_proj.scales), None)
         else:
+            if ready.shape != (T, d):  # (the library takes it as that)
+                raise ContractError(f"shared expert output {tuple(ready.shape)}, expected {(T, d)}")
             shared_args = (0, N.FMT_BF16, None, None, None, None, None, None, ready.data_ptr())
         k = cfg.num_experts_per_tok
         out = torch.empty((T, d), dtype=torch.float32, device=dev)
