@@ -748,7 +748,7 @@ int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_stride, int B
 #define GLM_ROWS_F32 1  /* f32 [T][K] */
 #define GLM_ROWS_FP8 2  /* codes and scales as above */
 
-/* Rows x (bf16 or f32) to codes and scales.  Limits: K % 8 == 0. */
+/* Rows x (bf16 or f32) to codes and scales.  Limits: K % 8 == 0, K <= 2^31 - 128. */
 int glm_fp8_quantize_rows(void *stream, const void *x, int x_type, int T, int K, uint8_t *codes,
                           float *scales);
 

@@ -188,7 +188,8 @@ extern "C" int glm_fp8_quantize_rows(void *stream, const void *x, int x_type, in
   glm::clear_error();
   GLM_REQUIRE(T >= 0 && K >= 1 && row_type(x_type), GLM_ERR_INVALID_ARGUMENT,
               "fp8_quantize_rows: invalid sizes or row type");
-  GLM_REQUIRE(K % 8 == 0, GLM_ERR_UNSUPPORTED_SHAPE, "fp8_quantize_rows: K %% 8 != 0 (K = %d)", K);
+  GLM_REQUIRE(K % 8 == 0 && K <= INT32_MAX - (kFp8Group - 1), GLM_ERR_UNSUPPORTED_SHAPE,
+              "fp8_quantize_rows: K = %d (a multiple of 8, whole groups of 128 below 2^31)", K);
   GLM_REQUIRE(x && codes && scales, GLM_ERR_INVALID_ARGUMENT, "fp8_quantize_rows: null pointer");
   GLM_REQUIRE(glm_aligned16({x, codes, scales}), GLM_ERR_INVALID_ARGUMENT,
               "fp8_quantize_rows: buffers must be 16-byte aligned");
