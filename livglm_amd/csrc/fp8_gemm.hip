@@ -123,8 +123,8 @@ __device__ __forceinline__ void wait_groups_ahead(int ahead) {
 // workgroup has 16 RB weight rows (of each projection); its four to eight waves take
 // the groups of K in turn, each through LDS of its own, and add up their f32
 // results at the end: no wave waits for another before that.  Gated pairs of
-// few row tiles are split along K too (blockIdx.z); what reads their sums joins
-// them.
+// few row tiles and at most 16 tokens a workgroup are split along K too (blockIdx.z);
+// what reads their sums joins them.
 //
 // Operands come by direct loads, 16 bytes a lane, whose lanes walk along a
 // row: an operand's own lanes lie in 16 rows, and loads into registers took 64
@@ -984,7 +984,9 @@ constexpr Fp8Cut kGatedCuts[] = {{16, 16, 44, 26}, {16, 32, 50, 35}, {16, 48, 30
                                  {128, 256, 0, 865}};
 constexpr int kGatedStreams = 6, kGatedWays = 9;
 struct GatedPlan {
-  int cut, splits;  // of K, where the workgroups are fewer than the CUs: as many as leave every wave a group
+  // splits of K, of the first cut where its workgroups are at most half the CUs: as many as leave
+  // every wave a group
+  int cut, splits;
 };
 static GatedPlan gated_plan(int T, int K, int N, int type) {
   GatedPlan plan{0, 1};
@@ -997,9 +999,11 @@ static GatedPlan gated_plan(int T, int K, int N, int type) {
       best = c;
     }
   }
-  if (plan.cut >= kGatedStreams) return plan;
-  const int waves = plan.cut < 3 ? 8 : 4, most = fp8_groups(K) / waves;
-  long long s = 256 / kGatedCuts[plan.cut].workgroups(T, N);
+  // (a larger cut costs less only where the one before it takes two rounds of 256 workgroups,
+  // and so has more than 128 itself: none of them has CUs to spare for splits)
+  if (plan.cut != 0) return plan;
+  const int most = fp8_groups(K) / 8;  // eight waves
+  long long s = 256 / kGatedCuts[0].workgroups(T, N);
   s = s < most ? s : most;
   plan.splits = s < 1 ? 1 : s < 8 ? (int)s : 8;
   return plan;
@@ -1014,11 +1018,11 @@ static int gated_product(hipStream_t stream, const Fp8Args &a, int type) {
   } else {
     switch (plan.cut) {
       case 0: rc = launch_stream<CodedStream<8, 2, 1, 1>>(stream, a, splits); break;
-      case 1: rc = launch_stream<CodedStream<8, 2, 1, 2>>(stream, a, splits); break;
-      case 2: rc = launch_stream<CodedStream<8, 2, 1, 3>>(stream, a, splits); break;
-      case 3: rc = launch_stream<CodedStream<4, 2, 2, 2>>(stream, a, splits); break;
-      case 4: rc = launch_stream<CodedStream<4, 2, 2, 3>>(stream, a, splits); break;
-      case 5: rc = launch_stream<CodedStream<4, 2, 2, 4>>(stream, a, splits); break;
+      case 1: rc = launch_stream<CodedStream<8, 2, 1, 2>>(stream, a); break;
+      case 2: rc = launch_stream<CodedStream<8, 2, 1, 3>>(stream, a); break;
+      case 3: rc = launch_stream<CodedStream<4, 2, 2, 2>>(stream, a); break;
+      case 4: rc = launch_stream<CodedStream<4, 2, 2, 3>>(stream, a); break;
+      case 5: rc = launch_stream<CodedStream<4, 2, 2, 4>>(stream, a); break;
       case 6: return launch_tile<2, Fp8Tile<4, 2, 4, 2>>(stream, a);
       case 7: return launch_tile<2, Fp8Tile<2, 4, 8, 2>>(stream, a);
       default: return launch_tile<2, Fp8Tile<2, 4, 8, 4>>(stream, a);
