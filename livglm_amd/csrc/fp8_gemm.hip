@@ -655,7 +655,7 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
       for (int p = NPROJ - 1; p >= 0; --p) s[p][t] = s[0][t] * wsc[p];
     side();
     now = Fp8Operand<FAST>(w[1]);
-    if (kAhead < BN) w[kAhead] = wfrag(kAhead);
+    if constexpr (kAhead < BN) w[kAhead] = wfrag(kAhead);
 #pragma unroll
     for (int b = 1; b <= BN; ++b) {
       Fp8Operand<FAST> next = now;
