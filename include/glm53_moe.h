@@ -741,8 +741,11 @@ int glm_paged_attention(void *stream, const uint16_t *q, int64_t q_stride, int B
  * finite magnitude of the group or block (448 2^-126 at least):
  *   scale = amax / 448,  code = e4m3(value * (448 / amax)), nearest even,
  * all in f32; an infinity or a NaN becomes E4M3's NaN.  Scales that a caller
- * brings may be any f32.  Every buffer is 16-byte aligned; outputs overlap no
- * input except where said.
+ * brings may be any f32 as long as a row's times a block's is a normal one: the
+ * two are multiplied first, in f32, and then meet the group's sum.  Past f32's
+ * range the row gets infinities or NaN there, of a group that sums to 0 too;
+ * below 2^-126 bits are lost.  Every buffer is 16-byte aligned; outputs overlap
+ * no input except where said.
  */
 #define GLM_ROWS_BF16 0 /* bf16 [T][K] */
 #define GLM_ROWS_F32 1  /* f32 [T][K] */

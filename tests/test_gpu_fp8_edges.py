@@ -124,3 +124,24 @@ def test_the_exact_cases_tell_the_sums_apart(F, T):
     many = F.linear(rows, gpu(P.encode(w)), ws)
     few = F.linear(F.Fp8Rows(rows.codes[:T].contiguous(), rows.scales[:T].contiguous()), gpu(P.encode(w)), ws)
     assert (many[:T] != few).float().mean() > 0.5
+
+
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_scales_of_products_near_the_ends_of_f32(F, T):
+    # a row's scale times a block's is formed in f32, before it meets the group's sum: within its range
+    # a zero group stays zero and a sum is right; a row whose product is infinite is no number, and alone so
+    K, N = 400, 48
+    rng = np.random.default_rng(T)
+    codes, w = P.encode(rng.integers(-8, 9, (T, K)).astype(np.float32)), P.encode(rng.integers(-8, 9, (N, K)).astype(np.float32))
+    codes[:, 128:256] = 0
+    xs = np.ones((T, 4), np.float32)
+    ws = np.ones((1, 4), np.float32)
+    ws[0, 1:3] = 2.0 ** 60, 2.0 ** -60
+    xs[:, 1:3] = 2.0 ** 67, 2.0 ** 62  # products of 2^127 and 4
+    xs[1, 1] = 2.0 ** 68               # 2^128
+    got = F.linear(F.Fp8Rows(gpu(codes), gpu(xs)), gpu(w), gpu(ws)).float().cpu().numpy()
+    assert np.isnan(got[1]).all()
+    x, one = P.decode(codes), P.decode(w)
+    want = x[:, :128] @ one[:, :128].T + 4 * (x[:, 256:384] @ one[:, 256:384].T) + x[:, 384:] @ one[:, 384:].T
+    rest = np.arange(T) != 1
+    assert np.array_equal(got[rest], torch.from_numpy(want[rest].astype(np.float32)).bfloat16().float().numpy())
