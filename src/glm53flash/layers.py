@@ -168,10 +168,10 @@ class DenseMLP:
         return fp8_block.linear(h, down, down_scales)
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
-        if self.block_scaled:
-            return self._block_scaled(x)
         fmt = self.fused_format()
         if fmt is None:
+            if self.block_scaled:
+                return self._block_scaled(x)
             return self.down_proj(limited_swiglu(self.gate_proj(x), self.up_proj(x),
                                                  self.swiglu_limit))
         N.require_device(x, "x", (torch.bfloat16,))

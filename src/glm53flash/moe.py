@@ -127,23 +127,22 @@ class ExpertSSDMoE:
         bank = self.experts
         bank._require_active()
         shared = self.shared_experts
-        # a block-scaled shared expert runs first, by itself; the layer adds its output
-        ready = shared(rows) if shared.block_scaled else None
-        if ready is None:
-            fmt = shared.fused_format()
-            if fmt is None:
-                raise ContractError("shared expert projections must share one storage format")
-            sg, su, sd = (require_weight(p.weight, f"shared {name}.weight") for name, p in (
-                ("gate_proj", shared.gate_proj), ("up_proj", shared.up_proj),
-                ("down_proj", shared.down_proj)))
+        fmt = shared.fused_format()
+        if fmt is not None:
+            sg = require_weight(shared.gate_proj.weight, "shared gate_proj.weight")
+            su = require_weight(shared.up_proj.weight, "shared up_proj.weight")
+            sd = require_weight(shared.down_proj.weight, "shared down_proj.weight")
             shared_args = (shared.intermediate_size, fmt, sg.data_ptr(),
                            N.ptr(shared.gate_proj.scales), su.data_ptr(),
                            N.ptr(shared.up_proj.scales), sd.data_ptr(),
                            N.ptr(shared.down_proj.scales), None)
-        else:
+        elif shared.block_scaled:  # runs first, by itself; the layer adds its output
+            ready = shared(rows)
             if ready.shape != (T, d):  # (the library takes it as that)
                 raise ContractError(f"shared expert output {tuple(ready.shape)}, expected {(T, d)}")
             shared_args = (0, N.FMT_BF16, None, None, None, None, None, None, ready.data_ptr())
+        else:
+            raise ContractError("shared expert projections must share one storage format")
         k = cfg.num_experts_per_tok
         out = torch.empty((T, d), dtype=torch.float32, device=dev)
         weights = torch.empty((T, k), dtype=torch.float32, device=dev)

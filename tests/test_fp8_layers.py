@@ -109,3 +109,16 @@ def test_a_shared_expert_of_another_width_never_reaches_the_layer(monkeypatch, p
     layer.shared_experts = attached(256, 128)
     layer(x)
     assert launched[-1] == "glm_moe_forward"
+
+
+def test_other_formats_do_not_pay_for_this_one(monkeypatch):
+    # a bf16 shared expert's call asks for its format once, as it did before there was a block-scaled mode
+    layer, launched = moe_on_the_cpu(monkeypatch)
+    for p in (layer.shared_experts.gate_proj, layer.shared_experts.up_proj, layer.shared_experts.down_proj):
+        p.weight = torch.zeros((p.output_dims, p.input_dims), dtype=torch.bfloat16)
+    monkeypatch.setattr(DenseMLP, "block_scaled", property(lambda self: pytest.fail("asked for")))
+    x = torch.zeros((3, 256), dtype=torch.bfloat16)
+    layer(x)
+    assert launched[-1] == "glm_moe_forward"
+    layer.shared_experts(x)
+    assert launched[-1] == "glm_dense_mlp"
