@@ -145,3 +145,53 @@ def test_scales_of_products_near_the_ends_of_f32(F, T):
     want = x[:, :128] @ one[:, :128].T + 4 * (x[:, 256:384] @ one[:, 256:384].T) + x[:, 384:] @ one[:, 384:].T
     rest = np.arange(T) != 1
     assert np.array_equal(got[rest], torch.from_numpy(want[rest].astype(np.float32)).bfloat16().float().numpy())
+
+
+@pytest.fixture(scope="module")
+def layer():
+    # the MoE layer with a block-scaled shared expert
+    import gpu_util as gu
+    from livglm_amd.workloads import SHAPES, make_layer
+    from test_gpu_mirror import _moe
+    shape = SHAPES["verify_t2"]
+    moe, _ = _moe(gu, shape, make_layer(shape, 7500))
+    s = moe.shared_experts
+    for p in (s.gate_proj, s.up_proj, s.down_proj):
+        p.quantize_to_fp8_block()
+    return moe, shape.d
+
+
+@pytest.mark.parametrize("T", [1, 5, 64, 300, 1100])
+def test_a_block_scaled_shared_expert_at_every_number_of_tokens(F, layer, T):
+    # few tokens, decode, the grouped products streamed and wide: each adds the ready output, the last of the f32 sum
+    moe, d = layer
+    x = gpu(np.random.default_rng(T).normal(0, 1, (T, d)).astype(np.float32), torch.bfloat16)
+    shared = moe.shared_experts(x)
+    out = moe(x)
+    scales = moe.shared_experts.down_proj.scales
+    moe.shared_experts.down_proj.scales = torch.zeros_like(scales)
+    rest = moe(x)
+    moe.shared_experts.down_proj.scales = scales
+    assert float(shared.float().abs().max()) > 0
+    assert bool(((out - (rest + shared.float())).abs() <= 2.0 ** -22 * (rest.abs() + shared.float().abs())).all())
+
+
+@pytest.mark.parametrize("T", [2, 64])
+def test_a_layer_with_a_block_scaled_shared_expert_in_a_graph(F, layer, T):
+    moe, d = layer
+    rng = np.random.default_rng(T)
+    x = gpu(rng.normal(0, 1, (T, d)).astype(np.float32), torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        moe(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = moe(x)
+    for _ in range(3):
+        x.copy_(gpu(rng.normal(0, 1, (T, d)).astype(np.float32), torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        again = got.clone()
+        assert torch.equal(moe(x), again)
