@@ -11,12 +11,11 @@
 // lane (r, q) holds weight rows 4q .. 4q + 3 for token r.
 //
 // Two forms of the inner sum.  As bf16 (every code is one, exactly) in four
-// v_mfma_f32_16x16x32_bf16: exact products, f32 sums (1e-8 relative error on
-// normal values).  As it is in one v_mfma_f32_16x16x128_f8f6f4, at twice the
-// rate: the core aligns eight products at a time to the largest of them and
-// drops what lies 2^-13 of it below, which is 1.5e-5 of the sum on normal
-// values, without a bias.  The latter serves products whose result is rounded
-// to bf16 (1.7e-3) and whose time the matrix cores set.
+// v_mfma_f32_16x16x32_bf16: exact products, f32 sums.  As it is in one
+// v_mfma_f32_16x16x128_f8f6f4, at twice the rate: the core aligns eight products
+// at a time to the largest of them and drops what lies 2^-13 of it below, which is
+// 1.5e-5 of the sum on normal values, without a bias.  The latter serves products
+// whose result is rounded to bf16 (1.7e-3) and whose time the matrix cores set.
 #include "fp8_rows.h"
 #include "fp8_span.h"
 #include "lds_stage.h"
@@ -474,7 +473,7 @@ __global__ __launch_bounds__(256) void fp8_gate_kernel(const float *h, int split
 // us, 2.2 to 2.35 PFLOP/s where a library's product of plain 8-bit matrices has
 // 2.8; 8192 rows, K and N 8192: 463 us, 2.37; the pair, 4001 rows, K 4096, 2 x 2048
 // features: 104 to 111 us, 1.25 where a bf16 one has 1.45.  Matrix cores are busy for
-// 56 to 58 % of the cycles, at a clock that power limits: without the loads 68.6 us
+// 55 to 59 % of the cycles, at a clock that power limits: without the loads 68.6 us
 // are 62.6, and without the conversions the pair takes longer.
 // ---------------------------------------------------------------------------
 constexpr int kTileXcds = 8;
@@ -734,7 +733,9 @@ __global__ __launch_bounds__(L::kThreads) void fp8_tile_kernel(Fp8TileArgs a) {
 
   const int fw = f0 + wn * HB * 16, tw = t0 + wt * BT * 16;  // the wave's first feature and token
   if constexpr (NPROJ == 1) {
-    if (N % 8 != 0) {  // rows of no 16-byte pieces: element by element
+    // rows of no 16-byte pieces: element by element (K 4096, N 4095 for 4096: 333 rows 16.5 us for
+    // 16.1, 1024 31.4 for 26.9, 4096 84.8 for 66.2)
+    if (N % 8 != 0) {
 #pragma unroll
       for (int b = 0; b < BN; ++b)
 #pragma unroll
@@ -900,9 +901,10 @@ static int launch_tile(hipStream_t stream, const Fp8Args &p) {
 // A way to cut a product: features and tokens of a workgroup, and its time in
 // tenths of a us at K 4096, base + each for every 256 workgroups begun (one a CU);
 // `groups` where the second part alone goes by K.  Over 9 pairs of K from 1024 to
-// 16384 and N from 1024 to 8192, 12 to 6000 rows, what the costs choose takes 0.5 %
-// more than the fastest cut on average, 26 % at most (72 rows, K 16384, N 4096); of
-// the gated pair's 5 % at most.
+// 16384 and N from 1024 to 8192, 12 to 6000 rows, each cut timed by a build that took
+// it as an argument, what the costs choose took 0.5 % more than the fastest on
+// average, 26 % at most (72 rows, K 16384, N 4096: above 64 rows the choice leaves K
+// out); of the gated pair's 5 % at most.
 struct Fp8Cut {
   int feat, tok, base, each;
   long long workgroups(int T, int N) const {

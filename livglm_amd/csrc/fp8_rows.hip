@@ -37,7 +37,8 @@ __global__ __launch_bounds__(kRowsThreads) void fp8_quantize_rows_kernel(
 
 // ---------------------------------------------------------------------------
 // Weights: a workgroup holds one 128 x 128 block, 64 values a thread, so that the
-// block is read once.  Done once, when a weight is loaded.
+// block is read once.  Done once, when a weight is loaded.  Bound by bytes: 8192 x
+// 8192 (201 MB) 43.0 us, 4.7 TB/s; 4096 x 4096 11.9, 4.2; 768 x 2048, 96 workgroups, 4.8.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kRowsThreads) void fp8_quantize_weight_kernel(
     const uint16_t *w, int N, int K, uint8_t *codes, float *scales) {

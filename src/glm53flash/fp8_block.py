@@ -18,8 +18,9 @@ Codes are u8 (a ``torch.float8_e4m3fn`` tensor is taken as its bytes): rows
 ``[..., K]`` with scales ``[..., ceil(K / 128)]``, weights ``[N, K]`` with
 scales ``[ceil(N / 128), ceil(K / 128)]``.  A row's scale times a block's is
 formed first, in f32: where that product is not finite, the row gets infinities
-or NaN, and below 2^-126 it loses bits.  Outputs that the caller brings
-share no memory with a call's other tensors, except where said.
+or NaN, and below 2^-126 it loses bits.  Every tensor's data begins on 16
+bytes.  Outputs that the caller brings share no memory with a call's other
+tensors, except where said.
 """
 
 from __future__ import annotations
